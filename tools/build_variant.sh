@@ -9,7 +9,7 @@ mkdir -p $root/ab /tmp/vitk_ab_$name
 obj=/tmp/vitk_ab_$name/${src%.hip}.o
 extra=""; [ "$src" = gemm.hip -o "$src" = gemm_ntq.hip ] && extra="-mllvm -amdgpu-atomic-optimizer-strategy=None"      # as build.py's EXTRA_FLAGS
 [ "$src" = attention.hip ] && extra="-fno-slp-vectorize"
-/opt/rocm/bin/hipcc -O3 -fPIC -std=c++17 --offload-arch=gfx950 -Wno-unused-function $extra $flags -Wno-inline-asm -Wno-cuda-compat -Wno-pass-failed -c $csrc/$src -o $obj
+/opt/rocm/bin/hipcc -O3 -fPIC -std=c++17 --offload-arch=gfx950 -Wno-unused-function $extra $flags -Wno-inline-asm -Wno-cuda-compat -Wno-pass-failed -Xclang -target-feature -Xclang -packed-fp32-ops -c $csrc/$src -o $obj
 others=$(ls $csrc/build/*.o | grep -v "/${src%.hip}.o")
 /opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -o $root/ab/libvitk_$name.so $obj $others
 echo $root/ab/libvitk_$name.so

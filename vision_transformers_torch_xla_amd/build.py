@@ -17,7 +17,10 @@ LIB_PATH = CSRC / "libvitk.so"
 SOURCES = ["api.hip", "layernorm.hip", "gemm.hip", "gemm_ntq.hip", "attention.hip", "elementwise.hip", "loss.hip", "optim.hip", "preprocess.hip"]
 HEADERS = [CSRC / "common.h", CSRC / "gemm_nt.h", CSRC.parent.parent / "include" / "vitk.h"]
 ARCH = "gfx950"
-FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function", "-Wno-inline-asm", "-Wno-cuda-compat", "-Wno-pass-failed"]
+FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function", "-Wno-inline-asm", "-Wno-cuda-compat", "-Wno-pass-failed",
+         # no packed fp32 instructions (v_pk_fma_f32 and its kin): some of their forms have given wrong results on this hardware now and
+         # then, and hipcc forms them by itself from ordinary float code; the host pass warns that it does not know the feature
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # gemm.hip: the tile claim of the persistent kernel is ONE lane's atomic whose result is used a whole tile later; hipcc's atomic
 # optimizer would turn it into a wave-wide reduction and wait for the result on the spot
 EXTRA_FLAGS = {"gemm.hip": ["-mllvm", "-amdgpu-atomic-optimizer-strategy=None"],

@@ -80,7 +80,7 @@ static __device__ __forceinline__ float dgelu_erf(float x) {
     const float pdf = 0.39894228040143267794f * __builtin_amdgcn_exp2f(-0.72134752044448170368f * u * u);
     return __builtin_fmaf(x, pdf, cdf);
 }
-// Two elements at a time: the polynomial runs on v_pk_fma_f32 (half the instructions of the VALU-bound GEMM epilogues).
+// Two elements at a time (two independent fma chains; the build forbids the packed fp32 instructions that hipcc would form from them).
 static __device__ __forceinline__ f32x2_t half_erfc_poly2(f32x2_t u) {
     const f32x2_t c6 = {-1.3601819546238403e-06f, -1.3601819546238403e-06f}, c5 = {5.1214541599620134e-05f, 5.1214541599620134e-05f};
     const f32x2_t c4 = {-0.0008435604977421463f, -0.0008435604977421463f}, c3 = {0.008160343393683434f, 0.008160343393683434f};
