@@ -320,6 +320,31 @@ int vitk_sumsq(const float* g, int64_t n, float* out, int accumulate, void* work
                void* stream);
 size_t vitk_sumsq_workspace(int64_t n);
 
+/* ---- global L2 norm of `count` gradient tensors and clipping by it (torch.nn.utils.clip_grad_norm_ over separate tensors,
+ * engine.py:175-177):  norm[0] = sqrt(sum g^2);  dst[t] = min(1, max_norm / (norm + 1e-6)) * src[t], rounded to the tensor's type.
+ * src / dst / numel / type are HOST arrays of `count` entries (device addresses, element counts, 0 fp32 / 1 bf16 / 2 fp16; src and dst of one
+ * tensor have the same type); they are copied into the kernel arguments, so the caller may reuse them at once.  dst[t] == src[t] clips
+ * in place (and writes nothing where the norm does not exceed max_norm); dst = NULL computes the norm alone.  Addresses need the alignment of
+ * the type only; tensors must not overlap except dst[t] == src[t].  The sum is formed in double, in a fixed order.
+ * workspace: vitk_clip_grads_workspace(count) bytes. */
+size_t vitk_clip_grads_workspace(int count);
+int vitk_clip_grads(const void* const* src, void* const* dst, const int64_t* numel, const int* type, int count, float max_norm,
+                    float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- token embeddings.  Types: 0 fp32, 1 bf16.  ids: T int64 (ids_are_64) or int32 on the device.  D and the row strides ldt, ldo, ldd are
+ * multiples of 8 elements, rows 16-byte aligned.
+ * forward: out[t] = scale * table[ids[t]]; the row of an id outside [0, V) is NaN. */
+int vitk_embedding_fwd(const void* ids, int ids_are_64, const void* table, int table_type, int64_t ldt, void* out, int out_type, int64_t ldo,
+                       int64_t T, int64_t V, int D, float scale, void* stream);
+/* gradient: dtable[v] = scale * sum over the tokens t with ids[t] == v of dout[t], in fp32 and in the order of the tokens whatever the
+ * schedule (the tokens are sorted by id), rounded once; zero for rows without a token.  accumulate: added to what dtable holds, rows
+ * without a token stay untouched.  Tokens with id padding_idx (negative: none) or an id outside [0, V) add nothing.
+ * T, V < 2^31.  workspace: vitk_embedding_bwd_workspace(T, V, D) bytes. */
+size_t vitk_embedding_bwd_workspace(int64_t T, int64_t V, int D);
+int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void* ids, int ids_are_64, void* dtable, int dtable_type, int64_t ldo,
+                       int64_t T, int64_t V, int D, float scale, int64_t padding_idx, int accumulate, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,336 @@
+"""Operators around a vocabulary, and clipping over many tensors: against plain forms in 64 bits on the CPU.
+
+Tolerances count roundings: a value rounded to a type is off by at most finfo(type).eps / 2 of itself, an fp32 sum of n terms in any
+order by at most n * 2^-24 of the sum of the terms' magnitudes."""
+import math
+
+import pytest
+import torch
+
+bf16, f16, f32, f64 = torch.bfloat16, torch.float16, torch.float32, torch.float64
+U32 = 2.0 ** -24
+
+
+def _ops():
+    from vision_transformers_torch_xla_amd import ops
+    return ops
+
+
+def _error():
+    from vision_transformers_torch_xla_amd._lib import VitkError
+    return VitkError
+
+
+def half_ulp(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+# ------------------------------------------------------------------------------------------------- clipping
+def plain_clip(grads, max_norm):
+    norm = math.sqrt(sum(float(g.double().pow(2).sum()) for g in grads))
+    coef = max_norm / (norm + 1e-6)
+    coef = 1.0 if coef > 1.0 else coef
+    return norm, [g.double() * coef for g in grads]
+
+
+def check_clipped(got, want):
+    for g, w in zip(got, want):
+        # fp32: the norm, norm + 1e-6, the quotient and the product are rounded (the quotient to an ulp), then the result's type
+        assert torch.all((g.cpu().double() - w).abs() <= (6 * U32 + (half_ulp(g.dtype) if g.dtype != f32 else 0.0)) * w.abs() + (2.0 ** -25 if g.dtype == f16 else 2.0 ** -133 if g.dtype == bf16 else 1e-45))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtypes", [(f32,), (bf16,), (f16,), (f32, bf16, f16)])
+@pytest.mark.parametrize("sizes", [(1,), (7, 0, 1, 8191, 8192, 8193), (64, 100000, 3), tuple(1 + 37 * i % 300 for i in range(300))])
+@pytest.mark.parametrize("factor", [0.3, 3.0])
+def test_clip_grads(device, dtypes, sizes, factor):
+    ops = _ops()
+    g = torch.Generator().manual_seed(len(sizes) * 10 + len(dtypes))
+    grads = [torch.randn(n, generator=g).to(dtypes[i % len(dtypes)]) for i, n in enumerate(sizes)]
+    norm, _ = plain_clip(grads, 1.0)
+    norm_, want = plain_clip(grads, factor * norm)
+    dev = [t.to(device) for t in grads]
+    got = ops.clip_grads(dev, None)
+    assert got.shape == () and got.dtype == f32 and abs(got.item() - norm) <= 2 * U32 * norm
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, grads))
+    out = [torch.full_like(t, 77.0) for t in dev]
+    assert torch.equal(ops.clip_grads(dev, factor * norm, out=out), got)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, grads))
+    check_clipped(out, want)
+    assert torch.equal(ops.clip_grads(dev, factor * norm), got)
+    assert all(torch.equal(a, b) for a, b in zip(dev, out))
+    if factor > 1:
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, grads))
+
+
+@pytest.mark.gpu
+def test_clip_grads_views_order_and_extremes(device):
+    ops = _ops()
+    flat = torch.randn(40000, generator=torch.Generator().manual_seed(1)).to(device)
+    before = flat.clone()
+    # a view that starts between 16-byte lines, a transposed (dense) one, a four-dimensional one with its dimensions in another order
+    views = [flat[1:9001], flat[10000:22000].view(100, 120).t(), flat[22004:22004 + 3 * 4 * 5 * 6].view(3, 4, 5, 6).permute(0, 3, 1, 2)]
+    norm, want = plain_clip([v.cpu() for v in views], 1.0)
+    got = ops.clip_grads(views, 1.0)
+    assert abs(got.item() - norm) <= 2 * U32 * norm
+    check_clipped(views, want)
+    for lo, hi in ((0, 1), (9001, 10000), (22000, 22004), (22364, 40000)):          # what lies between the views stays
+        assert torch.equal(flat[lo:hi], before[lo:hi])
+    # squares beyond the range of fp32, and far below it
+    for scale in (3e30, 2e-30):
+        t = torch.full((1000,), scale, device=device)
+        assert abs(ops.clip_grads([t], None).item() / (scale * math.sqrt(1000)) - 1) <= 4 * U32
+    t = torch.full((1000,), 3e30, device=device)
+    ops.clip_grads([t], 1.0)
+    assert torch.all((t * math.sqrt(1000) - 1).abs() <= 1e-6)
+    # zeros; infinities and NaN spread as in torch
+    z = torch.zeros(10, device=device)
+    assert ops.clip_grads([z], 1.0).item() == 0.0 and torch.all(z == 0)
+    a, b = torch.tensor([1.0, math.inf], device=device), torch.ones(3, device=device)
+    assert ops.clip_grads([a, b], 1.0).item() == math.inf
+    assert a[0] == 0 and torch.isnan(a[1]) and torch.all(b == 0)
+    a, b = torch.tensor([1.0, math.nan], device=device), torch.ones(3, device=device)
+    assert math.isnan(ops.clip_grads([a, b], 1.0).item()) and torch.isnan(a).all() and torch.isnan(b).all()
+    b = torch.ones(3, device=device)
+    ops.clip_grads([b], 0.0)
+    assert torch.all(b == 0)
+    e = torch.empty(0, device=device)
+    assert ops.clip_grads([e], 1.0).item() == 0.0
+
+
+@pytest.mark.gpu
+def test_clip_grads_in_a_graph_on_another_stream(device):
+    ops = _ops()
+    grads = [torch.randn(n, device=device).to(dt) for n, dt in ((5000, f32), (777, bf16))]
+    out = [torch.empty_like(t) for t in grads]
+    ops.clip_grads(grads, 2.0, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = ops.clip_grads(grads, 2.0, out=out)
+    for k in range(3):
+        for t in grads:
+            t.copy_(torch.randn(t.shape, device=device) * (k + 1))
+        graph.replay()
+        want = [torch.empty_like(t) for t in grads]
+        eager = ops.clip_grads(grads, 2.0, out=want)
+        torch.cuda.synchronize()
+        assert torch.equal(norm, eager) and all(torch.equal(a, b) for a, b in zip(out, want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = [torch.empty_like(t) for t in grads]
+        n2 = ops.clip_grads(grads, 2.0, out=other)
+    torch.cuda.synchronize()
+    assert torch.equal(n2, eager) and all(torch.equal(a, b) for a, b in zip(other, want))
+
+
+@pytest.mark.gpu
+def test_clip_grads_refuses(device):
+    ops, err = _ops(), _error()
+    a = torch.randn(64, device=device)
+    for call in (lambda: ops.clip_grads([], 1.0),
+                 lambda: ops.clip_grads([a, a], 1.0),                                    # scaled twice
+                 lambda: ops.clip_grads([a[:40], a[30:]], 1.0),
+                 lambda: ops.clip_grads([a], 1.0, out=[a[1:]]),
+                 lambda: ops.clip_grads([a[:32], a[32:]], 1.0, out=[a[32:], a[:32]]),     # an output on another gradient
+                 lambda: ops.clip_grads([a], 1.0, out=[]),
+                 lambda: ops.clip_grads([a], 1.0, out=[torch.empty(64, device=device, dtype=bf16)]),
+                 lambda: ops.clip_grads([a], None, out=[torch.empty_like(a)]),
+                 lambda: ops.clip_grads([a], -1.0),
+                 lambda: ops.clip_grads([a], math.nan),
+                 lambda: ops.clip_grads([a.double()], 1.0),
+                 lambda: ops.clip_grads([a[::2]], 1.0),
+                 lambda: ops.clip_grads([a[:1].expand(8)], 1.0),
+                 lambda: ops.clip_grads([a, torch.zeros(4)], 1.0)):
+        keep = a.clone()
+        with pytest.raises(err):
+            call()
+        assert torch.equal(a, keep)
+
+
+# ----------------------------------------------------------------------------------------------- embeddings
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D", [(1, 1, 8), (1, 1000, 768), (7, 33, 200), (1000, 50, 1024), (513, 100003, 64), (3, 5, 8200)])
+@pytest.mark.parametrize("tt,ot", [(bf16, bf16), (f32, f32), (f32, bf16), (bf16, f32)])
+@pytest.mark.parametrize("it", [torch.int64, torch.int32])
+def test_embedding_fwd(device, T, V, D, tt, ot, it):
+    ops = _ops()
+    g = torch.Generator().manual_seed(T + V + D)
+    table = torch.randn(V, D, generator=g).to(tt)
+    ids = torch.randint(0, V, (T,), generator=g)
+    scale = 0.37
+    want = (table[ids].float() * torch.tensor(scale, dtype=f32)).to(ot)          # the kernel's own roundings: product in fp32, then the type
+    got = ops.embedding_fwd(ids.to(device, it), table.to(device), scale=scale, out_dtype=ot)
+    assert got.dtype == ot and torch.equal(got.cpu(), want)
+    exact = table[ids].double() * scale
+    assert torch.all((got.cpu().double() - exact).abs() <= (half_ulp(ot) + 2 * U32) * exact.abs())
+
+
+@pytest.mark.gpu
+def test_embedding_fwd_shapes_strides_and_bad_ids(device):
+    ops = _ops()
+    big = torch.randn(40, 64, device=device)
+    table = big[:, 8:40]                                                           # rows with a stride, first column on a 16-byte line
+    ids = torch.tensor([[3, 39, 0], [40, -1, 7]], device=device)
+    got = ops.embedding_fwd(ids, table)
+    assert got.shape == (2, 3, 32)
+    assert torch.equal(got[0], table[ids[0]]) and torch.equal(got[1, 2], table[7]) and torch.isnan(got[1, :2]).all()
+    assert torch.isnan(ops.embedding_fwd(torch.tensor([2 ** 40], device=device), table)).all()
+    assert ops.embedding_fwd(torch.empty(0, 4, dtype=torch.int64, device=device), table).shape == (0, 4, 32)
+    assert torch.equal(ops.embedding_fwd(ids.t(), table)[2, 1], table[7])          # ids in another order of dimensions
+    assert ops.embedding_fwd(ids[0, 0], table).shape == (32,)
+
+
+def plain_embedding_grad(dout, ids, V, scale, padding):
+    ids = ids.reshape(-1).long()
+    rows = dout.reshape(ids.numel(), -1).double()
+    keep = (ids >= 0) & (ids < V) & (ids != (-1 if padding is None else padding))
+    out, mag, count = (torch.zeros(V, rows.shape[1], dtype=f64), torch.zeros(V, rows.shape[1], dtype=f64), torch.zeros(V, 1, dtype=f64))
+    out.index_add_(0, ids[keep], rows[keep])
+    mag.index_add_(0, ids[keep], rows[keep].abs())
+    count.index_add_(0, ids[keep], torch.ones(int(keep.sum()), 1, dtype=f64))
+    return out * scale, mag * abs(scale), count
+
+
+def check_embedding_grad(got, dout, ids, V, scale, padding, base=None):
+    want, mag, count = plain_embedding_grad(dout, ids, V, scale, padding)
+    if base is not None:
+        want, mag = want + base.double(), mag + base.double().abs()
+    # the fp32 sum of `count` terms, times the scale, plus what was there, then the type
+    tol = (count + 3) * U32 * mag + (half_ulp(got.dtype) * 1.01 * want.abs() if got.dtype != f32 else 0.0)
+    assert torch.all((got.cpu().double() - want).abs() <= tol)
+
+
+EMB_IDS = {
+    "uniform": lambda T, V, g: torch.randint(0, V, (T,), generator=g),
+    "one": lambda T, V, g: torch.full((T,), V - 1),
+    "hot": lambda T, V, g: torch.where(torch.rand(T, generator=g) < 0.5, torch.zeros(T, dtype=torch.int64), torch.randint(0, V, (T,), generator=g)),
+    "bad": lambda T, V, g: torch.randint(-2, V + 2, (T,), generator=g),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D", [(1, 1, 8), (1, 1000, 768), (63, 2, 8), (65, 511, 72), (1025, 512, 64), (2049, 513, 200), (16384, 20000, 64), (16385, 700, 64),
+                                   (5000, 262143, 16), (5000, 262144, 16), (40000, 300, 2064), (300000, 5000, 8)])
+@pytest.mark.parametrize("kind", list(EMB_IDS))
+def test_embedding_bwd(device, T, V, D, kind):
+    ops = _ops()
+    g = torch.Generator().manual_seed(T + V + D)
+    ids = EMB_IDS[kind](T, V, g)
+    dt = bf16 if kind in ("uniform", "hot") else f32
+    dout = torch.randn(T, D, generator=g).to(dt)
+    scale, padding = 1.7, (None if kind == "uniform" else V // 2)
+    got = ops.embedding_bwd(dout.to(device), ids.to(device), V, scale=scale, padding_idx=padding)
+    assert got.dtype == dt and got.shape == (V, D)
+    check_embedding_grad(got, dout, ids, V, scale, padding)
+    again = ops.embedding_bwd(dout.to(device), ids.to(device, torch.int32), V, scale=scale, padding_idx=padding)
+    assert torch.equal(got, again)                                                  # no order of the hardware's in it
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [500, 20000])
+def test_embedding_bwd_accumulates_into_a_part_of_a_buffer(device, T):
+    ops = _ops()
+    g = torch.Generator().manual_seed(T)
+    V, D = 700, 40
+    ids = torch.randint(0, 300, (T // 4, 4), generator=g) * 2
+    dout = torch.randn(T // 4, 4, D + 8, generator=g).to(bf16)[..., :D]             # rows with a stride
+    buf = torch.randn(V, D + 16, generator=g).to(device)
+    before = buf.clone()
+    out = buf[:, 8:8 + D]
+    got = ops.embedding_bwd(dout.to(device), ids.to(device), V, scale=0.5, out=out, accumulate=True)
+    assert got is out
+    check_embedding_grad(out, dout, ids, V, 0.5, None, base=before[:, 8:8 + D].cpu())
+    assert torch.equal(buf[:, :8], before[:, :8]) and torch.equal(buf[:, 8 + D:], before[:, 8 + D:])
+    missed = torch.ones(V, dtype=torch.bool)
+    missed[ids.reshape(-1)] = False
+    assert torch.equal(out.cpu()[missed], before[:, 8:8 + D].cpu()[missed])
+    whole = torch.full((V, D), 9.0, device=device)                                   # without accumulate everything is written
+    ops.embedding_bwd(dout.to(device), ids.to(device), V, scale=0.5, out=whole)
+    check_embedding_grad(whole, dout, ids, V, 0.5, None)
+    none = ops.embedding_bwd(dout[:0].to(device), ids[:0].to(device), V)
+    assert none.shape == (V, D) and torch.all(none == 0)
+    assert torch.all(ops.embedding_bwd(dout[:0].to(device), ids[:0].to(device), 300000) == 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V", [(3000, 400), (30000, 400)])
+def test_embedding_bwd_in_a_graph(device, T, V):
+    ops = _ops()
+    ids = torch.randint(0, V, (T,), device=device)
+    dout = torch.randn(T, 64, device=device, dtype=bf16)
+    ops.embedding_bwd(dout, ids, V)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.embedding_bwd(dout, ids, V)
+        out = ops.embedding_fwd(ids, got)
+    for k in range(3):
+        ids.copy_(torch.randint(0, V, (T,), device=device))
+        dout.copy_(torch.randn(T, 64, device=device))
+        graph.replay()
+        want = ops.embedding_bwd(dout, ids, V)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(out, ops.embedding_fwd(ids, want))
+
+
+@pytest.mark.gpu
+def test_embedding_refuses(device):
+    ops, err = _ops(), _error()
+    table, ids, dout = torch.randn(10, 16, device=device), torch.zeros(4, dtype=torch.int64, device=device), torch.randn(4, 16, device=device)
+    for call in (lambda: ops.embedding_fwd(ids.float(), table),
+                 lambda: ops.embedding_fwd(ids.cpu(), table),
+                 lambda: ops.embedding_fwd(ids, table.half()),
+                 lambda: ops.embedding_fwd(ids, table, out_dtype=f16),
+                 lambda: ops.embedding_fwd(ids, table[:, :12]),                       # D % 8
+                 lambda: ops.embedding_fwd(ids, table[:, ::2]),
+                 lambda: ops.embedding_fwd(ids, table[:, 1:9]),                       # rows off the 16-byte lines
+                 lambda: ops.embedding_fwd(ids, table[:0]),                           # no rows
+                 lambda: ops.embedding_bwd(dout, ids[:3], 10),
+                 lambda: ops.embedding_bwd(dout, ids, 10, accumulate=True),
+                 lambda: ops.embedding_bwd(dout, ids, 10, out=torch.empty(9, 16, device=device)),
+                 lambda: ops.embedding_bwd(dout, ids, 10, out=torch.empty(10, 32, device=device)[:, :16]),    # a stride without accumulate
+                 lambda: ops.embedding_bwd(dout, ids, 10, out=torch.empty(10, 16, device=device), out_dtype=bf16),
+                 lambda: ops.embedding_bwd(dout[:, :12], ids, 10),
+                 lambda: ops.embedding_bwd(dout.half(), ids, 10),
+                 lambda: ops.embedding_bwd(dout, ids, 0)):
+        with pytest.raises(err):
+            call()
+
+
+# --------------------------------------------------------------------------------------- checks without a GPU
+def test_cpu_tensors_are_refused():
+    ops, err = _ops(), _error()
+    x = torch.zeros(4, 16)
+    ids = torch.zeros(4, dtype=torch.int64)
+    for call in (lambda: ops.clip_grads([x], 1.0), lambda: ops.embedding_fwd(ids, x), lambda: ops.embedding_bwd(x, ids, 4)):
+        with pytest.raises(err, match="GPU"):
+            call()
+
+
+def test_entry_points_check_before_they_launch():
+    import ctypes as C
+    from tests.test_abi_and_host import _lib
+    lib = _lib().load()
+    buf = C.create_string_buffer(65536)
+    p = (C.cast(buf, C.c_void_p).value + 255) // 256 * 256
+    one = lambda v, t: (t * 1)(v)          # noqa: E731
+    src, n, ty = one(p, C.c_void_p), one(4, C.c_int64), one(0, C.c_int)
+    need = lib.vitk_clip_grads_workspace(1)
+    assert need > 0 and lib.vitk_clip_grads_workspace(300) > need and lib.vitk_clip_grads_workspace(-1) == 0
+    assert lib.vitk_clip_grads(src, src, n, ty, 1, 1.0, p, p, 16, None) == -28
+    assert lib.vitk_clip_grads(src, src, n, ty, 1, -1.0, p, p, need, None) == -22
+    assert lib.vitk_clip_grads(src, src, n, one(3, C.c_int), 1, 1.0, p, p, need, None) == -22
+    assert lib.vitk_clip_grads(one(p + 2, C.c_void_p), src, n, ty, 1, 1.0, p, p, need, None) == -22
+    assert lib.vitk_clip_grads(src, src, one(-1, C.c_int64), ty, 1, 1.0, p, p, need, None) == -22
+    assert lib.vitk_clip_grads(src, src, n, ty, 1, 1.0, None, p, need, None) == -22
+    assert lib.vitk_embedding_fwd(p, 1, p, 0, 12, p, 0, 16, 4, 4, 12, 1.0, None) == -22 and b"multiples of 8" in lib.vitk_last_error()
+    assert lib.vitk_embedding_fwd(p, 1, p, 2, 16, p, 0, 16, 4, 4, 16, 1.0, None) == -22
+    assert lib.vitk_embedding_fwd(p, 1, p + 4, 0, 16, p, 0, 16, 4, 4, 16, 1.0, None) == -22
+    assert lib.vitk_embedding_fwd(None, 1, None, 0, 16, None, 0, 16, 0, 4, 16, 1.0, None) == 0          # nothing to do
+    need = lib.vitk_embedding_bwd_workspace(4, 4, 16)
+    assert lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 16, 4, 4, 16, 1.0, -1, 0, p, need - 1, None) == -28
+    assert lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 24, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22
+    assert lib.vitk_embedding_bwd(p, 0, 8, p, 1, p, 0, 16, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22
+    assert lib.vitk_embedding_bwd(None, 0, 16, p, 1, p, 0, 16, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22

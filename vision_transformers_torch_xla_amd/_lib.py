@@ -86,6 +86,11 @@ SIGNATURES = {
     "vitk_clip_grad_scale": (_i, [_p, _i64, _p, _f, _p]),
     "vitk_sumsq": (_i, [_p, _i64, _p, _i, _p, _sz, _p]),
     "vitk_sumsq_workspace": (_sz, [_i64]),
+    "vitk_clip_grads_workspace": (_sz, [_i]),
+    "vitk_clip_grads": (_i, [_p, _p, _p, _p, _i, _f, _p, _p, _sz, _p]),
+    "vitk_embedding_fwd": (_i, [_p, _i, _p, _i, _i64, _p, _i, _i64, _i64, _i64, _i, _f, _p]),
+    "vitk_embedding_bwd_workspace": (_sz, [_i64, _i64, _i]),
+    "vitk_embedding_bwd": (_i, [_p, _i, _i64, _p, _i, _p, _i, _i64, _i64, _i64, _i, _f, _i64, _i, _p, _sz, _p]),
 }
 
 EPI_PLAIN, EPI_BIAS, EPI_BIAS_F32, EPI_BIAS_GELU, EPI_BIAS_RES, EPI_PATCH, EPI_DGELU, EPI_BIAS_GELU_DG, EPI_MUL = range(9)

@@ -1,0 +1,496 @@
+// Lookup of token embeddings with scaling, out[t] = scale * table[ids[t]], and the gradient of the table,
+// dtable[v] (+)= scale * sum over {t : ids[t] = v} of dout[t].  Both are HBM-bound.
+//
+// The gradient is summed without atomics: the tokens are sorted by id (stable, so the order inside a row is the order of the tokens),
+// the sorted list is cut into pieces of equal length whatever the ids are, and a workgroup adds up the runs of equal ids inside its
+// piece in fp32.  A run that ends inside its piece is final; the parts of a run that crosses pieces go to fp32 partial rows that a
+// second kernel joins in order.  So one id that is half of all tokens costs what any other mix costs, and the result does not depend
+// on the schedule.
+// Ids outside [0, V) never become an address: the lookup gives a row of NaN for them, the gradient leaves them out.
+#include "common.h"
+
+struct EmbFwdParams {
+    const void* ids; const void* table; void* out;
+    long long T, V, ldt, ldo;
+    int chunks;             // 8-element chunks per row
+    int rows_per_block;
+    float scale;
+};
+
+template <typename T8> struct Emb8;
+template <> struct Emb8<bf16_t> {
+    static __device__ __forceinline__ void load(const bf16_t* p, float (&v)[8]) { load8(p, v); }
+    static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[8]) { store8(p, v); }
+};
+template <> struct Emb8<float> {
+    static __device__ __forceinline__ void load(const float* p, float (&v)[8]) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+    static __device__ __forceinline__ void store(float* p, const float (&v)[8]) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+};
+
+template <typename I>
+static __device__ __forceinline__ long long emb_id(const void* ids, long long t) { return (long long)reinterpret_cast<const I*>(ids)[t]; }
+
+// A block takes rows_per_block rows, flattened into 8-element chunks; a thread has up to four chunks in flight.
+template <typename I, typename TI, typename TO>
+__global__ __launch_bounds__(256) void embedding_fwd_kernel(const EmbFwdParams p) {
+    const long long row0 = (long long)blockIdx.x * p.rows_per_block;
+    const long long left = p.T - row0;
+    const unsigned rows = left < p.rows_per_block ? (unsigned)left : (unsigned)p.rows_per_block;
+    const unsigned total = rows * (unsigned)p.chunks;
+    const TI* table = reinterpret_cast<const TI*>(p.table);
+    TO* out = reinterpret_cast<TO*>(p.out);
+    for (unsigned base = threadIdx.x; base < total; base += 1024) {
+        float v[4][8];
+        unsigned row[4], col[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned c = base + j * 256;
+            row[j] = c / (unsigned)p.chunks;
+            col[j] = (c - row[j] * (unsigned)p.chunks) * 8u;
+            if (c < total) {
+                const long long id = emb_id<I>(p.ids, row0 + row[j]);
+                if (id >= 0 && id < p.V) {
+                    Emb8<TI>::load(table + id * p.ldt + col[j], v[j]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[j][k] = __builtin_nanf("");
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (base + j * 256 < total) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[j][k] *= p.scale;
+                Emb8<TO>::store(out + (row0 + row[j]) * p.ldo + col[j], v[j]);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- sorting
+// Stable radix sort of (key, position) by key, 9 bits a pass.  Key V is the sentinel of tokens without a gradient (padding, an id out
+// of range); it sorts behind every row.
+#define SORT_BINS 512
+#define SORT_BITS 9
+#define SORT_ITEMS 16
+
+template <typename I>
+static __device__ __forceinline__ unsigned emb_key(const void* ids, long long t, long long V, long long padding) {
+    const long long id = emb_id<I>(ids, t);
+    return id >= 0 && id < V && id != padding ? (unsigned)id : (unsigned)V;
+}
+// lanes of the wave with the same digit: their mask
+static __device__ __forceinline__ unsigned long long sort_peers(unsigned digit) {
+    unsigned long long m = ~0ull;
+#pragma unroll
+    for (int b = 0; b < SORT_BITS; ++b) {
+        const unsigned long long bal = __ballot((digit >> b) & 1u);
+        m &= (digit >> b) & 1u ? bal : ~bal;
+    }
+    return m;
+}
+// inclusive sum over the wave
+static __device__ __forceinline__ unsigned wave_scan(unsigned v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+// rank of the thread's items among the block's: items j = 0.. of wave w are tokens w * 64 * SORT_ITEMS + j * 64 + lane, so the order of
+// (wave, item, lane) is the order of the input.  hist[wave][bin] holds the wave's first rank per bin and is moved on.
+static __device__ __forceinline__ unsigned sort_rank(unsigned* hist_wave, unsigned digit) {
+    const int lane = threadIdx.x & 63;
+    const unsigned long long m = sort_peers(digit);
+    const unsigned before = (unsigned)__popcll(m & ((1ull << lane) - 1ull));
+    const unsigned base = hist_wave[digit];         // the wave's LDS operations run in order: all lanes read before the first of a bin writes
+    asm volatile("" ::: "memory");
+    if (before == 0) hist_wave[digit] = base + (unsigned)__popcll(m);
+    asm volatile("" ::: "memory");
+    return base + before;
+}
+
+// The whole sort in one workgroup, for up to 16384 tokens of a vocabulary below 2^18: key and position share one word.  One pass over
+// 16384 tokens takes the compute unit a few microseconds, less than the two launches that a pass over several workgroups needs.
+// The blocks behind the first zero the gradient meanwhile.
+#define SORT1_MAX 16384
+template <typename I>
+__global__ __launch_bounds__(1024) void emb_sort_one_kernel(const void* ids, int T, long long V, long long padding, int passes, uint2* sorted,
+                                                            uint4* zero, long long zero16) {
+    extern __shared__ unsigned sh[];        // [16384] words, [16][512] counters, [16] scan
+    if (blockIdx.x > 0) {
+        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+        for (long long i = (long long)(blockIdx.x - 1) * 1024 + threadIdx.x; i < zero16; i += (long long)(gridDim.x - 1) * 1024) zero[i] = z;
+        return;
+    }
+    unsigned* buf = sh;
+    unsigned* hist = sh + SORT1_MAX;
+    unsigned* sums = hist + 16 * SORT_BINS;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    unsigned* mine = hist + wave * SORT_BINS;
+    const int items = (T + 1023) / 1024;        // per thread; a wave's items are consecutive in the input
+    unsigned word[SORT_ITEMS];
+#pragma unroll
+    for (int j = 0; j < SORT_ITEMS; ++j) {
+        const int t = (wave * items + j) * 64 + lane;
+        word[j] = j < items && t < T ? (emb_key<I>(ids, t, V, padding) << 14) | (unsigned)t : 0xffffffffu;
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = 14 + pass * SORT_BITS;
+        for (int i = threadIdx.x; i < 16 * SORT_BINS; i += 1024) hist[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < SORT_ITEMS; ++j)
+            if (j < items) atomicAdd(&mine[(word[j] >> shift) & (SORT_BINS - 1)], 1u);
+        __syncthreads();
+        unsigned total = 0;
+        if (threadIdx.x < SORT_BINS)
+            for (int w = 0; w < 16; ++w) { const unsigned c = hist[w * SORT_BINS + threadIdx.x]; hist[w * SORT_BINS + threadIdx.x] = total; total += c; }
+        const unsigned incl = wave_scan(total);
+        if (lane == 63) sums[wave] = incl;
+        __syncthreads();
+        if (threadIdx.x < SORT_BINS) {
+            unsigned base = incl - total;
+            for (int w = 0; w < wave; ++w) base += sums[w];
+            for (int w = 0; w < 16; ++w) hist[w * SORT_BINS + threadIdx.x] += base;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < SORT_ITEMS; ++j)
+            if (j < items) buf[sort_rank(mine, (word[j] >> shift) & (SORT_BINS - 1))] = word[j];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < SORT_ITEMS; ++j)
+            if (j < items) word[j] = buf[(wave * items + j) * 64 + lane];
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < SORT_ITEMS; ++j) {
+        const int t = (wave * items + j) * 64 + lane;
+        if (j < items && t < T) sorted[t] = make_uint2(word[j] >> 14, word[j] & 16383u);
+    }
+}
+
+// Several workgroups: per pass a histogram launch (counts[block][bin]) and a launch that turns the counts into ranks and scatters.
+#define SORT_BLOCK (256 * SORT_ITEMS)       // tokens per workgroup
+
+template <typename I, bool FIRST>
+static __device__ __forceinline__ uint2 sort_item(const void* ids, const uint2* in, long long t, long long T, long long V, long long padding) {
+    if (t >= T) return make_uint2(0xffffffffu, 0u);
+    if (FIRST) return make_uint2(emb_key<I>(ids, t, V, padding), (unsigned)t);
+    return in[t];
+}
+
+template <typename I, bool FIRST>
+__global__ __launch_bounds__(256) void emb_hist_kernel(const void* ids, const uint2* in, long long T, long long V, long long padding, int shift,
+                                                       unsigned* counts, int blocks, uint4* zero, long long zero16) {
+    __shared__ unsigned hist[SORT_BINS];
+    if ((int)blockIdx.x >= blocks) {        // the blocks behind the sort's zero the gradient (first pass only)
+        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+        const long long step = (long long)(gridDim.x - blocks) * 256;
+        for (long long i = (long long)(blockIdx.x - blocks) * 256 + threadIdx.x; i < zero16; i += step) zero[i] = z;
+        return;
+    }
+    hist[threadIdx.x] = 0;
+    hist[threadIdx.x + 256] = 0;
+    __syncthreads();
+    const long long t0 = (long long)blockIdx.x * SORT_BLOCK;
+#pragma unroll
+    for (int j = 0; j < SORT_ITEMS; ++j) {
+        const long long t = t0 + j * 256 + threadIdx.x;
+        const uint2 it = sort_item<I, FIRST>(ids, in, t, T, V, padding);
+        if (t < T) atomicAdd(&hist[(it.x >> shift) & (SORT_BINS - 1)], 1u);
+    }
+    __syncthreads();
+    counts[(size_t)blockIdx.x * SORT_BINS + threadIdx.x] = hist[threadIdx.x];
+    counts[(size_t)blockIdx.x * SORT_BINS + threadIdx.x + 256] = hist[threadIdx.x + 256];
+}
+
+template <typename I, bool FIRST>
+__global__ __launch_bounds__(256) void emb_scatter_kernel(const void* ids, const uint2* in, long long T, long long V, long long padding, int shift,
+                                                          const unsigned* __restrict__ counts, int blocks, uint2* out) {
+    __shared__ unsigned hist[4 * SORT_BINS];
+    __shared__ unsigned sums[4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    unsigned* mine = hist + wave * SORT_BINS;
+    for (int i = threadIdx.x; i < 4 * SORT_BINS; i += 256) hist[i] = 0;
+    __syncthreads();
+    uint2 item[SORT_ITEMS];
+    const long long t0 = (long long)blockIdx.x * SORT_BLOCK + wave * (64 * SORT_ITEMS);
+#pragma unroll
+    for (int j = 0; j < SORT_ITEMS; ++j) {
+        const long long t = t0 + j * 64 + lane;
+        item[j] = sort_item<I, FIRST>(ids, in, t, T, V, padding);
+        if (t < T) atomicAdd(&mine[(item[j].x >> shift) & (SORT_BINS - 1)], 1u);
+    }
+    // thread i owns bins 2i and 2i + 1: their totals and the share of the blocks before this one
+    const int b0 = 2 * threadIdx.x;
+    unsigned tot0 = 0, tot1 = 0, pre0 = 0, pre1 = 0;
+    for (int b = 0; b < blocks; ++b) {
+        const uint2 c = *reinterpret_cast<const uint2*>(counts + (size_t)b * SORT_BINS + b0);
+        if (b == (int)blockIdx.x) { pre0 = tot0; pre1 = tot1; }
+        tot0 += c.x; tot1 += c.y;
+    }
+    const unsigned incl = wave_scan(tot0 + tot1);
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    unsigned base = incl - tot0 - tot1;
+    for (int w = 0; w < wave; ++w) base += sums[w];
+    unsigned r0 = base + pre0, r1 = base + tot0 + pre1;
+    for (int w = 0; w < 4; ++w) {
+        const unsigned c0 = hist[w * SORT_BINS + b0], c1 = hist[w * SORT_BINS + b0 + 1];
+        hist[w * SORT_BINS + b0] = r0; hist[w * SORT_BINS + b0 + 1] = r1;
+        r0 += c0; r1 += c1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < SORT_ITEMS; ++j) {
+        const long long t = t0 + j * 64 + lane;
+        // tokens behind the last one take ranks of bin 511 behind every real one of this block, which is the last block; they are not stored
+        const unsigned r = sort_rank(mine, (item[j].x >> shift) & (SORT_BINS - 1));
+        if (t < T) out[r] = item[j];
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- sums
+struct EmbBwdParams {
+    const uint2* sorted; const void* dout; void* out; float* partial;       // partial: [pieces][2][D]: the piece's head run, its tail run
+    long long T, V, ldd, ldo;
+    int D, piece, pieces, accumulate;
+    float scale;
+};
+
+template <typename TO>
+static __device__ __forceinline__ void emb_put(const EmbBwdParams& p, unsigned key, int col, float (&acc)[8]) {
+    TO* q = reinterpret_cast<TO*>(p.out) + (long long)key * p.ldo + col;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] *= p.scale;
+    if (p.accumulate) {
+        float o[8];
+        Emb8<TO>::load(q, o);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += o[k];
+    }
+    Emb8<TO>::store(q, acc);
+}
+
+// One workgroup per piece of the sorted list and slice of 8 * blockDim columns.  The rows of a piece are independent loads: EMB_AHEAD
+// of them are in flight while the sums are formed in order.
+#define EMB_AHEAD 8
+template <typename TI, typename TO>
+__global__ __launch_bounds__(256) void embedding_bwd_kernel(const EmbBwdParams p) {
+    const int col = ((int)blockIdx.y * (int)blockDim.x + (int)threadIdx.x) * 8;
+    if (col >= p.D) return;
+    const long long i0 = (long long)blockIdx.x * p.piece;
+    const long long i1 = i0 + p.piece < p.T ? i0 + p.piece : p.T;
+    const TI* dout = reinterpret_cast<const TI*>(p.dout);
+    float* part = p.partial + (size_t)blockIdx.x * 2 * p.D + col;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    unsigned key = p.sorted[i0].x;
+    bool head = i0 > 0 && p.sorted[i0 - 1].x == key;        // the run began in an earlier piece
+    for (long long i = i0; i < i1; i += EMB_AHEAD) {
+        float v[EMB_AHEAD][8];
+        uint2 it[EMB_AHEAD];
+#pragma unroll
+        for (int j = 0; j < EMB_AHEAD; ++j) {
+            const long long at = i + j < i1 ? i + j : i1 - 1;
+            it[j] = p.sorted[at];
+        }
+#pragma unroll
+        for (int j = 0; j < EMB_AHEAD; ++j) Emb8<TI>::load(dout + (long long)it[j].y * p.ldd + col, v[j]);
+#pragma unroll
+        for (int j = 0; j < EMB_AHEAD; ++j) {
+            if (i + j >= i1) break;
+            if (it[j].x != key) {
+                if ((long long)key < p.V) {
+                    if (head) Emb8<float>::store(part, acc);
+                    else emb_put<TO>(p, key, col, acc);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+                key = it[j].x;
+                head = false;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] += v[j][k];
+        }
+        if ((long long)key >= p.V) break;       // only tokens without a gradient follow
+    }
+    if ((long long)key >= p.V) return;
+    const bool goes_on = i1 < p.T && p.sorted[i1].x == key;
+    if (head) Emb8<float>::store(part, acc);
+    else if (goes_on) Emb8<float>::store(part + p.D, acc);
+    else emb_put<TO>(p, key, col, acc);
+}
+
+// Runs that cross pieces: the workgroup of the piece a run begins in (as its tail) adds the head sums of the pieces that follow.
+template <typename TO>
+__global__ __launch_bounds__(256) void embedding_join_kernel(const EmbBwdParams p) {
+    const int col = ((int)blockIdx.y * (int)blockDim.x + (int)threadIdx.x) * 8;
+    if (col >= p.D) return;
+    const long long i1 = (long long)(blockIdx.x + 1) * p.piece;       // the grid has one block less than there are pieces
+    const unsigned key = p.sorted[i1 - 1].x;
+    if ((long long)key >= p.V || p.sorted[i1].x != key) return;       // nothing crosses this border
+    const long long i0 = i1 - p.piece;
+    if (p.sorted[i0].x == key && i0 > 0 && p.sorted[i0 - 1].x == key) return;       // the run began earlier
+    float acc[8];
+    Emb8<float>::load(p.partial + ((size_t)blockIdx.x * 2 + 1) * p.D + col, acc);
+    // how many pieces the run enters (the sorted keys: first piece whose first key is another one)
+    long long lo = blockIdx.x + 1, hi = p.pieces;
+    while (lo < hi) {
+        const long long mid = (lo + hi) >> 1;
+        if (p.sorted[mid * p.piece].x == key) lo = mid + 1; else hi = mid;
+    }
+    const float* q = p.partial + col;
+#pragma unroll 8
+    for (long long c = blockIdx.x + 1; c < lo; ++c) {
+        float v[8];
+        Emb8<float>::load(q + (size_t)c * 2 * p.D, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += v[k];
+    }
+    emb_put<TO>(p, key, col, acc);
+}
+
+// pieces of the sorted list: about 2048 workgroups where there are enough tokens, 8 to 512 tokens each
+static int emb_piece(long long T) {
+    long long c = (T + 2047) / 2048;
+    c = (c + 7) / 8 * 8;
+    return (int)(c < 8 ? 8 : c > 512 ? 512 : c);
+}
+static int emb_passes(long long V) {
+    int bits = 0;
+    while (bits < 32 && (V >> bits) != 0) ++bits;        // keys 0 .. V
+    return (bits + SORT_BITS - 1) / SORT_BITS;
+}
+static bool emb_one(long long T, long long V) { return T == 0 || (T <= SORT1_MAX && V < (1 << 18)); }
+static size_t emb_up(size_t n) { return (n + 255) & ~(size_t)255; }
+
+extern "C" {
+
+int vitk_embedding_fwd(const void* ids, int ids_are_64, const void* table, int table_type, int64_t ldt, void* out, int out_type, int64_t ldo,
+                       int64_t T, int64_t V, int D, float scale, void* stream) {
+    VITK_REQUIRE(T >= 0 && V > 0 && D > 0, "embedding_fwd: bad shape T=%lld V=%lld D=%d", (long long)T, (long long)V, D);
+    VITK_REQUIRE((table_type == 0 || table_type == 1) && (out_type == 0 || out_type == 1), "embedding_fwd: types are 0 (fp32) and 1 (bf16)");
+    if (T == 0) return VITK_OK;
+    VITK_REQUIRE(ids && table && out, "embedding_fwd: null pointer");
+    VITK_REQUIRE(D % 8 == 0 && ldt % 8 == 0 && ldo % 8 == 0 && ldt >= D && ldo >= D, "embedding_fwd: D and the row strides must be multiples of 8, strides >= D (D=%d ldt=%lld ldo=%lld)",
+                 D, (long long)ldt, (long long)ldo);
+    VITK_REQUIRE(vitk_aligned(table, 16) && vitk_aligned(out, 16) && vitk_aligned(ids, ids_are_64 ? 8 : 4), "embedding_fwd: rows must be 16-byte aligned");
+    EmbFwdParams p;
+    p.ids = ids; p.table = table; p.out = out; p.T = T; p.V = V; p.ldt = ldt; p.ldo = ldo; p.scale = scale;
+    p.chunks = D / 8;
+    p.rows_per_block = p.chunks >= 1024 ? 1 : 1024 / p.chunks;
+    const long long blocks = (T + p.rows_per_block - 1) / p.rows_per_block;
+    VITK_REQUIRE(blocks < 0x7fffffff, "embedding_fwd: too many tokens (%lld)", (long long)T);
+    hipStream_t s = (hipStream_t)stream;
+#define EMB_FWD(I, TI, TO) embedding_fwd_kernel<I, TI, TO><<<(int)blocks, 256, 0, s>>>(p)
+    switch ((ids_are_64 ? 4 : 0) | (table_type << 1) | out_type) {
+        case 0: EMB_FWD(int32_t, float, float); break;
+        case 1: EMB_FWD(int32_t, float, bf16_t); break;
+        case 2: EMB_FWD(int32_t, bf16_t, float); break;
+        case 3: EMB_FWD(int32_t, bf16_t, bf16_t); break;
+        case 4: EMB_FWD(int64_t, float, float); break;
+        case 5: EMB_FWD(int64_t, float, bf16_t); break;
+        case 6: EMB_FWD(int64_t, bf16_t, float); break;
+        default: EMB_FWD(int64_t, bf16_t, bf16_t); break;
+    }
+#undef EMB_FWD
+    return vitk_check_launch("embedding_fwd");
+}
+
+size_t vitk_embedding_bwd_workspace(int64_t T, int64_t V, int D) {
+    if (T <= 0 || V <= 0 || D <= 0) return 16;
+    const long long pieces = (T + emb_piece(T) - 1) / emb_piece(T);
+    size_t n = emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)pieces * 2 * D * sizeof(float));
+    if (!emb_one(T, V)) n += emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)((T + SORT_BLOCK - 1) / SORT_BLOCK) * SORT_BINS * sizeof(unsigned));
+    return n;
+}
+
+int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void* ids, int ids_are_64, void* dtable, int dtable_type, int64_t ldo,
+                       int64_t T, int64_t V, int D, float scale, int64_t padding_idx, int accumulate, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+    VITK_REQUIRE(T >= 0 && V > 0 && D > 0, "embedding_bwd: bad shape T=%lld V=%lld D=%d", (long long)T, (long long)V, D);
+    VITK_REQUIRE((dout_type == 0 || dout_type == 1) && (dtable_type == 0 || dtable_type == 1), "embedding_bwd: types are 0 (fp32) and 1 (bf16)");
+    VITK_REQUIRE(T < 0x7fffffffll && V < 0x7fffffffll, "embedding_bwd: T and V must be below 2^31");
+    VITK_REQUIRE(dtable && workspace && (T == 0 || (dout && ids)), "embedding_bwd: null pointer");
+    VITK_REQUIRE(D % 8 == 0 && ldd % 8 == 0 && ldo % 8 == 0 && ldd >= D && ldo >= D, "embedding_bwd: D and the row strides must be multiples of 8, strides >= D (D=%d ldd=%lld ldo=%lld)",
+                 D, (long long)ldd, (long long)ldo);
+    VITK_REQUIRE(vitk_aligned(dtable, 16) && vitk_aligned(workspace, 16) && (T == 0 || (vitk_aligned(dout, 16) && vitk_aligned(ids, ids_are_64 ? 8 : 4))),
+                 "embedding_bwd: rows must be 16-byte aligned");
+    VITK_REQUIRE(accumulate || ldo == D, "embedding_bwd: without accumulate the gradient must be contiguous (ldo == D)");
+    if (workspace_bytes < vitk_embedding_bwd_workspace(T, V, D)) {
+        vitk_set_error("embedding_bwd: workspace %zu < %zu", workspace_bytes, vitk_embedding_bwd_workspace(T, V, D));
+        return VITK_ENOSPC;
+    }
+    hipStream_t s = (hipStream_t)stream;
+    const long long zero16 = accumulate ? 0 : (long long)V * D * (dtable_type == 0 ? 4 : 2) / 16;
+    const int zero_blocks = (int)(zero16 / 4096 < 1024 ? (zero16 + 4095) / 4096 : 1024);
+    const int passes = emb_passes(V);
+    char* ws = (char*)workspace;
+    uint2* sorted = (uint2*)ws;
+    ws += emb_up((size_t)T * sizeof(uint2));
+    EmbBwdParams p;
+    p.piece = emb_piece(T);
+    p.pieces = (int)((T + p.piece - 1) / p.piece);
+    p.partial = (float*)ws;
+    ws += emb_up((size_t)p.pieces * 2 * D * sizeof(float));
+    if (emb_one(T, V)) {
+        const size_t lds = (SORT1_MAX + 16 * SORT_BINS + 16) * sizeof(unsigned);
+        static VitkLdsOnce once64 = {}, once32 = {};
+        if (int rc = ids_are_64 ? vitk_lds_once(once64, (const void*)emb_sort_one_kernel<int64_t>, lds, "embedding_bwd")
+                                : vitk_lds_once(once32, (const void*)emb_sort_one_kernel<int32_t>, lds, "embedding_bwd"))
+            return rc;
+        if (ids_are_64) emb_sort_one_kernel<int64_t><<<1 + zero_blocks, 1024, lds, s>>>(ids, (int)T, V, padding_idx, passes, sorted, (uint4*)dtable, zero16);
+        else emb_sort_one_kernel<int32_t><<<1 + zero_blocks, 1024, lds, s>>>(ids, (int)T, V, padding_idx, passes, sorted, (uint4*)dtable, zero16);
+        if (int rc = vitk_check_launch("embedding_bwd_sort")) return rc;
+    } else {
+        uint2* other = (uint2*)ws;
+        ws += emb_up((size_t)T * sizeof(uint2));
+        unsigned* counts = (unsigned*)ws;
+        const int blocks = (int)((T + SORT_BLOCK - 1) / SORT_BLOCK);
+        // the last pass has to write `sorted`
+        uint2* to = passes & 1 ? sorted : other;
+        uint2* from = nullptr;
+        for (int pass = 0; pass < passes; ++pass) {
+            const int shift = pass * SORT_BITS, extra = pass == 0 ? zero_blocks : 0;
+#define EMB_PASS(I, F)                                                                                                                       \
+    emb_hist_kernel<I, F><<<blocks + extra, 256, 0, s>>>(ids, from, T, V, padding_idx, shift, counts, blocks, (uint4*)dtable, zero16);      \
+    emb_scatter_kernel<I, F><<<blocks, 256, 0, s>>>(ids, from, T, V, padding_idx, shift, counts, blocks, to)
+            if (pass > 0) { EMB_PASS(int64_t, false); }
+            else if (ids_are_64) { EMB_PASS(int64_t, true); }
+            else { EMB_PASS(int32_t, true); }
+#undef EMB_PASS
+            if (int rc = vitk_check_launch("embedding_bwd_sort")) return rc;
+            from = to;
+            to = to == sorted ? other : sorted;
+        }
+    }
+    if (T == 0) return VITK_OK;
+    p.sorted = sorted; p.dout = dout; p.out = dtable; p.T = T; p.V = V; p.ldd = ldd; p.ldo = ldo; p.D = D; p.accumulate = accumulate; p.scale = scale;
+    const int lanes = D / 8;
+    const int threads = lanes >= 256 ? 256 : (lanes + 63) / 64 * 64;
+    const dim3 grid(p.pieces, (lanes + threads - 1) / threads), join(p.pieces > 1 ? p.pieces - 1 : 1, grid.y);
+#define EMB_BWD(TI, TO)                                                                                  \
+    embedding_bwd_kernel<TI, TO><<<grid, threads, 0, s>>>(p);                                            \
+    if (p.pieces > 1) embedding_join_kernel<TO><<<join, threads, 0, s>>>(p)
+    switch ((dout_type << 1) | dtable_type) {
+        case 0: EMB_BWD(float, float); break;
+        case 1: EMB_BWD(float, bf16_t); break;
+        case 2: EMB_BWD(bf16_t, float); break;
+        default: EMB_BWD(bf16_t, bf16_t); break;
+    }
+#undef EMB_BWD
+    return vitk_check_launch("embedding_bwd");
+}
+
+}  // extern "C"

@@ -466,6 +466,165 @@ def clip_grad_scale(g, sumsq_t, max_norm):
     check(_lib.load().vitk_clip_grad_scale(_ptr(g), g.numel(), _ptr(sumsq_t), float(max_norm), _stream()), "clip_grad_scale")
 
 
+# ------------------------------------------------------------------------- gradients of many tensors, token embeddings
+def _here(t, name):
+    """a tensor a kernel of the current stream may use: on the current device (one process drives one GPU at a time)"""
+    if not t.is_cuda:
+        raise _lib.VitkError(f"{name}: expected a GPU tensor (the HIP kernels are the only implementation), got {t.device}")
+    if _cur_device is not None and t.device.index != _cur_device():
+        raise _lib.VitkError(f"{name}: the tensor is on {t.device}, the current device is cuda:{_cur_device()}; "
+                             "make it current (torch.cuda.set_device) before the call")
+
+
+def _dense(t):
+    """every element of the tensor's memory range belongs to it, once, in whatever order of its dimensions"""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+_CLIP_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _clip_table(tensors, what):
+    """(addresses, element counts, type codes) of a list of dense gradients as numpy arrays"""
+    if not tensors:
+        return np.zeros(0, np.int64), np.zeros(0, np.int64), np.zeros(0, np.int32)
+    _here(tensors[0], what)
+    device = tensors[0].device
+    types = []
+    for i, t in enumerate(tensors):
+        code = _CLIP_TYPES.get(t.dtype)
+        if code is None:
+            raise _lib.VitkError(f"{what}[{i}]: expected float32, bfloat16 or float16, got {t.dtype}")
+        if t.layout is not torch.strided or not (t.is_contiguous() or _dense(t)):
+            raise _lib.VitkError(f"{what}[{i}]: expected a dense tensor, got shape {tuple(t.shape)} with strides "
+                                 f"{t.stride() if t.layout is torch.strided else t.layout}")
+        if t.device != device:
+            raise _lib.VitkError(f"{what}: tensors on {device} and {t.device} in one call")
+        types.append(code)
+    return (np.array([t.data_ptr() for t in tensors], np.int64), np.array([t.numel() for t in tensors], np.int64), np.array(types, np.int32))
+
+
+def _overlap(first, size):
+    """whether any two of the byte ranges [first, first + size) meet"""
+    keep = size > 0
+    first, size = first[keep], size[keep]
+    order = np.argsort(first, kind="stable")
+    first, size = first[order], size[order]
+    return bool((first[:-1] + size[:-1] > first[1:]).any())
+
+
+def clip_grads(tensors, max_norm, out=None):
+    """Global L2 norm of a list of gradient tensors (fp32, bf16, fp16 in any mix, dense) and clipping by it, in two launches for up to 128
+    tensors: t *= min(1, max_norm / (norm + 1e-6)).  Returns the norm before clipping as a 0-d fp32 GPU tensor; nothing is copied to
+    the host.  out: tensors of the same shapes, strides and types that receive the clipped gradients (tensors themselves stay as
+    they are); None: in place.  max_norm None: the norm alone.  A norm that is infinite or NaN spreads as in torch's clip_grad_norm_
+    (finite gradients become 0 or NaN)."""
+    tensors = list(tensors)
+    src, numel, types = _clip_table(tensors, "tensors")
+    if not tensors:
+        raise _lib.VitkError("clip_grads: no tensors (a device is needed for the norm)")
+    if max_norm is not None and not max_norm >= 0.0:
+        raise _lib.VitkError(f"clip_grads: max_norm must not be negative, got {max_norm}")
+    dst = None
+    if max_norm is not None:
+        size = numel * np.where(types == 0, 4, 2)
+        dst = src
+        if out is not None:
+            out = list(out)
+            if len(out) != len(tensors):
+                raise _lib.VitkError(f"clip_grads: {len(tensors)} tensors, {len(out)} outputs")
+            dst, _, _ = _clip_table(out, "out")
+            for i, (a, b) in enumerate(zip(tensors, out)):
+                if a.dtype != b.dtype or a.shape != b.shape or a.device != b.device or a.stride() != b.stride():
+                    raise _lib.VitkError(f"clip_grads: out[{i}] must have the shape, strides, type and device of tensors[{i}]")
+            other = dst != src
+            if _overlap(np.concatenate([dst, src[other]]), np.concatenate([size, size[other]])):
+                raise _lib.VitkError("clip_grads: the outputs overlap each other or another gradient")
+        elif _overlap(src, size):
+            raise _lib.VitkError("clip_grads: the same memory is in the list twice (it would be scaled twice)")
+    elif out is not None:
+        raise _lib.VitkError("clip_grads: out needs a max_norm")
+    lib = _lib.load()
+    norm = torch.empty((), dtype=f32, device=tensors[0].device)
+    ws = torch.empty(lib.vitk_clip_grads_workspace(len(tensors)), dtype=torch.uint8, device=norm.device)
+    check(lib.vitk_clip_grads(src.ctypes.data, None if dst is None else dst.ctypes.data, numel.ctypes.data, types.ctypes.data, len(tensors),
+                              float(max_norm or 0.0), _ptr(norm), _ptr(ws), ws.numel(), _stream()), "clip_grads")
+    return norm
+
+
+_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _rows2d(t, name):
+    """an fp32 / bf16 matrix with contiguous rows -> (type code, row stride)"""
+    _here(t, name)
+    code = _ROW_TYPES.get(t.dtype)
+    if code is None:
+        raise _lib.VitkError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise _lib.VitkError(f"{name}: expected a matrix with contiguous rows, got shape {tuple(t.shape)} with strides {t.stride()}")
+    return code, t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _ids1d(ids):
+    _here(ids, "ids")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise _lib.VitkError(f"ids: expected int64 or int32, got {ids.dtype}")
+    return ids.reshape(-1).contiguous()
+
+
+def embedding_fwd(ids, table, scale=1.0, out_dtype=None):
+    """out[..., :] = scale * table[ids[...], :] for ids (int64 / int32) of any shape, table fp32 / bf16 [V, D]; out in the table's type or
+    out_dtype.  D % 8 == 0; the table's rows may have a stride.  An id outside [0, V) gives a row of NaN."""
+    code, ldt = _rows2d(table, "table")
+    V, D = table.shape
+    flat = _ids1d(ids)
+    out_dtype = table.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _ROW_TYPES:
+        raise _lib.VitkError(f"embedding_fwd: out_dtype must be float32 or bfloat16, got {out_dtype}")
+    out = torch.empty((*ids.shape, D), dtype=out_dtype, device=table.device)
+    check(_lib.load().vitk_embedding_fwd(_ptr(flat), int(flat.dtype == torch.int64), _ptr(table), code, ldt, _ptr(out), _ROW_TYPES[out_dtype], D,
+                                         flat.numel(), V, D, float(scale), _stream()), "embedding_fwd")
+    return out
+
+
+def embedding_bwd(dout, ids, num_rows, scale=1.0, padding_idx=None, out=None, accumulate=False, out_dtype=None):
+    """Gradient of embedding_fwd's table: [num_rows, D] with row v = scale * sum of dout over the tokens with id v (fp32 sums in the order of
+    the tokens, the same bits on every run), zero where there is none; dout fp32 / bf16 [..., D].  Tokens with id padding_idx or an id
+    outside [0, num_rows) add nothing.  out: where it goes (fp32 / bf16 [num_rows, D]); with accumulate it is added there, and only the
+    rows that have tokens are touched.  Without out: a new tensor of out_dtype (default: dout's type)."""
+    if dout.dim() < 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
+        raise _lib.VitkError(f"embedding_bwd: dout must be {tuple(ids.shape)} + (D,), got {tuple(dout.shape)}")
+    D = dout.shape[-1]
+    flat = _ids1d(ids)
+    rows = dout.reshape(flat.numel(), D)
+    if D > 1 and rows.stride(1) != 1:
+        rows = rows.contiguous()
+    dcode, ldd = _rows2d(rows, "dout")
+    if out is None:
+        if accumulate:
+            raise _lib.VitkError("embedding_bwd: accumulate needs out")
+        out = torch.empty((int(num_rows), D), dtype=dout.dtype if out_dtype is None else out_dtype, device=dout.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise _lib.VitkError(f"embedding_bwd: out is {out.dtype}, out_dtype says {out_dtype}")
+    if tuple(out.shape) != (int(num_rows), D):
+        raise _lib.VitkError(f"embedding_bwd: out must be [{num_rows}, {D}], got {tuple(out.shape)}")
+    ocode, ldo = _rows2d(out, "out")
+    lib = _lib.load()
+    ws = torch.empty(lib.vitk_embedding_bwd_workspace(flat.numel(), int(num_rows), D), dtype=torch.uint8, device=out.device)
+    check(lib.vitk_embedding_bwd(_ptr(rows), dcode, ldd, _ptr(flat), int(flat.dtype == torch.int64), _ptr(out), ocode, ldo, flat.numel(), int(num_rows),
+                                 D, float(scale), -1 if padding_idx is None else int(padding_idx), int(bool(accumulate)), _ptr(ws), ws.numel(),
+                                 _stream()), "embedding_bwd")
+    return out
+
+
 _prof_on = False
 
 
