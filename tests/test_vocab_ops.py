@@ -299,12 +299,249 @@ def test_embedding_refuses(device):
             call()
 
 
+# ------------------------------------------------------------------------------------ linear cross entropy
+def plain_linear_xent(x, w, target, bias, smoothing, ignore, mean):
+    """the operator in 64 bits, and how far bf16 / fp32 arithmetic may be off it: (loss, rows, dx, dw, db), (tolerances of the same)"""
+    x, w = x.double(), w.double()
+    V, D = w.shape
+    b = torch.zeros(V, dtype=f64) if bias is None else bias.double()
+    z = x @ w.t() + b
+    counted = target != ignore
+    bad = counted & ((target < 0) | (target >= V))
+    t = torch.where(counted & ~bad, target, torch.zeros_like(target))
+    q = torch.full_like(z, smoothing / V)
+    q[torch.arange(len(t)), t] += 1.0 - smoothing
+    lse = torch.logsumexp(z, 1)
+    smooth = smoothing * (lse - z.mean(1)) if smoothing > 0 else 0.0            # no 0 * inf where a class is masked out
+    rows = (1.0 - smoothing) * (lse - z.gather(1, t[:, None])[:, 0]) + smooth
+    rows[~counted] = 0.0
+    rows[bad] = math.nan
+    n = int(counted.sum())
+    g = (1.0 / n if mean else 1.0) if n else 0.0
+    loss = rows.sum() * g
+    p = (z - lse[:, None]).exp()
+    dz = p - q
+    dz[~counted], p[~counted] = 0.0, 0.0
+    # a logit is an fp32 sum of D products of bf16 factors, plus the bias
+    zerr = ((D + 2) * U32 * (x.abs() @ w.abs().t() + torch.where(b.isinf(), torch.zeros_like(b), b.abs()))).max(1).values
+    # its exponential: relative error of the argument's error and of the exponent's rounding; sums over at most V of them
+    perr = 2 * zerr + (V / 64 + 200) * U32 * (1 + torch.where(lse.isfinite(), lse.abs(), torch.zeros_like(lse)))
+    rtol = perr * (1 + smoothing)
+    # the kept factor is fp16 relative to its piece's maximum, the gradient factor bf16
+    E = p * (2.0 ** -11 + perr[:, None]) * 1.01 + 2.0 ** -24 + dz.abs() * 2.0 ** -8 * 1.01
+    E[~counted] = 0.0
+    dx, dw, db = g * (dz @ w), g * (dz.t() @ x), g * dz.sum(0)
+    dxt = g * (E @ w.abs() + (V + 4) * U32 * (dz.abs() @ w.abs()))
+    dwt = g * (E.t() @ x.abs() + (len(t) + 4) * U32 * (dz.abs().t() @ x.abs()))
+    dbt = g * (E.sum(0) + (len(t) + 4) * U32 * dz.abs().sum(0))
+    lt = rtol[counted].sum() * g + 4 * U32 * abs(loss)
+    return (loss, rows, dx, dw, db), (lt, rtol, dxt, dwt, dbt)
+
+
+def check_linear_xent(r, x, w, target, bias=None, smoothing=0.0, ignore=-100, mean=True, grad=True):
+    want, tol = plain_linear_xent(x, w, target, bias, smoothing, ignore, mean)
+    for name, got, v, t in zip(("loss", "rows", "dx", "dweight", "dbias"), r, want, tol):
+        if not grad and name[0] == "d":
+            assert got is None
+            continue
+        if name == "dbias" and bias is None:
+            assert got is None
+            continue
+        got = got.cpu()
+        extra = half_ulp(got.dtype) * 1.01 * (v.abs() + t) + (2.0 ** -133 if got.dtype == bf16 else 0.0)
+        off = (got.double() - v).abs()
+        bad = ~(off <= t + extra) & ~(got.double() == v)
+        assert not bad.any(), f"{name}: {int(bad.sum())} of {bad.numel()} off, worst {float((off / (t + extra)).nan_to_num(9e9).max()):.3g} of its tolerance"
+
+
+def xent_inputs(T, V, D, g, ignored=0.2, sharp=1.0):
+    w = (torch.randn(V, D, generator=g) * (2.0 / math.sqrt(D))).to(bf16)
+    target = torch.randint(0, V, (T,), generator=g)
+    x = (torch.randn(T, D, generator=g) + sharp * w[target].float()).to(bf16)
+    target[torch.rand(T, generator=g) < ignored] = -100
+    return x, w, target
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D", [(1, 1, 8), (1, 1000, 192), (3, 2, 16), (17, 63, 64), (64, 64, 72), (65, 257, 128), (255, 300, 136), (256, 256, 64), (257, 1023, 200),
+                                   (300, 5000, 64), (700, 700, 384), (40, 33000, 64), (1500, 130, 1032)])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+@pytest.mark.parametrize("btype", [None, bf16, f32])
+def test_linear_xent(device, T, V, D, smoothing, btype):
+    ops = _ops()
+    g = torch.Generator().manual_seed(T * 7 + V + D)
+    x, w, target = xent_inputs(T, V, D, g)
+    bias = None if btype is None else (torch.randn(V, generator=g) * 0.5).to(btype)
+    args = (x.to(device), w.to(device), target.to(device), None if bias is None else bias.to(device))
+    r = ops.linear_xent(*args, smoothing=smoothing)
+    check_linear_xent(r, x, w, target, bias, smoothing)
+    alone = ops.linear_xent(*args, smoothing=smoothing, want_grad=False)
+    assert torch.equal(alone.loss, r.loss) and torch.equal(alone.rows, r.rows) and alone.dx is None
+    again = ops.linear_xent(*args, smoothing=smoothing)
+    assert all(a is None or torch.equal(a, b) for a, b in zip(again, r))
+    s = ops.linear_xent(*args, smoothing=smoothing, reduction="sum", dweight_dtype=f32)
+    assert s.dweight.dtype == f32
+    check_linear_xent(s, x, w, target, bias, smoothing, mean=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wtype", [bf16, f32])
+def test_linear_xent_in_several_blocks_of_rows(device, wtype):
+    ops = _ops()
+    g = torch.Generator().manual_seed(5)
+    x, w, target = xent_inputs(1300, 700, 72, g)
+    bias = torch.randn(700, generator=g)
+    args = (x.to(device), w.to(device), target.to(device), bias.to(device))
+    whole = ops.linear_xent(*args, smoothing=0.1, dweight_dtype=wtype)
+    for block_bytes in (1, 768 * 2 * 600):                  # 256 rows, 512 rows at a time
+        r = ops.linear_xent(*args, smoothing=0.1, dweight_dtype=wtype, block_bytes=block_bytes)
+        check_linear_xent(r, x, w, target, bias, 0.1)
+        assert torch.equal(r.rows, whole.rows) and torch.equal(r.loss, whole.loss)
+        e = ops.linear_xent(*args, smoothing=0.1, want_grad=False, block_bytes=block_bytes)
+        assert torch.equal(e.rows, whole.rows) and torch.equal(e.loss, whole.loss)
+
+
+@pytest.mark.gpu
+def test_linear_xent_strides(device):
+    ops = _ops()
+    g = torch.Generator().manual_seed(6)
+    x, w, target = xent_inputs(100, 300, 64, g)
+    bx, bw = torch.full((100, 96), math.nan, dtype=bf16), torch.full((300, 80), math.nan, dtype=bf16)
+    bx[:, 16:80], bw[:, 8:72] = x, w
+    tg = torch.stack([target, target + 1], 1).to(device)[:, 0]
+    r = ops.linear_xent(bx.to(device)[:, 16:80], bw.to(device)[:, 8:72], tg)
+    check_linear_xent(r, x, w, target)
+    assert all(torch.equal(a, b) for a, b in zip(r, ops.linear_xent(x.to(device), w.to(device), target.to(device))) if a is not None)
+
+
+@pytest.mark.gpu
+def test_linear_xent_rows_that_do_not_count_and_labels_that_are_none(device):
+    ops = _ops()
+    g = torch.Generator().manual_seed(7)
+    x, w, target = xent_inputs(70, 500, 64, g)
+    dev = lambda t: ops.linear_xent(x.to(device), w.to(device), t.to(device), ignore_index=3)          # noqa: E731
+    target[target < 0] = 5
+    target[10:40] = 3
+    check_linear_xent(dev(target), x, w, target, ignore=3)
+    nothing = dev(torch.full_like(target, 3))
+    assert all(torch.all(t == 0) for t in (nothing.loss, nothing.rows, nothing.dx, nothing.dweight))
+    bad = target.clone()
+    bad[0], bad[1] = 500, -7
+    r = dev(bad)
+    ok = torch.ones(70, dtype=torch.bool)
+    ok[:2] = False
+    assert torch.isnan(r.loss) and torch.isnan(r.rows[:2]).all() and torch.isnan(r.dx[:2]).all() and torch.isnan(r.dweight).all()
+    assert torch.equal(r.rows[2:], dev(target).rows[2:]) and torch.isfinite(r.dx[2:]).all() and torch.all(r.dx[10:40] == 0)
+    one = ops.linear_xent(x[:0].to(device), w.to(device), target[:0].to(device))
+    assert one.loss.item() == 0 and one.rows.shape == (0,) and one.dx.shape == (0, 64) and torch.all(one.dweight == 0)
+
+
+@pytest.mark.gpu
+def test_linear_xent_extreme_logits(device):
+    ops = _ops()
+    g = torch.Generator().manual_seed(8)
+    x, w, target = xent_inputs(60, 400, 64, g, ignored=0.0)
+    # classes that a bias masks out: with -inf, with the type's lowest value; whole pieces of 64 columns among them
+    for low in (-math.inf, torch.finfo(f32).min):
+        bias = torch.randn(400, generator=g)
+        bias[64:200] = low
+        t = target.clone()
+        t[(t >= 64) & (t < 200)] = 1
+        r = ops.linear_xent(x.to(device), w.to(device), t.to(device), bias.to(device))
+        check_linear_xent(r, x, w, t, torch.where(bias < -1e30, torch.full_like(bias, -math.inf), bias))
+        assert torch.all(r.dweight[64:200] == 0) and torch.all(r.dbias[64:200] == 0)
+    # logits of thousands: one class has everything
+    big = (x.float() * 40).to(bf16)
+    r = ops.linear_xent(big.to(device), (w.float() * 40).to(bf16).to(device), target.to(device))
+    check_linear_xent(r, big, (w.float() * 40).to(bf16), target)
+    # equal logits everywhere
+    zero = torch.zeros_like(x)
+    r = ops.linear_xent(zero.to(device), w.to(device), target.to(device))
+    check_linear_xent(r, zero, w, target)
+    assert torch.all((r.rows - math.log(400)).abs() < 1e-5)
+    # NaN and infinity in one row stay in that row (and in dweight)
+    y = x.clone()
+    y[3, 5] = math.nan
+    y[4, 5] = math.inf
+    r = ops.linear_xent(y.to(device), w.to(device), target.to(device))
+    assert torch.isnan(r.rows[3:5]).all() and torch.isnan(r.loss) and torch.isnan(r.dx[3:5]).all()
+    keep = [i for i in range(60) if i not in (3, 4)]
+    clean = ops.linear_xent(x.to(device), w.to(device), target.to(device))
+    assert torch.equal(r.rows[keep], clean.rows[keep]) and torch.equal(r.dx[keep], clean.dx[keep])
+
+
+@pytest.mark.gpu
+def test_linear_xent_gradient_against_differences(device):
+    ops = _ops()
+    g = torch.Generator().manual_seed(9)
+    x, w, target = xent_inputs(90, 310, 48, g)
+    bias = torch.randn(310, generator=g)
+    r = ops.linear_xent(x.to(device), w.to(device), target.to(device), bias.to(device), smoothing=0.1, dweight_dtype=f32)
+    _, tol = plain_linear_xent(x, w, target, bias, 0.1, -100, True)
+    loss = lambda a, b, c: plain_linear_xent(a, b, target, c, 0.1, -100, True)[0][0]            # noqa: E731
+    h = 1e-5
+    for k in range(3):
+        args = [x.double(), w.double(), bias.double()]
+        u = torch.randn(args[k].shape, generator=g, dtype=f64)
+        up, down = list(args), list(args)
+        up[k], down[k] = args[k] + h * u, args[k] - h * u
+        slope = (loss(*up) - loss(*down)) / (2 * h)
+        got = r[2 + k].cpu().double()
+        # every element may be off by its own tolerance; the difference quotient of the 64-bit function by 1e-8
+        allow = ((tol[2 + k] + half_ulp(r[2 + k].dtype) * (got.abs() + tol[2 + k])) * u.abs()).sum()
+        assert abs((got * u).sum() - slope) <= allow + 1e-8
+        assert allow < 0.2 * (got * u).abs().sum()                                             # the bound says something
+
+
+@pytest.mark.gpu
+def test_linear_xent_in_a_graph_on_another_stream(device):
+    ops = _ops()
+    g = torch.Generator().manual_seed(10)
+    x, w, target = (t.to(device) for t in xent_inputs(600, 900, 64, g))
+    ops.linear_xent(x, w, target)
+    ops.linear_xent(x[:5], w, target[:5])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, few = ops.linear_xent(x, w, target), ops.linear_xent(x[:5], w, target[:5])
+    side = torch.cuda.Stream()
+    for k in range(3):
+        a, _, c = xent_inputs(600, 900, 64, g)
+        x.copy_(a), target.copy_(c)
+        if k == 2:
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                graph.replay()
+            torch.cuda.current_stream().wait_stream(side)
+        else:
+            graph.replay()
+        want, want_few = ops.linear_xent(x, w, target), ops.linear_xent(x[:5], w, target[:5])
+        torch.cuda.synchronize()
+        assert all(u is None or torch.equal(u, v) for u, v in zip((*got, *few), (*want, *want_few)))
+
+
+@pytest.mark.gpu
+def test_linear_xent_refuses(device):
+    ops, err = _ops(), _error()
+    x, w, t = torch.randn(6, 16, device=device).to(bf16), torch.randn(9, 16, device=device).to(bf16), torch.zeros(6, dtype=torch.int64, device=device)
+    b = torch.zeros(9, device=device)
+    for call in (lambda: ops.linear_xent(x.float(), w, t), lambda: ops.linear_xent(x, w.half(), t), lambda: ops.linear_xent(x, w, t.int()),
+                 lambda: ops.linear_xent(x, w, t[:5]), lambda: ops.linear_xent(x, w[:, :8], t), lambda: ops.linear_xent(x[:, :12], w[:, :12], t),
+                 lambda: ops.linear_xent(x, w, t, b[:8]), lambda: ops.linear_xent(x, w, t, b.half()), lambda: ops.linear_xent(x, w, t.cpu()),
+                 lambda: ops.linear_xent(x, w, t, smoothing=1.5), lambda: ops.linear_xent(x, w, t, smoothing=math.nan),
+                 lambda: ops.linear_xent(x, w, t, reduction="none"), lambda: ops.linear_xent(x, w, t, dweight_dtype=f16),
+                 lambda: ops.linear_xent(x[:, ::2], w[:, ::2], t), lambda: ops.linear_xent(x[:, 1:9], w[:, 1:9], t), lambda: ops.linear_xent(x, w[:0], t)):
+        with pytest.raises(err):
+            call()
+
+
 # --------------------------------------------------------------------------------------- checks without a GPU
 def test_cpu_tensors_are_refused():
     ops, err = _ops(), _error()
     x = torch.zeros(4, 16)
     ids = torch.zeros(4, dtype=torch.int64)
-    for call in (lambda: ops.clip_grads([x], 1.0), lambda: ops.embedding_fwd(ids, x), lambda: ops.embedding_bwd(x, ids, 4)):
+    for call in (lambda: ops.clip_grads([x], 1.0), lambda: ops.embedding_fwd(ids, x), lambda: ops.embedding_bwd(x, ids, 4),
+                 lambda: ops.linear_xent(x.to(bf16), x.to(bf16), ids)):
         with pytest.raises(err, match="GPU"):
             call()
 
@@ -334,3 +571,22 @@ def test_entry_points_check_before_they_launch():
     assert lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 24, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22
     assert lib.vitk_embedding_bwd(p, 0, 8, p, 1, p, 0, 16, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22
     assert lib.vitk_embedding_bwd(None, 0, 16, p, 1, p, 0, 16, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22
+    need = lib.vitk_linear_xent_workspace(4, 4, 16, 1, 0, 0, 0, 1 << 20)
+
+    def xent(x=p, ldx=16, w=p, V=4, D=16, eps=0.0, dx=p, dw=p, db=None, nbytes=need, T=4, ld=16):
+        return lib.vitk_linear_xent(x, ldx, w, 16, None, 0, p, T, V, D, eps, -100, 1, p, p, dx, ld, dw, ld, 0, db, 0, p, nbytes, 1 << 20, None)
+    assert need > 0 and lib.vitk_linear_xent_workspace(0, 4, 16, 1, 0, 0, 0, 1 << 20) == 0
+    assert xent(nbytes=need - 1) == -28
+    for kw in ({"x": None}, {"ldx": 12}, {"D": 12}, {"V": 0}, {"V": 1 << 23}, {"eps": -0.1}, {"eps": 1.1}, {"dx": None}, {"db": p}, {"x": p + 8}, {"T": 0}, {"ld": 8}):
+        assert xent(**kw) == -22, kw
+
+
+def test_linear_xent_workspace_stays_within_its_blocks():
+    from tests.test_abi_and_host import _lib
+    size = _lib().load().vitk_linear_xent_workspace
+    budget = 1 << 30
+    for T, V, D in ((8192, 100003, 2048), (1 << 20, 100003, 64), (100352, 8192, 768), (1, 4000000, 8), (300, 1 << 22, 64)):
+        n = size(T, V, D, 1, 1, 0, 0, budget)
+        rows256 = 256 * ((V + 255) // 256 * 256) * 2.25
+        other = 4 * V * D + 8 * 256 * 256 * max(1, D // 256) * 256                 # the fp32 sum of dw, the partial sums of dx
+        assert n <= max(budget, rows256) + other + (1 << 20), (T, V, D, n)

@@ -80,6 +80,8 @@ SIGNATURES = {
     "vitk_xent_label_fwd_bwd": (_i, [_p, _i, _p, _f, _p, _p, _i, _f, _i, _i, _p]),
     "vitk_xent_soft_fwd_bwd": (_i, [_p, _i, _p, _i, _p, _p, _i, _f, _i, _i, _p]),
     "vitk_kd_kl_fwd_bwd": (_i, [_p, _i, _p, _i, _f, _p, _p, _i, _f, _i, _i, _p]),
+    "vitk_linear_xent_workspace": (_sz, [_i64, _i, _i, _i, _i, _i, _i, _sz]),
+    "vitk_linear_xent": (_i, [_p, _i64, _p, _i64, _p, _i, _p, _i64, _i, _i, _f, _i64, _i, _p, _p, _p, _i64, _p, _i64, _i, _p, _i, _p, _sz, _sz, _p]),
     "vitk_argmax_rows": (_i, [_p, _i, _p, _i, _i, _p]),
     "vitk_adamw_step": (_i, [_p, _p, _p, _p, _p, _p, _d, _i64, _d, _d, _d, _d, _d, _i, _f, _p]),
     "vitk_ema_update": (_i, [_p, _p, _d, _i64, _p]),

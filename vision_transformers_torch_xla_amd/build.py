@@ -14,7 +14,7 @@ from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent / "csrc"
 LIB_PATH = CSRC / "libvitk.so"
-SOURCES = ["api.hip", "layernorm.hip", "gemm.hip", "gemm_ntq.hip", "attention.hip", "elementwise.hip", "loss.hip", "optim.hip", "clip.hip", "embedding.hip", "preprocess.hip"]
+SOURCES = ["api.hip", "layernorm.hip", "gemm.hip", "gemm_ntq.hip", "attention.hip", "elementwise.hip", "loss.hip", "linear_xent.hip", "optim.hip", "clip.hip", "embedding.hip", "preprocess.hip"]
 HEADERS = [CSRC / "common.h", CSRC / "gemm_nt.h", CSRC.parent.parent / "include" / "vitk.h"]
 ARCH = "gfx950"
 FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function", "-Wno-inline-asm", "-Wno-cuda-compat", "-Wno-pass-failed",

@@ -6,6 +6,8 @@ device/dtype/contiguity, then hands raw device pointers, shapes and ``torch.cuda
 """
 from __future__ import annotations
 
+from typing import NamedTuple, Optional
+
 import numpy as np
 import torch
 
@@ -623,6 +625,75 @@ def embedding_bwd(dout, ids, num_rows, scale=1.0, padding_idx=None, out=None, ac
                                  D, float(scale), -1 if padding_idx is None else int(padding_idx), int(bool(accumulate)), _ptr(ws), ws.numel(),
                                  _stream()), "embedding_bwd")
     return out
+
+
+class LinearXent(NamedTuple):
+    """what linear_xent returns; the gradients are None where they were not asked for"""
+    loss: torch.Tensor
+    rows: torch.Tensor
+    dx: Optional[torch.Tensor] = None
+    dweight: Optional[torch.Tensor] = None
+    dbias: Optional[torch.Tensor] = None
+
+
+LINEAR_XENT_BLOCK = 2 << 30          # bytes of probabilities that linear_xent holds at a time by default
+
+
+def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, reduction="mean", want_grad=True, dweight_dtype=None,
+                block_bytes=LINEAR_XENT_BLOCK):
+    """Cross entropy of the logits x @ weight.T + bias against int64 targets, with the gradients of the reduced loss, without the logits in
+    memory: x bf16 [T, D], weight bf16 [V, D] (rows may have a stride), bias fp32 / bf16 [V], target [T].  D % 8 == 0, V <= 2^22.
+
+    rows[i] = (1 - smoothing) * nll + smoothing * mean_j(-logp_ij), 0 where target == ignore_index; loss = their mean over the counted
+    rows, or their sum (reduction 'sum'); 0 with zero gradients where no row counts.  Any other target outside [0, V) gives NaN.
+    want_grad: dx bf16 [T, D], dweight [V, D] in dweight_dtype (bf16, the default, or float32), dbias in the bias's type.
+    block_bytes: the rows are worked through in blocks that hold about this many bytes of probabilities (at least 256 rows); more than
+    one block costs an fp32 copy of a bf16 dweight."""
+    for t, n in ((x, "x"), (weight, "weight")):
+        _here(t, n)
+        if t.dtype != bf16 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+            raise _lib.VitkError(f"linear_xent: {n} must be a bf16 matrix with contiguous rows, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+    T, D = x.shape
+    V = weight.shape[0]
+    if weight.shape[1] != D:
+        raise _lib.VitkError(f"linear_xent: x has {D} columns, weight {weight.shape[1]}")
+    _here(target, "target")
+    if target.dtype != torch.int64 or tuple(target.shape) != (T,):
+        raise _lib.VitkError(f"linear_xent: target must be int64 [{T}], got {target.dtype} {tuple(target.shape)}")
+    if reduction not in ("mean", "sum"):
+        raise _lib.VitkError(f"linear_xent: reduction must be 'mean' or 'sum' (rows are returned beside either), got {reduction!r}")
+    btype = 0
+    if bias is not None:
+        _here(bias, "bias")
+        if bias.dtype not in _ROW_TYPES or tuple(bias.shape) != (V,):
+            raise _lib.VitkError(f"linear_xent: bias must be float32 or bfloat16 [{V}], got {bias.dtype} {tuple(bias.shape)}")
+        bias = bias.contiguous()
+        btype = _ROW_TYPES[bias.dtype]
+    wtype = bf16 if dweight_dtype is None else dweight_dtype
+    if wtype not in _ROW_TYPES:
+        raise _lib.VitkError(f"linear_xent: dweight_dtype must be bfloat16 or float32, got {wtype}")
+    target = target.contiguous()
+    dev = x.device
+    rows = torch.empty(T, dtype=f32, device=dev)
+    loss = torch.empty((), dtype=f32, device=dev)
+    dx = dw = db = None
+    if want_grad:
+        dx = torch.empty((T, D), dtype=bf16, device=dev)
+        dw = torch.empty((V, D), dtype=wtype, device=dev)
+        db = torch.empty(V, dtype=bias.dtype, device=dev) if bias is not None else None
+    if T == 0 and V > 0:
+        for t in (loss, dw, db):
+            if t is not None:
+                t.zero_()
+        return LinearXent(loss, rows, dx, dw, db)
+    lib = _lib.load()
+    wf32, smooth = int(wtype == f32), float(smoothing)
+    need = lib.vitk_linear_xent_workspace(T, V, D, int(want_grad), int(smooth > 0), wf32, int(db is not None), int(block_bytes))
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    check(lib.vitk_linear_xent(_ptr(x), x.stride(0) if T > 1 else max(D, 1), _ptr(weight), weight.stride(0) if V > 1 else max(D, 1), _ptr(bias), btype, _ptr(target),
+                               T, V, D, smooth, int(ignore_index), int(reduction == "mean"), _ptr(loss), _ptr(rows), _ptr(dx), D, _ptr(dw), D, wf32,
+                               _ptr(db), int(db is not None and db.dtype == f32), _ptr(ws), ws.numel(), int(block_bytes), _stream()), "linear_xent")
+    return LinearXent(loss, rows, dx, dw, db)
 
 
 _prof_on = False
