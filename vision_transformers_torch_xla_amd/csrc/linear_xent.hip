@@ -24,19 +24,22 @@
 #define LX_STAT 64                                            // columns per entry of the statistics table
 
 enum { LX_NT = 0, LX_NN = 1, LX_TN = 2 };
-enum { LX_OUT = 0, LX_XENT = 1 };
+enum { LX_OUT = 0, LX_XENT = 1, LX_XENT_BIAS = 2 };       // LX_XENT_BIAS: with a bias or the sums of the logits
 
 // 512 bytes of zeros (never written): what rows and columns behind the contraction's end are read from
 __device__ __attribute__((aligned(512))) unsigned lx_zero_row[128];
 
 struct LxGemmParams {
     const bf16_t* A; const bf16_t* B;       // NT: A [M][KA], B [N][KB];  NN: B [KB][N];  TN: A [KA][M], B [KB][N]
-    long long lda, ldb;
+    int lda, ldb;
     int M, N;
     int KA, KB;             // valid extent of the contraction in each operand; behind it zeros are read
     int steps;              // 64-deep steps over the whole contraction
-    int tiles_m, tiles_n, band, splits;
-    // LX_OUT: out[m][n] = scale[0] * acc (+ add[m][n]), bf16 or fp32; or slab[split][m][n] = acc
+    int tiles_m, tiles_n, band;
+    // work: workgroup g of G takes the whole tiles g, g + G, ... below `whole`; the `rest` tiles behind them are one sequence of rest * steps
+    // steps cut into G equal ranges (LX_OUT only), whose parts of tiles go to slab[2 range + part][256][256] as fp32 sums
+    int whole, rest;
+    // LX_OUT: out[m][n] = scale[0] * acc (+ add[m][n]), bf16 or fp32
     const float* scale;
     const float* add;
     void* out; long long ldo; int out_f32;
@@ -68,6 +71,13 @@ static __device__ __forceinline__ unsigned lx_pack_h(float a, float b) {
 // swapped, so a lane holds four consecutive columns of one output row.  Tiles are dealt by number (no counters: a captured graph may be
 // replayed on any stream); a tile order in bands of 8 column tiles keeps what the 32 workgroups of an XCD read at a time to 4 row panels
 // and 8 column panels.
+// range g of G of `total` steps: total / G each, the first total % G one more
+static __host__ __device__ __forceinline__ void lx_range(int g, int total, int G, int& from, int& to) {
+    const int q = total / G, r = total - q * G;
+    from = g * q + (g < r ? g : r);
+    to = from + q + (g < r ? 1 : 0);
+}
+
 template <int LAY, int EPI>
 __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
     constexpr bool AT = LAY == LX_TN, BT = LAY != LX_NT;        // operand stored with the contraction as its slow dimension
@@ -81,21 +91,46 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
     const unsigned lds_base = __builtin_amdgcn_readfirstlane(lds_addr(lsm));
     const unsigned lds_stage = (unsigned)(wave * 4 * 1024);
 
-    const int tiles = p.tiles_m * p.tiles_n, items = tiles * p.splits, G = gridDim.x;
+    const int G = gridDim.x;
+    // this workgroup's items: whole tiles, then at most two parts of tiles (its range of the rest is no longer than a tile)
+    const int whole_items = (int)blockIdx.x < p.whole ? (p.whole - 1 - (int)blockIdx.x) / G + 1 : 0;
+    int r0 = 0, r1 = 0, range = 0, rt = 0, parts = 0;
+    if constexpr (EPI == LX_OUT) {
+        if (p.rest > 0) {
+            range = __builtin_amdgcn_readfirstlane(xcd_remap(blockIdx.x, G));       // neighbouring ranges on one XCD
+            lx_range(range, p.rest * p.steps, G, r0, r1);
+            r0 = __builtin_amdgcn_readfirstlane(r0);
+            r1 = __builtin_amdgcn_readfirstlane(r1);
+            rt = __builtin_amdgcn_readfirstlane(r0 / p.steps);        // tile (of the rest) of the first part
+            parts = r1 <= r0 ? 0 : r1 > (rt + 1) * p.steps ? 2 : 1;
+        }
+    }
+    const int items = whole_items + parts;
 
-    // ---- staging: where the next step's operands come from
-    // [256][64] image: wave w, piece j: rows (4 w + j) * 8 + lane / 8; LDS position lane % 8 receives chunk (lane % 8) ^ (row & 7)
-    // [64][256] image: wave w, piece j: rows (4 w + j) * 2 + lane / 32; LDS position lane % 32 receives chunk (lane % 32) ^ lx_swz(row)
-    const int srow = lane >> 3, sch = (lane & 7) ^ srow;
-    const int shalf = lane >> 5, spos = lane & 31;
-    int sv = blockIdx.x, sk = 0, sk_end = 0;
+    // ---- staging: where the next step's operands come from.  A is staged in two halves, the rows that are the first 64 of a wave's 128
+    // (half 0) and the others, because the two are read at different times.  A piece is one instruction of one wave, 1 KB of LDS.
+    // K-contiguous: image [256][64]; a piece is 8 rows, LDS position lane % 8 receives chunk (lane % 8) ^ (row & 7)
+    // A, K-strided: image [2 halves][64][128]; a piece is 4 rows, position lane % 16 receives chunk (lane % 16) ^ lx_swz(row)
+    // B, K-strided: image [64][256]; a piece is 2 rows, position lane % 32 receives chunk (lane % 32) ^ lx_swz(row)
+    int sv = 0, sk = 0, sk_end = 0;
     const bf16_t* sA = p.A;
     const bf16_t* sB = p.B;
     unsigned voA[4], voB[4];
-    auto locate = [&](int v, int& split, int& m0, int& n0) {
-        const int id = xcd_remap(v, items);
-        split = id / tiles;
-        const int tile = id - split * tiles;
+    // item v: where its tile is, its steps k0 .. k1 - 1, and which part it is (-1: a whole tile)
+    auto locate = [&](int v, int& m0, int& n0, int& k0, int& k1, int& part) {
+        int tile;
+        k0 = 0;
+        k1 = p.steps;
+        if (EPI != LX_OUT || v < whole_items) {
+            part = -1;
+            tile = xcd_remap(blockIdx.x + v * G, p.whole);
+        } else {
+            part = v - whole_items;
+            tile = p.whole + rt + part;
+            if (part == 0) k0 = r0 - rt * p.steps;
+            const int left = r1 - (rt + part) * p.steps;
+            k1 = left < p.steps ? left : p.steps;
+        }
         const int full = p.tiles_m * p.band;
         const int blk = tile / full;
         const int rem = tile - blk * full;
@@ -103,29 +138,31 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
         const int width = p.tiles_n - c0 < p.band ? p.tiles_n - c0 : p.band;
         const int tm = rem / width;
         // the divisions run on the vector unit: say that their results are the same in every lane
-        split = __builtin_amdgcn_readfirstlane(split);
         m0 = __builtin_amdgcn_readfirstlane(tm * LX_TILE);
         n0 = __builtin_amdgcn_readfirstlane((c0 + rem - tm * width) * LX_TILE);
     };
-    // split s of S takes steps [s * steps / S, (s + 1) * steps / S): q = steps / S each, the first steps % S one more
-    const int sq = __builtin_amdgcn_readfirstlane(p.steps / p.splits), sr = p.steps - sq * p.splits;
-    auto first_step = [&](int split) { return split * sq + (split < sr ? split : sr); };
     auto aim = [&](int v) {
-        int split, m0, n0;
-        locate(v, split, m0, n0);
-        sk = first_step(split);
-        sk_end = first_step(split + 1);
+        int m0, n0, part;
+        locate(v, m0, n0, sk, sk_end, part);
         sA = p.A + (AT ? (size_t)m0 : (size_t)m0 * p.lda);
         sB = p.B + (BT ? (size_t)n0 : (size_t)n0 * p.ldb);
         // rows and columns behind the edge of the output read the last valid ones: their results are not stored
         const int ma = p.M - 1 - m0, mb = p.N - 1 - n0;
+        // the lane number passes through an empty asm, so that what is derived from it here is not kept in registers over the main loop
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int srow = ln >> 3, sch = (ln & 7) ^ srow;
+        const int shalf = ln >> 5, spos = ln & 31;
+        const int arow = ln >> 4, apos = ln & 15;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (AT) {
-                const int r = (wave * 4 + j) * 2 + shalf;
-                voA[j] = (unsigned)((r * p.lda + (spos ^ lx_swz(r)) * 8) * 2);      // A's rows are padded to a multiple of 256
+                const int r = (wave * 2 + (j & 1)) * 4 + arow;
+                const int c = apos ^ lx_swz(r);
+                voA[j] = (unsigned)((r * p.lda + (c >> 3) * 128 + (j >> 1) * 64 + (c & 7) * 8) * 2);      // A's rows are padded to a multiple of 256
             } else {
-                const int r = (wave * 4 + j) * 8 + srow;
+                const int b = wave * 2 + (j & 1);
+                const int r = (b >> 3) * 128 + (j >> 1) * 64 + (b & 7) * 8 + srow;
                 voA[j] = (unsigned)(((r < ma ? r : ma) * p.lda + sch * 8) * 2);
             }
             if (BT) {
@@ -138,26 +175,45 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
             }
         }
     };
-    // one operand's 64-deep step kstep -> LDS; what lies behind the contraction's end K comes from the zero row
-    auto stage = [&](const bf16_t* base, const unsigned (&vo)[4], bool slow, long long ld, int K, int kstep, unsigned dst) {
-        const bf16_t* src = base + (slow ? (size_t)kstep * LX_BK * ld : (size_t)kstep * LX_BK);
-        if ((kstep + 1) * LX_BK <= K) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) glds16(src, vo[j], dst + j * 1024);
+    // what lies behind the contraction's end comes from the zero row (the lane number passes through an empty asm as in aim)
+    auto stageA = [&](int par, int half) {
+        const bf16_t* src = sA + (AT ? (size_t)sk * LX_BK * p.lda : (size_t)sk * LX_BK);
+        const unsigned dst = lds_base + (unsigned)(par * 2 * LX_ELEMS * 2) +
+                             (AT ? half * 16384 + wave * 2048 : (wave >> 2) * 16384 + half * 8192 + (wave & 3) * 2048);
+        if ((sk + 1) * LX_BK <= p.KA) {
+            glds16(src, voA[2 * half], dst);
+            glds16(src, voA[2 * half + 1], dst + 1024);
         } else {
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            const void* zrow = (const char*)lx_zero_row + (ln & 31) * 16;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int k = kstep * LX_BK + (slow ? (wave * 4 + j) * 2 + shalf : sch * 8);
-                const void* z = (const char*)lx_zero_row + (lane & 31) * 16;
-                glds16_v(k < K ? (const void*)((const char*)src + vo[j]) : z, dst + j * 1024);
+            for (int j = 0; j < 2; ++j) {
+                const int k = sk * LX_BK + (AT ? (wave * 2 + j) * 4 + (ln >> 4) : ((ln & 7) ^ (ln >> 3)) * 8);
+                glds16_v(k < p.KA ? (const void*)((const char*)src + voA[2 * half + j]) : zrow, dst + j * 1024);
             }
         }
     };
-    auto stageA = [&](int par) { stage(sA, voA, AT, p.lda, p.KA, sk, lds_base + (unsigned)(par * 2 * LX_ELEMS * 2) + lds_stage); };
-    auto stageB = [&](int par) { stage(sB, voB, BT, p.ldb, p.KB, sk, lds_base + (unsigned)((par * 2 + 1) * LX_ELEMS * 2) + lds_stage); };
+    auto stageB = [&](int par) {
+        const bf16_t* src = sB + (BT ? (size_t)sk * LX_BK * p.ldb : (size_t)sk * LX_BK);
+        const unsigned dst = lds_base + (unsigned)((par * 2 + 1) * LX_ELEMS * 2) + lds_stage;
+        if ((sk + 1) * LX_BK <= p.KB) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) glds16(src, voB[j], dst + j * 1024);
+        } else {
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            const void* zrow = (const char*)lx_zero_row + (ln & 31) * 16;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = sk * LX_BK + (BT ? (wave * 4 + j) * 2 + (ln >> 5) : ((ln & 7) ^ (ln >> 3)) * 8);
+                glds16_v(k < p.KB ? (const void*)((const char*)src + voB[j]) : zrow, dst + j * 1024);
+            }
+        }
+    };
     auto advance = [&]() {
         if (++sk == sk_end) {
-            sv += G;
+            ++sv;
             if (sv < items) aim(sv);
         }
     };
@@ -173,9 +229,9 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
     }
     if (AT || BT) {
         const int sw = lx_swz(8 * lg + lq);
-        preA = ((wm * 16) | (lp >> 1)) ^ sw;
+        preA = ((wm * 8) | (lp >> 1)) ^ sw;
         preB = ((wn * 8) | (lp >> 1)) ^ sw;
-        rbase = (8 * lg + lq) * 256 + (lp & 1) * 4;
+        rbase = 8 * lg + lq;
     }
     f32x4 acc[8][4];
     bf16x8 faE[4], faO[4], fbE[4], fbO[4];
@@ -183,8 +239,8 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             if (AT) {
-                const bf16_t* q = cA + ks * 32 * 256 + rbase + ((preA ^ (2 * (4 * h + t))) << 3);
-                f[t] = lx_tr(q, q + 4 * 256);
+                const bf16_t* q = cA + h * 8192 + (ks * 32 + rbase) * 128 + (lp & 1) * 4 + ((preA ^ (2 * t)) << 3);
+                f[t] = lx_tr(q, q + 4 * 128);
             } else {
                 f[t] = *reinterpret_cast<const bf16x8*>(cA + offA[ks] + (4 * h + t) * 16 * LX_BK);
             }
@@ -194,7 +250,7 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             if (BT) {
-                const bf16_t* q = cB + ks * 32 * 256 + rbase + ((preB ^ (2 * t)) << 3);
+                const bf16_t* q = cB + (ks * 32 + rbase) * 256 + (lp & 1) * 4 + ((preB ^ (2 * t)) << 3);
                 f[t] = lx_tr(q, q + 4 * 256);
             } else {
                 f[t] = *reinterpret_cast<const bf16x8*>(cB + offB[ks] + t * 16 * LX_BK);
@@ -216,26 +272,46 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                            \
     }                                                                                 \
     __builtin_amdgcn_sched_barrier(0)
+#define LX_WAIT(n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n) : "memory")
+#define LX_BARRIER()                       \
+    __builtin_amdgcn_s_barrier();          \
+    asm volatile("" ::: "memory")
 
-    if (sv >= items) return;
-    int v = sv;
-    aim(sv);
-    stageA(0);
-    stageB(0);
+    // The steps of all items of a workgroup form one stream, requested two steps ahead into the buffer of the current one.  A step is four
+    // phases: (A half 0, k 0..31), (half 0, k 32..63), (half 1, k 0..31), (half 1, k 32..63), fragments read one phase ahead, so that B
+    // and half 0 of the buffer have been read after the first phase and half 1 after the third.  Two schedules:
+    //   DEEP (dz W): barriers X behind the first and Y behind the third phase.  Behind X the requests for B and half 0 of step s + 2 go
+    //     out, behind Y those for half 1.  Y publishes B and half 0 of step s + 1, X half 1 of step s: a request has 1.25 to 1.5 steps to
+    //     arrive.  vmcnt counts in issue order (4 for B, 2 for a half): at X what is younger than half 1 of s are the 8 requests of s + 1,
+    //     at Y half 1 of s + 1 and the 6 of s + 2.
+    //   else: one barrier, Y.  Behind it the requests for A of step s + 2 go out, a phase later those for B; they have 0.75 to 1 step.
+    // The second barrier costs a step 8 % where the operands come out of the caches (x W^T, dz^T x: 2625 -> 2840 us and 2610 -> 2830
+    // us at 8192 x 100003 x 2048); dz W streams dz from memory along its long contraction and gains 9 % (2755 -> 2500 us).
+    // The output stores of a full tile (16 of a wave at least) between two steps may stay in flight over the first step's waits.
+    constexpr bool DEEP = LAY == LX_NN;
+    if (items == 0) return;
+    aim(0);
+    stageB(0); stageA(0, 0); stageA(0, 1);
     advance();
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (sv < items) { stageA(1); stageB(1); advance(); }
+    bool n1 = sv < items;       // step s + 1 is on its way
+    if (n1) {
+        stageB(1); stageA(1, 0); stageA(1, 1);
+        advance();
+        LX_WAIT(8);
+    } else {
+        LX_WAIT(0);
+    }
+    LX_BARRIER();
     ldB(fbE, lsm + LX_ELEMS, 0);
     ldA(faE, lsm, 0, 0);
     int par = 0;
-    bool pend = false;          // the A half of a step is on its way into buffer par ^ 1, the B half is not yet requested
+    bool loose = false;         // at least 16 output stores of this wave are younger than its requests
+    bool pend = false;          // not DEEP: A of a step is on its way into the other buffer, B is not yet requested
 
-    for (; v < items; v += G) {
-        int split, m0, n0;
-        locate(v, split, m0, n0);
-        const int nk = first_step(split + 1) - first_step(split);
+    for (int v = 0; v < items; ++v) {
+        int m0, n0, k0, k1, part;
+        locate(v, m0, n0, k0, k1, part);
+        const int nk = k1 - k0;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -245,30 +321,58 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
             const bf16_t* cB = cA + LX_ELEMS;
             const bf16_t* nA = lsm + (par ^ 1) * 2 * LX_ELEMS;
             const bf16_t* nB = nA + LX_ELEMS;
-            if (pend) { stageB(par ^ 1); advance(); pend = false; }
-            mma(faE, fbE, 0);
-            ldA(faO, cA, 0, 1);
-            LX_MIX(RA);
-            mma(faO, fbE, 1);
-            ldB(fbO, cB, 1);
-            ldA(faE, cA, 1, 0);
-            LX_MIX(RAB);
-            mma(faE, fbO, 0);
-            ldA(faO, cA, 1, 1);
-            LX_MIX(RA);
-            // every wave has read the current buffer; the next step has landed: publish it, refill the current buffer
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            if (sv < items) { stageA(par); pend = true; }
-            mma(faO, fbO, 1);
+            if constexpr (DEEP) {
+                const bool n2 = sv < items;
+                mma(faE, fbE, 0);
+                ldB(fbO, cB, 1);
+                ldA(faO, cA, 1, 0);
+                LX_MIX(RAB);
+                if (!n1) LX_WAIT(0);
+                else if (loose) LX_WAIT(24);
+                else LX_WAIT(8);
+                LX_BARRIER();
+                if (n2) stageB(par);
+                mma(faO, fbO, 0);
+                ldA(faE, cA, 0, 1);
+                LX_MIX(RA);
+                if (n2) stageA(par, 0);
+                mma(faE, fbE, 1);
+                ldA(faO, cA, 1, 1);
+                LX_MIX(RA);
+                if (!n2) LX_WAIT(0);
+                else if (loose) LX_WAIT(24);
+                else LX_WAIT(8);
+                LX_BARRIER();
+                if (n2) { stageA(par, 1); advance(); }
+                mma(faO, fbO, 1);
+                n1 = n2;
+            } else {
+                if (pend) { stageB(par ^ 1); advance(); pend = false; }
+                mma(faE, fbE, 0);
+                ldA(faO, cA, 0, 1);
+                LX_MIX(RA);
+                mma(faO, fbE, 1);
+                ldB(fbO, cB, 1);
+                ldA(faE, cA, 1, 0);
+                LX_MIX(RAB);
+                mma(faE, fbO, 0);
+                ldA(faO, cA, 1, 1);
+                LX_MIX(RA);
+                if (loose) LX_WAIT(16);
+                else LX_WAIT(0);
+                LX_BARRIER();
+                if (sv < items) { stageA(par, 0); stageA(par, 1); pend = true; }
+                mma(faO, fbO, 1);
+            }
             ldB(fbE, nB, 0);
             ldA(faE, nA, 0, 0);
             LX_MIX(RAB);
+            loose = false;
             par ^= 1;
         }
-        if (pend) { stageB(par ^ 1); advance(); pend = false; }
+        if (pend) { stageB(par ^ 1); advance(); pend = false; }      // before the stores: vmcnt counts in issue order
 
+        const int srow = lane >> 3;
         if constexpr (EPI == LX_OUT) {
             // accumulators -> rows of 64 columns through the wave's 4 KB of LDS, so that a store covers whole lines
             float* stg = reinterpret_cast<float*>(lsm + 4 * LX_ELEMS) + wave * (16 * 64);
@@ -286,8 +390,8 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
                     f32x4 hi = *reinterpret_cast<const f32x4*>(stg + r * 64 + (((2 * (lane & 7) + 1) ^ srow) << 2));
                     const int m = m0 + wm * 128 + tm * 16 + r;
                     if (m < p.M && n < p.N) {
-                        if (p.slab != nullptr) {
-                            float* q = p.slab + ((size_t)split * p.M + m) * p.N + n;
+                        if (part >= 0) {
+                            float* q = p.slab + (size_t)(2 * range + part) * 65536 + (m - m0) * 256 + (n - n0);
                             __builtin_nontemporal_store(lo, reinterpret_cast<f32x4*>(q));
                             __builtin_nontemporal_store(hi, reinterpret_cast<f32x4*>(q + 4));
                         } else {
@@ -312,19 +416,30 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
             }
         } else {
             bf16_t* stg = reinterpret_cast<bf16_t*>(reinterpret_cast<float*>(lsm + 4 * LX_ELEMS) + wave * (16 * 64));
-            // bias of the lane's 16 columns; columns behind the vocabulary count as logits of -inf
-            float bias[4][4];
-            bool in[4][4];
+            const int first = n0 + wn * 64 + 4 * lg;         // the lane's columns are first + 16 tn + j
+            const int room = p.N - first;                    // those with 16 tn + j < room are columns of the vocabulary
+            if constexpr (EPI == LX_XENT_BIAS) {
+                if (p.bias != nullptr) {
 #pragma unroll
-            for (int tn = 0; tn < 4; ++tn)
+                    for (int tn = 0; tn < 4; ++tn) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int n = n0 + wn * 64 + tn * 16 + 4 * lg + j;
-                    in[tn][j] = n < p.N;
-                    const int nc = in[tn][j] ? n : p.N - 1;
-                    bias[tn][j] = 0.f;
-                    if (p.bias != nullptr) bias[tn][j] = p.bias_type == 1 ? bf2f(reinterpret_cast<const bf16_t*>(p.bias)[nc]) : reinterpret_cast<const float*>(p.bias)[nc];
+                        for (int j = 0; j < 4; ++j) {
+                            const int n = first + tn * 16 + j < p.N ? first + tn * 16 + j : p.N - 1;
+                            const float u = p.bias_type == 1 ? bf2f(reinterpret_cast<const bf16_t*>(p.bias)[n]) : reinterpret_cast<const float*>(p.bias)[n];
+#pragma unroll
+                            for (int tm = 0; tm < 8; ++tm) acc[tm][tn][j] += u;
+                        }
+                    }
                 }
+            }
+            if (n0 + LX_TILE > p.N) {           // columns behind the vocabulary count as logits of -inf
+#pragma unroll
+                for (int tm = 0; tm < 8; ++tm)
+#pragma unroll
+                    for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[tm][tn][j] = tn * 16 + j < room ? acc[tm][tn][j] : -INFINITY;
+            }
             const int sc = (n0 >> 6) + wn;
 #pragma unroll
             for (int tm = 0; tm < 8; ++tm) {
@@ -334,10 +449,9 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
                 for (int tn = 0; tn < 4; ++tn)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float u = acc[tm][tn][j] + bias[tn][j];
-                        zs += in[tn][j] ? u : 0.f;
-                        z[tn][j] = in[tn][j] ? u : -INFINITY;
+                        z[tn][j] = acc[tm][tn][j];
                         mx = fmaxf(mx, z[tn][j]);
+                        if constexpr (EPI == LX_XENT_BIAS) zs += tn * 16 + j < room ? z[tn][j] : 0.f;
                     }
                 mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -353,7 +467,7 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
                 s += __shfl_xor(s, 16, 64);
                 s += __shfl_xor(s, 32, 64);
                 if (lg == 0 && m < p.M) p.stats[(size_t)m * p.stat_cols + sc] = make_float2(mx, s);
-                if (p.zsum != nullptr) {
+                if (EPI == LX_XENT_BIAS && p.zsum != nullptr) {
                     zs += __shfl_xor(zs, 16, 64);
                     zs += __shfl_xor(zs, 32, 64);
                     if (lg == 0 && m < p.M) p.zsum[(size_t)m * p.stat_cols + sc] = zs;
@@ -377,6 +491,7 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
                 }
             }
         }
+        loose = m0 + LX_TILE <= p.M && (EPI != LX_OUT ? p.P != nullptr : n0 + LX_TILE <= p.N);       // a full tile: 16 stores at least
     }
 }
 
@@ -510,27 +625,52 @@ __global__ __launch_bounds__(1024) void lx_loss_kernel(const long long* __restri
     }
 }
 
-// out = scale * sum over the splits of slab[s] (+ add), fixed order; N % 4 == 0
-__global__ __launch_bounds__(256) void lx_reduce_kernel(const float* __restrict__ slab, int splits, int M, int N, const float* __restrict__ scale,
-                                                        const float* __restrict__ add, void* __restrict__ out, long long ldo, int out_f32) {
-    const size_t total = (size_t)M * N / 4, stride = (size_t)M * N;
-    const float sc = scale != nullptr ? scale[0] : 1.0f;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
-        const float* q = slab + i * 4;
-        f32x4 s = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(q));
+// the tiles of the rest: out = scale * sum of their parts (+ add), in the order of the contraction; 8 rows of a tile per workgroup
+__global__ __launch_bounds__(256) void lx_join_kernel(const LxGemmParams p, int G) {
+    const int r = blockIdx.x >> 5;
+    const int tile = p.whole + r;
+    const int full = p.tiles_m * p.band;
+    const int blk = tile / full;
+    const int rem = tile - blk * full;
+    const int c0 = blk * p.band;
+    const int width = p.tiles_n - c0 < p.band ? p.tiles_n - c0 : p.band;
+    const int tm = rem / width;
+    const int m0 = tm * LX_TILE, n0 = (c0 + rem - tm * width) * LX_TILE;
+    const int row = (int)(blockIdx.x & 31) * 8 + (int)(threadIdx.x >> 5), col = (int)(threadIdx.x & 31) * 8;
+    const int m = m0 + row, n = n0 + col;
+    if (m >= p.M || n >= p.N) return;
+    // the ranges that meet this tile's steps, from the one its first step lies in to the one of its last; the tile is the second part of
+    // the first of them if that range began in the tile before
+    const int s0 = r * p.steps, total = p.rest * p.steps;
+    const int q = total / G, more = total - q * G;
+    auto owner = [&](int step) { return step < more * (q + 1) ? step / (q + 1) : more + (step - more * (q + 1)) / q; };
+    const int first = owner(s0), last = owner(s0 + p.steps - 1);
+    int from, to;
+    lx_range(first, total, G, from, to);
+    const float* at = p.slab + row * 256 + col;
+    const float* w0 = at + (size_t)(2 * first + (from < s0 ? 1 : 0)) * 65536;
+    f32x4 lo = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(w0)), hi = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(w0 + 4));
 #pragma unroll 4
-        for (int k = 1; k < splits; ++k) s += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(q + k * stride));
-        s *= sc;
-        if (add != nullptr) s += *reinterpret_cast<const f32x4*>(add + i * 4);
-        const size_t m = i * 4 / N, n = i * 4 - m * N;
-        if (out_f32) {
-            *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(out) + m * ldo + n) = s;
-        } else {
-            uint2 o;
-            o.x = pack2bf(s[0], s[1]);
-            o.y = pack2bf(s[2], s[3]);
-            *reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(out) + m * ldo + n) = o;
-        }
+    for (int g = first + 1; g <= last; ++g) {
+        const float* w = at + (size_t)g * 131072;
+        lo += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(w));
+        hi += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(w + 4));
+    }
+    const float sc = p.scale != nullptr ? p.scale[0] : 1.0f;
+    lo *= sc;
+    hi *= sc;
+    if (p.add != nullptr) {
+        const float* w = p.add + (size_t)m * p.N + n;
+        lo += *reinterpret_cast<const f32x4*>(w);
+        hi += *reinterpret_cast<const f32x4*>(w + 4);
+    }
+    if (p.out_f32) {
+        float* w = reinterpret_cast<float*>(p.out) + (size_t)m * p.ldo + n;
+        *reinterpret_cast<f32x4*>(w) = lo;
+        *reinterpret_cast<f32x4*>(w + 4) = hi;
+    } else {
+        const u32x4 o = {pack2bf(lo[0], lo[1]), pack2bf(lo[2], lo[3]), pack2bf(hi[0], hi[1]), pack2bf(hi[2], hi[3])};
+        *reinterpret_cast<u32x4*>(reinterpret_cast<bf16_t*>(p.out) + (size_t)m * p.ldo + n) = o;
     }
 }
 
@@ -586,20 +726,31 @@ static int lx_cus() {
 }
 static size_t lx_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
+struct LxDeal { int G, whole, rest; };          // workgroups, whole tiles, tiles behind them that are cut
 // how the rows are cut and where everything lies in the workspace
 struct LxPlan {
     long long ldp, stat_cols;
     int block, blocks;              // rows per block, blocks
-    int dx_splits;
+    LxDeal dx[2], dw[2];            // of a block, of the last one
     size_t scale, stats, zsum, P, acc, slab, colpart, colsum, total;
 };
-// dx = dz W has few output tiles and a long contraction: it is cut so that about every compute unit has a share, at least 8 steps each
-static int lx_dx_splits(int rows, int V, int D) {
-    const long long tiles = (long long)((rows + LX_TILE - 1) / LX_TILE) * ((D + LX_TILE - 1) / LX_TILE);
-    const long long steps = (V + LX_BK - 1) / LX_BK;
-    long long s = 256 / tiles;
-    if (s > steps / 8) s = steps / 8;
-    return (int)(s < 1 ? 1 : s);
+// How the tiles of an output product are dealt.  Whole tiles on G workgroups take ceil(tiles / G) rounds; cutting what does not fill a round into
+// equal ranges of steps fills it at the price of fp32 parts written and read.  Costs in steps (about 1.4 us): a tile's epilogue and the
+// fill of the pipeline 4, a part of 256 x 256 that is written and read 0.09 (512 KB at 4 TB/s).  Measured: 294 tiles of 128 steps 384 -> 296 us, 96 of
+// 392 527 -> 300 us, 6 of 342 (42 equal splits, one range each) 60 -> 45 us.
+static LxDeal lx_deal(int M, int N, int steps, int cus) {
+    const long long tiles = (long long)((M + LX_TILE - 1) / LX_TILE) * ((N + LX_TILE - 1) / LX_TILE);
+    const int rounds = (int)(tiles / cus), rest = (int)(tiles - (long long)rounds * cus);
+    LxDeal d = {(int)(tiles < cus ? tiles : cus), (int)tiles, 0};
+    if (rest == 0 || (long long)rest * steps > 0x7fffffff) return d;
+    const double part = 0.09 * (M < LX_TILE ? M : LX_TILE) / LX_TILE;
+    double best = 0.98 * (rounds + 1) * (steps + 4.0);
+    for (int G = rounds > 0 ? cus : (rest + 8) & ~7; G <= cus; G += 8) {
+        if ((long long)rest * steps / G < 2) break;
+        const double cost = rounds * (steps + 4.0) + (double)rest * steps / G + 8.0 + 4.0 + part * (G + rest);
+        if (cost < best) { best = cost; d.G = G; d.whole = rounds * cus; d.rest = rest; }
+    }
+    return d;
 }
 static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw_f32, int bias, size_t block_bytes) {
     LxPlan q = {};
@@ -624,8 +775,16 @@ static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw
     if (grad) {
         q.P = take((size_t)rows * q.ldp * 2);
         if (q.blocks > 1 && !dw_f32) q.acc = take((size_t)V * D * sizeof(float));
-        q.dx_splits = lx_dx_splits((int)rows, V, D);
-        if (q.dx_splits > 1) q.slab = take((size_t)q.dx_splits * rows * D * sizeof(float));
+        const int cus = lx_cus();
+        int ranges = 0;
+        for (int last = 0; last < 2; ++last) {
+            const int n = last ? (int)(T - (long long)(q.blocks - 1) * rows) : (int)rows;
+            q.dx[last] = lx_deal(n, D, (V + LX_BK - 1) / LX_BK, cus);
+            q.dw[last] = lx_deal(V, D, (n + LX_BK - 1) / LX_BK, cus);
+            if (q.dx[last].rest && q.dx[last].G > ranges) ranges = q.dx[last].G;
+            if (q.dw[last].rest && q.dw[last].G > ranges) ranges = q.dw[last].G;
+        }
+        if (ranges > 0) q.slab = take((size_t)ranges * 2 * 65536 * sizeof(float));
         if (bias) {
             q.colpart = take((size_t)LX_RANGES * q.ldp * sizeof(float));
             q.colsum = take((size_t)V * sizeof(float));
@@ -636,13 +795,12 @@ static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw
 }
 
 template <int LAY, int EPI>
-static int lx_launch(const LxGemmParams& p, hipStream_t s, const char* what) {
+static int lx_launch(const LxGemmParams& p, int grid, hipStream_t s, const char* what) {
     static VitkLdsOnce once = {};
     if (int rc = vitk_lds_once(once, (const void*)lx_gemm_kernel<LAY, EPI>, LX_LDS, what)) return rc;
-    const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
-    const int cus = lx_cus();
-    const int grid = items < cus ? (int)items : cus;
     lx_gemm_kernel<LAY, EPI><<<grid, 512, LX_LDS, s>>>(p);
+    if (int rc = vitk_check_launch(what)) return rc;
+    if (p.rest > 0) lx_join_kernel<<<p.rest * 32, 256, 0, s>>>(p, grid);
     return vitk_check_launch(what);
 }
 
@@ -675,6 +833,7 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         return VITK_ENOSPC;
     }
     hipStream_t s = (hipStream_t)stream;
+    const int cus = lx_cus();
     char* ws = (char*)workspace;
     float* scale = (float*)(ws + q.scale);
     const long long* tg = (const long long*)target;
@@ -687,13 +846,16 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         const int n = (int)(T - r0 < q.block ? T - r0 : q.block);
         const bool last = b == q.blocks - 1;
         LxGemmParams g = {};
-        g.A = (const bf16_t*)x + r0 * ldx; g.lda = ldx; g.B = (const bf16_t*)w; g.ldb = ldw;
+        g.A = (const bf16_t*)x + r0 * ldx; g.lda = (int)ldx; g.B = (const bf16_t*)w; g.ldb = (int)ldw;
         g.M = n; g.N = V; g.KA = g.KB = D; g.steps = (D + LX_BK - 1) / LX_BK;
-        g.tiles_m = (n + LX_TILE - 1) / LX_TILE; g.tiles_n = (int)(q.ldp / LX_TILE); g.band = 8; g.splits = 1;
+        g.tiles_m = (n + LX_TILE - 1) / LX_TILE; g.tiles_n = (int)(q.ldp / LX_TILE); g.band = 8; g.whole = g.tiles_m * g.tiles_n;
         g.bias = bias; g.bias_type = bias_type;
         g.stats = (float2*)(ws + q.stats); g.stat_cols = (int)q.stat_cols; g.zsum = smoothing > 0.f ? (float*)(ws + q.zsum) : nullptr;
         g.P = grad ? (_Float16*)(ws + q.P) : nullptr; g.ldp = q.ldp;
-        if (int rc = lx_launch<LX_NT, LX_XENT>(g, s, "linear_xent_logits")) return rc;
+        const int grid = g.whole < cus ? g.whole : cus;
+        if (int rc = g.bias || g.zsum ? lx_launch<LX_NT, LX_XENT_BIAS>(g, grid, s, "linear_xent_logits")
+                                      : lx_launch<LX_NT, LX_XENT>(g, grid, s, "linear_xent_logits"))
+            return rc;
         LxRowParams r = {};
         r.x = g.A; r.ldx = ldx; r.w = g.B; r.ldw = ldw; r.bias = bias; r.bias_type = bias_type; r.target = tg + r0; r.ignore_index = ignore_index;
         r.stats = g.stats; r.zsum = g.zsum; r.stat_cols = g.stat_cols; r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.smoothing = smoothing;
@@ -707,26 +869,24 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         const bf16_t* dz = (const bf16_t*)(ws + q.P);
         // dx = dz W: dz is zero behind the vocabulary up to its row stride
         LxGemmParams d = {};
-        d.A = dz; d.lda = q.ldp; d.B = (const bf16_t*)w; d.ldb = ldw; d.M = n; d.N = D; d.KA = (int)q.ldp; d.KB = V; d.steps = (V + LX_BK - 1) / LX_BK;
-        d.tiles_m = (n + LX_TILE - 1) / LX_TILE; d.tiles_n = (D + LX_TILE - 1) / LX_TILE; d.band = 8; d.splits = q.dx_splits;
-        d.scale = scale; d.out = (bf16_t*)dx + r0 * lddx; d.ldo = lddx; d.slab = q.dx_splits > 1 ? (float*)(ws + q.slab) : nullptr;
-        if (int rc = lx_launch<LX_NN, LX_OUT>(d, s, "linear_xent_dx")) return rc;
-        if (d.slab != nullptr) {
-            const long long total = (long long)n * D / 4;
-            const int grid = (int)((total + 255) / 256 < 2048 ? (total + 255) / 256 : 2048);
-            lx_reduce_kernel<<<grid, 256, 0, s>>>(d.slab, d.splits, n, D, scale, nullptr, d.out, lddx, 0);
-            if (int rc = vitk_check_launch("linear_xent_dx_sum")) return rc;
-        }
+        d.A = dz; d.lda = (int)q.ldp; d.B = (const bf16_t*)w; d.ldb = (int)ldw; d.M = n; d.N = D; d.KA = (int)q.ldp; d.KB = V; d.steps = (V + LX_BK - 1) / LX_BK;
+        d.tiles_m = (n + LX_TILE - 1) / LX_TILE; d.tiles_n = (D + LX_TILE - 1) / LX_TILE; d.band = 8;
+        const LxDeal dd = q.dx[last];
+        d.whole = dd.whole; d.rest = dd.rest;
+        d.scale = scale; d.out = (bf16_t*)dx + r0 * lddx; d.ldo = lddx; d.slab = (float*)(ws + q.slab);
+        if (int rc = lx_launch<LX_NN, LX_OUT>(d, dd.G, s, "linear_xent_dx")) return rc;
         // dW = dz^T x, summed over the blocks in fp32
         LxGemmParams e = {};
-        e.A = dz; e.lda = q.ldp; e.B = g.A; e.ldb = ldx; e.M = V; e.N = D; e.KA = e.KB = n; e.steps = (n + LX_BK - 1) / LX_BK;
-        e.tiles_m = (V + LX_TILE - 1) / LX_TILE; e.tiles_n = (D + LX_TILE - 1) / LX_TILE; e.band = 8; e.splits = 1;
-        e.scale = scale;
+        e.A = dz; e.lda = (int)q.ldp; e.B = g.A; e.ldb = (int)ldx; e.M = V; e.N = D; e.KA = e.KB = n; e.steps = (n + LX_BK - 1) / LX_BK;
+        e.tiles_m = (V + LX_TILE - 1) / LX_TILE; e.tiles_n = (D + LX_TILE - 1) / LX_TILE; e.band = 8;
+        const LxDeal de = q.dw[last];
+        e.whole = de.whole; e.rest = de.rest;
+        e.scale = scale; e.slab = d.slab;
         float* acc = dw_f32 ? (float*)dw : (float*)(ws + q.acc);
         e.add = b > 0 ? acc : nullptr;
         if (last) { e.out = dw; e.ldo = lddw; e.out_f32 = dw_f32; }
         else { e.out = acc; e.ldo = D; e.out_f32 = 1; }
-        if (int rc = lx_launch<LX_TN, LX_OUT>(e, s, "linear_xent_dw")) return rc;
+        if (int rc = lx_launch<LX_TN, LX_OUT>(e, de.G, s, "linear_xent_dw")) return rc;
         if (db != nullptr) {
             float* part = (float*)(ws + q.colpart);
             int per = (n + LX_RANGES - 1) / LX_RANGES;
