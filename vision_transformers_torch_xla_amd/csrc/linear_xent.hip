@@ -35,10 +35,10 @@ struct LxGemmParams {
     int M, N;
     int KA, KB;             // valid extent of the contraction in each operand; behind it zeros are read
     int steps;              // 64-deep steps over the whole contraction
-    int tiles_m, tiles_n, band;
-    // work: workgroup g of G takes the whole tiles g, g + G, ... below `whole`; the `rest` tiles behind them are one sequence of rest * steps
-    // steps cut into G equal ranges (LX_OUT only), whose parts of tiles go to slab[2 range + part][256][256] as fp32 sums
-    int whole, rest;
+    int tiles_m, tiles_n;
+    // work, LX_XENT*: workgroup g of G takes the tiles g, g + G, ... (in bands of 8 column tiles)
+    // work, LX_OUT: see LxDeal
+    int width, teams, whole, rest, ranges;
     // LX_OUT: out[m][n] = scale[0] * acc (+ add[m][n]), bf16 or fp32
     const float* scale;
     const float* add;
@@ -92,18 +92,22 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
     const unsigned lds_stage = (unsigned)(wave * 4 * 1024);
 
     const int G = gridDim.x;
-    // this workgroup's items: whole tiles, then at most two parts of tiles (its range of the rest is no longer than a tile)
-    const int whole_items = (int)blockIdx.x < p.whole ? (p.whole - 1 - (int)blockIdx.x) / G + 1 : 0;
-    int r0 = 0, r1 = 0, range = 0, rt = 0, parts = 0;
+    int whole_items, parts = 0, r0 = 0, r1 = 0, rt = 0, team = 0, member = 0;
     if constexpr (EPI == LX_OUT) {
-        if (p.rest > 0) {
-            range = __builtin_amdgcn_readfirstlane(xcd_remap(blockIdx.x, G));       // neighbouring ranges on one XCD
-            lx_range(range, p.rest * p.steps, G, r0, r1);
+        const int id = xcd_remap(blockIdx.x, G);        // a team's workgroups are neighbours on one XCD
+        team = __builtin_amdgcn_readfirstlane(id / p.width);
+        member = __builtin_amdgcn_readfirstlane(id - team * p.width);
+        whole_items = __builtin_amdgcn_readfirstlane(team < p.whole ? (p.whole - 1 - team) / p.teams + 1 : 0);
+        if (team < p.ranges) {
+            lx_range(team, p.rest * p.steps, p.ranges, r0, r1);
             r0 = __builtin_amdgcn_readfirstlane(r0);
             r1 = __builtin_amdgcn_readfirstlane(r1);
-            rt = __builtin_amdgcn_readfirstlane(r0 / p.steps);        // tile (of the rest) of the first part
-            parts = r1 <= r0 ? 0 : r1 > (rt + 1) * p.steps ? 2 : 1;
+            rt = __builtin_amdgcn_readfirstlane(r0 / p.steps);        // row (of the rest) of the first part
+            parts = r1 > (rt + 1) * p.steps ? 2 : 1;
         }
+    } else {
+        const int tiles = p.tiles_m * p.tiles_n;
+        whole_items = __builtin_amdgcn_readfirstlane((int)blockIdx.x < tiles ? (tiles - 1 - (int)blockIdx.x) / G + 1 : 0);
     }
     const int items = whole_items + parts;
 
@@ -118,28 +122,35 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
     unsigned voA[4], voB[4];
     // item v: where its tile is, its steps k0 .. k1 - 1, and which part it is (-1: a whole tile)
     auto locate = [&](int v, int& m0, int& n0, int& k0, int& k1, int& part) {
-        int tile;
         k0 = 0;
         k1 = p.steps;
-        if (EPI != LX_OUT || v < whole_items) {
-            part = -1;
-            tile = xcd_remap(blockIdx.x + v * G, p.whole);
+        part = -1;
+        int tm, tn;
+        if constexpr (EPI == LX_OUT) {
+            int row = v * p.teams + team;
+            if (v >= whole_items) {
+                part = v - whole_items;
+                row = p.whole + rt + part;
+                if (part == 0) k0 = r0 - rt * p.steps;
+                const int left = r1 - (rt + part) * p.steps;
+                k1 = left < p.steps ? left : p.steps;
+            }
+            const int blk = row / p.tiles_m;
+            tm = row - blk * p.tiles_m;
+            tn = blk * p.width + member;
         } else {
-            part = v - whole_items;
-            tile = p.whole + rt + part;
-            if (part == 0) k0 = r0 - rt * p.steps;
-            const int left = r1 - (rt + part) * p.steps;
-            k1 = left < p.steps ? left : p.steps;
+            const int tile = xcd_remap(blockIdx.x + v * G, p.tiles_m * p.tiles_n);
+            const int full = p.tiles_m * 8;
+            const int blk = tile / full;
+            const int rem = tile - blk * full;
+            const int c0 = blk * 8;
+            const int width = p.tiles_n - c0 < 8 ? p.tiles_n - c0 : 8;
+            tm = rem / width;
+            tn = c0 + rem - tm * width;
         }
-        const int full = p.tiles_m * p.band;
-        const int blk = tile / full;
-        const int rem = tile - blk * full;
-        const int c0 = blk * p.band;
-        const int width = p.tiles_n - c0 < p.band ? p.tiles_n - c0 : p.band;
-        const int tm = rem / width;
         // the divisions run on the vector unit: say that their results are the same in every lane
         m0 = __builtin_amdgcn_readfirstlane(tm * LX_TILE);
-        n0 = __builtin_amdgcn_readfirstlane((c0 + rem - tm * width) * LX_TILE);
+        n0 = __builtin_amdgcn_readfirstlane(tn * LX_TILE);
     };
     auto aim = [&](int v) {
         int m0, n0, part;
@@ -391,7 +402,7 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
                     const int m = m0 + wm * 128 + tm * 16 + r;
                     if (m < p.M && n < p.N) {
                         if (part >= 0) {
-                            float* q = p.slab + (size_t)(2 * range + part) * 65536 + (m - m0) * 256 + (n - n0);
+                            float* q = p.slab + (size_t)((2 * team + part) * p.width + member) * 65536 + (m - m0) * 256 + (n - n0);
                             __builtin_nontemporal_store(lo, reinterpret_cast<f32x4*>(q));
                             __builtin_nontemporal_store(hi, reinterpret_cast<f32x4*>(q + 4));
                         } else {
@@ -626,33 +637,28 @@ __global__ __launch_bounds__(1024) void lx_loss_kernel(const long long* __restri
 }
 
 // the tiles of the rest: out = scale * sum of their parts (+ add), in the order of the contraction; 8 rows of a tile per workgroup
-__global__ __launch_bounds__(256) void lx_join_kernel(const LxGemmParams p, int G) {
-    const int r = blockIdx.x >> 5;
-    const int tile = p.whole + r;
-    const int full = p.tiles_m * p.band;
-    const int blk = tile / full;
-    const int rem = tile - blk * full;
-    const int c0 = blk * p.band;
-    const int width = p.tiles_n - c0 < p.band ? p.tiles_n - c0 : p.band;
-    const int tm = rem / width;
-    const int m0 = tm * LX_TILE, n0 = (c0 + rem - tm * width) * LX_TILE;
+__global__ __launch_bounds__(256) void lx_join_kernel(const LxGemmParams p) {
+    const int r = (int)(blockIdx.x >> 5) / p.width, member = (int)(blockIdx.x >> 5) - r * p.width;
+    const int blk = (p.whole + r) / p.tiles_m;
+    const int m0 = (p.whole + r - blk * p.tiles_m) * LX_TILE, n0 = (blk * p.width + member) * LX_TILE;
     const int row = (int)(blockIdx.x & 31) * 8 + (int)(threadIdx.x >> 5), col = (int)(threadIdx.x & 31) * 8;
     const int m = m0 + row, n = n0 + col;
     if (m >= p.M || n >= p.N) return;
-    // the ranges that meet this tile's steps, from the one its first step lies in to the one of its last; the tile is the second part of
-    // the first of them if that range began in the tile before
+    // the ranges that meet this row's steps, from the one its first step lies in to the one of its last; the tile is the second part of
+    // the first of them if that range began in the row before
     const int s0 = r * p.steps, total = p.rest * p.steps;
-    const int q = total / G, more = total - q * G;
+    const int q = total / p.ranges, more = total - q * p.ranges;
     auto owner = [&](int step) { return step < more * (q + 1) ? step / (q + 1) : more + (step - more * (q + 1)) / q; };
     const int first = owner(s0), last = owner(s0 + p.steps - 1);
     int from, to;
-    lx_range(first, total, G, from, to);
-    const float* at = p.slab + row * 256 + col;
-    const float* w0 = at + (size_t)(2 * first + (from < s0 ? 1 : 0)) * 65536;
+    lx_range(first, total, p.ranges, from, to);
+    const float* at = p.slab + (size_t)member * 65536 + row * 256 + col;
+    const size_t tile = (size_t)p.width * 65536;
+    const float* w0 = at + (2 * first + (from < s0 ? 1 : 0)) * tile;
     f32x4 lo = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(w0)), hi = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(w0 + 4));
 #pragma unroll 4
     for (int g = first + 1; g <= last; ++g) {
-        const float* w = at + (size_t)g * 131072;
+        const float* w = at + 2 * g * tile;
         lo += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(w));
         hi += __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(w + 4));
     }
@@ -726,7 +732,11 @@ static int lx_cus() {
 }
 static size_t lx_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
-struct LxDeal { int G, whole, rest; };          // workgroups, whole tiles, tiles behind them that are cut
+// How the tiles of dx and dW are dealt.  `width` column tiles side by side form a row, worked on by a team of as many workgroups in step, so
+// that what they share of the other operand is fetched once; there are tiles_m * tiles_n / width rows.  Of `teams` teams, team t takes the
+// whole rows t, t + teams, ... below `whole`; the `rest` rows behind them are one sequence of rest * steps steps, cut into `ranges`
+// equal ranges (at most two parts of rows each) whose fp32 sums go to slab[2 range + part][width][256][256] and are joined in order.
+struct LxDeal { int width, teams, whole, rest, ranges; };
 // how the rows are cut and where everything lies in the workspace
 struct LxPlan {
     long long ldp, stat_cols;
@@ -734,21 +744,26 @@ struct LxPlan {
     LxDeal dx[2], dw[2];            // of a block, of the last one
     size_t scale, stats, zsum, P, acc, slab, colpart, colsum, total;
 };
-// How the tiles of an output product are dealt.  Whole tiles on G workgroups take ceil(tiles / G) rounds; cutting what does not fill a round into
-// equal ranges of steps fills it at the price of fp32 parts written and read.  Costs in steps (about 1.4 us): a tile's epilogue and the
-// fill of the pipeline 4, a part of 256 x 256 that is written and read 0.09 (512 KB at 4 TB/s).  Measured: 294 tiles of 128 steps 384 -> 296 us, 96 of
-// 392 527 -> 300 us, 6 of 342 (42 equal splits, one range each) 60 -> 45 us.
+// Whole rows alone take ceil(rows / teams) rounds; cutting what does not fill a round into ranges fills it at the price of parts written and
+// read.  Costs in steps (about 1.4 us): a tile's epilogue and the fill of the pipeline 4, a part of 256 x 256 that is written and read 0.09
+// (512 KB at 4 TB/s).
 static LxDeal lx_deal(int M, int N, int steps, int cus) {
-    const long long tiles = (long long)((M + LX_TILE - 1) / LX_TILE) * ((N + LX_TILE - 1) / LX_TILE);
-    const int rounds = (int)(tiles / cus), rest = (int)(tiles - (long long)rounds * cus);
-    LxDeal d = {(int)(tiles < cus ? tiles : cus), (int)tiles, 0};
+    const int tiles_n = (N + LX_TILE - 1) / LX_TILE;
+    LxDeal d = {};
+    for (d.width = tiles_n < 8 ? tiles_n : 8; tiles_n % d.width; --d.width) {}
+    const int rows = (M + LX_TILE - 1) / LX_TILE * (tiles_n / d.width);
+    const int most = cus / d.width > 0 ? cus / d.width : 1;
+    const int rounds = rows / most, rest = rows - rounds * most;
+    d.teams = rows < most ? rows : most;
+    d.whole = rows;
     if (rest == 0 || (long long)rest * steps > 0x7fffffff) return d;
-    const double part = 0.09 * (M < LX_TILE ? M : LX_TILE) / LX_TILE;
+    const double part = 0.09 * (M < LX_TILE ? M : LX_TILE) / LX_TILE * d.width;
     double best = 0.98 * (rounds + 1) * (steps + 4.0);
-    for (int G = rounds > 0 ? cus : (rest + 8) & ~7; G <= cus; G += 8) {
-        if ((long long)rest * steps / G < 2) break;
-        const double cost = rounds * (steps + 4.0) + (double)rest * steps / G + 8.0 + 4.0 + part * (G + rest);
-        if (cost < best) { best = cost; d.G = G; d.whole = rounds * cus; d.rest = rest; }
+    for (int k = 1; k <= 16; ++k) {
+        const int ranges = most * k / 16;
+        if (ranges <= rest || (long long)rest * steps / ranges < 2) continue;
+        const double cost = rounds * (steps + 4.0) + (double)rest * steps / ranges + 12.0 + part * (ranges + rest);
+        if (cost < best) { best = cost; d.teams = rounds > 0 ? most : ranges; d.whole = rounds * most; d.rest = rest; d.ranges = ranges; }
     }
     return d;
 }
@@ -776,15 +791,17 @@ static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw
         q.P = take((size_t)rows * q.ldp * 2);
         if (q.blocks > 1 && !dw_f32) q.acc = take((size_t)V * D * sizeof(float));
         const int cus = lx_cus();
-        int ranges = 0;
+        size_t parts = 0;           // tiles of partial sums; dx and dW use them one after the other
         for (int last = 0; last < 2; ++last) {
             const int n = last ? (int)(T - (long long)(q.blocks - 1) * rows) : (int)rows;
             q.dx[last] = lx_deal(n, D, (V + LX_BK - 1) / LX_BK, cus);
             q.dw[last] = lx_deal(V, D, (n + LX_BK - 1) / LX_BK, cus);
-            if (q.dx[last].rest && q.dx[last].G > ranges) ranges = q.dx[last].G;
-            if (q.dw[last].rest && q.dw[last].G > ranges) ranges = q.dw[last].G;
+            for (const LxDeal& d : {q.dx[last], q.dw[last]}) {
+                const size_t need = (size_t)2 * d.ranges * d.width;
+                if (need > parts) parts = need;
+            }
         }
-        if (ranges > 0) q.slab = take((size_t)ranges * 2 * 65536 * sizeof(float));
+        if (parts > 0) q.slab = take(parts * 65536 * sizeof(float));
         if (bias) {
             q.colpart = take((size_t)LX_RANGES * q.ldp * sizeof(float));
             q.colsum = take((size_t)V * sizeof(float));
@@ -800,7 +817,7 @@ static int lx_launch(const LxGemmParams& p, int grid, hipStream_t s, const char*
     if (int rc = vitk_lds_once(once, (const void*)lx_gemm_kernel<LAY, EPI>, LX_LDS, what)) return rc;
     lx_gemm_kernel<LAY, EPI><<<grid, 512, LX_LDS, s>>>(p);
     if (int rc = vitk_check_launch(what)) return rc;
-    if (p.rest > 0) lx_join_kernel<<<p.rest * 32, 256, 0, s>>>(p, grid);
+    if (p.rest > 0) lx_join_kernel<<<p.rest * p.width * 32, 256, 0, s>>>(p);
     return vitk_check_launch(what);
 }
 
@@ -848,11 +865,12 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         LxGemmParams g = {};
         g.A = (const bf16_t*)x + r0 * ldx; g.lda = (int)ldx; g.B = (const bf16_t*)w; g.ldb = (int)ldw;
         g.M = n; g.N = V; g.KA = g.KB = D; g.steps = (D + LX_BK - 1) / LX_BK;
-        g.tiles_m = (n + LX_TILE - 1) / LX_TILE; g.tiles_n = (int)(q.ldp / LX_TILE); g.band = 8; g.whole = g.tiles_m * g.tiles_n;
+        g.tiles_m = (n + LX_TILE - 1) / LX_TILE; g.tiles_n = (int)(q.ldp / LX_TILE);
         g.bias = bias; g.bias_type = bias_type;
         g.stats = (float2*)(ws + q.stats); g.stat_cols = (int)q.stat_cols; g.zsum = smoothing > 0.f ? (float*)(ws + q.zsum) : nullptr;
         g.P = grad ? (_Float16*)(ws + q.P) : nullptr; g.ldp = q.ldp;
-        const int grid = g.whole < cus ? g.whole : cus;
+        const long long tiles = (long long)g.tiles_m * g.tiles_n;
+        const int grid = tiles < cus ? (int)tiles : cus;
         if (int rc = g.bias || g.zsum ? lx_launch<LX_NT, LX_XENT_BIAS>(g, grid, s, "linear_xent_logits")
                                       : lx_launch<LX_NT, LX_XENT>(g, grid, s, "linear_xent_logits"))
             return rc;
@@ -870,23 +888,23 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         // dx = dz W: dz is zero behind the vocabulary up to its row stride
         LxGemmParams d = {};
         d.A = dz; d.lda = (int)q.ldp; d.B = (const bf16_t*)w; d.ldb = (int)ldw; d.M = n; d.N = D; d.KA = (int)q.ldp; d.KB = V; d.steps = (V + LX_BK - 1) / LX_BK;
-        d.tiles_m = (n + LX_TILE - 1) / LX_TILE; d.tiles_n = (D + LX_TILE - 1) / LX_TILE; d.band = 8;
-        const LxDeal dd = q.dx[last];
-        d.whole = dd.whole; d.rest = dd.rest;
+        d.tiles_m = (n + LX_TILE - 1) / LX_TILE; d.tiles_n = (D + LX_TILE - 1) / LX_TILE;
+        const LxDeal& dd = q.dx[last];
+        d.width = dd.width; d.teams = dd.teams; d.whole = dd.whole; d.rest = dd.rest; d.ranges = dd.ranges;
         d.scale = scale; d.out = (bf16_t*)dx + r0 * lddx; d.ldo = lddx; d.slab = (float*)(ws + q.slab);
-        if (int rc = lx_launch<LX_NN, LX_OUT>(d, dd.G, s, "linear_xent_dx")) return rc;
+        if (int rc = lx_launch<LX_NN, LX_OUT>(d, dd.teams * dd.width, s, "linear_xent_dx")) return rc;
         // dW = dz^T x, summed over the blocks in fp32
         LxGemmParams e = {};
         e.A = dz; e.lda = (int)q.ldp; e.B = g.A; e.ldb = (int)ldx; e.M = V; e.N = D; e.KA = e.KB = n; e.steps = (n + LX_BK - 1) / LX_BK;
-        e.tiles_m = (V + LX_TILE - 1) / LX_TILE; e.tiles_n = (D + LX_TILE - 1) / LX_TILE; e.band = 8;
-        const LxDeal de = q.dw[last];
-        e.whole = de.whole; e.rest = de.rest;
+        e.tiles_m = (V + LX_TILE - 1) / LX_TILE; e.tiles_n = (D + LX_TILE - 1) / LX_TILE;
+        const LxDeal& de = q.dw[last];
+        e.width = de.width; e.teams = de.teams; e.whole = de.whole; e.rest = de.rest; e.ranges = de.ranges;
         e.scale = scale; e.slab = d.slab;
         float* acc = dw_f32 ? (float*)dw : (float*)(ws + q.acc);
         e.add = b > 0 ? acc : nullptr;
         if (last) { e.out = dw; e.ldo = lddw; e.out_f32 = dw_f32; }
         else { e.out = acc; e.ldo = D; e.out_f32 = 1; }
-        if (int rc = lx_launch<LX_TN, LX_OUT>(e, de.G, s, "linear_xent_dw")) return rc;
+        if (int rc = lx_launch<LX_TN, LX_OUT>(e, de.teams * de.width, s, "linear_xent_dw")) return rc;
         if (db != nullptr) {
             float* part = (float*)(ws + q.colpart);
             int per = (n + LX_RANGES - 1) / LX_RANGES;
