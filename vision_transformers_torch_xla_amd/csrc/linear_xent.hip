@@ -5,7 +5,7 @@
 //
 // x bf16 [T, D], W bf16 [V, D].  The rows are worked through in blocks whose size the workspace bounds; per block
 //   1. x W^T tile by tile (lx_gemm_kernel, NT).  The epilogue takes a tile's logits in fp32 from the accumulators: per row and 64
-//      columns their maximum m and s = sum exp(z - m) go to a small table; exp(z - m) itself, in [0, 1], goes to the block's
+//      columns their maximum m and s = sum exp(z - m) go to a small table (in powers of two); exp(z - m) itself, in [0, 1], goes to the block's
 //      matrix P in fp16 (11 bits; bf16 would round it 8 times as far; what falls below fp16's 6e-8 of its maximum is below what the
 //      later bf16 rounding of its larger neighbours leaves).  Loss alone: only the table is written.
 //   2. one workgroup per row (lx_row_kernel): lse from the table, the target's logit as a dot product of its own, the row's loss, and
@@ -46,7 +46,7 @@ struct LxGemmParams {
     float* slab;
     // LX_XENT
     const void* bias; int bias_type;        // 0 fp32, 1 bf16, null: none
-    float2* stats; int stat_cols;           // [M][stat_cols]: (m, s) of 64 columns
+    float2* stats; int stat_cols;           // [M][stat_cols]: (m log2 e, s) of 64 columns
     float* zsum;                            // [M][stat_cols] sums of the logits, null: not wanted (no smoothing)
     _Float16* P; long long ldp;             // null: loss alone
 };
@@ -466,13 +466,15 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
                     }
                 mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float ref = mx == -INFINITY ? 0.f : mx;        // a row of -inf only: exp(-inf - 0) = 0
+                // From here on in powers of two, relative to m = max * log2(e) as rounded: z * log2(e) - m is one fma, exact up to its own rounding
+                mx *= 1.44269504088896340736f;
+                const float ref = mx == -INFINITY ? 0.f : mx;        // a row of -inf only: 2^(-inf - 0) = 0
                 float s = 0.f;
 #pragma unroll
                 for (int tn = 0; tn < 4; ++tn)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        z[tn][j] = __builtin_amdgcn_exp2f((z[tn][j] - ref) * 1.44269504088896340736f);
+                        z[tn][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[tn][j], 1.44269504088896340736f, -ref));
                         s += z[tn][j];
                     }
                 s += __shfl_xor(s, 16, 64);
@@ -557,7 +559,7 @@ __global__ __launch_bounds__(256) void lx_row_kernel(const LxRowParams p) {
     float s = 0.f, zs = 0.f;
     for (int c = threadIdx.x; c < p.stat_cols; c += 256) {
         const float2 v = st[c];
-        s += v.y * (v.x == -INFINITY ? 1.f : __expf(v.x - ref));         // an all -inf entry has s = 0, or NaN where a logit was NaN
+        s += v.y * (v.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(v.x - ref));         // an all -inf entry has s = 0, or NaN where a logit was NaN
         if (p.smoothing > 0.f) zs += p.zsum[(size_t)row * p.stat_cols + c];
     }
     s = lx_block_sum(s, sh);
@@ -575,7 +577,7 @@ __global__ __launch_bounds__(256) void lx_row_kernel(const LxRowParams p) {
     dot = lx_block_sum(dot, sh);
     if (p.smoothing > 0.f) zs = lx_block_sum(zs, sh);
     if (p.bias != nullptr) dot += p.bias_type == 1 ? bf2f(reinterpret_cast<const bf16_t*>(p.bias)[t]) : reinterpret_cast<const float*>(p.bias)[t];
-    const float lse = ref + logf(s);
+    const float lse2 = ref + log2f(s), lse = lse2 * 0.69314718055994530942f;
     if (threadIdx.x == 0) {
         float l = lse - dot;
         if (p.smoothing > 0.f) l = (1.f - p.smoothing) * l + p.smoothing * (lse - zs / (float)p.V);
@@ -585,7 +587,7 @@ __global__ __launch_bounds__(256) void lx_row_kernel(const LxRowParams p) {
     const float u = p.smoothing / (float)p.V, hit = 1.f - p.smoothing;
     for (int c = threadIdx.x; c < chunks; c += 256) {
         const u32x4 r = reinterpret_cast<const u32x4*>(P)[c];
-        const float f = __expf(st[c >> 3].x - lse);
+        const float f = __builtin_amdgcn_exp2f(st[c >> 3].x - lse2);
         float v[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
