@@ -124,6 +124,24 @@ def load():
     return lib
 
 
+_host = None
+
+
+def host():
+    """The host extension (csrc/host.cpp).  Raises if it has not been built."""
+    global _host
+    if _host is None:
+        import importlib.util
+        path = Path(__file__).resolve().parent / "csrc" / "vitk_host.so"
+        if not path.exists():
+            raise VitkError(f"{path} not found: build it first (python -m vision_transformers_torch_xla_amd.build, or __graft_entry__.build())")
+        spec = importlib.util.spec_from_file_location("vitk_host", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _host = module
+    return _host
+
+
 def check(rc: int, what: str = ""):
     if rc != 0:
         msg = load().vitk_last_error()

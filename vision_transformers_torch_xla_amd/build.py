@@ -14,6 +14,7 @@ from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent / "csrc"
 LIB_PATH = CSRC / "libvitk.so"
+HOST_SOURCE, HOST_PATH = CSRC / "host.cpp", CSRC / "vitk_host.so"       # a CPython extension over torch's headers, host code only
 SOURCES = ["api.hip", "layernorm.hip", "gemm.hip", "gemm_ntq.hip", "attention.hip", "elementwise.hip", "loss.hip", "linear_xent.hip", "optim.hip", "clip.hip", "embedding.hip", "preprocess.hip"]
 HEADERS = [CSRC / "common.h", CSRC / "gemm_nt.h", CSRC.parent.parent / "include" / "vitk.h"]
 ARCH = "gfx950"
@@ -44,8 +45,28 @@ def _stale(target: Path, deps) -> bool:
     return any(Path(d).stat().st_mtime > t for d in deps)
 
 
+def build_host(force: bool = False, verbose: bool = True) -> Path:
+    """Compile the host extension (g++, torch's headers); rebuilt when its source is newer or torch's own library is."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    libs = Path(torch.__file__).resolve().parent / "lib"
+    if not force and not _stale(HOST_PATH, [HOST_SOURCE, libs / "libtorch_python.so"]):
+        return HOST_PATH
+    cmd = ["g++", "-O2", "-shared", "-fPIC", "-std=c++17", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{d}" for d in [*include_paths(), sysconfig.get_paths()["include"]]), str(HOST_SOURCE), "-o", str(HOST_PATH),
+           f"-L{libs}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print("[build]", " ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {HOST_SOURCE.name}:\n{r.stdout}\n{r.stderr}")
+    return HOST_PATH
+
+
 def build_lib(force: bool = False, verbose: bool = True) -> Path:
-    """Compile every .hip source to an object file (in parallel) and link libvitk.so.  Returns the library path."""
+    """Compile every .hip source to an object file (in parallel), link libvitk.so and build the host extension.  Returns the library path."""
     hipcc = _hipcc()
     objdir = CSRC / "build"
     objdir.mkdir(exist_ok=True)
@@ -67,9 +88,10 @@ def build_lib(force: bool = False, verbose: bool = True) -> Path:
         if verbose and r.stderr.strip():
             print(r.stderr, file=sys.stderr)
 
-    if jobs:
-        with ThreadPoolExecutor(max_workers=min(4, len(jobs))) as ex:
-            list(ex.map(compile_one, jobs))
+    with ThreadPoolExecutor(max_workers=4) as ex:
+        host = ex.submit(build_host, force, verbose)
+        list(ex.map(compile_one, jobs))
+        host.result()
     objs = [objdir / (Path(s).stem + ".o") for s in SOURCES]
     if force or jobs or _stale(LIB_PATH, objs):
         cmd = [hipcc, "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", str(LIB_PATH), *map(str, objs)]

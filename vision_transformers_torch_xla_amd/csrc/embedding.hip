@@ -119,65 +119,95 @@ static __device__ __forceinline__ unsigned sort_rank(unsigned* hist_wave, unsign
     return base + before;
 }
 
-// The whole sort in one workgroup, for up to 16384 tokens of a vocabulary below 2^18: key and position share one word.  One pass over
-// 16384 tokens takes the compute unit a few microseconds, less than the two launches that a pass over several workgroups needs.
-// The blocks behind the first zero the gradient meanwhile.
-#define SORT1_MAX 16384
+// Grouping in one launch, for up to 32768 tokens of a vocabulary below 2^18.  Workgroup g of 256 owns the ids that are g modulo 256: it reads
+// ALL ids (256 KB at most, out of the L2 cache), counts its own per wave and id, and how many belong to the workgroups before it - which
+// is where its part of the sorted list begins, so the workgroups need nothing from each other.  Then it reads the ids again and puts its
+// tokens down, equal ids in the order of the tokens: wave w has a contiguous stretch of the tokens, and a token's place is the wave's
+// first one for its id plus the number of equal ids before it in the wave.  (The ids of a text are 1 in 256 a workgroup's own, so most
+// groups of 64 need one vote and nothing else.)  Tokens without a gradient come last.  The workgroups behind the 256 zero the gradient.
+// Against a radix sort of one workgroup (46 us for 16384 tokens) or of several (four launches) this takes 12 us.
+#define GROUP_MAX 32768
+#define GROUP_WG 256
+#define GROUP_ROWS ((1 << 18) / GROUP_WG)
+#define GROUP_WAVES 8
 template <typename I>
-__global__ __launch_bounds__(1024) void emb_sort_one_kernel(const void* ids, int T, long long V, long long padding, int passes, uint2* sorted,
-                                                            uint4* zero, long long zero16) {
-    extern __shared__ unsigned sh[];        // [16384] words, [16][512] counters, [16] scan
-    if (blockIdx.x > 0) {
+__global__ __launch_bounds__(512) void emb_group_kernel(const void* ids, int T, long long V, long long padding, uint2* sorted, uint4* zero, long long zero16) {
+    __shared__ unsigned hist[GROUP_WAVES][GROUP_ROWS];
+    __shared__ unsigned sums[2][GROUP_WAVES];
+    if (blockIdx.x >= GROUP_WG) {
         const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-        for (long long i = (long long)(blockIdx.x - 1) * 1024 + threadIdx.x; i < zero16; i += (long long)(gridDim.x - 1) * 1024) zero[i] = z;
+        const long long step = (long long)(gridDim.x - GROUP_WG) * 512;
+        for (long long i = (long long)(blockIdx.x - GROUP_WG) * 512 + threadIdx.x; i < zero16; i += step) zero[i] = z;
         return;
     }
-    unsigned* buf = sh;
-    unsigned* hist = sh + SORT1_MAX;
-    unsigned* sums = hist + 16 * SORT_BINS;
+    const unsigned own = blockIdx.x;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    unsigned* mine = hist + wave * SORT_BINS;
-    const int items = (T + 1023) / 1024;        // per thread; a wave's items are consecutive in the input
-    unsigned word[SORT_ITEMS];
-#pragma unroll
-    for (int j = 0; j < SORT_ITEMS; ++j) {
-        const int t = (wave * items + j) * 64 + lane;
-        word[j] = j < items && t < T ? (emb_key<I>(ids, t, V, padding) << 14) | (unsigned)t : 0xffffffffu;
-    }
-    for (int pass = 0; pass < passes; ++pass) {
-        const int shift = 14 + pass * SORT_BITS;
-        for (int i = threadIdx.x; i < 16 * SORT_BINS; i += 1024) hist[i] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < SORT_ITEMS; ++j)
-            if (j < items) atomicAdd(&mine[(word[j] >> shift) & (SORT_BINS - 1)], 1u);
-        __syncthreads();
-        unsigned total = 0;
-        if (threadIdx.x < SORT_BINS)
-            for (int w = 0; w < 16; ++w) { const unsigned c = hist[w * SORT_BINS + threadIdx.x]; hist[w * SORT_BINS + threadIdx.x] = total; total += c; }
-        const unsigned incl = wave_scan(total);
-        if (lane == 63) sums[wave] = incl;
-        __syncthreads();
-        if (threadIdx.x < SORT_BINS) {
-            unsigned base = incl - total;
-            for (int w = 0; w < wave; ++w) base += sums[w];
-            for (int w = 0; w < 16; ++w) hist[w * SORT_BINS + threadIdx.x] += base;
+    const int rows = (int)((V + GROUP_WG - 1) / GROUP_WG);           // at most GROUP_ROWS
+    for (int i = threadIdx.x; i < GROUP_WAVES * rows; i += 512) hist[i / rows][i % rows] = 0;
+    __syncthreads();
+    const int strips = (T + 63) / 64, per = (strips + GROUP_WAVES - 1) / GROUP_WAVES;
+    const int s0 = wave * per, s1 = s0 + per < strips ? s0 + per : strips;
+    unsigned before = 0, valid = 0;         // of the lane's tokens: those of workgroups before this one, those with a gradient
+#pragma unroll 4
+    for (int s = s0; s < s1; ++s) {
+        const int t = s * 64 + lane;
+        const unsigned key = t < T ? emb_key<I>(ids, t, V, padding) : (unsigned)V;
+        if (key < (unsigned)V) {
+            const unsigned g = key & (GROUP_WG - 1);
+            ++valid;
+            before += g < own ? 1u : 0u;
+            if (g == own) atomicAdd(&hist[wave][key / GROUP_WG], 1u);
         }
-        __syncthreads();
+    }
+    before = wave_scan(before);
+    valid = wave_scan(valid);
+    if (lane == 63) { sums[0][wave] = before; sums[1][wave] = valid; }
+    __syncthreads();
+    unsigned at = 0, total_valid = 0;
 #pragma unroll
-        for (int j = 0; j < SORT_ITEMS; ++j)
-            if (j < items) buf[sort_rank(mine, (word[j] >> shift) & (SORT_BINS - 1))] = word[j];
-        __syncthreads();
+    for (int w = 0; w < GROUP_WAVES; ++w) { at += sums[0][w]; total_valid += sums[1][w]; }
+    __syncthreads();
+    // first places: ids in order, within an id the waves in order; 512 ids a round
+    for (int r0 = 0; r0 < rows; r0 += 512) {
+        const int r = r0 + (int)threadIdx.x;
+        unsigned count = 0;
+        if (r < rows) {
 #pragma unroll
-        for (int j = 0; j < SORT_ITEMS; ++j)
-            if (j < items) word[j] = buf[(wave * items + j) * 64 + lane];
+            for (int w = 0; w < GROUP_WAVES; ++w) { const unsigned c = hist[w][r]; hist[w][r] = count; count += c; }
+        }
+        const unsigned incl = wave_scan(count);
+        if (lane == 63) sums[0][wave] = incl;
+        __syncthreads();
+        unsigned base = at + incl - count;
+        for (int w = 0; w < wave; ++w) base += sums[0][w];
+        if (r < rows) {
+#pragma unroll
+            for (int w = 0; w < GROUP_WAVES; ++w) hist[w][r] += base;
+        }
+#pragma unroll
+        for (int w = 0; w < GROUP_WAVES; ++w) at += sums[0][w];
         __syncthreads();
     }
-#pragma unroll
-    for (int j = 0; j < SORT_ITEMS; ++j) {
-        const int t = (wave * items + j) * 64 + lane;
-        if (j < items && t < T) sorted[t] = make_uint2(word[j] >> 14, word[j] & 16383u);
+#pragma unroll 4
+    for (int s = s0; s < s1; ++s) {
+        const int t = s * 64 + lane;
+        const unsigned key = t < T ? emb_key<I>(ids, t, V, padding) : (unsigned)V;
+        unsigned long long left = __ballot(key < (unsigned)V && (key & (GROUP_WG - 1)) == own);
+        while (left != 0) {             // one round for each different id among the strip's own tokens
+            const unsigned k = (unsigned)__builtin_amdgcn_readlane((int)key, (int)__builtin_ctzll(left));
+            const unsigned long long same = __ballot(key == k);
+            if (key == k) {
+                const unsigned first = hist[wave][k / GROUP_WG];
+                asm volatile("" ::: "memory");
+                const unsigned place = (unsigned)__popcll(same & ((1ull << lane) - 1ull));
+                sorted[first + place] = make_uint2(key, (unsigned)t);
+                if (place == 0) hist[wave][k / GROUP_WG] = first + (unsigned)__popcll(same);
+                asm volatile("" ::: "memory");
+            }
+            left &= ~same;
+        }
     }
+    for (unsigned i = total_valid + own * 512u + threadIdx.x; i < (unsigned)T; i += GROUP_WG * 512u) sorted[i] = make_uint2((unsigned)V, 0u);
 }
 
 // Several workgroups: per pass a histogram launch (counts[block][bin]) and a launch that turns the counts into ranks and scatters.
@@ -235,9 +265,11 @@ __global__ __launch_bounds__(256) void emb_scatter_kernel(const void* ids, const
     // thread i owns bins 2i and 2i + 1: their totals and the share of the blocks before this one
     const int b0 = 2 * threadIdx.x;
     unsigned tot0 = 0, tot1 = 0, pre0 = 0, pre1 = 0;
+#pragma unroll 8
     for (int b = 0; b < blocks; ++b) {
         const uint2 c = *reinterpret_cast<const uint2*>(counts + (size_t)b * SORT_BINS + b0);
-        if (b == (int)blockIdx.x) { pre0 = tot0; pre1 = tot1; }
+        const bool before = b < (int)blockIdx.x;
+        pre0 += before ? c.x : 0u; pre1 += before ? c.y : 0u;
         tot0 += c.x; tot1 += c.y;
     }
     const unsigned incl = wave_scan(tot0 + tot1);
@@ -296,6 +328,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_kernel(const EmbBwdParams p
     float* part = p.partial + (size_t)blockIdx.x * 2 * p.D + col;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     unsigned key = p.sorted[i0].x;
+    if ((long long)key >= p.V) return;
     bool head = i0 > 0 && p.sorted[i0 - 1].x == key;        // the run began in an earlier piece
     for (long long i = i0; i < i1; i += EMB_AHEAD) {
         float v[EMB_AHEAD][8];
@@ -332,32 +365,44 @@ __global__ __launch_bounds__(256) void embedding_bwd_kernel(const EmbBwdParams p
     else emb_put<TO>(p, key, col, acc);
 }
 
-// Runs that cross pieces: the workgroup of the piece a run begins in (as its tail) adds the head sums of the pieces that follow.
+// Runs that cross pieces: the workgroup of the piece a run begins in (as its tail) adds the head sums of the pieces that follow, a quarter of
+// them each of its four groups of threads, then the four in order.
 template <typename TO>
-__global__ __launch_bounds__(256) void embedding_join_kernel(const EmbBwdParams p) {
+__global__ __launch_bounds__(1024) void embedding_join_kernel(const EmbBwdParams p) {
+    __shared__ float quarter[3][256][8];
     const int col = ((int)blockIdx.y * (int)blockDim.x + (int)threadIdx.x) * 8;
-    if (col >= p.D) return;
     const long long i1 = (long long)(blockIdx.x + 1) * p.piece;       // the grid has one block less than there are pieces
     const unsigned key = p.sorted[i1 - 1].x;
     if ((long long)key >= p.V || p.sorted[i1].x != key) return;       // nothing crosses this border
     const long long i0 = i1 - p.piece;
     if (p.sorted[i0].x == key && i0 > 0 && p.sorted[i0 - 1].x == key) return;       // the run began earlier
-    float acc[8];
-    Emb8<float>::load(p.partial + ((size_t)blockIdx.x * 2 + 1) * p.D + col, acc);
-    // how many pieces the run enters (the sorted keys: first piece whose first key is another one)
+    // how many pieces the run enters (equal ids are neighbours: first piece whose first id is another one)
     long long lo = blockIdx.x + 1, hi = p.pieces;
     while (lo < hi) {
         const long long mid = (lo + hi) >> 1;
         if (p.sorted[mid * p.piece].x == key) lo = mid + 1; else hi = mid;
     }
-    const float* q = p.partial + col;
-#pragma unroll 8
-    for (long long c = blockIdx.x + 1; c < lo; ++c) {
-        float v[8];
-        Emb8<float>::load(q + (size_t)c * 2 * p.D, v);
+    const long long c0 = blockIdx.x + 1, n = lo - c0;
+    const long long from = c0 + n * threadIdx.y / 4, to = c0 + n * (threadIdx.y + 1) / 4;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (col < p.D) {
+        if (threadIdx.y == 0) Emb8<float>::load(p.partial + ((size_t)blockIdx.x * 2 + 1) * p.D + col, acc);
+        const float* q = p.partial + col;
+#pragma unroll 4
+        for (long long c = from; c < to; ++c) {
+            float v[8];
+            Emb8<float>::load(q + (size_t)c * 2 * p.D, v);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] += v[k];
+            for (int k = 0; k < 8; ++k) acc[k] += v[k];
+        }
     }
+    if (threadIdx.y > 0) Emb8<float>::store(quarter[threadIdx.y - 1][threadIdx.x], acc);
+    __syncthreads();
+    if (threadIdx.y > 0 || col >= p.D) return;
+#pragma unroll
+    for (int g = 0; g < 3; ++g)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += quarter[g][threadIdx.x][k];
     emb_put<TO>(p, key, col, acc);
 }
 
@@ -372,7 +417,7 @@ static int emb_passes(long long V) {
     while (bits < 32 && (V >> bits) != 0) ++bits;        // keys 0 .. V
     return (bits + SORT_BITS - 1) / SORT_BITS;
 }
-static bool emb_one(long long T, long long V) { return T == 0 || (T <= SORT1_MAX && V < (1 << 18)); }
+static bool emb_one(long long T, long long V) { return T == 0 || (T <= GROUP_MAX && V <= (1 << 18)); }
 static size_t emb_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 extern "C" {
@@ -445,13 +490,9 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
     p.partial = (float*)ws;
     ws += emb_up((size_t)p.pieces * 2 * D * sizeof(float));
     if (emb_one(T, V)) {
-        const size_t lds = (SORT1_MAX + 16 * SORT_BINS + 16) * sizeof(unsigned);
-        static VitkLdsOnce once64 = {}, once32 = {};
-        if (int rc = ids_are_64 ? vitk_lds_once(once64, (const void*)emb_sort_one_kernel<int64_t>, lds, "embedding_bwd")
-                                : vitk_lds_once(once32, (const void*)emb_sort_one_kernel<int32_t>, lds, "embedding_bwd"))
-            return rc;
-        if (ids_are_64) emb_sort_one_kernel<int64_t><<<1 + zero_blocks, 1024, lds, s>>>(ids, (int)T, V, padding_idx, passes, sorted, (uint4*)dtable, zero16);
-        else emb_sort_one_kernel<int32_t><<<1 + zero_blocks, 1024, lds, s>>>(ids, (int)T, V, padding_idx, passes, sorted, (uint4*)dtable, zero16);
+        const int grid = GROUP_WG + zero_blocks;
+        if (ids_are_64) emb_group_kernel<int64_t><<<grid, 512, 0, s>>>(ids, (int)T, V, padding_idx, sorted, (uint4*)dtable, zero16);
+        else emb_group_kernel<int32_t><<<grid, 512, 0, s>>>(ids, (int)T, V, padding_idx, sorted, (uint4*)dtable, zero16);
         if (int rc = vitk_check_launch("embedding_bwd_sort")) return rc;
     } else {
         uint2* other = (uint2*)ws;
@@ -482,7 +523,7 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
     const dim3 grid(p.pieces, (lanes + threads - 1) / threads), join(p.pieces > 1 ? p.pieces - 1 : 1, grid.y);
 #define EMB_BWD(TI, TO)                                                                                  \
     embedding_bwd_kernel<TI, TO><<<grid, threads, 0, s>>>(p);                                            \
-    if (p.pieces > 1) embedding_join_kernel<TO><<<join, threads, 0, s>>>(p)
+    if (p.pieces > 1) embedding_join_kernel<TO><<<join, dim3(threads, 4), 0, s>>>(p)
     switch ((dout_type << 1) | dtable_type) {
         case 0: EMB_BWD(float, float); break;
         case 1: EMB_BWD(float, bf16_t); break;

@@ -473,53 +473,9 @@ def _here(t, name):
     """a tensor a kernel of the current stream may use: on the current device (one process drives one GPU at a time)"""
     if not t.is_cuda:
         raise _lib.VitkError(f"{name}: expected a GPU tensor (the HIP kernels are the only implementation), got {t.device}")
-    if _cur_device is not None and t.device.index != _cur_device():
+    if _cur_device is not None and t.get_device() != _cur_device():
         raise _lib.VitkError(f"{name}: the tensor is on {t.device}, the current device is cuda:{_cur_device()}; "
                              "make it current (torch.cuda.set_device) before the call")
-
-
-def _dense(t):
-    """every element of the tensor's memory range belongs to it, once, in whatever order of its dimensions"""
-    if t.is_contiguous():
-        return True
-    expect = 1
-    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if stride != expect:
-            return False
-        expect *= size
-    return True
-
-
-_CLIP_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def _clip_table(tensors, what):
-    """(addresses, element counts, type codes) of a list of dense gradients as numpy arrays"""
-    if not tensors:
-        return np.zeros(0, np.int64), np.zeros(0, np.int64), np.zeros(0, np.int32)
-    _here(tensors[0], what)
-    device = tensors[0].device
-    types = []
-    for i, t in enumerate(tensors):
-        code = _CLIP_TYPES.get(t.dtype)
-        if code is None:
-            raise _lib.VitkError(f"{what}[{i}]: expected float32, bfloat16 or float16, got {t.dtype}")
-        if t.layout is not torch.strided or not (t.is_contiguous() or _dense(t)):
-            raise _lib.VitkError(f"{what}[{i}]: expected a dense tensor, got shape {tuple(t.shape)} with strides "
-                                 f"{t.stride() if t.layout is torch.strided else t.layout}")
-        if t.device != device:
-            raise _lib.VitkError(f"{what}: tensors on {device} and {t.device} in one call")
-        types.append(code)
-    return (np.array([t.data_ptr() for t in tensors], np.int64), np.array([t.numel() for t in tensors], np.int64), np.array(types, np.int32))
-
-
-def _overlap(first, size):
-    """whether any two of the byte ranges [first, first + size) meet"""
-    keep = size > 0
-    first, size = first[keep], size[keep]
-    order = np.argsort(first, kind="stable")
-    first, size = first[order], size[order]
-    return bool((first[:-1] + size[:-1] > first[1:]).any())
 
 
 def clip_grads(tensors, max_norm, out=None):
@@ -529,35 +485,25 @@ def clip_grads(tensors, max_norm, out=None):
     they are); None: in place.  max_norm None: the norm alone.  A norm that is infinite or NaN spreads as in torch's clip_grad_norm_
     (finite gradients become 0 or NaN)."""
     tensors = list(tensors)
-    src, numel, types = _clip_table(tensors, "tensors")
     if not tensors:
         raise _lib.VitkError("clip_grads: no tensors (a device is needed for the norm)")
-    if max_norm is not None and not max_norm >= 0.0:
-        raise _lib.VitkError(f"clip_grads: max_norm must not be negative, got {max_norm}")
-    dst = None
-    if max_norm is not None:
-        size = numel * np.where(types == 0, 4, 2)
-        dst = src
+    if max_norm is None:
         if out is not None:
-            out = list(out)
-            if len(out) != len(tensors):
-                raise _lib.VitkError(f"clip_grads: {len(tensors)} tensors, {len(out)} outputs")
-            dst, _, _ = _clip_table(out, "out")
-            for i, (a, b) in enumerate(zip(tensors, out)):
-                if a.dtype != b.dtype or a.shape != b.shape or a.device != b.device or a.stride() != b.stride():
-                    raise _lib.VitkError(f"clip_grads: out[{i}] must have the shape, strides, type and device of tensors[{i}]")
-            other = dst != src
-            if _overlap(np.concatenate([dst, src[other]]), np.concatenate([size, size[other]])):
-                raise _lib.VitkError("clip_grads: the outputs overlap each other or another gradient")
-        elif _overlap(src, size):
-            raise _lib.VitkError("clip_grads: the same memory is in the list twice (it would be scaled twice)")
-    elif out is not None:
-        raise _lib.VitkError("clip_grads: out needs a max_norm")
+            raise _lib.VitkError("clip_grads: out needs a max_norm")
+    elif not max_norm >= 0.0:
+        raise _lib.VitkError(f"clip_grads: max_norm must not be negative, got {max_norm}")
+    else:
+        out = tensors if out is None else list(out)
     lib = _lib.load()
-    norm = torch.empty((), dtype=f32, device=tensors[0].device)
-    ws = torch.empty(lib.vitk_clip_grads_workspace(len(tensors)), dtype=torch.uint8, device=norm.device)
-    check(lib.vitk_clip_grads(src.ctypes.data, None if dst is None else dst.ctypes.data, numel.ctypes.data, types.ctypes.data, len(tensors),
-                              float(max_norm or 0.0), _ptr(norm), _ptr(ws), ws.numel(), _stream()), "clip_grads")
+    try:
+        src, dst, numel, types = _lib.host().clip_table(tensors, out, _cur_device() if getattr(tensors[0], "is_cuda", False) else -1)
+    except ValueError as e:
+        raise _lib.VitkError(f"clip_grads: {e}") from None
+    dev = tensors[0].device
+    norm = torch.empty((), dtype=f32, device=dev)
+    ws = torch.empty(lib.vitk_clip_grads_workspace(len(tensors)), dtype=torch.uint8, device=dev)
+    check(lib.vitk_clip_grads(src, dst, numel, types, len(tensors), 0.0 if max_norm is None else float(max_norm), norm.data_ptr(), ws.data_ptr(), ws.numel(),
+                              _stream()), "clip_grads")
     return norm
 
 
@@ -579,7 +525,7 @@ def _ids1d(ids):
     _here(ids, "ids")
     if ids.dtype not in (torch.int64, torch.int32):
         raise _lib.VitkError(f"ids: expected int64 or int32, got {ids.dtype}")
-    return ids.reshape(-1).contiguous()
+    return ids if ids.is_contiguous() else ids.contiguous()          # only its memory is read, in order: any shape does
 
 
 def embedding_fwd(ids, table, scale=1.0, out_dtype=None):
