@@ -212,7 +212,7 @@ EMB_IDS = {
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,V,D", [(1, 1, 8), (1, 1000, 768), (63, 2, 8), (65, 511, 72), (1025, 512, 64), (2049, 513, 200), (16384, 20000, 64), (16385, 700, 64),
-                                   (5000, 262143, 16), (5000, 262144, 16), (40000, 300, 2064), (300000, 5000, 8)])
+                                   (5000, 262143, 16), (5000, 262144, 16), (5000, 262145, 16), (40000, 300, 2064), (300000, 5000, 8)])
 @pytest.mark.parametrize("kind", list(EMB_IDS))
 def test_embedding_bwd(device, T, V, D, kind):
     ops = _ops()
@@ -533,6 +533,181 @@ def test_linear_xent_refuses(device):
                  lambda: ops.linear_xent(x[:, ::2], w[:, ::2], t), lambda: ops.linear_xent(x[:, 1:9], w[:, 1:9], t), lambda: ops.linear_xent(x, w[:0], t)):
         with pytest.raises(err):
             call()
+
+
+# --------------------------------------------------------------------------------------- modules and the path
+def close(got, want, rel):
+    got, want = got.detach().double().cpu(), want.double()
+    return float((got - want).norm() / want.norm()) <= rel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wtype", [f32, bf16])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_linear_cross_entropy_module(device, wtype, reduction):
+    from vision_transformers_torch_xla_amd.losses import LinearCrossEntropy
+    g = torch.Generator().manual_seed(3)
+    torch.manual_seed(3)
+    m = LinearCrossEntropy(64, 211, smoothing=0.1, ignore_index=-1, reduction=reduction).to(device)
+    assert m.weight.dtype == f32 and m.weight.std() < 0.03 and torch.all(m.bias == 0)
+    with torch.no_grad():
+        m.weight.copy_(torch.randn(211, 64, generator=g) * 0.3)
+        m.bias.copy_(torch.randn(211, generator=g))
+    m = m.to(wtype)
+    x = torch.randn(6, 20, 64, generator=g).to(device, bf16).requires_grad_(True)
+    t = torch.randint(-1, 211, (6, 20), generator=g)
+    loss = m(x, t.to(device))
+    (3.0 * loss).backward()
+    (want, _, dx, dw, db), (lt, _, dxt, dwt, dbt) = plain_linear_xent(x.detach().cpu().view(-1, 64), m.weight.detach().to(bf16).cpu(), t.view(-1),
+                                                                     m.bias.detach().cpu(), 0.1, -1, reduction == "mean")
+    assert abs(loss.item() - want) <= lt + U32 * abs(want)
+    for got, v, tol in ((x.grad.view(-1, 64), dx, dxt), (m.weight.grad, dw, dwt), (m.bias.grad, db, dbt)):
+        # the gradient and its product with the upstream 3 are rounded to the type
+        assert torch.all((got.cpu().double() - 3 * v).abs() <= 3 * (tol + 2.02 * half_ulp(got.dtype) * (v.abs() + tol) + 1e-38))
+        assert got.dtype == (bf16 if got.shape == x.grad.view(-1, 64).shape and got.data_ptr() == x.grad.data_ptr() else wtype)
+    with torch.no_grad():
+        assert torch.equal(m(x, t.to(device)), loss)
+    again = m(x, t.to(device))
+    again.backward(retain_graph=True)
+    with pytest.raises(_error(), match="second time"):
+        again.backward()
+
+
+@pytest.mark.gpu
+def test_token_embedding_module(device):
+    from vision_transformers_torch_xla_amd.embedding import TokenEmbedding
+    torch.manual_seed(4)
+    m = TokenEmbedding(50, 16, scale=4.0, padding_idx=-1).to(device)
+    assert torch.all(m.weight[49] == 0)
+    with torch.no_grad():
+        m.weight[49] = 1.0
+    ids = torch.randint(0, 50, (7, 30), device=device)
+    ids[0] = 49
+    out = m(ids)
+    assert out.dtype == bf16 and torch.equal(out, (m.weight.detach()[ids] * 4.0).to(bf16))
+    up = torch.randn(7, 30, 16, device=device).to(bf16)
+    out.backward(up)
+    check_embedding_grad(m.weight.grad, up.cpu(), ids.cpu(), 50, 4.0, 49)
+    assert torch.all(m.weight.grad[49] == 0)
+    # a gradient that is one broadcast row
+    m.weight.grad = None
+    m(ids).sum().backward()
+    check_embedding_grad(m.weight.grad, torch.ones(7, 30, 16), ids.cpu(), 50, 4.0, 49)
+
+
+def test_module_arguments_are_checked():
+    from vision_transformers_torch_xla_amd.embedding import TokenEmbedding, embedding
+    from vision_transformers_torch_xla_amd.losses import LinearCrossEntropy, linear_cross_entropy
+    err = _error()
+    w, i = torch.zeros(8, 16), torch.zeros(3, dtype=torch.int64)
+    for call in (lambda: TokenEmbedding(0, 16), lambda: TokenEmbedding(8, 12), lambda: TokenEmbedding(8, 16, padding_idx=8),
+                 lambda: embedding(i, w, padding_idx=-9), lambda: embedding(i, w), lambda: LinearCrossEntropy(12, 8), lambda: LinearCrossEntropy(16, 0),
+                 lambda: LinearCrossEntropy(16, 8, smoothing=2.0), lambda: LinearCrossEntropy(16, 8, reduction="none"),
+                 lambda: linear_cross_entropy(torch.zeros(3, 16), w, i), lambda: linear_cross_entropy(torch.zeros(2, 16), w, i),
+                 lambda: linear_cross_entropy(torch.zeros(3, 16, dtype=f64), w, i)):
+        with pytest.raises(err):
+            call()
+
+
+@pytest.mark.gpu
+def test_lookup_loss_clip_and_step_together(device):
+    """one training step of the smallest model that has all of it: tokens -> table -> the same table as the head -> loss, the two gradients of
+    the shared table, their common norm with a second parameter, the clipped step of the fused AdamW"""
+    from vision_transformers_torch_xla_amd import engine, ops
+    from vision_transformers_torch_xla_amd.embedding import embedding
+    from vision_transformers_torch_xla_amd.losses import linear_cross_entropy
+    g = torch.Generator().manual_seed(12)
+    V, D, T = 300, 64, 500
+    table = (torch.randn(V, D, generator=g) * 0.3).to(bf16).float()          # bf16 values, so that the plain form has the same products
+    gain = torch.ones(D) * 1.5
+    ids, target = torch.randint(0, V, (T,), generator=g), torch.randint(0, V, (T,), generator=g)
+    target[::5] = -100
+
+    p, q = torch.nn.Parameter(table.to(device)), torch.nn.Parameter(gain.to(device))
+    x = embedding(ids.to(device), p, scale=2.0) * q                            # bf16 * fp32 -> fp32
+    loss = linear_cross_entropy(x, p, target.to(device))
+    loss.backward()
+    norm = engine.clip_grad_norm_([p, [q], p], 0.05)                            # p is reached twice and counts once
+
+    P, Q = table.double().requires_grad_(True), gain.double().requires_grad_(True)
+    X = P[ids] * 2.0 * Q
+    keep = target >= 0
+    L = torch.nn.functional.cross_entropy(X[keep] @ P.t(), target[keep])
+    L.backward()
+    N = torch.sqrt(P.grad.pow(2).sum() + Q.grad.pow(2).sum())
+    # x is rounded to bf16 before the products, its gradient and the loss factor too: three roundings of 2^-8 at most, incoherent
+    tol = 3 * 2.0 ** -8
+    assert abs(loss.item() - L.item()) <= 2 * 2.0 ** -8 * abs(L.item())
+    assert abs(norm.item() / N.item() - 1) <= tol and N > 0.05
+    coef = 0.05 / (N + 1e-6)
+    assert close(p.grad, P.grad * coef, 2 * tol) and close(q.grad, Q.grad * coef, 2 * tol)
+    clipped = math.sqrt(float(p.grad.double().pow(2).sum() + q.grad.double().pow(2).sum()))
+    assert abs(clipped / 0.05 - 1) <= 1e-4
+    m, v = torch.zeros_like(p.data), torch.zeros_like(p.data)
+    before, grad = p.data.clone(), p.grad.clone()
+    ops.adamw_step(p.data, grad, m, v, lr=0.1, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, step=1)
+    # the first step moves every weight with a gradient by lr against its sign
+    big = grad.abs() > 1e-6
+    assert torch.all((p.data - before)[big].sign() == -grad.sign()[big])
+
+
+@pytest.mark.gpu
+def test_clip_grad_norm_takes_modules_and_parameters(device):
+    from vision_transformers_torch_xla_amd import engine
+    from vision_transformers_torch_xla_amd.vit import create_model
+    torch.manual_seed(5)
+    lin = torch.nn.Linear(24, 40).to(device)
+    other = torch.nn.Parameter(torch.zeros(33, device=device, dtype=bf16))
+    unused = torch.nn.Parameter(torch.zeros(5, device=device))
+    for t in (lin.weight, lin.bias, other):
+        t.grad = torch.randn_like(t)
+    want = [t.grad.double().cpu() for t in (lin.weight, lin.bias, other)]
+    norm, clipped = plain_clip(want, 0.7)
+    got = engine.clip_grad_norm_((lin, other, unused), 0.7)
+    assert abs(got.item() - norm) <= 2 * U32 * norm
+    check_clipped([lin.weight.grad, lin.bias.grad, other.grad], clipped)
+    assert engine.clip_grad_norm_(unused, 1.0).item() == 0.0
+    # a flat-buffer model beside a head with parameters of its own
+    model = create_model("vit_tiny_patch16_224", num_classes=8, depth=1).to(device)
+    flat = model._ensure_grad_buffer()
+    flat.copy_(torch.randn(flat.shape, device=device))
+    lin.weight.grad, lin.bias.grad = torch.randn_like(lin.weight), torch.randn_like(lin.bias)
+    norm, clipped = plain_clip([flat.cpu(), lin.weight.grad.cpu(), lin.bias.grad.cpu()], 1.0)
+    assert abs(engine.clip_grad_norm_([model, lin], 1.0).item() / norm - 1) <= 2 * U32
+    check_clipped([flat, lin.weight.grad, lin.bias.grad], clipped)
+
+
+@pytest.mark.gpu
+def test_train_one_epoch_with_a_criterion_that_holds_the_head(device):
+    from vision_transformers_torch_xla_amd import engine
+    from vision_transformers_torch_xla_amd.embedding import TokenEmbedding
+    from vision_transformers_torch_xla_amd.losses import LinearCrossEntropy
+    torch.manual_seed(6)
+    model, criterion = TokenEmbedding(100, 32).to(device), LinearCrossEntropy(32, 100).to(device)
+    with torch.no_grad():
+        model.weight.mul_(20)
+        criterion.weight.mul_(20)
+    opt = torch.optim.SGD([*model.parameters(), *criterion.parameters()], lr=0.5)
+    data = [(torch.randint(0, 100, (64,)), torch.randint(0, 100, (64,))) for _ in range(3)]
+    want_model, want_head = model.weight.detach().double().cpu(), criterion.weight.detach().double().cpu()
+    bias = torch.zeros(100, dtype=f64)
+    losses = []
+    for ids, t in data:
+        a, w, b = want_model.clone().requires_grad_(True), want_head.clone().requires_grad_(True), bias.clone().requires_grad_(True)
+        loss = torch.nn.functional.cross_entropy(a[ids] @ w.t() + b, t)
+        loss.backward()
+        norm = math.sqrt(sum(float(v.grad.pow(2).sum()) for v in (a, w, b)))
+        c = min(1.0, 0.1 / (norm + 1e-6))
+        assert c < 1.0
+        want_model, want_head, bias = (v.detach() - 0.5 * c * v.grad for v in (a, w, b))
+        losses.append(loss.item())
+    start = model.weight.detach().double().cpu()
+    stats = engine.train_one_epoch(model, criterion, data, opt, device, 0, max_norm=0.1)
+    assert "class_acc" not in stats and abs(stats["loss"] - sum(losses) / 3) <= 2 * 2.0 ** -8 * sum(losses) / 3
+    # the weights have moved by three clipped steps of 0.05 in all; a step is off by a few roundings of 2^-8
+    assert float((model.weight.detach().double().cpu() - want_model).norm()) <= 3 * 0.05 * 6 * 2.0 ** -8
+    assert float((criterion.weight.detach().double().cpu() - want_head).norm()) <= 3 * 0.05 * 6 * 2.0 ** -8
+    assert float((want_model - start).norm()) > 0.01
 
 
 # --------------------------------------------------------------------------------------- checks without a GPU

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const EmbFwdParams p
 // of range); it sorts behind every row.
 #define SORT_BINS 512
 #define SORT_BITS 9
-#define SORT_ITEMS 16
+#define SORT_ITEMS 8            // (16: the four launches take 39 us for 100352 tokens, 8: 29 us, 4: 30 us)
 
 template <typename I>
 static __device__ __forceinline__ unsigned emb_key(const void* ids, long long t, long long V, long long padding) {
@@ -119,95 +119,121 @@ static __device__ __forceinline__ unsigned sort_rank(unsigned* hist_wave, unsign
     return base + before;
 }
 
-// Grouping in one launch, for up to 32768 tokens of a vocabulary below 2^18.  Workgroup g of 256 owns the ids that are g modulo 256: it reads
-// ALL ids (256 KB at most, out of the L2 cache), counts its own per wave and id, and how many belong to the workgroups before it - which
-// is where its part of the sorted list begins, so the workgroups need nothing from each other.  Then it reads the ids again and puts its
-// tokens down, equal ids in the order of the tokens: wave w has a contiguous stretch of the tokens, and a token's place is the wave's
-// first one for its id plus the number of equal ids before it in the wave.  (The ids of a text are 1 in 256 a workgroup's own, so most
-// groups of 64 need one vote and nothing else.)  Tokens without a gradient come last.  The workgroups behind the 256 zero the gradient.
-// Against a radix sort of one workgroup (46 us for 16384 tokens) or of several (four launches) this takes 12 us.
+// Grouping in one launch, for up to 32768 tokens of a vocabulary up to 2^18.  Workgroup g of 256 owns the ids that are g modulo 256.  It
+// reads ALL ids (out of the L2 cache), counts how many belong to the workgroups before it - which is where its part of the sorted list
+// begins, so the workgroups need nothing from each other - and keeps its own tokens in a list in LDS, one in 256 of a text's.  Wave w has
+// a contiguous stretch of the tokens, so its list is in their order; a token's place is the wave's first one for its id plus the number of
+// equal ids before it in the wave.  A wave with more own tokens than its list holds reads its stretch again instead.  Tokens without a
+// gradient come last.  The workgroups behind the 256 zero the gradient meanwhile.  16384 tokens and 77 MB of zeros take 19 us together
+// (a radix sort in one workgroup 46 us); 100352 tokens 48 us, where the four launches below take 29 us.
 #define GROUP_MAX 32768
 #define GROUP_WG 256
-#define GROUP_ROWS ((1 << 18) / GROUP_WG)
-#define GROUP_WAVES 8
+#define GROUP_WAVES 16
+#define GROUP_LIST 192          // list entries of a wave
+#define GROUP_AHEAD 8           // strips of 64 ids in flight
+static size_t emb_group_lds(long long V) {
+    return (size_t)GROUP_WAVES * GROUP_LIST * sizeof(uint2) + (size_t)GROUP_WAVES * ((V + GROUP_WG - 1) / GROUP_WG) * sizeof(unsigned) + 2 * GROUP_WAVES * sizeof(unsigned);
+}
 template <typename I>
-__global__ __launch_bounds__(512) void emb_group_kernel(const void* ids, int T, long long V, long long padding, uint2* sorted, uint4* zero, long long zero16) {
-    __shared__ unsigned hist[GROUP_WAVES][GROUP_ROWS];
-    __shared__ unsigned sums[2][GROUP_WAVES];
+__global__ __launch_bounds__(1024) void emb_group_kernel(const void* ids, int T, long long V, long long padding, uint2* sorted, uint4* zero, long long zero16) {
+    extern __shared__ uint2 group_sh[];         // [16][GROUP_LIST] own tokens, [16][rows] counts, [2][16] sums
     if (blockIdx.x >= GROUP_WG) {
         const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-        const long long step = (long long)(gridDim.x - GROUP_WG) * 512;
-        for (long long i = (long long)(blockIdx.x - GROUP_WG) * 512 + threadIdx.x; i < zero16; i += step) zero[i] = z;
+        const long long step = (long long)(gridDim.x - GROUP_WG) * 1024;
+        for (long long i = (long long)(blockIdx.x - GROUP_WG) * 1024 + threadIdx.x; i < zero16; i += step) zero[i] = z;
         return;
     }
     const unsigned own = blockIdx.x;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int rows = (int)((V + GROUP_WG - 1) / GROUP_WG);           // at most GROUP_ROWS
-    for (int i = threadIdx.x; i < GROUP_WAVES * rows; i += 512) hist[i / rows][i % rows] = 0;
+    const unsigned long long lower = (1ull << lane) - 1ull;
+    const int rows = (int)((V + GROUP_WG - 1) / GROUP_WG);
+    uint2* list = group_sh + wave * GROUP_LIST;
+    unsigned* hist = reinterpret_cast<unsigned*>(group_sh + GROUP_WAVES * GROUP_LIST);
+    unsigned* sums = hist + GROUP_WAVES * rows;
+    unsigned* mine = hist + wave * rows;
+    for (int i = threadIdx.x; i < GROUP_WAVES * rows; i += 1024) hist[i] = 0;
     __syncthreads();
     const int strips = (T + 63) / 64, per = (strips + GROUP_WAVES - 1) / GROUP_WAVES;
     const int s0 = wave * per, s1 = s0 + per < strips ? s0 + per : strips;
     unsigned before = 0, valid = 0;         // of the lane's tokens: those of workgroups before this one, those with a gradient
-#pragma unroll 4
-    for (int s = s0; s < s1; ++s) {
-        const int t = s * 64 + lane;
-        const unsigned key = t < T ? emb_key<I>(ids, t, V, padding) : (unsigned)V;
-        if (key < (unsigned)V) {
-            const unsigned g = key & (GROUP_WG - 1);
-            ++valid;
-            before += g < own ? 1u : 0u;
-            if (g == own) atomicAdd(&hist[wave][key / GROUP_WG], 1u);
+    int listed = 0;                         // the wave's own tokens
+    for (int s = s0; s < s1; s += GROUP_AHEAD) {
+        unsigned key[GROUP_AHEAD];
+#pragma unroll
+        for (int j = 0; j < GROUP_AHEAD; ++j) {
+            const int t = (s + j) * 64 + lane;
+            key[j] = s + j < s1 && t < T ? emb_key<I>(ids, t, V, padding) : (unsigned)V;
+        }
+#pragma unroll
+        for (int j = 0; j < GROUP_AHEAD; ++j) {
+            const unsigned g = key[j] & (GROUP_WG - 1);
+            const bool ok = key[j] < (unsigned)V, hit = ok && g == own;
+            valid += ok ? 1u : 0u;
+            before += ok && g < own ? 1u : 0u;
+            const unsigned long long m = __ballot(hit);
+            if (m != 0) {
+                if (hit) {
+                    atomicAdd(&mine[key[j] / GROUP_WG], 1u);
+                    const int at = listed + __popcll(m & lower);
+                    if (at < GROUP_LIST) list[at] = make_uint2(key[j], (unsigned)((s + j) * 64 + lane));
+                }
+                listed += __popcll(m);
+            }
         }
     }
     before = wave_scan(before);
     valid = wave_scan(valid);
-    if (lane == 63) { sums[0][wave] = before; sums[1][wave] = valid; }
+    if (lane == 63) { sums[wave] = before; sums[GROUP_WAVES + wave] = valid; }
     __syncthreads();
     unsigned at = 0, total_valid = 0;
 #pragma unroll
-    for (int w = 0; w < GROUP_WAVES; ++w) { at += sums[0][w]; total_valid += sums[1][w]; }
+    for (int w = 0; w < GROUP_WAVES; ++w) { at += sums[w]; total_valid += sums[GROUP_WAVES + w]; }
     __syncthreads();
-    // first places: ids in order, within an id the waves in order; 512 ids a round
-    for (int r0 = 0; r0 < rows; r0 += 512) {
-        const int r = r0 + (int)threadIdx.x;
+    // first places: ids in order, within an id the waves in order; `rows` is at most 1024
+    {
+        const int r = (int)threadIdx.x;
         unsigned count = 0;
-        if (r < rows) {
-#pragma unroll
-            for (int w = 0; w < GROUP_WAVES; ++w) { const unsigned c = hist[w][r]; hist[w][r] = count; count += c; }
-        }
+        if (r < rows)
+            for (int w = 0; w < GROUP_WAVES; ++w) { const unsigned c = hist[w * rows + r]; hist[w * rows + r] = count; count += c; }
         const unsigned incl = wave_scan(count);
-        if (lane == 63) sums[0][wave] = incl;
+        if (lane == 63) sums[wave] = incl;
         __syncthreads();
         unsigned base = at + incl - count;
-        for (int w = 0; w < wave; ++w) base += sums[0][w];
-        if (r < rows) {
-#pragma unroll
-            for (int w = 0; w < GROUP_WAVES; ++w) hist[w][r] += base;
-        }
-#pragma unroll
-        for (int w = 0; w < GROUP_WAVES; ++w) at += sums[0][w];
+        for (int w = 0; w < wave; ++w) base += sums[w];
+        if (r < rows)
+            for (int w = 0; w < GROUP_WAVES; ++w) hist[w * rows + r] += base;
         __syncthreads();
     }
-#pragma unroll 4
-    for (int s = s0; s < s1; ++s) {
-        const int t = s * 64 + lane;
-        const unsigned key = t < T ? emb_key<I>(ids, t, V, padding) : (unsigned)V;
-        unsigned long long left = __ballot(key < (unsigned)V && (key & (GROUP_WG - 1)) == own);
-        while (left != 0) {             // one round for each different id among the strip's own tokens
+    // the wave's own tokens of one group of 64 are put down; one round for each different id among them
+    auto place = [&](unsigned key, unsigned t, bool hit) {
+        unsigned long long left = __ballot(hit);
+        while (left != 0) {
             const unsigned k = (unsigned)__builtin_amdgcn_readlane((int)key, (int)__builtin_ctzll(left));
-            const unsigned long long same = __ballot(key == k);
-            if (key == k) {
-                const unsigned first = hist[wave][k / GROUP_WG];
+            const unsigned long long same = __ballot(hit && key == k);
+            if (hit && key == k) {
+                const unsigned first = mine[k / GROUP_WG];
                 asm volatile("" ::: "memory");
-                const unsigned place = (unsigned)__popcll(same & ((1ull << lane) - 1ull));
-                sorted[first + place] = make_uint2(key, (unsigned)t);
-                if (place == 0) hist[wave][k / GROUP_WG] = first + (unsigned)__popcll(same);
+                const unsigned n = (unsigned)__popcll(same & lower);
+                sorted[first + n] = make_uint2(key, t);
+                if (n == 0) mine[k / GROUP_WG] = first + (unsigned)__popcll(same);
                 asm volatile("" ::: "memory");
             }
             left &= ~same;
         }
+    };
+    if (listed <= GROUP_LIST) {
+        for (int i = 0; i < listed; i += 64) {
+            const uint2 e = i + lane < listed ? list[i + lane] : make_uint2(0u, 0u);
+            place(e.x, e.y, i + lane < listed);
+        }
+    } else {
+        for (int s = s0; s < s1; ++s) {
+            const int t = s * 64 + lane;
+            const unsigned key = t < T ? emb_key<I>(ids, t, V, padding) : (unsigned)V;
+            place(key, (unsigned)t, key < (unsigned)V && (key & (GROUP_WG - 1)) == own);
+        }
     }
-    for (unsigned i = total_valid + own * 512u + threadIdx.x; i < (unsigned)T; i += GROUP_WG * 512u) sorted[i] = make_uint2((unsigned)V, 0u);
+    for (unsigned i = total_valid + own * 1024u + threadIdx.x; i < (unsigned)T; i += GROUP_WG * 1024u) sorted[i] = make_uint2((unsigned)V, 0u);
 }
 
 // Several workgroups: per pass a histogram launch (counts[block][bin]) and a launch that turns the counts into ranks and scatters.
@@ -406,11 +432,12 @@ __global__ __launch_bounds__(1024) void embedding_join_kernel(const EmbBwdParams
     emb_put<TO>(p, key, col, acc);
 }
 
-// pieces of the sorted list: about 2048 workgroups where there are enough tokens, 8 to 512 tokens each
+// pieces of the sorted list: about 1024 workgroups where there are enough tokens, 16 to 512 tokens each (2048 of 8 and more: the sums take as
+// long, the joining of their parts 7.4 and 10.9 instead of 6.1 and 6.6 us for 16384 and 100352 tokens of 768 columns)
 static int emb_piece(long long T) {
-    long long c = (T + 2047) / 2048;
+    long long c = (T + 1023) / 1024;
     c = (c + 7) / 8 * 8;
-    return (int)(c < 8 ? 8 : c > 512 ? 512 : c);
+    return (int)(c < 16 ? 16 : c > 512 ? 512 : c);
 }
 static int emb_passes(long long V) {
     int bits = 0;
@@ -491,8 +518,13 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
     ws += emb_up((size_t)p.pieces * 2 * D * sizeof(float));
     if (emb_one(T, V)) {
         const int grid = GROUP_WG + zero_blocks;
-        if (ids_are_64) emb_group_kernel<int64_t><<<grid, 512, 0, s>>>(ids, (int)T, V, padding_idx, sorted, (uint4*)dtable, zero16);
-        else emb_group_kernel<int32_t><<<grid, 512, 0, s>>>(ids, (int)T, V, padding_idx, sorted, (uint4*)dtable, zero16);
+        const size_t lds = emb_group_lds(V);
+        static VitkLdsOnce once64 = {}, once32 = {};        // the largest is allowed once; a launch asks for what its vocabulary needs
+        if (int rc = ids_are_64 ? vitk_lds_once(once64, (const void*)emb_group_kernel<int64_t>, emb_group_lds(1 << 18), "embedding_bwd")
+                                : vitk_lds_once(once32, (const void*)emb_group_kernel<int32_t>, emb_group_lds(1 << 18), "embedding_bwd"))
+            return rc;
+        if (ids_are_64) emb_group_kernel<int64_t><<<grid, 1024, lds, s>>>(ids, (int)T, V, padding_idx, sorted, (uint4*)dtable, zero16);
+        else emb_group_kernel<int32_t><<<grid, 1024, lds, s>>>(ids, (int)T, V, padding_idx, sorted, (uint4*)dtable, zero16);
         if (int rc = vitk_check_launch("embedding_bwd_sort")) return rc;
     } else {
         uint2* other = (uint2*)ws;

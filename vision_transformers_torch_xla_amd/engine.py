@@ -31,10 +31,31 @@ def _core_model(model):
     return m.student if hasattr(m, "student") else m
 
 
+def _grad_tensors(source):
+    """the gradient tensors behind a module, a tensor or a nested iterable of them; a flat-buffer model counts as its one buffer"""
+    if isinstance(source, torch.Tensor):
+        return [] if source.grad is None else [source.grad.detach()]
+    if isinstance(source, torch.nn.Module):
+        core = _core_model(source)
+        if hasattr(core, "_ensure_grad_buffer"):
+            return [core._ensure_grad_buffer()]
+        return [p.grad.detach() for p in source.parameters() if p.grad is not None]
+    return [g for item in source for g in _grad_tensors(item)]
+
+
 def clip_grad_norm_(model, max_norm: float):
-    """torch.nn.utils.clip_grad_norm_ (L2) over the flat gradient buffer: one sum-of-squares reduction and one
-    scaling launch, the norm never leaves the GPU.  Returns the total norm as a 0-d GPU tensor."""
-    core = _core_model(model)
+    """torch.nn.utils.clip_grad_norm_ (L2); the norm never leaves the GPU and is returned as a 0-d GPU tensor.
+
+    model: the flat-buffer VisionTransformer (one sum-of-squares reduction and one scaling launch over its gradient buffer), or any other
+    module, parameter, or iterable of modules and parameters - a head or an embedding with parameters of its own beside the model -
+    whose gradients (fp32 / bf16 / fp16) are then clipped together by their common norm (ops.clip_grads).  A parameter that is reached
+    twice counts once."""
+    core = _core_model(model) if isinstance(model, torch.nn.Module) else None
+    if core is None or not hasattr(core, "_ensure_grad_buffer"):
+        grads = list({(g.data_ptr(), g.numel()): g for g in _grad_tensors(model)}.values())
+        if not grads:
+            return torch.zeros((), device="cuda" if torch.cuda.is_available() else "cpu")
+        return ops.clip_grads(grads, max_norm)
     g = core._ensure_grad_buffer()
     if not hasattr(core, "_sumsq"):
         core._sumsq = torch.zeros(1, dtype=torch.float32, device=g.device)
@@ -191,14 +212,15 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
                 if reducer is not None:
                     reducer.wait()
                 if max_norm is not None and max_norm > 0:
-                    clip_grad_norm_(model, max_norm)
+                    own = isinstance(criterion, torch.nn.Module) and any(p.grad is not None for p in criterion.parameters())
+                    clip_grad_norm_([model, criterion] if own else model, max_norm)      # a criterion may hold a head (LinearCrossEntropy)
                 optimizer.step()
                 optimizer.zero_grad()
                 if model_ema is not None:
                     model_ema.update(model)
 
             class_acc = None
-            if mixup_fn is None:
+            if mixup_fn is None and not getattr(criterion, "takes_features", False):
                 out0 = output[0] if isinstance(output, tuple) else output
                 class_acc = (ops.argmax_rows(out0.detach().float()) == targets).float().mean()
 

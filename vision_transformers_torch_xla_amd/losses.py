@@ -1,5 +1,6 @@
 """Criteria of the reference's training loop, computed by fused HIP kernels (log-softmax, loss and gradient in
-one pass over fp32 logits).
+one pass over fp32 logits; linear_cross_entropy / LinearCrossEntropy take the features and the head's weight instead, for label sets
+whose logits are too large to hold).
 
 Mirrors main.py:926-935 (criterion choice: timm SoftTargetCrossEntropy when mixup is on, timm
 LabelSmoothingCrossEntropy(smoothing) when smoothing > 0, else nn.CrossEntropyLoss) and the inline knowledge
@@ -15,6 +16,8 @@ import torch.nn as nn
 
 from . import ops
 from ._lib import VitkError
+
+bf16, f32 = torch.bfloat16, torch.float32
 
 
 def _as_logits(x):
@@ -76,6 +79,79 @@ class SoftTargetCrossEntropy(nn.Module):
         if t.dtype != torch.float32 or t.stride(-1) != 1:
             t = t.float().contiguous()
         return _FusedLoss.apply(_as_logits(x), "soft", t, None)
+
+
+def _bf16_rows(t):
+    """a bf16 matrix with contiguous, 16-byte aligned rows holding t's values (t itself where it is one)"""
+    if t.dtype == f32:
+        return ops.cast_f32_to_bf16(t.detach().contiguous())
+    t = t.detach()
+    if t.stride(-1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+        t = t.contiguous()
+    return t
+
+
+class _LinearXent(torch.autograd.Function):
+    """The loss and, where anything needs them, its gradients in one call of ops.linear_xent; backward multiplies them by the upstream scalar."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, smoothing, ignore_index, reduction):
+        want = any(ctx.needs_input_grad[:3])
+        wtype = weight.dtype
+        r = ops.linear_xent(_bf16_rows(x), _bf16_rows(weight), target, None if bias is None else bias.detach(), smoothing=smoothing,
+                            ignore_index=ignore_index, reduction=reduction, want_grad=want, dweight_dtype=wtype if wtype in (bf16, f32) else None)
+        ctx.grads = (r.dx, r.dweight, r.dbias) if want else None
+        ctx.xtype = x.dtype
+        return r.loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go):
+        if ctx.grads is None:
+            raise VitkError("linear_cross_entropy: backward was called a second time (the gradients are handed over, not kept)")
+        (dx, dw, db), ctx.grads = ctx.grads, None
+        need = ctx.needs_input_grad
+        scaled = lambda g: None if g is None else ops.rowscale(g, go.reshape(1).float(), g.shape[0], out=g) if g.dtype == bf16 and g.dim() == 2 \
+            else (g * go.float()).to(g.dtype)                     # the upstream scalar stays fp32: a bf16 gradient is rounded once more, not it
+        dx = scaled(dx).to(ctx.xtype) if need[0] else None
+        return dx, scaled(dw) if need[1] else None, scaled(db) if need[2] else None, None, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, bias=None, smoothing: float = 0.0, ignore_index: int = -100, reduction: str = "mean"):
+    """cross entropy of the logits x @ weight.T + bias without the logits in memory (ops.linear_xent): x [..., D], weight [V, D] (bf16, or fp32
+    masters, which are rounded to bf16 for the products as every linear of this package does), bias [V], target [...] int64.
+    Differentiable in x, weight and bias, once.  reduction 'mean' (over the targets that are not ignore_index) or 'sum'."""
+    if x.dim() < 1 or tuple(x.shape[:-1]) != tuple(target.shape):
+        raise VitkError(f"linear_cross_entropy: target must be {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
+    for t, n in ((x, "x"), (weight, "weight")):
+        if t.dtype not in (bf16, f32):
+            raise VitkError(f"linear_cross_entropy: {n} must be bfloat16 or float32, got {t.dtype}")
+    if not x.is_cuda:
+        raise VitkError("linear_cross_entropy: x must be on the GPU; the fused loss kernels are the only implementation")
+    return _LinearXent.apply(x.reshape(-1, x.shape[-1]), weight, bias, target.reshape(-1), float(smoothing), int(ignore_index), reduction)
+
+
+class LinearCrossEntropy(nn.Module):
+    """A classification head and its criterion in one: owns weight [num_classes, in_features] and bias (fp32 masters, timm's head
+    initialisation), takes the features instead of the logits.  For label sets so large that the logits and their gradient are what fills
+    the memory: 21 843 classes, or the vocabulary of a token-prediction objective over every position.  As a criterion of train_one_epoch it is
+    clipped together with the model; its parameters belong into the optimizer beside the model's."""
+
+    takes_features = True           # train_one_epoch: the model's output is not a matrix of logits
+
+    def __init__(self, in_features: int, num_classes: int, bias: bool = True, smoothing: float = 0.0, ignore_index: int = -100, reduction: str = "mean"):
+        super().__init__()
+        if in_features < 8 or in_features % 8 or num_classes < 1:
+            raise VitkError(f"LinearCrossEntropy: in_features must be a multiple of 8, num_classes positive, got {in_features}, {num_classes}")
+        if not 0.0 <= smoothing <= 1.0 or reduction not in ("mean", "sum"):
+            raise VitkError(f"LinearCrossEntropy: smoothing outside [0, 1] or unknown reduction: {smoothing}, {reduction!r}")
+        self.smoothing, self.ignore_index, self.reduction = float(smoothing), int(ignore_index), reduction
+        self.weight = nn.Parameter(torch.empty(num_classes, in_features))
+        nn.init.trunc_normal_(self.weight, std=0.02)
+        self.bias = nn.Parameter(torch.zeros(num_classes)) if bias else None
+
+    def forward(self, x, target):
+        return linear_cross_entropy(x, self.weight, target, self.bias, self.smoothing, self.ignore_index, self.reduction)
 
 
 class DistillationLoss(nn.Module):
