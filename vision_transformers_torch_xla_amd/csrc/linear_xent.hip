@@ -39,6 +39,7 @@ struct LxGemmParams {
     // work, LX_XENT*: workgroup g of G takes the tiles g, g + G, ... (in bands of 8 column tiles)
     // work, LX_OUT: see LxDeal
     int width, teams, whole, rest, ranges;
+    int splits;             // the small kernel: ranges of steps
     // LX_OUT: out[m][n] = scale[0] * acc (+ add[m][n]), bf16 or fp32
     const float* scale;
     const float* add;
@@ -61,6 +62,89 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 static __device__ __forceinline__ unsigned lx_pack_h(float a, float b) {
     const f32x2_t v = {a, b};
     return __builtin_bit_cast(unsigned, __builtin_convertvector(v, f16x2));
+}
+
+// The loss's epilogue of a wave that holds FM * 16 rows (from m0) by 64 columns (from n0) of logits: lane (lr, lg) has columns 16 tn + 4 lg + j
+// of row 16 tm + lr.  stg: 2 KB of LDS of the wave's own, through which P leaves in rows of 64 columns so that a store covers whole lines.
+// EXTRA: with a bias or the sums of the logits.
+template <int FM, bool EXTRA>
+static __device__ __forceinline__ void lx_loss_epilogue(const LxGemmParams& p, f32x4 (&acc)[FM][4], int m0, int n0, bf16_t* stg) {
+    const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4, srow = lane >> 3;
+    const int first = n0 + 4 * lg;                   // the lane's columns are first + 16 tn + j
+    const int room = p.N - first;                    // those with 16 tn + j < room are columns of the vocabulary
+    if constexpr (EXTRA) {
+        if (p.bias != nullptr) {
+#pragma unroll
+            for (int tn = 0; tn < 4; ++tn) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int n = first + tn * 16 + j < p.N ? first + tn * 16 + j : p.N - 1;
+                    const float u = p.bias_type == 1 ? bf2f(reinterpret_cast<const bf16_t*>(p.bias)[n]) : reinterpret_cast<const float*>(p.bias)[n];
+#pragma unroll
+                    for (int tm = 0; tm < FM; ++tm) acc[tm][tn][j] += u;
+                }
+            }
+        }
+    }
+    if (n0 + 64 > p.N) {           // columns behind the vocabulary count as logits of -inf
+#pragma unroll
+        for (int tm = 0; tm < FM; ++tm)
+#pragma unroll
+            for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[tm][tn][j] = tn * 16 + j < room ? acc[tm][tn][j] : -INFINITY;
+    }
+    const int sc = n0 >> 6;
+#pragma unroll
+    for (int tm = 0; tm < FM; ++tm) {
+        const int m = m0 + tm * 16 + lr;
+        float z[4][4], mx = -INFINITY, zs = 0.f;
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                z[tn][j] = acc[tm][tn][j];
+                mx = fmaxf(mx, z[tn][j]);
+                if constexpr (EXTRA) zs += tn * 16 + j < room ? z[tn][j] : 0.f;
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        // From here on in powers of two, relative to m = max * log2(e) as rounded: z * log2(e) - m is one fma, exact up to its own rounding
+        mx *= 1.44269504088896340736f;
+        const float ref = mx == -INFINITY ? 0.f : mx;        // a row of -inf only: 2^(-inf - 0) = 0
+        float s = 0.f;
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                z[tn][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[tn][j], 1.44269504088896340736f, -ref));
+                s += z[tn][j];
+            }
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        if (lg == 0 && m < p.M) p.stats[(size_t)m * p.stat_cols + sc] = make_float2(mx, s);
+        if (EXTRA && p.zsum != nullptr) {
+            zs += __shfl_xor(zs, 16, 64);
+            zs += __shfl_xor(zs, 32, 64);
+            if (lg == 0 && m < p.M) p.zsum[(size_t)m * p.stat_cols + sc] = zs;
+        }
+        if (p.P != nullptr) {
+#pragma unroll
+            for (int tn = 0; tn < 4; ++tn) {
+                uint2 w;
+                w.x = lx_pack_h(z[tn][0], z[tn][1]);
+                w.y = lx_pack_h(z[tn][2], z[tn][3]);
+                *reinterpret_cast<uint2*>(stg + lr * 64 + (((tn * 2 + (lg >> 1)) ^ (lr & 7)) << 3) + (lg & 1) * 4) = w;
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = half * 8 + srow;
+                const u32x4 o = *reinterpret_cast<const u32x4*>(stg + r * 64 + (((lane & 7) ^ srow) << 3));
+                const int mr = m0 + tm * 16 + r;
+                if (mr < p.M) __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(p.P + (size_t)mr * p.ldp + n0 + (lane & 7) * 8));
+            }
+        }
+    }
 }
 
 // One 512-thread workgroup per compute unit works through 256 x 256 tiles of the output, 8 waves (2 x 4) of 128 x 64 = 128 accumulator
@@ -426,83 +510,7 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
                 }
             }
         } else {
-            bf16_t* stg = reinterpret_cast<bf16_t*>(reinterpret_cast<float*>(lsm + 4 * LX_ELEMS) + wave * (16 * 64));
-            const int first = n0 + wn * 64 + 4 * lg;         // the lane's columns are first + 16 tn + j
-            const int room = p.N - first;                    // those with 16 tn + j < room are columns of the vocabulary
-            if constexpr (EPI == LX_XENT_BIAS) {
-                if (p.bias != nullptr) {
-#pragma unroll
-                    for (int tn = 0; tn < 4; ++tn) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int n = first + tn * 16 + j < p.N ? first + tn * 16 + j : p.N - 1;
-                            const float u = p.bias_type == 1 ? bf2f(reinterpret_cast<const bf16_t*>(p.bias)[n]) : reinterpret_cast<const float*>(p.bias)[n];
-#pragma unroll
-                            for (int tm = 0; tm < 8; ++tm) acc[tm][tn][j] += u;
-                        }
-                    }
-                }
-            }
-            if (n0 + LX_TILE > p.N) {           // columns behind the vocabulary count as logits of -inf
-#pragma unroll
-                for (int tm = 0; tm < 8; ++tm)
-#pragma unroll
-                    for (int tn = 0; tn < 4; ++tn)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[tm][tn][j] = tn * 16 + j < room ? acc[tm][tn][j] : -INFINITY;
-            }
-            const int sc = (n0 >> 6) + wn;
-#pragma unroll
-            for (int tm = 0; tm < 8; ++tm) {
-                const int m = m0 + wm * 128 + tm * 16 + lr;
-                float z[4][4], mx = -INFINITY, zs = 0.f;
-#pragma unroll
-                for (int tn = 0; tn < 4; ++tn)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        z[tn][j] = acc[tm][tn][j];
-                        mx = fmaxf(mx, z[tn][j]);
-                        if constexpr (EPI == LX_XENT_BIAS) zs += tn * 16 + j < room ? z[tn][j] : 0.f;
-                    }
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                // From here on in powers of two, relative to m = max * log2(e) as rounded: z * log2(e) - m is one fma, exact up to its own rounding
-                mx *= 1.44269504088896340736f;
-                const float ref = mx == -INFINITY ? 0.f : mx;        // a row of -inf only: 2^(-inf - 0) = 0
-                float s = 0.f;
-#pragma unroll
-                for (int tn = 0; tn < 4; ++tn)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        z[tn][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[tn][j], 1.44269504088896340736f, -ref));
-                        s += z[tn][j];
-                    }
-                s += __shfl_xor(s, 16, 64);
-                s += __shfl_xor(s, 32, 64);
-                if (lg == 0 && m < p.M) p.stats[(size_t)m * p.stat_cols + sc] = make_float2(mx, s);
-                if (EPI == LX_XENT_BIAS && p.zsum != nullptr) {
-                    zs += __shfl_xor(zs, 16, 64);
-                    zs += __shfl_xor(zs, 32, 64);
-                    if (lg == 0 && m < p.M) p.zsum[(size_t)m * p.stat_cols + sc] = zs;
-                }
-                if (p.P != nullptr) {
-#pragma unroll
-                    for (int tn = 0; tn < 4; ++tn) {
-                        uint2 w;
-                        w.x = lx_pack_h(z[tn][0], z[tn][1]);
-                        w.y = lx_pack_h(z[tn][2], z[tn][3]);
-                        *reinterpret_cast<uint2*>(stg + lr * 64 + (((tn * 2 + (lg >> 1)) ^ (lr & 7)) << 3) + (lg & 1) * 4) = w;
-                    }
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int r = half * 8 + srow;
-                        const u32x4 o = *reinterpret_cast<const u32x4*>(stg + r * 64 + (((lane & 7) ^ srow) << 3));
-                        const int mr = m0 + wm * 128 + tm * 16 + r;
-                        if (mr < p.M)
-                            __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(p.P + (size_t)mr * p.ldp + n0 + wn * 64 + (lane & 7) * 8));
-                    }
-                }
-            }
+            lx_loss_epilogue<8, EPI == LX_XENT_BIAS>(p, acc, m0 + wm * 128, n0 + wn * 64, reinterpret_cast<bf16_t*>(lsm + 4 * LX_ELEMS) + wave * (16 * 64 * 2));
         }
         loose = m0 + LX_TILE <= p.M && (EPI != LX_OUT ? p.P != nullptr : n0 + LX_TILE <= p.N);       // a full tile: 16 stores at least
     }
@@ -515,126 +523,389 @@ struct LxRowParams {
     const void* bias; int bias_type;
     const long long* target; long long ignore_index;
     const float2* stats; const float* zsum; int stat_cols;
+    unsigned* ticket;                  // zeroed for lx_loss_kernel
     bf16_t* P; long long ldp;          // fp16 on entry, bf16 dz on exit; null: loss alone
     float* rows;
-    int V, D;
+    int V, D, rows_n;
     float smoothing;
 };
 
+template <int WAVES>
 static __device__ __forceinline__ float lx_block_max(float v, float* sh) {
     v = wave_max(v);
+    if (WAVES == 1) return v;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
     __syncthreads();
-    return fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) v = fmaxf(v, sh[w]);
+    return v;
 }
+template <int WAVES>
 static __device__ __forceinline__ float lx_block_sum(float v, float* sh) {
     v = wave_sum(v);
+    if (WAVES == 1) return v;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) v += sh[w];
+    return v;
 }
 
-__global__ __launch_bounds__(256) void lx_row_kernel(const LxRowParams p) {
-    __shared__ float sh[4];
-    const int row = blockIdx.x;
+// 8 columns of P -> dz
+static __device__ __forceinline__ u32x4 lx_dz8(const u32x4 r, float f, float u, float hit, int n, int t, int V, bool valid) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const unsigned word = r[k];         // (a bit cast of the vector's element itself reads element 0)
+        const f16x2 h = __builtin_bit_cast(f16x2, word);
+        v[2 * k] = __builtin_fmaf((float)h[0], f, -u);
+        v[2 * k + 1] = __builtin_fmaf((float)h[1], f, -u);
+    }
+    if ((t & ~7) == n) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (n + k == t) v[k] -= hit;
+    }
+    if (!valid) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = __builtin_nanf("");
+    }
+    if (n + 8 > V) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (n + k >= V) v[k] = 0.f;
+    }
+    return (u32x4){pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])};
+}
+
+// WAVES waves per row: one workgroup, or for short rows one wave of a workgroup of four.  Bound by memory: 4 bytes per logit where the gradient
+// is wanted, nothing to speak of where it is not.
+#ifndef LX_NTS
+#define LX_NTS 0
+#endif
+#define LX_AHEAD 4          // chunks of 8 columns a thread has in flight
+template <int WAVES, bool STREAM>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(const LxRowParams p) {
+    constexpr int NT = WAVES * 64;
+    __shared__ float sh[WAVES];
+    const int tid = WAVES == 1 ? (int)threadIdx.x & 63 : (int)threadIdx.x;
+    const int row = WAVES == 1 ? (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6) : (int)blockIdx.x;
+    if (row >= p.rows_n) return;
+    if (row == 0 && tid == 0) *p.ticket = 0u;
     const long long t64 = p.target[row];
     bf16_t* P = p.P != nullptr ? p.P + (size_t)row * p.ldp : nullptr;
     const int chunks = (int)(p.ldp / 8);
     if (t64 == p.ignore_index) {
-        if (threadIdx.x == 0) p.rows[row] = 0.f;
+        if (tid == 0) p.rows[row] = 0.f;
         if (P != nullptr)
-            for (int c = threadIdx.x; c < chunks; c += 256) reinterpret_cast<u32x4*>(P)[c] = (u32x4){0u, 0u, 0u, 0u};
+            for (int c = tid; c < chunks; c += NT) __builtin_nontemporal_store((u32x4){0u, 0u, 0u, 0u}, reinterpret_cast<u32x4*>(P) + c);
         return;
     }
     // a label outside [0, V) never becomes an address: the row's loss and gradient are NaN
     const bool valid = t64 >= 0 && t64 < (long long)p.V;
     const int t = valid ? (int)t64 : 0;
     const float2* st = p.stats + (size_t)row * p.stat_cols;
-    float mx = -INFINITY;
-    for (int c = threadIdx.x; c < p.stat_cols; c += 256) mx = fmaxf(mx, st[c].x);
-    mx = lx_block_max(mx, sh);
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    float s = 0.f, zs = 0.f;
-    for (int c = threadIdx.x; c < p.stat_cols; c += 256) {
-        const float2 v = st[c];
-        s += v.y * (v.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(v.x - ref));         // an all -inf entry has s = 0, or NaN where a logit was NaN
-        if (p.smoothing > 0.f) zs += p.zsum[(size_t)row * p.stat_cols + c];
-    }
-    s = lx_block_sum(s, sh);
+    const int entries = (p.V + LX_STAT - 1) / LX_STAT;          // what lies behind them up to stat_cols need not have been written
     // the target's logit
     const bf16_t* xr = p.x + (size_t)row * p.ldx;
     const bf16_t* wr = p.w + (size_t)t * p.ldw;
     float dot = 0.f;
-    for (int c = threadIdx.x; c < p.D / 8; c += 256) {
+    for (int c = tid; c < p.D / 8; c += NT) {
         float a[8], b[8];
         load8(xr + c * 8, a);
         load8(wr + c * 8, b);
 #pragma unroll
         for (int k = 0; k < 8; ++k) dot = __builtin_fmaf(a[k], b[k], dot);
     }
-    dot = lx_block_sum(dot, sh);
-    if (p.smoothing > 0.f) zs = lx_block_sum(zs, sh);
+    float mx = -INFINITY;
+#pragma unroll 4
+    for (int c = tid; c < entries; c += NT) mx = fmaxf(mx, st[c].x);
+    mx = lx_block_max<WAVES>(mx, sh);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float s = 0.f, zs = 0.f;
+#pragma unroll 4
+    for (int c = tid; c < entries; c += NT) {
+        const float2 v = st[c];
+        s += v.y * (v.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(v.x - ref));         // an all -inf entry has s = 0, or NaN where a logit was NaN
+        if (p.smoothing > 0.f) zs += p.zsum[(size_t)row * p.stat_cols + c];
+    }
+    s = lx_block_sum<WAVES>(s, sh);
+    dot = lx_block_sum<WAVES>(dot, sh);
+    if (p.smoothing > 0.f) zs = lx_block_sum<WAVES>(zs, sh);
     if (p.bias != nullptr) dot += p.bias_type == 1 ? bf2f(reinterpret_cast<const bf16_t*>(p.bias)[t]) : reinterpret_cast<const float*>(p.bias)[t];
     const float lse2 = ref + log2f(s), lse = lse2 * 0.69314718055994530942f;
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         float l = lse - dot;
         if (p.smoothing > 0.f) l = (1.f - p.smoothing) * l + p.smoothing * (lse - zs / (float)p.V);
         p.rows[row] = valid ? l : __builtin_nanf("");
     }
     if (P == nullptr) return;
     const float u = p.smoothing / (float)p.V, hit = 1.f - p.smoothing;
-    for (int c = threadIdx.x; c < chunks; c += 256) {
-        const u32x4 r = reinterpret_cast<const u32x4*>(P)[c];
-        const float f = __builtin_amdgcn_exp2f(st[c >> 3].x - lse2);
-        float v[8];
+    u32x4* q = reinterpret_cast<u32x4*>(P);
+    for (int c0 = tid; c0 < chunks; c0 += LX_AHEAD * NT) {
+        u32x4 r[LX_AHEAD];
+        float m[LX_AHEAD];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const unsigned word = r[k];         // (a bit cast of the vector's element itself reads element 0)
-            const f16x2 h = __builtin_bit_cast(f16x2, word);
-            v[2 * k] = (float)h[0] * f - u;
-            v[2 * k + 1] = (float)h[1] * f - u;
+        for (int j = 0; j < LX_AHEAD; ++j) {
+            const int c = c0 + j * NT < chunks ? c0 + j * NT : c0;
+            r[j] = STREAM ? __builtin_nontemporal_load(q + c) : q[c];
+            m[j] = st[c >> 3].x;
         }
-        const int n = c * 8;
-        if ((t >> 3) == c) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (n + k == t) v[k] -= hit;
+        for (int j = 0; j < LX_AHEAD; ++j) {
+            const int c = c0 + j * NT;
+            if (c < chunks) {
+                const u32x4 o = lx_dz8(r[j], __builtin_amdgcn_exp2f(m[j] - lse2), u, hit, c * 8, t, p.V, valid);
+                if (STREAM || LX_NTS) __builtin_nontemporal_store(o, q + c);
+                else q[c] = o;
+            }
         }
-        if (!valid) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = __builtin_nanf("");
-        }
-        if (n + 8 > p.V) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (n + k >= p.V) v[k] = 0.f;
-        }
-        const u32x4 o = {pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])};
-        reinterpret_cast<u32x4*>(P)[c] = o;
     }
 }
 
-// count of the counted rows, the scale of the gradients (1 / count, or 1 for a sum; 0 without a counted row) and the loss, by one workgroup
-__global__ __launch_bounds__(1024) void lx_loss_kernel(const long long* __restrict__ target, long long ignore_index, const float* __restrict__ rows, int T,
-                                                       int mean, float* __restrict__ scale, float* __restrict__ loss) {
-    __shared__ double sh[16];
-    __shared__ int shc[16];
+// Count of the counted rows, the scale of the gradients (1 / count, or 1 for a sum; 0 without a counted row) and the loss.  Workgroup b sums
+// a stretch of the rows into part[b]; the last one to finish adds the parts in order (lx_row_kernel has zeroed the ticket).
+#define LX_LOSS_WGS 64
+struct LxLossPart { double sum; long long count; };
+__global__ __launch_bounds__(256) void lx_loss_kernel(const long long* __restrict__ target, long long ignore_index, const float* __restrict__ rows, int T, int per,
+                                                      int mean, LxLossPart* part, unsigned* ticket, float* __restrict__ scale, float* __restrict__ loss) {
+    __shared__ double sh[4];
+    __shared__ int shc[4];
+    const int i1 = (int)((blockIdx.x + 1ll) * per < T ? (blockIdx.x + 1ll) * per : T);
     double s = 0.0;
     int n = 0;
-    for (int i = threadIdx.x; i < T; i += 1024) {
-        if (target[i] != ignore_index) ++n;
-        if (rows != nullptr) s += (double)rows[i];
+    for (int i0 = blockIdx.x * per + (int)threadIdx.x; i0 < i1; i0 += 8 * 256) {
+        long long t[8];
+        float r[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + j * 256 < i1 ? i0 + j * 256 : i0;
+            t[j] = target[i];
+            r[j] = rows != nullptr ? rows[i] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i0 + j * 256 < i1) {
+                n += t[j] != ignore_index;
+                s += (double)r[j];
+            }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); n += __shfl_xor(n, o, 64); }
     if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = s; shc[threadIdx.x >> 6] = n; }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) { s += sh[w]; n += shc[w]; }
-        if (scale != nullptr) *scale = n == 0 ? 0.f : mean ? (float)(1.0 / (double)n) : 1.f;
-        if (loss != nullptr) *loss = (float)(n == 0 ? 0.0 : mean ? s / (double)n : s);
+    if (threadIdx.x != 0) return;
+    s = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+    long long count = (long long)shc[0] + shc[1] + shc[2] + shc[3];
+    if (gridDim.x > 1) {
+        __hip_atomic_store(&part[blockIdx.x].sum, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&part[blockIdx.x].count, count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) != gridDim.x - 1) return;
+        s = 0.0;
+        count = 0;
+        for (unsigned b = 0; b < gridDim.x; ++b) {
+            s += __hip_atomic_load(&part[b].sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            count += __hip_atomic_load(&part[b].count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    if (scale != nullptr) *scale = count == 0 ? 0.f : mean ? (float)(1.0 / (double)count) : 1.f;
+    if (loss != nullptr) *loss = (float)(count == 0 ? 0.0 : mean ? s / (double)count : s);
+}
+// The same products for outputs too small to fill the chip with 256 x 256 tiles, which also cost a call 8 to 10 us of pipeline fill and epilogue
+// however short it is: one tile of (16 FM WM) x (64 WN) and one range of steps per 256-thread workgroup, several workgroups on a compute unit
+// in place of a deep pipeline within one.  FM = 4, waves 2 x 2: 128 x 128 tiles, 64 KB of LDS; FM = 1, waves 4 x 1: 64 x 64, 32 KB.
+// LX_OUT with p.splits > 1: the fp32 sums of range s go to slab[s][M][N].
+template <int LAY, int EPI, int FM, int WM, int WN>
+__global__ __launch_bounds__(256) void lx_small_kernel(const LxGemmParams p) {
+    constexpr bool AT = LAY == LX_TN, BT = LAY != LX_NT;
+    constexpr int TM = FM * 16 * WM, TN = 64 * WN;              // the tile
+    constexpr int PA = TM / 32, PB = TN / 32;                   // 1 KB pieces of an operand's step per wave
+    constexpr int EA = TM * LX_BK, EB = TN * LX_BK;             // elements of a buffer
+    __shared__ __attribute__((aligned(1024))) bf16_t sm[2 * (EA + EB)];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const int lr = lane & 15, lg = lane >> 4, lq = lr >> 2, lp = lr & 3;
+    const unsigned lds_base = __builtin_amdgcn_readfirstlane(lds_addr(sm));
+
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int tiles = p.tiles_m * p.tiles_n;
+    const int split = __builtin_amdgcn_readfirstlane(id / tiles);
+    const int tile = id - split * tiles;
+    const int tm_ = tile / p.tiles_n;
+    const int m0 = __builtin_amdgcn_readfirstlane(tm_ * TM), n0 = __builtin_amdgcn_readfirstlane((tile - tm_ * p.tiles_n) * TN);
+    int k0, k1;
+    lx_range(split, p.steps, p.splits, k0, k1);
+    k0 = __builtin_amdgcn_readfirstlane(k0);
+    k1 = __builtin_amdgcn_readfirstlane(k1);
+
+    // K-contiguous image [T][64]: a piece is 8 rows, position lane % 8 receives chunk (lane % 8) ^ (row & 7).  K-strided image [64][T]: a piece
+    // is 512 / T rows; chunks are XOR-swizzled by the row so that the transposing read's 8 rows of a half wave meet different banks
+    // (rows r and r + 4 have the same swizzle)
+    auto swz = [](int r, int T) { return T == 128 ? lx_swz(r) : (((r >> 1) & 1) << 1) | (((r >> 3) & 1) << 2); };
+    const bf16_t* gA = p.A + (AT ? (size_t)m0 : (size_t)m0 * p.lda);
+    const bf16_t* gB = p.B + (BT ? (size_t)n0 : (size_t)n0 * p.ldb);
+    unsigned voA[PA], voB[PB];
+    int kA[PA], kB[PB];         // the lane's place in a step's contraction, per piece
+#pragma unroll
+    for (int j = 0; j < PA; ++j) {
+        if (AT) {
+            constexpr int CH = TM / 8;          // chunks of a row
+            const int r = (wave * PA + j) * (64 / CH) + lane / CH;
+            kA[j] = r;
+            voA[j] = (unsigned)((r * p.lda + ((lane % CH) ^ swz(r, TM)) * 8) * 2);         // A's rows are padded to a multiple of 256
+        } else {
+            const int r = (wave * PA + j) * 8 + (lane >> 3), most = p.M - 1 - m0;
+            kA[j] = ((lane & 7) ^ (r & 7)) * 8;
+            voA[j] = (unsigned)(((r < most ? r : most) * p.lda + kA[j]) * 2);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < PB; ++j) {
+        if (BT) {
+            constexpr int CH = TN / 8;
+            const int r = (wave * PB + j) * (64 / CH) + lane / CH, c = ((lane % CH) ^ swz(r, TN)) * 8;
+            kB[j] = r;
+            voB[j] = (unsigned)((r * p.ldb + (n0 + c < p.N ? c : p.N - 8 - n0)) * 2);
+        } else {
+            const int r = (wave * PB + j) * 8 + (lane >> 3), most = p.N - 1 - n0;
+            kB[j] = ((lane & 7) ^ (r & 7)) * 8;
+            voB[j] = (unsigned)(((r < most ? r : most) * p.ldb + kB[j]) * 2);
+        }
+    }
+    const void* zrow = (const char*)lx_zero_row + (lane & 31) * 16;
+    auto stage = [&](int k, int par) {
+        const bf16_t* a = gA + (AT ? (size_t)k * LX_BK * p.lda : (size_t)k * LX_BK);
+        const bf16_t* b = gB + (BT ? (size_t)k * LX_BK * p.ldb : (size_t)k * LX_BK);
+        const unsigned dA = lds_base + (unsigned)(par * (EA + EB) * 2) + wave * PA * 1024, dB = lds_base + (unsigned)((par * (EA + EB) + EA) * 2) + wave * PB * 1024;
+        if ((k + 1) * LX_BK <= p.KA) {
+#pragma unroll
+            for (int j = 0; j < PA; ++j) glds16(a, voA[j], dA + j * 1024);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PA; ++j) glds16_v(k * LX_BK + kA[j] < p.KA ? (const void*)((const char*)a + voA[j]) : zrow, dA + j * 1024);
+        }
+        if ((k + 1) * LX_BK <= p.KB) {
+#pragma unroll
+            for (int j = 0; j < PB; ++j) glds16(b, voB[j], dB + j * 1024);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PB; ++j) glds16_v(k * LX_BK + kB[j] < p.KB ? (const void*)((const char*)b + voB[j]) : zrow, dB + j * 1024);
+        }
+    };
+    f32x4 acc[FM][4];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    stage(k0, 0);
+    for (int k = k0; k < k1; ++k) {
+        const int par = (k - k0) & 1;
+        LX_WAIT(0);             // this step's operands have landed, the other buffer has been read
+        LX_BARRIER();
+        if (k + 1 < k1) stage(k + 1, par ^ 1);
+        const bf16_t* cA = sm + par * (EA + EB);
+        const bf16_t* cB = cA + EA;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            bf16x8 fa[FM], fb[4];
+            const int r = ks * 32 + 8 * lg + lq, ch = ks * 4 + lg;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if (BT) {
+                    const bf16_t* q = cB + r * TN + ((((wn * 64 + t * 16) >> 3) + (lp >> 1)) ^ swz(r, TN)) * 8 + (lp & 1) * 4;
+                    fb[t] = lx_tr(q, q + 4 * TN);
+                } else {
+                    const int row = wn * 64 + t * 16 + lr;
+                    fb[t] = *reinterpret_cast<const bf16x8*>(cB + row * LX_BK + ((ch ^ (row & 7)) << 3));
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < FM; ++t) {
+                if (AT) {
+                    const bf16_t* q = cA + r * TM + ((((wm * FM * 16 + t * 16) >> 3) + (lp >> 1)) ^ swz(r, TM)) * 8 + (lp & 1) * 4;
+                    fa[t] = lx_tr(q, q + 4 * TM);
+                } else {
+                    const int row = wm * FM * 16 + t * 16 + lr;
+                    fa[t] = *reinterpret_cast<const bf16x8*>(cA + row * LX_BK + ((ch ^ (row & 7)) << 3));
+                }
+            }
+#pragma unroll
+            for (int tm = 0; tm < FM; ++tm)
+#pragma unroll
+                for (int tn = 0; tn < 4; ++tn)
+                    acc[tm][tn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[tn], fa[tm], acc[tm][tn], 0, 0, 0);
+        }
+    }
+    LX_WAIT(0);
+    LX_BARRIER();           // every wave has read its operands: their LDS takes the epilogue's rows
+    if constexpr (EPI == LX_OUT) {
+        const float sc = p.scale != nullptr ? p.scale[0] : 1.0f;
+        bf16_t* stg = sm + wave * (16 * 64);
+        const int srow = lane >> 3;
+#pragma unroll
+        for (int tm = 0; tm < FM; ++tm) {
+            const int m = m0 + (wm * FM + tm) * 16 + lr;
+#pragma unroll
+            for (int tn = 0; tn < 4; ++tn) {
+                const int n = n0 + wn * 64 + tn * 16 + 4 * lg;
+                const bool in = m < p.M && n < p.N;
+                f32x4 v = acc[tm][tn];
+                if (p.splits > 1) {
+                    if (in) *reinterpret_cast<f32x4*>(p.slab + ((size_t)split * p.M + m) * p.N + n) = v;
+                    continue;
+                }
+                v *= sc;
+                if (p.add != nullptr && in) v += *reinterpret_cast<const f32x4*>(p.add + (size_t)m * p.N + n);
+                if (p.out_f32) {
+                    if (in) *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + (size_t)m * p.ldo + n) = v;
+                } else {            // bf16: through the wave's 2 KB of LDS, so that a store covers whole lines
+                    uint2 o;
+                    o.x = pack2bf(v[0], v[1]);
+                    o.y = pack2bf(v[2], v[3]);
+                    *reinterpret_cast<uint2*>(stg + lr * 64 + (((tn * 2 + (lg >> 1)) ^ (lr & 7)) << 3) + (lg & 1) * 4) = o;
+                }
+            }
+            if (p.splits == 1 && !p.out_f32) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int r = half * 8 + srow;
+                    const u32x4 o = *reinterpret_cast<const u32x4*>(stg + r * 64 + (((lane & 7) ^ srow) << 3));
+                    const int mr = m0 + (wm * FM + tm) * 16 + r, n = n0 + wn * 64 + (lane & 7) * 8;
+                    if (mr < p.M && n < p.N) __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(reinterpret_cast<bf16_t*>(p.out) + (size_t)mr * p.ldo + n));
+                }
+            }
+        }
+    } else {
+        lx_loss_epilogue<FM, true>(p, acc, m0 + wm * FM * 16, n0 + wn * 64, sm + wave * (16 * 64));
+    }
+}
+
+// out = scale * sum over the splits of slab[s] (+ add), fixed order; N % 4 == 0
+__global__ __launch_bounds__(256) void lx_reduce_kernel(const LxGemmParams p) {
+    const size_t total = (size_t)p.M * p.N / 4, stride = (size_t)p.M * p.N;
+    const float sc = p.scale != nullptr ? p.scale[0] : 1.0f;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+        const float* q = p.slab + i * 4;
+        f32x4 s = *reinterpret_cast<const f32x4*>(q);
+#pragma unroll 4
+        for (int k = 1; k < p.splits; ++k) s += *reinterpret_cast<const f32x4*>(q + k * stride);
+        s *= sc;
+        if (p.add != nullptr) s += *reinterpret_cast<const f32x4*>(p.add + i * 4);
+        const size_t m = i * 4 / p.N, n = i * 4 - m * p.N;
+        if (p.out_f32) {
+            *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.out) + m * p.ldo + n) = s;
+        } else {
+            uint2 o;
+            o.x = pack2bf(s[0], s[1]);
+            o.y = pack2bf(s[2], s[3]);
+            *reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(p.out) + m * p.ldo + n) = o;
+        }
     }
 }
 
@@ -720,6 +991,7 @@ __global__ __launch_bounds__(256) void lx_colsum_final_kernel(const float* __res
 
 // ---------------------------------------------------------------------------------------------------- host
 #define LX_RANGES 64
+#define LX_CACHED ((size_t)640 << 20)
 
 static int lx_cus() {
     static int cache[64] = {0};
@@ -738,7 +1010,9 @@ static size_t lx_up(size_t n) { return (n + 255) & ~(size_t)255; }
 // that what they share of the other operand is fetched once; there are tiles_m * tiles_n / width rows.  Of `teams` teams, team t takes the
 // whole rows t, t + teams, ... below `whole`; the `rest` rows behind them are one sequence of rest * steps steps, cut into `ranges`
 // equal ranges (at most two parts of rows each) whose fp32 sums go to slab[2 range + part][width][256][256] and are joined in order.
-struct LxDeal { int width, teams, whole, rest, ranges; };
+// The small kernel (kind LX_SMALL64, LX_SMALL128): `splits` ranges of steps per tile, slab[splits][M][N].
+enum { LX_BIG = 0, LX_SMALL128 = 1, LX_SMALL64 = 2 };
+struct LxDeal { int kind, width, teams, whole, rest, ranges, splits; size_t slab; double us; };
 // how the rows are cut and where everything lies in the workspace
 struct LxPlan {
     long long ldp, stat_cols;
@@ -746,26 +1020,70 @@ struct LxPlan {
     LxDeal dx[2], dw[2];            // of a block, of the last one
     size_t scale, stats, zsum, P, acc, slab, colpart, colsum, total;
 };
-// Whole rows alone take ceil(rows / teams) rounds; cutting what does not fill a round into ranges fills it at the price of parts written and
-// read.  Costs in steps (about 1.4 us): a tile's epilogue and the fill of the pipeline 4, a part of 256 x 256 that is written and read 0.09
-// (512 KB at 4 TB/s).
-static LxDeal lx_deal(int M, int N, int steps, int cus) {
-    const int tiles_n = (N + LX_TILE - 1) / LX_TILE;
+// The kernel and its cut that a model of the time finds fastest, in microseconds on 256 compute units, from 28 shapes between 1 x 1000 x 192 and
+// 512 x 100003 x 1024 measured with each of the three kernels (time of x W^T / dz W / dz^T x in us, large : 128 : 64):
+//   1 x 1000 x 192       10 24 8 : 7 8 7 : 4 7 4              512 x 8192 x 768     22 32 17 : 15 21 14 : 19 19 16
+//   1024 x 1024 x 1024   30 31 29 : 16 17 16 : 11 12 10       8192 x 8192 x 768    92 129 129 : 157 114 99 : 244 154 156
+//   512 x 21843 x 768    25 50 31 : 31 36 34 : 47 33 36       512 x 100003 x 1024  117 131 125 : 158 156 189 : 245 262 260
+// Large: whole rows alone take ceil(rows / teams) rounds; cutting what does not fill a round into ranges fills it at the price of parts written
+// and read, 0.13 us for one of 256 x 256 (512 KB at 4 TB/s).
+#define LX_US_STEP 1.25
+#define LX_US_PART 0.13
+static LxDeal lx_deal_big(int M, int N, int steps, int cus, bool loss) {
     LxDeal d = {};
+    d.kind = LX_BIG;
+    d.splits = 1;
+    const int tiles_m = (M + LX_TILE - 1) / LX_TILE, tiles_n = (N + LX_TILE - 1) / LX_TILE;
+    if (loss) {             // the logits: whole tiles, dealt one by one
+        const long long tiles = (long long)tiles_m * tiles_n;
+        d.teams = tiles < cus ? (int)tiles : cus;
+        d.us = 4.0 + (double)((tiles + cus - 1) / cus) * (steps * LX_US_STEP + 7.5);
+        return d;
+    }
+    const double tile = 6.0;
     for (d.width = tiles_n < 8 ? tiles_n : 8; tiles_n % d.width; --d.width) {}
-    const int rows = (M + LX_TILE - 1) / LX_TILE * (tiles_n / d.width);
+    const int rows = tiles_m * (tiles_n / d.width);
     const int most = cus / d.width > 0 ? cus / d.width : 1;
     const int rounds = rows / most, rest = rows - rounds * most;
     d.teams = rows < most ? rows : most;
     d.whole = rows;
+    d.us = 4.0 + (rounds + (rest > 0)) * (steps * LX_US_STEP + tile);
     if (rest == 0 || (long long)rest * steps > 0x7fffffff) return d;
-    const double part = 0.09 * (M < LX_TILE ? M : LX_TILE) / LX_TILE * d.width;
-    double best = 0.98 * (rounds + 1) * (steps + 4.0);
+    const double part = LX_US_PART * (M < LX_TILE ? M : LX_TILE) / LX_TILE * d.width;
     for (int k = 1; k <= 16; ++k) {
         const int ranges = most * k / 16;
         if (ranges <= rest || (long long)rest * steps / ranges < 2) continue;
-        const double cost = rounds * (steps + 4.0) + (double)rest * steps / ranges + 12.0 + part * (ranges + rest);
-        if (cost < best) { best = cost; d.teams = rounds > 0 ? most : ranges; d.whole = rounds * most; d.rest = rest; d.ranges = ranges; }
+        const double us = 8.0 + rounds * (steps * LX_US_STEP + tile) + (double)rest * steps / ranges * LX_US_STEP + 2 * tile + part * (ranges + rest);
+        if (us < 0.98 * d.us) { d.us = us; d.teams = rounds > 0 ? most : ranges; d.whole = rounds * most; d.rest = rest; d.ranges = ranges; }
+    }
+    d.slab = (size_t)2 * d.ranges * d.width * 65536;
+    return d;
+}
+// Small: a step of a workgroup alone on its compute unit takes `alone`, workgroups that share one get a step in `shared` each in turn.
+static LxDeal lx_deal_small(int M, int N, int steps, int cus, bool loss, int kind) {
+    const bool s64 = kind == LX_SMALL64;
+    const int tile = s64 ? 64 : 128;
+    const double alone = s64 ? 0.30 : 0.62, shared = s64 ? 0.31 : loss ? 0.52 : 0.45, base = s64 ? 3.2 : 4.0, last = loss ? (s64 ? 0.6 : 2.5) : (s64 ? 0.3 : 0.8);
+    const long long tiles = (long long)((M + tile - 1) / tile) * ((N + tile - 1) / tile);
+    LxDeal best = {};
+    best.us = 1e30;
+    for (int splits = 1; splits <= (loss ? 1 : 256); splits += splits < 8 ? 1 : splits / 4) {
+        if (splits > 1 && steps / splits < 4) break;
+        const long long wgs = tiles * splits, per = (wgs + cus - 1) / cus;
+        if (wgs > 0x7fffffff) break;
+        double us = base + ((steps + splits - 1) / splits) * (per > 1 ? shared * per : alone) + last * per;
+        if (splits > 1) us += 3.0 + 2e-6 * splits * M * N;          // the sums written and read at 4 TB/s, and another launch
+        if (us >= best.us) continue;
+        best.us = us; best.kind = kind; best.splits = splits;
+        best.slab = splits > 1 ? (size_t)splits * M * N : 0;
+    }
+    return best;
+}
+static LxDeal lx_deal(int M, int N, int steps, int cus, bool loss) {
+    LxDeal d = lx_deal_big(M, N, steps, cus, loss);
+    for (int kind : {LX_SMALL128, LX_SMALL64}) {
+        const LxDeal e = lx_deal_small(M, N, steps, cus, loss, kind);
+        if (e.us < d.us) d = e;
     }
     return d;
 }
@@ -786,24 +1104,22 @@ static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw
     q.blocks = (int)((T + rows - 1) / rows);
     size_t at = 0;
     auto take = [&](size_t n) { const size_t here = at; at += lx_up(n); return here; };
-    q.scale = take(16);
+    q.scale = take(16 + LX_LOSS_WGS * sizeof(LxLossPart));          // scale, ticket, the loss's parts
     q.stats = take((size_t)rows * q.stat_cols * sizeof(float2));
     q.zsum = smoothing ? take((size_t)rows * q.stat_cols * sizeof(float)) : 0;
     if (grad) {
         q.P = take((size_t)rows * q.ldp * 2);
         if (q.blocks > 1 && !dw_f32) q.acc = take((size_t)V * D * sizeof(float));
         const int cus = lx_cus();
-        size_t parts = 0;           // tiles of partial sums; dx and dW use them one after the other
+        size_t slab = 0;            // dx and dW use it one after the other
         for (int last = 0; last < 2; ++last) {
             const int n = last ? (int)(T - (long long)(q.blocks - 1) * rows) : (int)rows;
-            q.dx[last] = lx_deal(n, D, (V + LX_BK - 1) / LX_BK, cus);
-            q.dw[last] = lx_deal(V, D, (n + LX_BK - 1) / LX_BK, cus);
-            for (const LxDeal& d : {q.dx[last], q.dw[last]}) {
-                const size_t need = (size_t)2 * d.ranges * d.width;
-                if (need > parts) parts = need;
-            }
+            q.dx[last] = lx_deal(n, D, (V + LX_BK - 1) / LX_BK, cus, false);
+            q.dw[last] = lx_deal(V, D, (n + LX_BK - 1) / LX_BK, cus, false);
+            if (q.dx[last].slab > slab) slab = q.dx[last].slab;
+            if (q.dw[last].slab > slab) slab = q.dw[last].slab;
         }
-        if (parts > 0) q.slab = take(parts * 65536 * sizeof(float));
+        if (slab > 0) q.slab = take(slab * sizeof(float));
         if (bias) {
             q.colpart = take((size_t)LX_RANGES * q.ldp * sizeof(float));
             q.colsum = take((size_t)V * sizeof(float));
@@ -814,12 +1130,30 @@ static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw
 }
 
 template <int LAY, int EPI>
-static int lx_launch(const LxGemmParams& p, int grid, hipStream_t s, const char* what) {
+static int lx_launch(LxGemmParams& p, const LxDeal& d, hipStream_t s, const char* what) {
+    const int tile = d.kind == LX_SMALL64 ? 64 : d.kind == LX_SMALL128 ? 128 : LX_TILE;
+    p.tiles_m = (p.M + tile - 1) / tile;
+    p.tiles_n = (p.N + tile - 1) / tile;
+    if (d.kind != LX_BIG) {
+        constexpr int E = EPI == LX_OUT ? LX_OUT : LX_XENT_BIAS;
+        p.splits = d.splits;
+        const int grid = p.tiles_m * p.tiles_n * d.splits;
+        if (d.kind == LX_SMALL64) lx_small_kernel<LAY, E, 1, 4, 1><<<grid, 256, 0, s>>>(p);
+        else lx_small_kernel<LAY, E, 4, 2, 2><<<grid, 256, 0, s>>>(p);
+        if (int rc = vitk_check_launch(what)) return rc;
+        if (d.splits > 1) {
+            const long long quads = (long long)p.M * p.N / 4;
+            lx_reduce_kernel<<<(int)((quads + 255) / 256 < 4096 ? (quads + 255) / 256 : 4096), 256, 0, s>>>(p);
+        }
+        return vitk_check_launch(what);
+    }
     static VitkLdsOnce once = {};
     if (int rc = vitk_lds_once(once, (const void*)lx_gemm_kernel<LAY, EPI>, LX_LDS, what)) return rc;
+    p.width = d.width; p.teams = d.teams; p.whole = d.whole; p.rest = d.rest; p.ranges = d.ranges;
+    const int grid = EPI == LX_OUT ? d.teams * d.width : d.teams;
     lx_gemm_kernel<LAY, EPI><<<grid, 512, LX_LDS, s>>>(p);
     if (int rc = vitk_check_launch(what)) return rc;
-    if (p.rest > 0) lx_join_kernel<<<p.rest * p.width * 32, 256, 0, s>>>(p);
+    if (EPI == LX_OUT && p.rest > 0) lx_join_kernel<<<p.rest * p.width * 32, 256, 0, s>>>(p);
     return vitk_check_launch(what);
 }
 
@@ -855,9 +1189,10 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
     const int cus = lx_cus();
     char* ws = (char*)workspace;
     float* scale = (float*)(ws + q.scale);
+    unsigned* ticket = (unsigned*)(ws + q.scale + 8);
     const long long* tg = (const long long*)target;
     if (q.blocks > 1 && grad) {
-        lx_loss_kernel<<<1, 1024, 0, s>>>(tg, ignore_index, nullptr, (int)T, mean, scale, nullptr);
+        lx_loss_kernel<<<1, 256, 0, s>>>(tg, ignore_index, nullptr, (int)T, (int)T, mean, nullptr, nullptr, scale, nullptr);
         if (int rc = vitk_check_launch("linear_xent_count")) return rc;
     }
     for (int b = 0; b < q.blocks; ++b) {
@@ -867,22 +1202,38 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         LxGemmParams g = {};
         g.A = (const bf16_t*)x + r0 * ldx; g.lda = (int)ldx; g.B = (const bf16_t*)w; g.ldb = (int)ldw;
         g.M = n; g.N = V; g.KA = g.KB = D; g.steps = (D + LX_BK - 1) / LX_BK;
-        g.tiles_m = (n + LX_TILE - 1) / LX_TILE; g.tiles_n = (int)(q.ldp / LX_TILE);
         g.bias = bias; g.bias_type = bias_type;
         g.stats = (float2*)(ws + q.stats); g.stat_cols = (int)q.stat_cols; g.zsum = smoothing > 0.f ? (float*)(ws + q.zsum) : nullptr;
         g.P = grad ? (_Float16*)(ws + q.P) : nullptr; g.ldp = q.ldp;
-        const long long tiles = (long long)g.tiles_m * g.tiles_n;
-        const int grid = tiles < cus ? (int)tiles : cus;
-        if (int rc = g.bias || g.zsum ? lx_launch<LX_NT, LX_XENT_BIAS>(g, grid, s, "linear_xent_logits")
-                                      : lx_launch<LX_NT, LX_XENT>(g, grid, s, "linear_xent_logits"))
+        const LxDeal dz_deal = lx_deal(n, V, g.steps, cus, true);
+        if (int rc = g.bias || g.zsum ? lx_launch<LX_NT, LX_XENT_BIAS>(g, dz_deal, s, "linear_xent_logits")
+                                      : lx_launch<LX_NT, LX_XENT>(g, dz_deal, s, "linear_xent_logits"))
             return rc;
         LxRowParams r = {};
         r.x = g.A; r.ldx = ldx; r.w = g.B; r.ldw = ldw; r.bias = bias; r.bias_type = bias_type; r.target = tg + r0; r.ignore_index = ignore_index;
-        r.stats = g.stats; r.zsum = g.zsum; r.stat_cols = g.stat_cols; r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.smoothing = smoothing;
-        lx_row_kernel<<<n, 256, 0, s>>>(r);
+        r.stats = g.stats; r.zsum = g.zsum; r.stat_cols = g.stat_cols; r.ticket = ticket; r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.rows_n = n; r.smoothing = smoothing;
+        // long rows get more waves.  By the vocabulary alone, so that a row's sums do not depend on how many rows there are or what is wanted.
+        // STREAM: past the caches, where the block is larger than they are.
+        const bool stream = grad && (size_t)n * q.ldp * 2 > LX_CACHED;
+        if (q.ldp >= 65536) {
+            if (stream) lx_row_kernel<16, true><<<n, 1024, 0, s>>>(r);
+            else lx_row_kernel<16, false><<<n, 1024, 0, s>>>(r);
+        } else if (q.ldp >= 16384) {
+            if (stream) lx_row_kernel<8, true><<<n, 512, 0, s>>>(r);
+            else lx_row_kernel<8, false><<<n, 512, 0, s>>>(r);
+        } else if (q.ldp >= 4096) {
+            if (stream) lx_row_kernel<4, true><<<n, 256, 0, s>>>(r);
+            else lx_row_kernel<4, false><<<n, 256, 0, s>>>(r);
+        } else {
+            if (stream) lx_row_kernel<1, true><<<(n + 3) / 4, 256, 0, s>>>(r);
+            else lx_row_kernel<1, false><<<(n + 3) / 4, 256, 0, s>>>(r);
+        }
         if (int rc = vitk_check_launch("linear_xent_rows")) return rc;
         if (last) {
-            lx_loss_kernel<<<1, 1024, 0, s>>>(tg, ignore_index, rows, (int)T, mean, q.blocks > 1 ? nullptr : scale, loss);
+            int per = (int)((T + LX_LOSS_WGS - 1) / LX_LOSS_WGS);
+            if (per < 1024) per = 1024;
+            lx_loss_kernel<<<(int)((T + per - 1) / per), 256, 0, s>>>(tg, ignore_index, rows, (int)T, per, mean, (LxLossPart*)(ws + q.scale + 16), ticket,
+                                                                      q.blocks > 1 ? nullptr : scale, loss);
             if (int rc = vitk_check_launch("linear_xent_loss")) return rc;
         }
         if (!grad) continue;
@@ -890,23 +1241,17 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         // dx = dz W: dz is zero behind the vocabulary up to its row stride
         LxGemmParams d = {};
         d.A = dz; d.lda = (int)q.ldp; d.B = (const bf16_t*)w; d.ldb = (int)ldw; d.M = n; d.N = D; d.KA = (int)q.ldp; d.KB = V; d.steps = (V + LX_BK - 1) / LX_BK;
-        d.tiles_m = (n + LX_TILE - 1) / LX_TILE; d.tiles_n = (D + LX_TILE - 1) / LX_TILE;
-        const LxDeal& dd = q.dx[last];
-        d.width = dd.width; d.teams = dd.teams; d.whole = dd.whole; d.rest = dd.rest; d.ranges = dd.ranges;
         d.scale = scale; d.out = (bf16_t*)dx + r0 * lddx; d.ldo = lddx; d.slab = (float*)(ws + q.slab);
-        if (int rc = lx_launch<LX_NN, LX_OUT>(d, dd.teams * dd.width, s, "linear_xent_dx")) return rc;
+        if (int rc = lx_launch<LX_NN, LX_OUT>(d, q.dx[last], s, "linear_xent_dx")) return rc;
         // dW = dz^T x, summed over the blocks in fp32
         LxGemmParams e = {};
         e.A = dz; e.lda = (int)q.ldp; e.B = g.A; e.ldb = (int)ldx; e.M = V; e.N = D; e.KA = e.KB = n; e.steps = (n + LX_BK - 1) / LX_BK;
-        e.tiles_m = (V + LX_TILE - 1) / LX_TILE; e.tiles_n = (D + LX_TILE - 1) / LX_TILE;
-        const LxDeal& de = q.dw[last];
-        e.width = de.width; e.teams = de.teams; e.whole = de.whole; e.rest = de.rest; e.ranges = de.ranges;
         e.scale = scale; e.slab = d.slab;
         float* acc = dw_f32 ? (float*)dw : (float*)(ws + q.acc);
         e.add = b > 0 ? acc : nullptr;
         if (last) { e.out = dw; e.ldo = lddw; e.out_f32 = dw_f32; }
         else { e.out = acc; e.ldo = D; e.out_f32 = 1; }
-        if (int rc = lx_launch<LX_TN, LX_OUT>(e, de.teams * de.width, s, "linear_xent_dw")) return rc;
+        if (int rc = lx_launch<LX_TN, LX_OUT>(e, q.dw[last], s, "linear_xent_dw")) return rc;
         if (db != nullptr) {
             float* part = (float*)(ws + q.colpart);
             int per = (n + LX_RANGES - 1) / LX_RANGES;
