@@ -50,6 +50,7 @@ struct LxGemmParams {
     float2* stats; int stat_cols;           // [M][stat_cols]: (m log2 e, s) of 64 columns
     float* zsum;                            // [M][stat_cols] sums of the logits, null: not wanted (no smoothing)
     _Float16* P; long long ldp;             // null: loss alone
+    unsigned* ticket;                       // zeroed here for the kernels that follow
 };
 
 static __device__ __forceinline__ int lx_swz(int m) { return (((m >> 3) & 1) << 3) | ((m & 3) << 1); }
@@ -384,6 +385,7 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
     // us at 8192 x 100003 x 2048); dz W streams dz from memory along its long contraction and gains 9 % (2755 -> 2500 us).
     // The output stores of a full tile (16 of a wave at least) between two steps may stay in flight over the first step's waits.
     constexpr bool DEEP = LAY == LX_NN;
+    if (EPI != LX_OUT && blockIdx.x == 0 && tid == 0) *p.ticket = 0u;
     if (items == 0) return;
     aim(0);
     stageB(0); stageA(0, 0); stageA(0, 1);
@@ -523,7 +525,7 @@ struct LxRowParams {
     const void* bias; int bias_type;
     const long long* target; long long ignore_index;
     const float2* stats; const float* zsum; int stat_cols;
-    unsigned* ticket;                  // zeroed for lx_loss_kernel
+    unsigned* ticket; float* scale; float* loss; int mean;      // loss not null: the last row to finish adds the rows up (see lx_loss_kernel)
     bf16_t* P; long long ldp;          // fp16 on entry, bf16 dz on exit; null: loss alone
     float* rows;
     int V, D, rows_n;
@@ -582,6 +584,37 @@ static __device__ __forceinline__ u32x4 lx_dz8(const u32x4 r, float f, float u, 
     return (u32x4){pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])};
 }
 
+// the sum of up to LX_FUSED rows' losses and their count, by one wave, in an order of its own: lane by lane, then the lanes
+#define LX_FUSED 512
+static __device__ __forceinline__ void lx_finish(double s, long long count, int mean, float* scale, float* loss) {
+    if (scale != nullptr) *scale = count == 0 ? 0.f : mean ? (float)(1.0 / (double)count) : 1.f;
+    if (loss != nullptr) *loss = (float)(count == 0 ? 0.0 : mean ? s / (double)count : s);
+}
+// a row's loss is known: stored, and where p.loss is set the wave that is the last of all rows' first waves adds them up
+static __device__ __forceinline__ void lx_row_done(const LxRowParams& p, int row, int tid, float l) {
+    if (tid >= 64) return;
+    if (p.loss == nullptr) {
+        if (tid == 0) p.rows[row] = l;
+        return;
+    }
+    unsigned n = 0;
+    if (tid == 0) {
+        __hip_atomic_store(p.rows + row, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        n = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if ((int)__builtin_amdgcn_readfirstlane(n) != p.rows_n - 1) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    double s = 0.0;
+    int count = 0;
+    for (int i = tid; i < p.rows_n; i += 64) {
+        s += (double)__hip_atomic_load(p.rows + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        count += p.target[i] != p.ignore_index;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); count += __shfl_xor(count, o, 64); }
+    if (tid == 0) lx_finish(s, count, p.mean, p.scale, p.loss);
+}
+
 // WAVES waves per row: one workgroup, or for short rows one wave of a workgroup of four.  Bound by memory: 4 bytes per logit where the gradient
 // is wanted, nothing to speak of where it is not.
 #ifndef LX_NTS
@@ -595,14 +628,13 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
     const int tid = WAVES == 1 ? (int)threadIdx.x & 63 : (int)threadIdx.x;
     const int row = WAVES == 1 ? (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6) : (int)blockIdx.x;
     if (row >= p.rows_n) return;
-    if (row == 0 && tid == 0) *p.ticket = 0u;
     const long long t64 = p.target[row];
     bf16_t* P = p.P != nullptr ? p.P + (size_t)row * p.ldp : nullptr;
     const int chunks = (int)(p.ldp / 8);
     if (t64 == p.ignore_index) {
-        if (tid == 0) p.rows[row] = 0.f;
         if (P != nullptr)
             for (int c = tid; c < chunks; c += NT) __builtin_nontemporal_store((u32x4){0u, 0u, 0u, 0u}, reinterpret_cast<u32x4*>(P) + c);
+        lx_row_done(p, row, tid, 0.f);
         return;
     }
     // a label outside [0, V) never becomes an address: the row's loss and gradient are NaN
@@ -638,11 +670,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
     if (p.smoothing > 0.f) zs = lx_block_sum<WAVES>(zs, sh);
     if (p.bias != nullptr) dot += p.bias_type == 1 ? bf2f(reinterpret_cast<const bf16_t*>(p.bias)[t]) : reinterpret_cast<const float*>(p.bias)[t];
     const float lse2 = ref + log2f(s), lse = lse2 * 0.69314718055994530942f;
-    if (tid == 0) {
-        float l = lse - dot;
-        if (p.smoothing > 0.f) l = (1.f - p.smoothing) * l + p.smoothing * (lse - zs / (float)p.V);
-        p.rows[row] = valid ? l : __builtin_nanf("");
-    }
+    float l = lse - dot;
+    if (p.smoothing > 0.f) l = (1.f - p.smoothing) * l + p.smoothing * (lse - zs / (float)p.V);
+    lx_row_done(p, row, tid, valid ? l : __builtin_nanf(""));
     if (P == nullptr) return;
     const float u = p.smoothing / (float)p.V, hit = 1.f - p.smoothing;
     u32x4* q = reinterpret_cast<u32x4*>(P);
@@ -668,7 +698,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
 }
 
 // Count of the counted rows, the scale of the gradients (1 / count, or 1 for a sum; 0 without a counted row) and the loss.  Workgroup b sums
-// a stretch of the rows into part[b]; the last one to finish adds the parts in order (lx_row_kernel has zeroed the ticket).
+// a stretch of the rows into part[b]; the last one to finish adds the parts in order (the kernel that made the logits has zeroed the ticket).
 #define LX_LOSS_WGS 64
 struct LxLossPart { double sum; long long count; };
 __global__ __launch_bounds__(256) void lx_loss_kernel(const long long* __restrict__ target, long long ignore_index, const float* __restrict__ rows, int T, int per,
@@ -719,20 +749,20 @@ __global__ __launch_bounds__(256) void lx_loss_kernel(const long long* __restric
 // however short it is: one tile of (16 FM WM) x (64 WN) and one range of steps per 256-thread workgroup, several workgroups on a compute unit
 // in place of a deep pipeline within one.  FM = 4, waves 2 x 2: 128 x 128 tiles, 64 KB of LDS; FM = 1, waves 4 x 1: 64 x 64, 32 KB.
 // LX_OUT with p.splits > 1: the fp32 sums of range s go to slab[s][M][N].
+template <int FM, int WM, int WN> struct LxSmall { static constexpr int lds = 2 * (FM * 16 * WM + 64 * WN) * LX_BK; };       // elements
 template <int LAY, int EPI, int FM, int WM, int WN>
-__global__ __launch_bounds__(256) void lx_small_kernel(const LxGemmParams p) {
+static __device__ __forceinline__ void lx_small_body(const LxGemmParams& p, bf16_t* sm, int block, int blocks) {
     constexpr bool AT = LAY == LX_TN, BT = LAY != LX_NT;
     constexpr int TM = FM * 16 * WM, TN = 64 * WN;              // the tile
     constexpr int PA = TM / 32, PB = TN / 32;                   // 1 KB pieces of an operand's step per wave
     constexpr int EA = TM * LX_BK, EB = TN * LX_BK;             // elements of a buffer
-    __shared__ __attribute__((aligned(1024))) bf16_t sm[2 * (EA + EB)];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
     const int lr = lane & 15, lg = lane >> 4, lq = lr >> 2, lp = lr & 3;
     const unsigned lds_base = __builtin_amdgcn_readfirstlane(lds_addr(sm));
 
-    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int id = xcd_remap(block, blocks);
     const int tiles = p.tiles_m * p.tiles_n;
     const int split = __builtin_amdgcn_readfirstlane(id / tiles);
     const int tile = id - split * tiles;
@@ -885,6 +915,19 @@ __global__ __launch_bounds__(256) void lx_small_kernel(const LxGemmParams p) {
         lx_loss_epilogue<FM, true>(p, acc, m0 + wm * FM * 16, n0 + wn * 64, sm + wave * (16 * 64));
     }
 }
+template <int LAY, int EPI, int FM, int WM, int WN>
+__global__ __launch_bounds__(256) void lx_small_kernel(const LxGemmParams p) {
+    __shared__ __attribute__((aligned(1024))) bf16_t sm[LxSmall<FM, WM, WN>::lds];
+    if (EPI != LX_OUT && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0u;
+    lx_small_body<LAY, EPI, FM, WM, WN>(p, sm, blockIdx.x, gridDim.x);
+}
+// dx and dW in one launch: both need dz alone.  The first `blocks` workgroups are those of dx.
+template <int FM, int WM, int WN>
+__global__ __launch_bounds__(256) void lx_small_grads_kernel(const LxGemmParams dx, const LxGemmParams dw, int blocks) {
+    __shared__ __attribute__((aligned(1024))) bf16_t sm[LxSmall<FM, WM, WN>::lds];
+    if ((int)blockIdx.x < blocks) lx_small_body<LX_NN, LX_OUT, FM, WM, WN>(dx, sm, blockIdx.x, blocks);
+    else lx_small_body<LX_TN, LX_OUT, FM, WM, WN>(dw, sm, blockIdx.x - blocks, gridDim.x - blocks);
+}
 
 // out = scale * sum over the splits of slab[s] (+ add), fixed order; N % 4 == 0
 __global__ __launch_bounds__(256) void lx_reduce_kernel(const LxGemmParams p) {
@@ -989,6 +1032,32 @@ __global__ __launch_bounds__(256) void lx_colsum_final_kernel(const float* __res
     else reinterpret_cast<bf16_t*>(db)[n] = f2bf(s);
 }
 
+// the same for up to 1024 rows in one launch: a workgroup sums 128 columns, 16 rows at a time
+__global__ __launch_bounds__(256) void lx_colsum_few_kernel(const bf16_t* __restrict__ dz, long long ldp, int T, int V, const float* __restrict__ scale, void* __restrict__ db, int db_f32) {
+    __shared__ float sh[16][128];
+    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
+    const long long col = (long long)blockIdx.x * 128 + lane * 8;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int r = group; r < T; r += 16) {
+        float v[8];
+        load8(dz + (size_t)r * ldp + col, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += v[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sh[group][lane * 8 + k] = acc[k];
+    __syncthreads();
+    const int n = blockIdx.x * 128 + (int)threadIdx.x;
+    if (threadIdx.x >= 128 || n >= V) return;
+    float s = 0.f;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) s += sh[g][threadIdx.x];
+    s *= scale[0];
+    if (db_f32) reinterpret_cast<float*>(db)[n] = s;
+    else reinterpret_cast<bf16_t*>(db)[n] = f2bf(s);
+}
+
 // ---------------------------------------------------------------------------------------------------- host
 #define LX_RANGES 64
 #define LX_CACHED ((size_t)640 << 20)
@@ -1087,6 +1156,18 @@ static LxDeal lx_deal(int M, int N, int steps, int cus, bool loss) {
     }
     return d;
 }
+// dx and dW of the same small kind share a launch: about 5 us less for the two, and each fills what the other leaves
+static bool lx_one_launch(const LxDeal& dx, const LxDeal& dw) { return dx.kind == dw.kind && dx.kind != LX_BIG; }
+static void lx_deal_grads(int n, int V, int D, int cus, LxDeal& dx, LxDeal& dw) {
+    const int sx = (V + LX_BK - 1) / LX_BK, sw = (n + LX_BK - 1) / LX_BK;
+    dx = lx_deal(n, D, sx, cus, false);
+    dw = lx_deal(V, D, sw, cus, false);
+    if (lx_one_launch(dx, dw)) return;
+    for (int kind : {LX_SMALL128, LX_SMALL64}) {
+        const LxDeal x = lx_deal_small(n, D, sx, cus, false, kind), w = lx_deal_small(V, D, sw, cus, false, kind);
+        if (x.us + w.us < dx.us + dw.us + 5.0) { dx = x; dw = w; return; }
+    }
+}
 static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw_f32, int bias, size_t block_bytes) {
     LxPlan q = {};
     q.ldp = ((long long)V + LX_TILE - 1) / LX_TILE * LX_TILE;
@@ -1112,11 +1193,11 @@ static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw
         if (q.blocks > 1 && !dw_f32) q.acc = take((size_t)V * D * sizeof(float));
         const int cus = lx_cus();
         size_t slab = 0;            // dx and dW use it one after the other
-        for (int last = 0; last < 2; ++last) {
+        for (int last = q.blocks > 1 ? 0 : 1; last < 2; ++last) {          // [1]: the last block, which may be the only one
             const int n = last ? (int)(T - (long long)(q.blocks - 1) * rows) : (int)rows;
-            q.dx[last] = lx_deal(n, D, (V + LX_BK - 1) / LX_BK, cus, false);
-            q.dw[last] = lx_deal(V, D, (n + LX_BK - 1) / LX_BK, cus, false);
-            if (q.dx[last].slab > slab) slab = q.dx[last].slab;
+            lx_deal_grads(n, V, D, cus, q.dx[last], q.dw[last]);
+            const size_t need = q.dx[last].slab + (lx_one_launch(q.dx[last], q.dw[last]) ? q.dw[last].slab : 0);
+            if (need > slab) slab = need;
             if (q.dw[last].slab > slab) slab = q.dw[last].slab;
         }
         if (slab > 0) q.slab = take(slab * sizeof(float));
@@ -1129,23 +1210,27 @@ static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw
     return q;
 }
 
-template <int LAY, int EPI>
-static int lx_launch(LxGemmParams& p, const LxDeal& d, hipStream_t s, const char* what) {
+static void lx_tiles(LxGemmParams& p, const LxDeal& d) {
     const int tile = d.kind == LX_SMALL64 ? 64 : d.kind == LX_SMALL128 ? 128 : LX_TILE;
     p.tiles_m = (p.M + tile - 1) / tile;
     p.tiles_n = (p.N + tile - 1) / tile;
+    p.splits = d.splits;
+}
+static int lx_reduce(const LxGemmParams& p, hipStream_t s, const char* what) {
+    const long long quads = (long long)p.M * p.N / 4;
+    lx_reduce_kernel<<<(int)((quads + 255) / 256 < 4096 ? (quads + 255) / 256 : 4096), 256, 0, s>>>(p);
+    return vitk_check_launch(what);
+}
+template <int LAY, int EPI>
+static int lx_launch(LxGemmParams& p, const LxDeal& d, hipStream_t s, const char* what) {
+    lx_tiles(p, d);
     if (d.kind != LX_BIG) {
         constexpr int E = EPI == LX_OUT ? LX_OUT : LX_XENT_BIAS;
-        p.splits = d.splits;
         const int grid = p.tiles_m * p.tiles_n * d.splits;
         if (d.kind == LX_SMALL64) lx_small_kernel<LAY, E, 1, 4, 1><<<grid, 256, 0, s>>>(p);
         else lx_small_kernel<LAY, E, 4, 2, 2><<<grid, 256, 0, s>>>(p);
         if (int rc = vitk_check_launch(what)) return rc;
-        if (d.splits > 1) {
-            const long long quads = (long long)p.M * p.N / 4;
-            lx_reduce_kernel<<<(int)((quads + 255) / 256 < 4096 ? (quads + 255) / 256 : 4096), 256, 0, s>>>(p);
-        }
-        return vitk_check_launch(what);
+        return d.splits > 1 ? lx_reduce(p, s, what) : VITK_OK;
     }
     static VitkLdsOnce once = {};
     if (int rc = vitk_lds_once(once, (const void*)lx_gemm_kernel<LAY, EPI>, LX_LDS, what)) return rc;
@@ -1204,14 +1289,15 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         g.M = n; g.N = V; g.KA = g.KB = D; g.steps = (D + LX_BK - 1) / LX_BK;
         g.bias = bias; g.bias_type = bias_type;
         g.stats = (float2*)(ws + q.stats); g.stat_cols = (int)q.stat_cols; g.zsum = smoothing > 0.f ? (float*)(ws + q.zsum) : nullptr;
-        g.P = grad ? (_Float16*)(ws + q.P) : nullptr; g.ldp = q.ldp;
+        g.P = grad ? (_Float16*)(ws + q.P) : nullptr; g.ldp = q.ldp; g.ticket = ticket;
         const LxDeal dz_deal = lx_deal(n, V, g.steps, cus, true);
         if (int rc = g.bias || g.zsum ? lx_launch<LX_NT, LX_XENT_BIAS>(g, dz_deal, s, "linear_xent_logits")
                                       : lx_launch<LX_NT, LX_XENT>(g, dz_deal, s, "linear_xent_logits"))
             return rc;
         LxRowParams r = {};
         r.x = g.A; r.ldx = ldx; r.w = g.B; r.ldw = ldw; r.bias = bias; r.bias_type = bias_type; r.target = tg + r0; r.ignore_index = ignore_index;
-        r.stats = g.stats; r.zsum = g.zsum; r.stat_cols = g.stat_cols; r.ticket = ticket; r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.rows_n = n; r.smoothing = smoothing;
+        r.stats = g.stats; r.zsum = g.zsum; r.stat_cols = g.stat_cols; const bool fused = q.blocks == 1 && T <= LX_FUSED;
+        r.ticket = ticket; r.scale = scale; r.loss = fused ? loss : nullptr; r.mean = mean; r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.rows_n = n; r.smoothing = smoothing;
         // long rows get more waves.  By the vocabulary alone, so that a row's sums do not depend on how many rows there are or what is wanted.
         // STREAM: past the caches, where the block is larger than they are.
         const bool stream = grad && (size_t)n * q.ldp * 2 > LX_CACHED;
@@ -1229,7 +1315,7 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
             else lx_row_kernel<1, false><<<(n + 3) / 4, 256, 0, s>>>(r);
         }
         if (int rc = vitk_check_launch("linear_xent_rows")) return rc;
-        if (last) {
+        if (last && !fused) {
             int per = (int)((T + LX_LOSS_WGS - 1) / LX_LOSS_WGS);
             if (per < 1024) per = 1024;
             lx_loss_kernel<<<(int)((T + per - 1) / per), 256, 0, s>>>(tg, ignore_index, rows, (int)T, per, mean, (LxLossPart*)(ws + q.scale + 16), ticket,
@@ -1242,7 +1328,6 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         LxGemmParams d = {};
         d.A = dz; d.lda = (int)q.ldp; d.B = (const bf16_t*)w; d.ldb = (int)ldw; d.M = n; d.N = D; d.KA = (int)q.ldp; d.KB = V; d.steps = (V + LX_BK - 1) / LX_BK;
         d.scale = scale; d.out = (bf16_t*)dx + r0 * lddx; d.ldo = lddx; d.slab = (float*)(ws + q.slab);
-        if (int rc = lx_launch<LX_NN, LX_OUT>(d, q.dx[last], s, "linear_xent_dx")) return rc;
         // dW = dz^T x, summed over the blocks in fp32
         LxGemmParams e = {};
         e.A = dz; e.lda = (int)q.ldp; e.B = g.A; e.ldb = (int)ldx; e.M = V; e.N = D; e.KA = e.KB = n; e.steps = (n + LX_BK - 1) / LX_BK;
@@ -1251,8 +1336,28 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         e.add = b > 0 ? acc : nullptr;
         if (last) { e.out = dw; e.ldo = lddw; e.out_f32 = dw_f32; }
         else { e.out = acc; e.ldo = D; e.out_f32 = 1; }
-        if (int rc = lx_launch<LX_TN, LX_OUT>(e, q.dw[last], s, "linear_xent_dw")) return rc;
-        if (db != nullptr) {
+        const LxDeal& dd = q.dx[last];
+        const LxDeal& de = q.dw[last];
+        if (lx_one_launch(dd, de)) {
+            lx_tiles(d, dd);
+            lx_tiles(e, de);
+            e.slab = d.slab + dd.slab;
+            const int bx = d.tiles_m * d.tiles_n * dd.splits, bw = e.tiles_m * e.tiles_n * de.splits;
+            if (dd.kind == LX_SMALL64) lx_small_grads_kernel<1, 4, 1><<<bx + bw, 256, 0, s>>>(d, e, bx);
+            else lx_small_grads_kernel<4, 2, 2><<<bx + bw, 256, 0, s>>>(d, e, bx);
+            if (int rc = vitk_check_launch("linear_xent_grads")) return rc;
+            if (dd.splits > 1)
+                if (int rc = lx_reduce(d, s, "linear_xent_dx_sum")) return rc;
+            if (de.splits > 1)
+                if (int rc = lx_reduce(e, s, "linear_xent_dw_sum")) return rc;
+        } else {
+            if (int rc = lx_launch<LX_NN, LX_OUT>(d, dd, s, "linear_xent_dx")) return rc;
+            if (int rc = lx_launch<LX_TN, LX_OUT>(e, de, s, "linear_xent_dw")) return rc;
+        }
+        if (db != nullptr && q.blocks == 1 && n <= 1024) {
+            lx_colsum_few_kernel<<<(unsigned)(q.ldp / 128), 256, 0, s>>>(dz, q.ldp, n, V, scale, db, db_f32);
+            if (int rc = vitk_check_launch("linear_xent_db")) return rc;
+        } else if (db != nullptr) {
             float* part = (float*)(ws + q.colpart);
             int per = (n + LX_RANGES - 1) / LX_RANGES;
             if (per < 32) per = 32;
