@@ -212,7 +212,7 @@ EMB_IDS = {
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,V,D", [(1, 1, 8), (1, 1000, 768), (63, 2, 8), (65, 511, 72), (1025, 512, 64), (2049, 513, 200), (16384, 20000, 64), (16385, 700, 64),
-                                   (5000, 262143, 16), (5000, 262144, 16), (5000, 262145, 16), (40000, 300, 2064), (300000, 5000, 8)])
+                                   (5000, 262143, 16), (5000, 262144, 16), (5000, 262145, 16), (40000, 300, 2064), (50000, 4131, 24), (3000, 60, 256), (300000, 5000, 8)])
 @pytest.mark.parametrize("kind", list(EMB_IDS))
 def test_embedding_bwd(device, T, V, D, kind):
     ops = _ops()

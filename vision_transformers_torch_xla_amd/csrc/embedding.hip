@@ -119,14 +119,14 @@ static __device__ __forceinline__ unsigned sort_rank(unsigned* hist_wave, unsign
     return base + before;
 }
 
-// Grouping in one launch, for up to 32768 tokens of a vocabulary up to 2^18.  Workgroup g of 256 owns the ids that are g modulo 256.  It
+// Grouping in one launch, for up to 49152 tokens of a vocabulary up to 2^18.  Workgroup g of 256 owns the ids that are g modulo 256.  It
 // reads ALL ids (out of the L2 cache), counts how many belong to the workgroups before it - which is where its part of the sorted list
 // begins, so the workgroups need nothing from each other - and keeps its own tokens in a list in LDS, one in 256 of a text's.  Wave w has
 // a contiguous stretch of the tokens, so its list is in their order; a token's place is the wave's first one for its id plus the number of
 // equal ids before it in the wave.  A wave with more own tokens than its list holds reads its stretch again instead.  Tokens without a
 // gradient come last.  The workgroups behind the 256 zero the gradient meanwhile.  16384 tokens and 77 MB of zeros take 19 us together
 // (a radix sort in one workgroup 46 us); 100352 tokens 48 us, where the four launches below take 29 us.
-#define GROUP_MAX 32768
+#define GROUP_MAX 49152
 #define GROUP_WG 256
 #define GROUP_WAVES 16
 #define GROUP_LIST 192          // list entries of a wave
@@ -341,17 +341,18 @@ static __device__ __forceinline__ void emb_put(const EmbBwdParams& p, unsigned k
     Emb8<TO>::store(q, acc);
 }
 
-// One workgroup per piece of the sorted list and slice of 8 * blockDim columns.  The rows of a piece are independent loads: EMB_AHEAD
-// of them are in flight while the sums are formed in order.
+// A row of blockDim.x threads per piece of the sorted list and slice of 8 * blockDim.x columns; narrow tables have several pieces to a wave.
+// The rows of a piece are independent loads: EMB_AHEAD of them are in flight while the sums are formed in order.
 #define EMB_AHEAD 8
 template <typename TI, typename TO>
 __global__ __launch_bounds__(256) void embedding_bwd_kernel(const EmbBwdParams p) {
     const int col = ((int)blockIdx.y * (int)blockDim.x + (int)threadIdx.x) * 8;
-    if (col >= p.D) return;
-    const long long i0 = (long long)blockIdx.x * p.piece;
+    const long long piece = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+    if (col >= p.D || piece >= p.pieces) return;
+    const long long i0 = piece * p.piece;
     const long long i1 = i0 + p.piece < p.T ? i0 + p.piece : p.T;
     const TI* dout = reinterpret_cast<const TI*>(p.dout);
-    float* part = p.partial + (size_t)blockIdx.x * 2 * p.D + col;
+    float* part = p.partial + (size_t)piece * 2 * p.D + col;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     unsigned key = p.sorted[i0].x;
     if ((long long)key >= p.V) return;
@@ -391,51 +392,73 @@ __global__ __launch_bounds__(256) void embedding_bwd_kernel(const EmbBwdParams p
     else emb_put<TO>(p, key, col, acc);
 }
 
-// Runs that cross pieces: the workgroup of the piece a run begins in (as its tail) adds the head sums of the pieces that follow, a quarter of
-// them each of its four groups of threads, then the four in order.
-template <typename TO>
+// Runs that cross pieces: the threads of the piece a run begins in (as its tail) add the head sums of the pieces that follow; of a table that
+// takes a wave or more per piece (GROUPS = 4) a quarter of them each of four groups of threads, then the four in order.
+template <typename TO, int GROUPS>
 __global__ __launch_bounds__(1024) void embedding_join_kernel(const EmbBwdParams p) {
-    __shared__ float quarter[3][256][8];
+    __shared__ float quarter[GROUPS > 1 ? GROUPS - 1 : 1][256][8];
     const int col = ((int)blockIdx.y * (int)blockDim.x + (int)threadIdx.x) * 8;
-    const long long i1 = (long long)(blockIdx.x + 1) * p.piece;       // the grid has one block less than there are pieces
+    const int group = GROUPS > 1 ? (int)threadIdx.y : 0;
+    const long long piece = GROUPS > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * blockDim.y + threadIdx.y;
+    if (piece + 1 >= p.pieces) return;
+    const long long i1 = (piece + 1) * p.piece;
     const unsigned key = p.sorted[i1 - 1].x;
     if ((long long)key >= p.V || p.sorted[i1].x != key) return;       // nothing crosses this border
     const long long i0 = i1 - p.piece;
     if (p.sorted[i0].x == key && i0 > 0 && p.sorted[i0 - 1].x == key) return;       // the run began earlier
     // how many pieces the run enters (equal ids are neighbours: first piece whose first id is another one)
-    long long lo = blockIdx.x + 1, hi = p.pieces;
+    long long lo = piece + 1, hi = p.pieces;
     while (lo < hi) {
         const long long mid = (lo + hi) >> 1;
         if (p.sorted[mid * p.piece].x == key) lo = mid + 1; else hi = mid;
     }
-    const long long c0 = blockIdx.x + 1, n = lo - c0;
-    const long long from = c0 + n * threadIdx.y / 4, to = c0 + n * (threadIdx.y + 1) / 4;
+    const long long c0 = piece + 1, n = lo - c0;
+    const long long from = c0 + n * group / GROUPS, to = c0 + n * (group + 1) / GROUPS;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (col < p.D) {
-        if (threadIdx.y == 0) Emb8<float>::load(p.partial + ((size_t)blockIdx.x * 2 + 1) * p.D + col, acc);
+        if (group == 0) Emb8<float>::load(p.partial + ((size_t)piece * 2 + 1) * p.D + col, acc);
         const float* q = p.partial + col;
-#pragma unroll 4
-        for (long long c = from; c < to; ++c) {
-            float v[8];
-            Emb8<float>::load(q + (size_t)c * 2 * p.D, v);
+        constexpr int JOIN_AHEAD = GROUPS > 1 ? 4 : 8;        // partial rows in flight (8 in each of four groups: 9.4 instead of 6.3 us where most runs end at once)
+        for (long long c = from; c < to; c += JOIN_AHEAD) {
+            float v[JOIN_AHEAD][8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) acc[k] += v[k];
+            for (int j = 0; j < JOIN_AHEAD; ++j)
+                if (j == 0 || c + j < to) Emb8<float>::load(q + (size_t)(c + j) * 2 * p.D, v[j]);
+#pragma unroll
+            for (int j = 0; j < JOIN_AHEAD; ++j)
+                if (c + j < to) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) acc[k] += v[j][k];
+                }
         }
     }
-    if (threadIdx.y > 0) Emb8<float>::store(quarter[threadIdx.y - 1][threadIdx.x], acc);
-    __syncthreads();
-    if (threadIdx.y > 0 || col >= p.D) return;
+    if constexpr (GROUPS > 1) {
+        if (group > 0) Emb8<float>::store(quarter[group - 1][threadIdx.x], acc);
+        __syncthreads();
+        if (group > 0 || col >= p.D) return;
 #pragma unroll
-    for (int g = 0; g < 3; ++g)
+        for (int g = 0; g < GROUPS - 1; ++g)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] += quarter[g][threadIdx.x][k];
-    emb_put<TO>(p, key, col, acc);
+            for (int k = 0; k < 8; ++k) acc[k] += quarter[g][threadIdx.x][k];
+    }
+    if (col < p.D) emb_put<TO>(p, key, col, acc);
 }
 
-// pieces of the sorted list: about 1024 workgroups where there are enough tokens, 16 to 512 tokens each (2048 of 8 and more: the sums take as
-// long, the joining of their parts 7.4 and 10.9 instead of 6.1 and 6.6 us for 16384 and 100352 tokens of 768 columns)
-static int emb_piece(long long T) {
-    long long c = (T + 1023) / 1024;
+// threads per piece: the columns in eights, a power of two below a wave and whole waves above
+static int emb_lanes(int D) {
+    const int n = D / 8;
+    if (n >= 256) return 256;
+    if (n > 32) return (n + 63) / 64 * 64;
+    int w = 1;
+    while (w < n) w *= 2;
+    return w;
+}
+// tokens per piece: about 1024 workgroups where there are enough tokens, 16 to 512 tokens each (2048 of 8 and more: the sums take as long, the
+// joining of their parts 7.4 and 10.9 instead of 6.1 and 6.6 us for 16384 and 100352 tokens of 768 columns)
+static int emb_piece(long long T, int D) {
+    const int lanes = emb_lanes(D), side = lanes < 64 ? 256 / lanes : 1;
+    const long long wgs = side > 1 ? 512 * side : 1024;
+    long long c = (T + wgs - 1) / wgs;
     c = (c + 7) / 8 * 8;
     return (int)(c < 16 ? 16 : c > 512 ? 512 : c);
 }
@@ -482,7 +505,7 @@ int vitk_embedding_fwd(const void* ids, int ids_are_64, const void* table, int t
 
 size_t vitk_embedding_bwd_workspace(int64_t T, int64_t V, int D) {
     if (T <= 0 || V <= 0 || D <= 0) return 16;
-    const long long pieces = (T + emb_piece(T) - 1) / emb_piece(T);
+    const long long pieces = (T + emb_piece(T, D) - 1) / emb_piece(T, D);
     size_t n = emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)pieces * 2 * D * sizeof(float));
     if (!emb_one(T, V)) n += emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)((T + SORT_BLOCK - 1) / SORT_BLOCK) * SORT_BINS * sizeof(unsigned));
     return n;
@@ -512,7 +535,7 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
     uint2* sorted = (uint2*)ws;
     ws += emb_up((size_t)T * sizeof(uint2));
     EmbBwdParams p;
-    p.piece = emb_piece(T);
+    p.piece = emb_piece(T, D);
     p.pieces = (int)((T + p.piece - 1) / p.piece);
     p.partial = (float*)ws;
     ws += emb_up((size_t)p.pieces * 2 * D * sizeof(float));
@@ -550,12 +573,12 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
     }
     if (T == 0) return VITK_OK;
     p.sorted = sorted; p.dout = dout; p.out = dtable; p.T = T; p.V = V; p.ldd = ldd; p.ldo = ldo; p.D = D; p.accumulate = accumulate; p.scale = scale;
-    const int lanes = D / 8;
-    const int threads = lanes >= 256 ? 256 : (lanes + 63) / 64 * 64;
-    const dim3 grid(p.pieces, (lanes + threads - 1) / threads), join(p.pieces > 1 ? p.pieces - 1 : 1, grid.y);
-#define EMB_BWD(TI, TO)                                                                                  \
-    embedding_bwd_kernel<TI, TO><<<grid, threads, 0, s>>>(p);                                            \
-    if (p.pieces > 1) embedding_join_kernel<TO><<<join, dim3(threads, 4), 0, s>>>(p)
+    const int lanes = emb_lanes(D), side = lanes < 64 ? 256 / lanes : 1, slices = (D / 8 + lanes - 1) / lanes;
+    const dim3 block(lanes, side), grid((p.pieces + side - 1) / side, slices);
+#define EMB_BWD(TI, TO)                                                                                                            \
+    embedding_bwd_kernel<TI, TO><<<grid, block, 0, s>>>(p);                                                                        \
+    if (p.pieces > 1 && side > 1) embedding_join_kernel<TO, 1><<<grid, block, 0, s>>>(p);                                          \
+    else if (p.pieces > 1) embedding_join_kernel<TO, 4><<<dim3(p.pieces - 1, slices), dim3(lanes, 4), 0, s>>>(p)
     switch ((dout_type << 1) | dtable_type) {
         case 0: EMB_BWD(float, float); break;
         case 1: EMB_BWD(float, bf16_t); break;
