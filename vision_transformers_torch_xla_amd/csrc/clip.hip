@@ -9,7 +9,7 @@
 // overflows nor vanishes where sums in float would, at the same speed (the loads are what the kernel waits for).
 #include "common.h"
 
-#define MT_MAX 128
+#define MT_MAX 180             // what 4 KB of arguments hold (128 with an 8-byte count each: 152 tensors took 14 us more in two launches a stage)
 #define MT_CHUNK 8192          // elements per chunk: 32 per thread
 #define MT_BLOCKS 2048         // blocks of a launch at most: 8 per compute unit
 
@@ -18,11 +18,11 @@ enum { MT_F32 = 0, MT_BF16 = 1, MT_F16 = 2 };
 struct MtList {
     const void* src[MT_MAX];
     void* dst[MT_MAX];
-    unsigned long long n_type[MT_MAX];      // element count in the low 60 bits, type above
     unsigned first[MT_MAX + 1];             // first chunk of each tensor; first[count] = chunks of this launch
+    unsigned short tail_type[MT_MAX];       // elements of the last chunk less one, type from bit 13 on
     int count;
 };
-static_assert(sizeof(MtList) <= 3700, "kernel arguments are limited to 4 KB");
+static_assert(MT_CHUNK <= 1 << 13 && sizeof(MtList) <= 4000, "kernel arguments are limited to 4 KB");
 
 static __device__ __forceinline__ int mt_find(const MtList& l, unsigned chunk) {
     int lo = 0, hi = l.count - 1;           // largest t with first[t] <= chunk
@@ -120,9 +120,9 @@ __global__ __launch_bounds__(256) void mt_sumsq_kernel(const MtList l, double* _
     const unsigned chunks = l.first[l.count];
     for (unsigned c = blockIdx.x; c < chunks; c += gridDim.x) {
         const int t = mt_find(l, c);
-        const int type = (int)(l.n_type[t] >> 60);
-        const size_t n = (size_t)(l.n_type[t] & 0x0fffffffffffffffull), at = (size_t)(c - l.first[t]) * MT_CHUNK;
-        const int m = n - at < MT_CHUNK ? (int)(n - at) : MT_CHUNK;
+        const int type = (int)(l.tail_type[t] >> 13);
+        const size_t at = (size_t)(c - l.first[t]) * MT_CHUNK;
+        const int m = c + 1 == l.first[t + 1] ? (int)(l.tail_type[t] & 8191) + 1 : MT_CHUNK;
         if (type == MT_F32) s += mt_chunk_sumsq<MT_F32>(l.src[t], at, m);
         else if (type == MT_BF16) s += mt_chunk_sumsq<MT_BF16>(l.src[t], at, m);
         else s += mt_chunk_sumsq<MT_F16>(l.src[t], at, m);
@@ -188,9 +188,9 @@ __global__ __launch_bounds__(256) void mt_scale_kernel(const MtList l, const dou
     for (unsigned k = blockIdx.x; k < chunks; k += gridDim.x) {
         const unsigned c = chunks - 1 - k;
         const int t = mt_find(l, c);
-        const int type = (int)(l.n_type[t] >> 60);
-        const size_t n = (size_t)(l.n_type[t] & 0x0fffffffffffffffull), at = (size_t)(c - l.first[t]) * MT_CHUNK;
-        const int m = n - at < MT_CHUNK ? (int)(n - at) : MT_CHUNK;
+        const int type = (int)(l.tail_type[t] >> 13);
+        const size_t at = (size_t)(c - l.first[t]) * MT_CHUNK;
+        const int m = c + 1 == l.first[t + 1] ? (int)(l.tail_type[t] & 8191) + 1 : MT_CHUNK;
         if (type == MT_F32) mt_chunk_scale<MT_F32>(l.src[t], l.dst[t], at, m, coef);
         else if (type == MT_BF16) mt_chunk_scale<MT_BF16>(l.src[t], l.dst[t], at, m, coef);
         else mt_chunk_scale<MT_F16>(l.src[t], l.dst[t], at, m, coef);
@@ -214,7 +214,7 @@ static int mt_fill(MtList& l, const void* const* src, void* const* dst, const in
         if (chunks + c > 0xf0000000ull) break;
         l.src[l.count] = src[t];
         l.dst[l.count] = dst ? dst[t] : nullptr;
-        l.n_type[l.count] = (unsigned long long)numel[t] | ((unsigned long long)type[t] << 60);
+        l.tail_type[l.count] = (unsigned short)(((unsigned long long)(numel[t] - 1) % MT_CHUNK) | ((unsigned)type[t] << 13));
         l.first[l.count] = (unsigned)chunks;
         chunks += c;
         ++l.count;

@@ -479,7 +479,7 @@ def _here(t, name):
 
 
 def clip_grads(tensors, max_norm, out=None):
-    """Global L2 norm of a list of gradient tensors (fp32, bf16, fp16 in any mix, dense) and clipping by it, in two launches for up to 128
+    """Global L2 norm of a list of gradient tensors (fp32, bf16, fp16 in any mix, dense) and clipping by it, in two launches for up to 180
     tensors: t *= min(1, max_norm / (norm + 1e-6)).  Returns the norm before clipping as a 0-d fp32 GPU tensor; nothing is copied to
     the host.  out: tensors of the same shapes, strides and types that receive the clipped gradients (tensors themselves stay as
     they are); None: in place.  max_norm None: the norm alone.  A norm that is infinite or NaN spreads as in torch's clip_grad_norm_
