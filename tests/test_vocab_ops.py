@@ -142,7 +142,9 @@ def test_clip_grads_refuses(device):
                  lambda: ops.clip_grads([a.double()], 1.0),
                  lambda: ops.clip_grads([a[::2]], 1.0),
                  lambda: ops.clip_grads([a[:1].expand(8)], 1.0),
-                 lambda: ops.clip_grads([a, torch.zeros(4)], 1.0)):
+                 lambda: ops.clip_grads([a, torch.zeros(4)], 1.0),
+                 lambda: ops.clip_grads(a, 1.0),
+                 lambda: ops.clip_grads([a, 3.0], 1.0)):
         keep = a.clone()
         with pytest.raises(err):
             call()
@@ -294,6 +296,8 @@ def test_embedding_refuses(device):
                  lambda: ops.embedding_bwd(dout, ids, 10, out=torch.empty(10, 16, device=device), out_dtype=bf16),
                  lambda: ops.embedding_bwd(dout[:, :12], ids, 10),
                  lambda: ops.embedding_bwd(dout.half(), ids, 10),
+                 lambda: ops.embedding_bwd(dout, ids, 10, padding_idx=-1),
+                 lambda: ops.embedding_bwd(dout, ids, 10, padding_idx=10),
                  lambda: ops.embedding_bwd(dout, ids, 0)):
         with pytest.raises(err):
             call()
@@ -530,7 +534,8 @@ def test_linear_xent_refuses(device):
                  lambda: ops.linear_xent(x, w, t, b[:8]), lambda: ops.linear_xent(x, w, t, b.half()), lambda: ops.linear_xent(x, w, t.cpu()),
                  lambda: ops.linear_xent(x, w, t, smoothing=1.5), lambda: ops.linear_xent(x, w, t, smoothing=math.nan),
                  lambda: ops.linear_xent(x, w, t, reduction="none"), lambda: ops.linear_xent(x, w, t, dweight_dtype=f16),
-                 lambda: ops.linear_xent(x[:, ::2], w[:, ::2], t), lambda: ops.linear_xent(x[:, 1:9], w[:, 1:9], t), lambda: ops.linear_xent(x, w[:0], t)):
+                 lambda: ops.linear_xent(x[:, ::2], w[:, ::2], t), lambda: ops.linear_xent(x[:, 1:9], w[:, 1:9], t), lambda: ops.linear_xent(x, w[:0], t),
+                 lambda: ops.linear_xent(x, w, t, block_bytes=0), lambda: ops.linear_xent(x[:1].expand(6, 16), w, t)):
         with pytest.raises(err):
             call()
 
@@ -571,6 +576,80 @@ def test_linear_cross_entropy_module(device, wtype, reduction):
     again.backward(retain_graph=True)
     with pytest.raises(_error(), match="second time"):
         again.backward()
+
+
+@pytest.mark.gpu
+def test_linear_cross_entropy_inputs_of_every_layout(device, monkeypatch):
+    from vision_transformers_torch_xla_amd import losses
+    g = torch.Generator().manual_seed(8)
+    x, w, t = xent_inputs(24, 90, 32, g)
+    dev = [v.to(device) for v in (x, w, t)]
+    want = losses.linear_cross_entropy(*dev)
+    # fp32 holders of the same values, rows with an odd stride, a start between 16-byte lines, columns first, one row for all
+    odd = torch.zeros(24, 33, device=device, dtype=bf16)
+    odd[:, 1:] = dev[0]
+    line = torch.zeros(24 * 32 + 1, device=device)
+    line[1:] = dev[0].float().reshape(-1)
+    for v in (dev[0].float(), odd[:, 1:], line[1:].view(24, 32), dev[0].t().contiguous().t(), dev[0].view(4, 6, 32)):
+        v.requires_grad_(True)
+        got = losses.linear_cross_entropy(v, dev[1].float(), dev[2].view(v.shape[:-1]))
+        assert torch.equal(got, want)
+        got.backward()
+        assert v.grad.shape == v.shape and v.grad.dtype == v.dtype
+    row = dev[0][:1].detach().clone().requires_grad_(True)
+    losses.linear_cross_entropy(row.expand(24, 32), dev[1], dev[2]).backward()
+    (_, _, dx, _, _), (_, _, dxt, _, _) = plain_linear_xent(x[:1].expand(24, 32), w, t, None, 0.0, -100, True)
+    # 24 gradients, each rounded to bf16, then torch's sum of them in bf16
+    assert torch.all((row.grad.cpu().double() - dx.sum(0)).abs() <= dxt.sum(0) + 4 * 2.0 ** -8 * dx.abs().sum(0))
+    empty = dev[0][:0].detach().requires_grad_(True)
+    weight = dev[1].float().requires_grad_(True)
+    losses.linear_cross_entropy(empty, weight, dev[2][:0]).backward()
+    assert empty.grad.shape == (0, 32) and torch.all(weight.grad == 0)
+    # the gradients are computed where somebody can ask for them, and only there
+    asked = []
+    real = losses.ops.linear_xent
+    monkeypatch.setattr(losses.ops, "linear_xent", lambda *a, **k: (asked.append(k["want_grad"]), real(*a, **k))[1])
+    losses.linear_cross_entropy(dev[0], dev[1], dev[2])
+    losses.linear_cross_entropy(dev[0], weight, dev[2])
+    with torch.no_grad():
+        losses.linear_cross_entropy(dev[0], weight, dev[2])
+    assert asked == [False, True, False]
+
+
+@pytest.mark.gpu
+def test_modules_in_a_graph(device):
+    """forward and backward of lookup and loss captured and replayed; the eager graph of the same parameters is gone before the capture"""
+    from vision_transformers_torch_xla_amd.embedding import TokenEmbedding
+    from vision_transformers_torch_xla_amd.losses import LinearCrossEntropy
+    torch.manual_seed(9)
+    emb, head = TokenEmbedding(120, 32).to(device), LinearCrossEntropy(32, 120).to(device)
+    with torch.no_grad():
+        emb.weight.mul_(30), head.weight.mul_(30)
+    params = [*emb.parameters(), *head.parameters()]
+    ids, target = torch.randint(0, 120, (200,), device=device), torch.randint(0, 120, (200,), device=device)
+
+    def step():
+        for p in params:
+            p.grad = None
+        loss = head(emb(ids), target)
+        loss.backward()
+        return loss.detach()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(), step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = step()
+    held = [p.grad for p in params]
+    for k in range(3):
+        ids.copy_(torch.randint(0, 120, (200,), device=device)), target.copy_(torch.randint(0, 120, (200,), device=device))
+        graph.replay()
+        got = [loss.clone(), *(h.clone() for h in held)]
+        want = [step(), *(p.grad for p in params)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 @pytest.mark.gpu

@@ -131,8 +131,9 @@ __global__ __launch_bounds__(256) void mt_sumsq_kernel(const MtList l, double* _
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
+typedef __attribute__((ext_vector_type(4))) unsigned mt_u32x4;
 template <int TYPE>
-static __device__ __forceinline__ void mt_chunk_scale(const void* src, void* dst, size_t at, int n, float coef) {
+static __device__ __forceinline__ void mt_chunk_scale(const void* src, void* dst, size_t at, int n, float coef, bool stream) {
     constexpr int W = TYPE == MT_F32 ? 4 : 8, SIZE = TYPE == MT_F32 ? 4 : 2;
     const char* a = reinterpret_cast<const char*>(src) + at * SIZE;
     char* b = reinterpret_cast<char*>(dst) + at * SIZE;
@@ -153,7 +154,11 @@ static __device__ __forceinline__ void mt_chunk_scale(const void* src, void* dst
             mt_unpack(r[j], TYPE, v);
 #pragma unroll
             for (int k = 0; k < W; ++k) v[k] *= coef;
-            q[j * 256 + threadIdx.x] = mt_pack(v, TYPE);
+            // into other tensors: past the caches, which keep the gradients that are still to be read (152 tensors of 22 M values 57.8 -> 48.8 us,
+            // 400 of 600 M 1002 -> 968 us)
+            const uint4 w = mt_pack(v, TYPE);
+            if (stream) __builtin_nontemporal_store((mt_u32x4){w.x, w.y, w.z, w.w}, reinterpret_cast<mt_u32x4*>(q) + j * 256 + threadIdx.x);
+            else q[j * 256 + threadIdx.x] = w;
         }
         return;
     }
@@ -184,16 +189,14 @@ __global__ __launch_bounds__(256) void mt_scale_kernel(const MtList l, const dou
     if (coef > 1.0f) coef = 1.0f;                   // NaN stays NaN, an infinite norm gives 0 (and NaN where the gradient is infinite)
     if (in_place && coef == 1.0f) return;
     const unsigned chunks = l.first[l.count];
-    // last chunks first: they are what the first stage has left in the caches
-    for (unsigned k = blockIdx.x; k < chunks; k += gridDim.x) {
-        const unsigned c = chunks - 1 - k;
+    for (unsigned c = blockIdx.x; c < chunks; c += gridDim.x) {
         const int t = mt_find(l, c);
         const int type = (int)(l.tail_type[t] >> 13);
         const size_t at = (size_t)(c - l.first[t]) * MT_CHUNK;
         const int m = c + 1 == l.first[t + 1] ? (int)(l.tail_type[t] & 8191) + 1 : MT_CHUNK;
-        if (type == MT_F32) mt_chunk_scale<MT_F32>(l.src[t], l.dst[t], at, m, coef);
-        else if (type == MT_BF16) mt_chunk_scale<MT_BF16>(l.src[t], l.dst[t], at, m, coef);
-        else mt_chunk_scale<MT_F16>(l.src[t], l.dst[t], at, m, coef);
+        if (type == MT_F32) mt_chunk_scale<MT_F32>(l.src[t], l.dst[t], at, m, coef, !in_place);
+        else if (type == MT_BF16) mt_chunk_scale<MT_BF16>(l.src[t], l.dst[t], at, m, coef, !in_place);
+        else mt_chunk_scale<MT_F16>(l.src[t], l.dst[t], at, m, coef, !in_place);
     }
 }
 

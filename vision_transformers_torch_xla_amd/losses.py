@@ -83,20 +83,30 @@ class SoftTargetCrossEntropy(nn.Module):
 
 def _bf16_rows(t):
     """a bf16 matrix with contiguous, 16-byte aligned rows holding t's values (t itself where it is one)"""
-    if t.dtype == f32:
-        return ops.cast_f32_to_bf16(t.detach().contiguous())
     t = t.detach()
-    if t.stride(-1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+    if t.numel() == 0:
+        return t.to(bf16)
+    if t.dtype == f32 or t.stride(-1) != 1 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
         t = t.contiguous()
-    return t
+    if t.data_ptr() % 16:
+        t = t.clone()
+    return ops.cast_f32_to_bf16(t) if t.dtype == f32 else t
+
+
+def _times(g, go):
+    """g * go in place of g; the upstream scalar go stays fp32 where g is bf16, so that the product is what is rounded and not the scalar"""
+    if g is None or g.numel() == 0:
+        return g
+    if g.dtype == bf16 and g.dim() == 2:
+        return ops.rowscale(g, go.reshape(1).float(), g.shape[0], out=g)
+    return (g * go.float()).to(g.dtype)
 
 
 class _LinearXent(torch.autograd.Function):
     """The loss and, where anything needs them, its gradients in one call of ops.linear_xent; backward multiplies them by the upstream scalar."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, target, smoothing, ignore_index, reduction):
-        want = any(ctx.needs_input_grad[:3])
+    def forward(ctx, x, weight, bias, target, smoothing, ignore_index, reduction, want):
         wtype = weight.dtype
         r = ops.linear_xent(_bf16_rows(x), _bf16_rows(weight), target, None if bias is None else bias.detach(), smoothing=smoothing,
                             ignore_index=ignore_index, reduction=reduction, want_grad=want, dweight_dtype=wtype if wtype in (bf16, f32) else None)
@@ -111,10 +121,8 @@ class _LinearXent(torch.autograd.Function):
             raise VitkError("linear_cross_entropy: backward was called a second time (the gradients are handed over, not kept)")
         (dx, dw, db), ctx.grads = ctx.grads, None
         need = ctx.needs_input_grad
-        scaled = lambda g: None if g is None else ops.rowscale(g, go.reshape(1).float(), g.shape[0], out=g) if g.dtype == bf16 and g.dim() == 2 \
-            else (g * go.float()).to(g.dtype)                     # the upstream scalar stays fp32: a bf16 gradient is rounded once more, not it
-        dx = scaled(dx).to(ctx.xtype) if need[0] else None
-        return dx, scaled(dw) if need[1] else None, scaled(db) if need[2] else None, None, None, None, None
+        dx = _times(dx, go).to(ctx.xtype) if need[0] else None
+        return dx, _times(dw, go) if need[1] else None, _times(db, go) if need[2] else None, None, None, None, None, None
 
 
 def linear_cross_entropy(x, weight, target, bias=None, smoothing: float = 0.0, ignore_index: int = -100, reduction: str = "mean"):
@@ -126,9 +134,9 @@ def linear_cross_entropy(x, weight, target, bias=None, smoothing: float = 0.0, i
     for t, n in ((x, "x"), (weight, "weight")):
         if t.dtype not in (bf16, f32):
             raise VitkError(f"linear_cross_entropy: {n} must be bfloat16 or float32, got {t.dtype}")
-    if not x.is_cuda:
-        raise VitkError("linear_cross_entropy: x must be on the GPU; the fused loss kernels are the only implementation")
-    return _LinearXent.apply(x.reshape(-1, x.shape[-1]), weight, bias, target.reshape(-1), float(smoothing), int(ignore_index), reduction)
+        ops._here(t, f"linear_cross_entropy: {n}")
+    want = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
+    return _LinearXent.apply(x.reshape(-1, x.shape[-1]), weight, bias, target.reshape(-1), float(smoothing), int(ignore_index), reduction, want)
 
 
 class LinearCrossEntropy(nn.Module):

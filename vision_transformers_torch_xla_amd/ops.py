@@ -484,6 +484,8 @@ def clip_grads(tensors, max_norm, out=None):
     the host.  out: tensors of the same shapes, strides and types that receive the clipped gradients (tensors themselves stay as
     they are); None: in place.  max_norm None: the norm alone.  A norm that is infinite or NaN spreads as in torch's clip_grad_norm_
     (finite gradients become 0 or NaN)."""
+    if isinstance(tensors, torch.Tensor) or isinstance(out, torch.Tensor):
+        raise _lib.VitkError("clip_grads: expected lists of tensors, got one tensor (its rows would be taken for gradients)")
     tensors = list(tensors)
     if not tensors:
         raise _lib.VitkError("clip_grads: no tensors (a device is needed for the norm)")
@@ -548,6 +550,8 @@ def embedding_bwd(dout, ids, num_rows, scale=1.0, padding_idx=None, out=None, ac
     the tokens, the same bits on every run), zero where there is none; dout fp32 / bf16 [..., D].  Tokens with id padding_idx or an id
     outside [0, num_rows) add nothing.  out: where it goes (fp32 / bf16 [num_rows, D]); with accumulate it is added there, and only the
     rows that have tokens are touched.  Without out: a new tensor of out_dtype (default: dout's type)."""
+    if padding_idx is not None and not 0 <= int(padding_idx) < int(num_rows):
+        raise _lib.VitkError(f"embedding_bwd: padding_idx {padding_idx} outside the table of {num_rows} rows")
     if dout.dim() < 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
         raise _lib.VitkError(f"embedding_bwd: dout must be {tuple(ids.shape)} + (D,), got {tuple(dout.shape)}")
     D = dout.shape[-1]
@@ -606,6 +610,8 @@ def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, 
     _here(target, "target")
     if target.dtype != torch.int64 or tuple(target.shape) != (T,):
         raise _lib.VitkError(f"linear_xent: target must be int64 [{T}], got {target.dtype} {tuple(target.shape)}")
+    if int(block_bytes) <= 0:
+        raise _lib.VitkError(f"linear_xent: block_bytes must be positive, got {block_bytes}")
     if reduction not in ("mean", "sum"):
         raise _lib.VitkError(f"linear_xent: reduction must be 'mean' or 'sum' (rows are returned beside either), got {reduction!r}")
     btype = 0
