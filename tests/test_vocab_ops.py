@@ -308,13 +308,13 @@ def plain_linear_xent(x, w, target, bias, smoothing, ignore, mean):
     """the operator in 64 bits, and how far bf16 / fp32 arithmetic may be off it: (loss, rows, dx, dw, db), (tolerances of the same)"""
     x, w = x.double(), w.double()
     V, D = w.shape
-    b = torch.zeros(V, dtype=f64) if bias is None else bias.double()
+    b = torch.zeros(V, dtype=f64, device=w.device) if bias is None else bias.double()
     z = x @ w.t() + b
     counted = target != ignore
     bad = counted & ((target < 0) | (target >= V))
     t = torch.where(counted & ~bad, target, torch.zeros_like(target))
     q = torch.full_like(z, smoothing / V)
-    q[torch.arange(len(t)), t] += 1.0 - smoothing
+    q[torch.arange(len(t), device=t.device), t] += 1.0 - smoothing
     lse = torch.logsumexp(z, 1)
     smooth = smoothing * (lse - z.mean(1)) if smoothing > 0 else 0.0            # no 0 * inf where a class is masked out
     rows = (1.0 - smoothing) * (lse - z.gather(1, t[:, None])[:, 0]) + smooth
@@ -351,7 +351,7 @@ def check_linear_xent(r, x, w, target, bias=None, smoothing=0.0, ignore=-100, me
         if name == "dbias" and bias is None:
             assert got is None
             continue
-        got = got.cpu()
+        got = got.to(v.device)
         extra = half_ulp(got.dtype) * 1.01 * (v.abs() + t) + (2.0 ** -133 if got.dtype == bf16 else 0.0)
         off = (got.double() - v).abs()
         bad = ~(off <= t + extra) & ~(got.double() == v)
@@ -386,6 +386,27 @@ def test_linear_xent(device, T, V, D, smoothing, btype):
     s = ops.linear_xent(*args, smoothing=smoothing, reduction="sum", dweight_dtype=f32)
     assert s.dweight.dtype == f32
     check_linear_xent(s, x, w, target, bias, smoothing, mean=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D,block_bytes", [(1099, 24921, 424, 2 << 30), (8275, 8906, 392, 2 << 30), (8275, 8906, 392, 100 << 20), (16583, 8692, 168, 2 << 30),
+                                               (1680, 21915, 720, 2 << 30), (6800, 6618, 2384, 2 << 30), (3615, 3627, 2240, 40 << 20), (8062, 7972, 2048, 2 << 30),
+                                               (5225, 7940, 1896, 2 << 30)])
+def test_linear_xent_large(device, T, V, D, block_bytes):
+    """sizes that reach the large kernels: whole rounds of tiles, tiles cut into ranges of the contraction with and without whole rounds before
+    them, tile columns in teams of 2 to 8, several blocks of rows; the plain form in 64 bits runs on the GPU"""
+    ops = _ops()
+    g = torch.Generator().manual_seed(T + V + D)
+    x, w, target = (t.to(device) for t in xent_inputs(T, V, D, g))
+    bias = (torch.randn(V, generator=g) * 0.5).to(device) if D % 16 else None
+    smoothing = 0.1 if T % 2 else 0.0
+    wtype = f32 if V % 2 else bf16
+    r = ops.linear_xent(x, w, target, bias, smoothing=smoothing, dweight_dtype=wtype, block_bytes=block_bytes)
+    check_linear_xent(r, x, w, target, bias, smoothing)
+    again = ops.linear_xent(x, w, target, bias, smoothing=smoothing, dweight_dtype=wtype, block_bytes=block_bytes)
+    assert all(a is None or torch.equal(a, b) for a, b in zip(again, r))
+    alone = ops.linear_xent(x, w, target, bias, smoothing=smoothing, want_grad=False)
+    assert torch.equal(alone.rows, r.rows)
 
 
 @pytest.mark.gpu
