@@ -231,6 +231,25 @@ def test_embedding_bwd(device, T, V, D, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D", [(262144, 511, 8), (262145, 70000, 16), (1000003, 300001, 8)])       # on both sides of the sort's scan; one pass and more
+def test_embedding_bwd_of_very_many_tokens(device, T, V, D):
+    ops = _ops()
+    g = torch.Generator().manual_seed(T)
+    ids = EMB_IDS["hot"](T, V, g)
+    dout = torch.randn(T, D, generator=g)
+    check_embedding_grad(ops.embedding_bwd(dout.to(device), ids.to(device), V, scale=-0.3, padding_idx=1), dout, ids, V, -0.3, 1)
+
+
+@pytest.mark.gpu
+def test_embedding_bwd_without_tokens(device):
+    ops = _ops()
+    none = torch.empty(0, 8, device=device), torch.empty(0, dtype=torch.int64, device=device)
+    for V in (1, 300000, 5000000):
+        assert torch.all(ops.embedding_bwd(*none, V, out=torch.full((V, 8), 7.0, device=device)) == 0)
+        assert torch.all(ops.embedding_bwd(*none, V, out=torch.full((V, 8), 7.0, device=device), accumulate=True) == 7.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [500, 20000])
 def test_embedding_bwd_accumulates_into_a_part_of_a_buffer(device, T):
     ops = _ops()

@@ -236,8 +236,12 @@ __global__ __launch_bounds__(1024) void emb_group_kernel(const void* ids, int T,
     for (unsigned i = total_valid + own * 1024u + threadIdx.x; i < (unsigned)T; i += GROUP_WG * 1024u) sorted[i] = make_uint2((unsigned)V, 0u);
 }
 
-// Several workgroups: per pass a histogram launch (counts[block][bin]) and a launch that turns the counts into ranks and scatters.
+// Several workgroups: per pass a histogram launch (counts[block][bin]) and a launch that turns the counts into ranks and scatters.  For that a
+// workgroup adds up the counts of all others; from SORT_DIRECT workgroups on, a launch in between turns the counts of SORT_GROUP workgroups
+// into sums over those before and a total per group, so that only the totals are added up.
 #define SORT_BLOCK (256 * SORT_ITEMS)       // tokens per workgroup
+#define SORT_DIRECT 128
+#define SORT_GROUP 32
 
 template <typename I, bool FIRST>
 static __device__ __forceinline__ uint2 sort_item(const void* ids, const uint2* in, long long t, long long T, long long V, long long padding) {
@@ -271,9 +275,24 @@ __global__ __launch_bounds__(256) void emb_hist_kernel(const void* ids, const ui
     counts[(size_t)blockIdx.x * SORT_BINS + threadIdx.x + 256] = hist[threadIdx.x + 256];
 }
 
+__global__ __launch_bounds__(SORT_BINS) void emb_scan_kernel(unsigned* counts, int blocks, unsigned* totals) {
+    const int b0 = blockIdx.x * SORT_GROUP, n = blocks - b0 < SORT_GROUP ? blocks - b0 : SORT_GROUP;
+    unsigned* q = counts + (size_t)b0 * SORT_BINS + threadIdx.x;
+    unsigned c[SORT_GROUP], sum = 0;
+#pragma unroll
+    for (int b = 0; b < SORT_GROUP; ++b) c[b] = b < n ? q[b * SORT_BINS] : 0u;
+#pragma unroll
+    for (int b = 0; b < SORT_GROUP; ++b) {
+        if (b < n) q[b * SORT_BINS] = sum;
+        sum += c[b];
+    }
+    totals[(size_t)blockIdx.x * SORT_BINS + threadIdx.x] = sum;
+}
+
+// totals: the counts themselves and entries = blocks, or the groups' totals
 template <typename I, bool FIRST>
 __global__ __launch_bounds__(256) void emb_scatter_kernel(const void* ids, const uint2* in, long long T, long long V, long long padding, int shift,
-                                                          const unsigned* __restrict__ counts, int blocks, uint2* out) {
+                                                          const unsigned* __restrict__ counts, const unsigned* __restrict__ totals, int entries, uint2* out) {
     __shared__ unsigned hist[4 * SORT_BINS];
     __shared__ unsigned sums[4];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -290,11 +309,16 @@ __global__ __launch_bounds__(256) void emb_scatter_kernel(const void* ids, const
     }
     // thread i owns bins 2i and 2i + 1: their totals and the share of the blocks before this one
     const int b0 = 2 * threadIdx.x;
+    const int own = totals == counts ? (int)blockIdx.x : (int)blockIdx.x / SORT_GROUP;
     unsigned tot0 = 0, tot1 = 0, pre0 = 0, pre1 = 0;
+    if (totals != counts) {
+        const uint2 c = *reinterpret_cast<const uint2*>(counts + (size_t)blockIdx.x * SORT_BINS + b0);
+        pre0 = c.x; pre1 = c.y;
+    }
 #pragma unroll 8
-    for (int b = 0; b < blocks; ++b) {
-        const uint2 c = *reinterpret_cast<const uint2*>(counts + (size_t)b * SORT_BINS + b0);
-        const bool before = b < (int)blockIdx.x;
+    for (int b = 0; b < entries; ++b) {
+        const uint2 c = *reinterpret_cast<const uint2*>(totals + (size_t)b * SORT_BINS + b0);
+        const bool before = b < own;
         pre0 += before ? c.x : 0u; pre1 += before ? c.y : 0u;
         tot0 += c.x; tot1 += c.y;
     }
@@ -468,6 +492,8 @@ static int emb_passes(long long V) {
     return (bits + SORT_BITS - 1) / SORT_BITS;
 }
 static bool emb_one(long long T, long long V) { return T == 0 || (T <= GROUP_MAX && V <= (1 << 18)); }
+static long long emb_sort_blocks(long long T) { return (T + SORT_BLOCK - 1) / SORT_BLOCK; }
+static long long emb_sort_groups(long long T) { return emb_sort_blocks(T) > SORT_DIRECT ? (emb_sort_blocks(T) + SORT_GROUP - 1) / SORT_GROUP : 0; }
 static size_t emb_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 extern "C" {
@@ -507,7 +533,7 @@ size_t vitk_embedding_bwd_workspace(int64_t T, int64_t V, int D) {
     if (T <= 0 || V <= 0 || D <= 0) return 16;
     const long long pieces = (T + emb_piece(T, D) - 1) / emb_piece(T, D);
     size_t n = emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)pieces * 2 * D * sizeof(float));
-    if (!emb_one(T, V)) n += emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)((T + SORT_BLOCK - 1) / SORT_BLOCK) * SORT_BINS * sizeof(unsigned));
+    if (!emb_one(T, V)) n += emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)(emb_sort_blocks(T) + emb_sort_groups(T)) * SORT_BINS * sizeof(unsigned));
     return n;
 }
 
@@ -527,6 +553,7 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
         vitk_set_error("embedding_bwd: workspace %zu < %zu", workspace_bytes, vitk_embedding_bwd_workspace(T, V, D));
         return VITK_ENOSPC;
     }
+    if (T == 0 && accumulate) return VITK_OK;
     hipStream_t s = (hipStream_t)stream;
     const long long zero16 = accumulate ? 0 : (long long)V * D * (dtable_type == 0 ? 4 : 2) / 16;
     const int zero_blocks = (int)(zero16 / 4096 < 1024 ? (zero16 + 4095) / 4096 : 1024);
@@ -541,19 +568,21 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
     ws += emb_up((size_t)p.pieces * 2 * D * sizeof(float));
     if (emb_one(T, V)) {
         const int grid = GROUP_WG + zero_blocks;
-        const size_t lds = emb_group_lds(V);
+        const long long ids_of = T > 0 ? V : 1;         // no token: nothing to group, zeros alone
+        const size_t lds = emb_group_lds(ids_of);
         static VitkLdsOnce once64 = {}, once32 = {};        // the largest is allowed once; a launch asks for what its vocabulary needs
         if (int rc = ids_are_64 ? vitk_lds_once(once64, (const void*)emb_group_kernel<int64_t>, emb_group_lds(1 << 18), "embedding_bwd")
                                 : vitk_lds_once(once32, (const void*)emb_group_kernel<int32_t>, emb_group_lds(1 << 18), "embedding_bwd"))
             return rc;
-        if (ids_are_64) emb_group_kernel<int64_t><<<grid, 1024, lds, s>>>(ids, (int)T, V, padding_idx, sorted, (uint4*)dtable, zero16);
-        else emb_group_kernel<int32_t><<<grid, 1024, lds, s>>>(ids, (int)T, V, padding_idx, sorted, (uint4*)dtable, zero16);
+        if (ids_are_64) emb_group_kernel<int64_t><<<grid, 1024, lds, s>>>(ids, (int)T, ids_of, padding_idx, sorted, (uint4*)dtable, zero16);
+        else emb_group_kernel<int32_t><<<grid, 1024, lds, s>>>(ids, (int)T, ids_of, padding_idx, sorted, (uint4*)dtable, zero16);
         if (int rc = vitk_check_launch("embedding_bwd_sort")) return rc;
     } else {
         uint2* other = (uint2*)ws;
         ws += emb_up((size_t)T * sizeof(uint2));
         unsigned* counts = (unsigned*)ws;
-        const int blocks = (int)((T + SORT_BLOCK - 1) / SORT_BLOCK);
+        const int blocks = (int)emb_sort_blocks(T), groups = (int)emb_sort_groups(T), entries = groups > 0 ? groups : blocks;
+        unsigned* totals = groups > 0 ? counts + (size_t)blocks * SORT_BINS : counts;
         // the last pass has to write `sorted`
         uint2* to = passes & 1 ? sorted : other;
         uint2* from = nullptr;
@@ -561,7 +590,8 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
             const int shift = pass * SORT_BITS, extra = pass == 0 ? zero_blocks : 0;
 #define EMB_PASS(I, F)                                                                                                                       \
     emb_hist_kernel<I, F><<<blocks + extra, 256, 0, s>>>(ids, from, T, V, padding_idx, shift, counts, blocks, (uint4*)dtable, zero16);      \
-    emb_scatter_kernel<I, F><<<blocks, 256, 0, s>>>(ids, from, T, V, padding_idx, shift, counts, blocks, to)
+    if (groups > 0) emb_scan_kernel<<<groups, SORT_BINS, 0, s>>>(counts, blocks, totals);                                                    \
+    emb_scatter_kernel<I, F><<<blocks, 256, 0, s>>>(ids, from, T, V, padding_idx, shift, counts, totals, entries, to)
             if (pass > 0) { EMB_PASS(int64_t, false); }
             else if (ids_are_64) { EMB_PASS(int64_t, true); }
             else { EMB_PASS(int32_t, true); }
