@@ -35,6 +35,7 @@ static void check_one(const at::Tensor& t, Py_ssize_t i, const char* what, long 
         throw name + ": the tensor is on " + t.device().str() + ", the current device is cuda:" + std::to_string(device);
     if (t.layout() != at::kStrided) throw name + ": expected a dense tensor";
     if (type_code(t) < 0) throw name + ": expected float32, bfloat16 or float16, got " + std::string(at::toString(t.scalar_type()));
+    if (t.is_neg()) throw name + ": expected the values themselves, not a lazily negated view (resolve_neg)";
     if (!t.is_non_overlapping_and_dense()) throw name + ": expected a dense tensor (every element of its memory range, once)";
 }
 
@@ -95,6 +96,8 @@ static PyObject* clip_table(PyObject*, PyObject* args) {
         PyErr_SetString(PyExc_ValueError, why.c_str());
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_ValueError, e.what());
+    } catch (...) {
+        PyErr_SetString(PyExc_ValueError, "a tensor could not be read");
     }
     return nullptr;
 }
