@@ -148,6 +148,13 @@ static __device__ __forceinline__ void lx_loss_epilogue(const LxGemmParams& p, f
     }
 }
 
+// range g of G of `total` steps: total / G each, the first total % G one more
+static __host__ __device__ __forceinline__ void lx_range(int g, int total, int G, int& from, int& to) {
+    const int q = total / G, r = total - q * G;
+    from = g * q + (g < r ? g : r);
+    to = from + q + (g < r ? 1 : 0);
+}
+
 // One 512-thread workgroup per compute unit works through 256 x 256 tiles of the output, 8 waves (2 x 4) of 128 x 64 = 128 accumulator
 // registers each, 64-deep steps.  Operands go from memory to LDS by DMA, two steps ahead across tile borders, into a double buffer;
 // fragments are read one phase of 16 matrix instructions before their use.  An operand whose rows run along the contraction sits in LDS as
@@ -156,13 +163,6 @@ static __device__ __forceinline__ void lx_loss_epilogue(const LxGemmParams& p, f
 // swapped, so a lane holds four consecutive columns of one output row.  Tiles are dealt by number (no counters: a captured graph may be
 // replayed on any stream); a tile order in bands of 8 column tiles keeps what the 32 workgroups of an XCD read at a time to 4 row panels
 // and 8 column panels.
-// range g of G of `total` steps: total / G each, the first total % G one more
-static __host__ __device__ __forceinline__ void lx_range(int g, int total, int G, int& from, int& to) {
-    const int q = total / G, r = total - q * G;
-    from = g * q + (g < r ? g : r);
-    to = from + q + (g < r ? 1 : 0);
-}
-
 template <int LAY, int EPI>
 __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
     constexpr bool AT = LAY == LX_TN, BT = LAY != LX_NT;        // operand stored with the contraction as its slow dimension
@@ -584,13 +584,13 @@ static __device__ __forceinline__ u32x4 lx_dz8(const u32x4 r, float f, float u, 
     return (u32x4){pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])};
 }
 
-// the sum of up to LX_FUSED rows' losses and their count, by one wave, in an order of its own: lane by lane, then the lanes
-#define LX_FUSED 512
+// scale of the gradients and loss from the sum of the rows' losses and the count of the counted rows
 static __device__ __forceinline__ void lx_finish(double s, long long count, int mean, float* scale, float* loss) {
     if (scale != nullptr) *scale = count == 0 ? 0.f : mean ? (float)(1.0 / (double)count) : 1.f;
     if (loss != nullptr) *loss = (float)(count == 0 ? 0.0 : mean ? s / (double)count : s);
 }
-// a row's loss is known: stored, and where p.loss is set the wave that is the last of all rows' first waves adds them up
+// A row's loss is known: it is stored, and where p.loss is set the wave that is the last of all rows' first waves adds them up, lane by lane, then
+// the lanes.  That saves a call of few rows a launch (see LX_FUSED_ROWS).
 static __device__ __forceinline__ void lx_row_done(const LxRowParams& p, int row, int tid, float l) {
     if (tid >= 64) return;
     if (p.loss == nullptr) {
@@ -617,9 +617,6 @@ static __device__ __forceinline__ void lx_row_done(const LxRowParams& p, int row
 
 // WAVES waves per row: one workgroup, or for short rows one wave of a workgroup of four.  Bound by memory: 4 bytes per logit where the gradient
 // is wanted, nothing to speak of where it is not.
-#ifndef LX_NTS
-#define LX_NTS 0
-#endif
 #define LX_AHEAD 4          // chunks of 8 columns a thread has in flight
 template <int WAVES, bool STREAM>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(const LxRowParams p) {
@@ -690,7 +687,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
             const int c = c0 + j * NT;
             if (c < chunks) {
                 const u32x4 o = lx_dz8(r[j], __builtin_amdgcn_exp2f(m[j] - lse2), u, hit, c * 8, t, p.V, valid);
-                if (STREAM || LX_NTS) __builtin_nontemporal_store(o, q + c);
+                if (STREAM) __builtin_nontemporal_store(o, q + c);
                 else q[c] = o;
             }
         }
@@ -742,9 +739,9 @@ __global__ __launch_bounds__(256) void lx_loss_kernel(const long long* __restric
             count += __hip_atomic_load(&part[b].count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
     }
-    if (scale != nullptr) *scale = count == 0 ? 0.f : mean ? (float)(1.0 / (double)count) : 1.f;
-    if (loss != nullptr) *loss = (float)(count == 0 ? 0.0 : mean ? s / (double)count : s);
+    lx_finish(s, count, mean, scale, loss);
 }
+
 // The same products for outputs too small to fill the chip with 256 x 256 tiles, which also cost a call 8 to 10 us of pipeline fill and epilogue
 // however short it is: one tile of (16 FM WM) x (64 WN) and one range of steps per 256-thread workgroup, several workgroups on a compute unit
 // in place of a deep pipeline within one.  FM = 4, waves 2 x 2: 128 x 128 tiles, 64 KB of LDS; FM = 1, waves 4 x 1: 64 x 64, 32 KB.
@@ -1060,6 +1057,10 @@ __global__ __launch_bounds__(256) void lx_colsum_few_kernel(const bf16_t* __rest
 
 // ---------------------------------------------------------------------------------------------------- host
 #define LX_RANGES 64
+// the rows' kernel adds the losses up itself for up to 512 rows, unless it rewrites more than 1 MB of P (each row's ticket waits for the
+// stores before it to reach memory)
+#define LX_FUSED_ROWS 512
+#define LX_FUSED_BYTES ((size_t)1 << 20)
 #define LX_CACHED ((size_t)640 << 20)
 
 static int lx_cus() {
@@ -1175,7 +1176,7 @@ static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw
     const size_t row = (grad ? (size_t)q.ldp * 2 : 0) + (size_t)q.stat_cols * (smoothing ? 12 : 8);
     long long rows = (long long)(block_bytes / row) / LX_TILE * LX_TILE;
     if (rows < LX_TILE) rows = LX_TILE;
-    if (rows > (1 << 22)) rows = 1 << 22;
+    if (rows > (1 << 21)) rows = 1 << 21;
     if (rows > T) rows = T;
     q.blocks = (int)((T + rows - 1) / rows);
     // equal blocks: the last one is not a remnant
@@ -1245,14 +1246,14 @@ static int lx_launch(LxGemmParams& p, const LxDeal& d, hipStream_t s, const char
 extern "C" {
 
 size_t vitk_linear_xent_workspace(int64_t T, int V, int D, int want_grad, int smoothing, int dw_f32, int bias, size_t block_bytes) {
-    if (T <= 0 || T > 0x7fffffff || V <= 0 || V > (1 << 22) || D <= 0 || D > (1 << 20)) return 0;
+    if (T <= 0 || T > (1 << 30) || V <= 0 || V > (1 << 22) || D <= 0 || D > (1 << 20)) return 0;
     return lx_plan(T, V, D, want_grad, smoothing, dw_f32, bias, block_bytes).total;
 }
 
 int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_type, const int64_t* target, int64_t T, int V, int D,
                      float smoothing, int64_t ignore_index, int mean, float* loss, float* rows, void* dx, int64_t lddx, void* dw, int64_t lddw, int dw_f32,
                      void* db, int db_f32, void* workspace, size_t workspace_bytes, size_t block_bytes, void* stream) {
-    VITK_REQUIRE(T > 0 && T <= 0x7fffffff && V > 0 && V <= (1 << 22) && D > 0 && D <= (1 << 20), "linear_xent: bad shape T=%lld V=%d D=%d", (long long)T, V, D);
+    VITK_REQUIRE(T > 0 && T <= (1 << 30) && V > 0 && V <= (1 << 22) && D > 0 && D <= (1 << 20), "linear_xent: bad shape T=%lld V=%d D=%d", (long long)T, V, D);
     VITK_REQUIRE(x && w && target && loss && rows && workspace, "linear_xent: null pointer");
     VITK_REQUIRE(D % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 && ldx >= D && ldw >= D && ldx < (1 << 22) && ldw < (1 << 22),
                  "linear_xent: D and the row strides must be multiples of 8, strides from D to 2^22 (D=%d ldx=%lld ldw=%lld)", D, (long long)ldx, (long long)ldw);
@@ -1296,8 +1297,10 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
             return rc;
         LxRowParams r = {};
         r.x = g.A; r.ldx = ldx; r.w = g.B; r.ldw = ldw; r.bias = bias; r.bias_type = bias_type; r.target = tg + r0; r.ignore_index = ignore_index;
-        r.stats = g.stats; r.zsum = g.zsum; r.stat_cols = g.stat_cols; const bool fused = q.blocks == 1 && T <= LX_FUSED;
-        r.ticket = ticket; r.scale = scale; r.loss = fused ? loss : nullptr; r.mean = mean; r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.rows_n = n; r.smoothing = smoothing;
+        r.stats = g.stats; r.zsum = g.zsum; r.stat_cols = g.stat_cols;
+        const bool fused = q.blocks == 1 && T <= LX_FUSED_ROWS && (!grad || (size_t)T * q.ldp * 2 <= LX_FUSED_BYTES);
+        r.ticket = ticket; r.scale = scale; r.loss = fused ? loss : nullptr; r.mean = mean;
+        r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.rows_n = n; r.smoothing = smoothing;
         // long rows get more waves.  By the vocabulary alone, so that a row's sums do not depend on how many rows there are or what is wanted.
         // STREAM: past the caches, where the block is larger than they are.
         const bool stream = grad && (size_t)n * q.ldp * 2 > LX_CACHED;
