@@ -241,6 +241,26 @@ def test_embedding_bwd_of_very_many_tokens(device, T, V, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 9, 256, 257, 511, 512, 513])                   # on both sides of the form for few tokens
+@pytest.mark.parametrize("V,D", [(3, 8), (4099, 24), (40, 256), (700, 264), (100, 1032), (1, 16384), (300001, 8)])
+def test_embedding_bwd_of_few_tokens(device, T, V, D):
+    ops = _ops()
+    g = torch.Generator().manual_seed(T * V)
+    for kind, dt, ot in (("bad", f32, f32), ("hot", bf16, f32), ("one", f32, bf16), ("hot", bf16, bf16)):
+        ids = EMB_IDS[kind](T, V, g)
+        dout = torch.randn(T, D, generator=g).to(dt)
+        out = torch.full((V, D), math.nan, dtype=ot, device=device)
+        got = ops.embedding_bwd(dout.to(device), ids.to(device), V, scale=0.7, padding_idx=0 if kind == "hot" else None, out=out)
+        check_embedding_grad(got, dout, ids, V, 0.7, 0 if kind == "hot" else None)
+    base = torch.randn(V, D, generator=g)
+    wide = torch.zeros(V, D + 8, device=device)
+    wide[:, :D] = base.to(device)
+    ops.embedding_bwd(dout.to(device), ids.to(device, torch.int32), V, out=wide[:, :D], accumulate=True)
+    check_embedding_grad(wide[:, :D], dout, ids, V, 1.0, None, base=base)
+    assert torch.all(wide[:, D:] == 0)
+
+
+@pytest.mark.gpu
 def test_embedding_bwd_without_tokens(device):
     ops = _ops()
     none = torch.empty(0, 8, device=device), torch.empty(0, dtype=torch.int64, device=device)
@@ -276,7 +296,7 @@ def test_embedding_bwd_accumulates_into_a_part_of_a_buffer(device, T):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,V", [(3000, 400), (30000, 400)])
+@pytest.mark.parametrize("T,V", [(3000, 400), (30000, 400), (300, 400), (300000, 400)])
 def test_embedding_bwd_in_a_graph(device, T, V):
     ops = _ops()
     ids = torch.randint(0, V, (T,), device=device)

@@ -468,6 +468,94 @@ __global__ __launch_bounds__(1024) void embedding_join_kernel(const EmbBwdParams
     if (col < p.D) emb_put<TO>(p, key, col, acc);
 }
 
+// Few tokens: everything in one launch, without a list.  The last workgroups zero the rows that no token has; each of the others is one token
+// and a slice of the columns, and if its token is the first with its id it collects the tokens that have the same one, in order, and
+// adds them up: up to eight by one group of threads, more by 256 / lanes groups, a stretch each, whose sums are joined in order.
+// A call takes 13 us instead of 19 (512 tokens, 1000 x 768), with 50021 x 768 to zero 16 instead of 21; the worst mix, one id alone before so
+// large a table, 28 instead of 22.
+#define FEW_MAX 512
+#define FEW_AHEAD 16
+#define FEW_ROWS 2048           // rows of the gradient a workgroup zeroes at a time, at most
+template <typename I, typename TI, typename TO>
+__global__ __launch_bounds__(256) void embedding_bwd_few_kernel(const EmbBwdParams p, const void* ids, long long padding, int zero_wgs, int zero_rows, int slices, int lanes) {
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, T = (int)p.T;
+    unsigned key[FEW_MAX / 256];
+#pragma unroll
+    for (int r = 0; r < FEW_MAX / 256; ++r) key[r] = r * 256 + tid < T ? emb_key<I>(ids, r * 256 + tid, p.V, padding) : (unsigned)p.V;
+    const int block = (int)blockIdx.x - T * slices;
+    if (block >= 0) {
+        __shared__ unsigned taken[FEW_ROWS / 32];
+        const unsigned row16 = (unsigned)(p.D * sizeof(TO) / 16);
+        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+        for (long long r0 = (long long)block * zero_rows; r0 < p.V; r0 += (long long)zero_wgs * zero_rows) {
+            const int rows = p.V - r0 < zero_rows ? (int)(p.V - r0) : zero_rows;
+            if (tid < FEW_ROWS / 32) taken[tid] = 0u;
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < FEW_MAX / 256; ++r) {
+                const long long at = (long long)key[r] - r0;
+                if (key[r] < (unsigned)p.V && at >= 0 && at < rows) atomicOr(&taken[at >> 5], 1u << (at & 31));
+            }
+            __syncthreads();
+            uint4* q = reinterpret_cast<uint4*>(reinterpret_cast<TO*>(p.out) + r0 * p.D);
+            for (unsigned i = tid; i < rows * row16; i += 256) {
+                const unsigned r = i / row16;
+                if (((taken[r >> 5] >> (r & 31)) & 1u) == 0u) q[i] = z;
+            }
+            __syncthreads();
+        }
+        return;
+    }
+    __shared__ unsigned short list[FEW_MAX];
+    __shared__ int counts[FEW_MAX / 64];
+    __shared__ float sums[256][8];
+    const int t = (int)blockIdx.x / slices, slice = (int)blockIdx.x - t * slices;
+    const unsigned mine = emb_key<I>(ids, t, p.V, padding);
+    if (mine == (unsigned)p.V) return;
+    unsigned long long same[FEW_MAX / 256];
+#pragma unroll
+    for (int r = 0; r < FEW_MAX / 256; ++r) {
+        same[r] = __ballot(key[r] == mine);
+        if (lane == 0) counts[r * 4 + wave] = __popcll(same[r]);
+    }
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < FEW_MAX / 64; ++w) {
+        if ((w & 3) == wave && key[w >> 2] == mine) list[n + __popcll(same[w >> 2] & ((1ull << lane) - 1ull))] = (unsigned short)((w >> 2) * 256 + tid);
+        n += counts[w];
+    }
+    __syncthreads();
+    if (list[0] != t) return;
+    const int groups = n > 8 ? 256 / lanes : 1, g = tid / lanes, col = (slice * lanes + tid - g * lanes) * 8;
+    const int from = g < groups ? n * g / groups : 0, to = g < groups ? n * (g + 1) / groups : 0;
+    const TI* dout = reinterpret_cast<const TI*>(p.dout) + col;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (col < p.D) {
+        for (int i = from; i < to; i += FEW_AHEAD) {
+            float v[FEW_AHEAD][8];
+#pragma unroll
+            for (int j = 0; j < FEW_AHEAD; ++j)
+                if (i + j < to) Emb8<TI>::load(dout + (long long)list[i + j] * p.ldd, v[j]);
+#pragma unroll
+            for (int j = 0; j < FEW_AHEAD; ++j)
+                if (i + j < to) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) acc[k] += v[j][k];
+                }
+        }
+    }
+    if (groups > 1) {
+        if (g > 0) Emb8<float>::store(sums[tid], acc);
+        __syncthreads();
+        if (g == 0)
+            for (int o = 1; o < groups; ++o)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) acc[k] += sums[o * lanes + tid][k];
+    }
+    if (g == 0 && col < p.D) emb_put<TO>(p, mine, col, acc);
+}
+
 // threads per piece: the columns in eights, a power of two below a wave and whole waves above
 static int emb_lanes(int D) {
     const int n = D / 8;
@@ -491,7 +579,7 @@ static int emb_passes(long long V) {
     while (bits < 32 && (V >> bits) != 0) ++bits;        // keys 0 .. V
     return (bits + SORT_BITS - 1) / SORT_BITS;
 }
-static bool emb_one(long long T, long long V) { return T == 0 || (T <= GROUP_MAX && V <= (1 << 18)); }
+static bool emb_one(long long T, long long V) { return T <= GROUP_MAX && V <= (1 << 18); }
 static long long emb_sort_blocks(long long T) { return (T + SORT_BLOCK - 1) / SORT_BLOCK; }
 static long long emb_sort_groups(long long T) { return emb_sort_blocks(T) > SORT_DIRECT ? (emb_sort_blocks(T) + SORT_GROUP - 1) / SORT_GROUP : 0; }
 static size_t emb_up(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -530,7 +618,7 @@ int vitk_embedding_fwd(const void* ids, int ids_are_64, const void* table, int t
 }
 
 size_t vitk_embedding_bwd_workspace(int64_t T, int64_t V, int D) {
-    if (T <= 0 || V <= 0 || D <= 0) return 16;
+    if (T <= FEW_MAX || V <= 0 || D <= 0) return 16;
     const long long pieces = (T + emb_piece(T, D) - 1) / emb_piece(T, D);
     size_t n = emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)pieces * 2 * D * sizeof(float));
     if (!emb_one(T, V)) n += emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)(emb_sort_blocks(T) + emb_sort_groups(T)) * SORT_BINS * sizeof(unsigned));
@@ -542,7 +630,7 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
                        void* stream) {
     VITK_REQUIRE(T >= 0 && V > 0 && D > 0, "embedding_bwd: bad shape T=%lld V=%lld D=%d", (long long)T, (long long)V, D);
     VITK_REQUIRE((dout_type == 0 || dout_type == 1) && (dtable_type == 0 || dtable_type == 1), "embedding_bwd: types are 0 (fp32) and 1 (bf16)");
-    VITK_REQUIRE(T < 0x7fffffffll && V < 0x7fffffffll, "embedding_bwd: T and V must be below 2^31");
+    VITK_REQUIRE(T < 0x7fffffffll && V < 0x7fffffffll && D <= (1 << 23), "embedding_bwd: T and V must be below 2^31, D at most 2^23");
     VITK_REQUIRE(dtable && workspace && (T == 0 || (dout && ids)), "embedding_bwd: null pointer");
     VITK_REQUIRE(D % 8 == 0 && ldd % 8 == 0 && ldo % 8 == 0 && ldd >= D && ldo >= D, "embedding_bwd: D and the row strides must be multiples of 8, strides >= D (D=%d ldd=%lld ldo=%lld)",
                  D, (long long)ldd, (long long)ldo);
@@ -555,27 +643,46 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
     }
     if (T == 0 && accumulate) return VITK_OK;
     hipStream_t s = (hipStream_t)stream;
+    EmbBwdParams p = {};
+    p.dout = dout; p.out = dtable; p.T = T; p.V = V; p.ldd = ldd; p.ldo = ldo; p.D = D; p.accumulate = accumulate; p.scale = scale;
+    const int types = (dout_type << 1) | dtable_type;
+    if (T <= FEW_MAX) {
+        const int lanes = D > 256 ? 32 : emb_lanes(D), few_slices = (D / 8 + lanes - 1) / lanes;
+        const long long bytes = (long long)D * (dtable_type == 0 ? 4 : 2);
+        const int zero_rows = (int)(bytes >= 65536 ? 1 : 65536 / bytes < FEW_ROWS ? 65536 / bytes : FEW_ROWS);
+        const int zero_wgs = accumulate ? 0 : (int)((V + zero_rows - 1) / zero_rows < 1024 ? (V + zero_rows - 1) / zero_rows : 1024);
+#define EMB_FEW(TI, TO)                                                                                                                                    \
+    if (ids_are_64) embedding_bwd_few_kernel<int64_t, TI, TO><<<zero_wgs + (int)T * few_slices, 256, 0, s>>>(p, ids, padding_idx, zero_wgs, zero_rows, few_slices, lanes); \
+    else embedding_bwd_few_kernel<int32_t, TI, TO><<<zero_wgs + (int)T * few_slices, 256, 0, s>>>(p, ids, padding_idx, zero_wgs, zero_rows, few_slices, lanes)
+        switch (types) {
+            case 0: EMB_FEW(float, float); break;
+            case 1: EMB_FEW(float, bf16_t); break;
+            case 2: EMB_FEW(bf16_t, float); break;
+            default: EMB_FEW(bf16_t, bf16_t); break;
+        }
+#undef EMB_FEW
+        return vitk_check_launch("embedding_bwd_few");
+    }
     const long long zero16 = accumulate ? 0 : (long long)V * D * (dtable_type == 0 ? 4 : 2) / 16;
     const int zero_blocks = (int)(zero16 / 4096 < 1024 ? (zero16 + 4095) / 4096 : 1024);
     const int passes = emb_passes(V);
     char* ws = (char*)workspace;
     uint2* sorted = (uint2*)ws;
     ws += emb_up((size_t)T * sizeof(uint2));
-    EmbBwdParams p;
+    p.sorted = sorted;
     p.piece = emb_piece(T, D);
     p.pieces = (int)((T + p.piece - 1) / p.piece);
     p.partial = (float*)ws;
     ws += emb_up((size_t)p.pieces * 2 * D * sizeof(float));
     if (emb_one(T, V)) {
         const int grid = GROUP_WG + zero_blocks;
-        const long long ids_of = T > 0 ? V : 1;         // no token: nothing to group, zeros alone
-        const size_t lds = emb_group_lds(ids_of);
+        const size_t lds = emb_group_lds(V);
         static VitkLdsOnce once64 = {}, once32 = {};        // the largest is allowed once; a launch asks for what its vocabulary needs
         if (int rc = ids_are_64 ? vitk_lds_once(once64, (const void*)emb_group_kernel<int64_t>, emb_group_lds(1 << 18), "embedding_bwd")
                                 : vitk_lds_once(once32, (const void*)emb_group_kernel<int32_t>, emb_group_lds(1 << 18), "embedding_bwd"))
             return rc;
-        if (ids_are_64) emb_group_kernel<int64_t><<<grid, 1024, lds, s>>>(ids, (int)T, ids_of, padding_idx, sorted, (uint4*)dtable, zero16);
-        else emb_group_kernel<int32_t><<<grid, 1024, lds, s>>>(ids, (int)T, ids_of, padding_idx, sorted, (uint4*)dtable, zero16);
+        if (ids_are_64) emb_group_kernel<int64_t><<<grid, 1024, lds, s>>>(ids, (int)T, V, padding_idx, sorted, (uint4*)dtable, zero16);
+        else emb_group_kernel<int32_t><<<grid, 1024, lds, s>>>(ids, (int)T, V, padding_idx, sorted, (uint4*)dtable, zero16);
         if (int rc = vitk_check_launch("embedding_bwd_sort")) return rc;
     } else {
         uint2* other = (uint2*)ws;
@@ -601,15 +708,13 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
             to = to == sorted ? other : sorted;
         }
     }
-    if (T == 0) return VITK_OK;
-    p.sorted = sorted; p.dout = dout; p.out = dtable; p.T = T; p.V = V; p.ldd = ldd; p.ldo = ldo; p.D = D; p.accumulate = accumulate; p.scale = scale;
     const int lanes = emb_lanes(D), side = lanes < 64 ? 256 / lanes : 1, slices = (D / 8 + lanes - 1) / lanes;
     const dim3 block(lanes, side), grid((p.pieces + side - 1) / side, slices);
 #define EMB_BWD(TI, TO)                                                                                                            \
     embedding_bwd_kernel<TI, TO><<<grid, block, 0, s>>>(p);                                                                        \
     if (p.pieces > 1 && side > 1) embedding_join_kernel<TO, 1><<<grid, block, 0, s>>>(p);                                          \
     else if (p.pieces > 1) embedding_join_kernel<TO, 4><<<dim3(p.pieces - 1, slices), dim3(lanes, 4), 0, s>>>(p)
-    switch ((dout_type << 1) | dtable_type) {
+    switch (types) {
         case 0: EMB_BWD(float, float); break;
         case 1: EMB_BWD(float, bf16_t); break;
         case 2: EMB_BWD(bf16_t, float); break;
