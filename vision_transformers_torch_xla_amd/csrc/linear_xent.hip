@@ -4,14 +4,14 @@
 //   dz_ij = p_ij - (1 - e) [j = t(i)] - e/V            dx = g dz W      dW = g dz^T x      db = g sum_i dz_i
 //
 // x bf16 [T, D], W bf16 [V, D].  The rows are worked through in blocks whose size the workspace bounds; per block
-//   1. x W^T tile by tile (lx_gemm_kernel, NT).  The epilogue takes a tile's logits in fp32 from the accumulators: per row and 64
+//   1. x W^T tile by tile (lx_logits_kernel).  The epilogue takes a tile's logits in fp32 from the accumulators: per row and 64
 //      columns their maximum m and s = sum exp(z - m) go to a small table (in powers of two); exp(z - m) itself, in [0, 1], goes to the block's
 //      matrix P in fp16 (11 bits; bf16 would round it 8 times as far; what falls below fp16's 6e-8 of its maximum is below what the
 //      later bf16 rounding of its larger neighbours leaves).  Loss alone: only the table is written.
 //   2. one workgroup per row (lx_row_kernel): lse from the table, the target's logit as a dot product of its own, the row's loss, and
 //      P -> dz in place, now bf16: the one rounding of the gradient's factor.  g is not in it: a constant such as 1 / count would be
 //      rounded 1 part in 256 in the same direction everywhere; it multiplies the fp32 sums of the next step.
-//   3. dx = dz W (NN) and dW = dz^T x (TN) with the same kernel, and the column sums for db.
+//   3. dx = dz W and dW = dz^T x (lx_grad_kernel), and the column sums for db.
 // 6 T V D floating-point operations: nothing is computed twice.  Keeping one 16-bit factor per logit of a block costs 4 bytes of
 // traffic per logit for step 2, where computing the logits again for the gradients would cost 2 D operations.
 #include "common.h"
@@ -21,6 +21,7 @@
 #define LX_TILE 256
 #define LX_ELEMS (LX_TILE * LX_BK)                            // elements per operand tile
 #define LX_LDS (4 * LX_ELEMS * 2 + 8 * 16 * 64 * 4)           // two buffers of both tiles, 4 KB of epilogue staging per wave
+#define LX_GRAD_LDS (4 * LX_ELEMS * 2 + 4 * 16 * 64 * 4)
 #define LX_STAT 64                                            // columns per entry of the statistics table
 
 enum { LX_NT = 0, LX_NN = 1, LX_TN = 2 };
@@ -155,127 +156,76 @@ static __host__ __device__ __forceinline__ void lx_range(int g, int total, int G
     to = from + q + (g < r ? 1 : 0);
 }
 
-// One 512-thread workgroup per compute unit works through 256 x 256 tiles of the output, 8 waves (2 x 4) of 128 x 64 = 128 accumulator
-// registers each, 64-deep steps.  Operands go from memory to LDS by DMA, two steps ahead across tile borders, into a double buffer;
-// fragments are read one phase of 16 matrix instructions before their use.  An operand whose rows run along the contraction sits in LDS as
-// [256][64] (16-byte chunks XOR-swizzled by the row) and is read with ds_read_b128; one whose rows run along the output as [64][256]
-// and is read with the transposing ds_read_b64_tr_b16: no transposed copy of W or dz is made.  The matrix instruction's operands are
-// swapped, so a lane holds four consecutive columns of one output row.  Tiles are dealt by number (no counters: a captured graph may be
-// replayed on any stream); a tile order in bands of 8 column tiles keeps what the 32 workgroups of an XCD read at a time to 4 row panels
-// and 8 column panels.
-template <int LAY, int EPI>
-__global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
-    constexpr bool AT = LAY == LX_TN, BT = LAY != LX_NT;        // operand stored with the contraction as its slow dimension
+#define LX_WAIT(n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n) : "memory")
+#define LX_BARRIER()                       \
+    __builtin_amdgcn_s_barrier();          \
+    asm volatile("" ::: "memory")
+
+// The logits: one 512-thread workgroup per compute unit works through 256 x 256 tiles, 8 waves (2 x 4) of 128 x 64 = 128 accumulator registers each,
+// 64-deep steps.  Operands go from memory to LDS by DMA, two steps ahead across tile borders, into a double buffer; fragments are read one
+// phase of 16 matrix instructions before their use.  An operand sits in LDS as [256][64], its 16-byte chunks XOR-swizzled by the row, and is
+// read with ds_read_b128.  The matrix instruction's operands are swapped, so a lane holds four consecutive columns of one output row.
+// Tiles are dealt by number (no counters: a captured graph may be replayed on any stream): workgroup g of G takes the tiles g, g + G, ...,
+// in bands of 8 column tiles, which keeps what the 32 workgroups of an XCD read at a time to 4 row panels and 8 column panels.
+// Two waves share a SIMD because the loss's epilogue is vector arithmetic (an exponential per logit), which one wave's stalls would leave
+// uncovered: with four waves as in lx_grad_kernel 8192 x 100003 x 2048 takes 2820 instead of 2550 us, 2047 x 50021 x 1024 239 instead of 182.
+// Matrix pipe 68 % busy at the first of these; a library product of the two operands alone takes 2501 us.
+template <int EPI>
+__global__ __launch_bounds__(512) void lx_logits_kernel(const LxGemmParams p) {
     extern __shared__ __attribute__((aligned(16))) bf16_t lsm[];   // [2 buffers][A tile | B tile], [8 waves][16][64] fp32
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 2, wn = wave & 3;
     const int lr = lane & 15, lg = lane >> 4;
-    const int lq = lr >> 2, lp = lr & 3;
     const unsigned lds_base = __builtin_amdgcn_readfirstlane(lds_addr(lsm));
     const unsigned lds_stage = (unsigned)(wave * 4 * 1024);
 
-    const int G = gridDim.x;
-    int whole_items, parts = 0, r0 = 0, r1 = 0, rt = 0, team = 0, member = 0;
-    if constexpr (EPI == LX_OUT) {
-        const int id = xcd_remap(blockIdx.x, G);        // a team's workgroups are neighbours on one XCD
-        team = __builtin_amdgcn_readfirstlane(id / p.width);
-        member = __builtin_amdgcn_readfirstlane(id - team * p.width);
-        whole_items = __builtin_amdgcn_readfirstlane(team < p.whole ? (p.whole - 1 - team) / p.teams + 1 : 0);
-        if (team < p.ranges) {
-            lx_range(team, p.rest * p.steps, p.ranges, r0, r1);
-            r0 = __builtin_amdgcn_readfirstlane(r0);
-            r1 = __builtin_amdgcn_readfirstlane(r1);
-            rt = __builtin_amdgcn_readfirstlane(r0 / p.steps);        // row (of the rest) of the first part
-            parts = r1 > (rt + 1) * p.steps ? 2 : 1;
-        }
-    } else {
-        const int tiles = p.tiles_m * p.tiles_n;
-        whole_items = __builtin_amdgcn_readfirstlane((int)blockIdx.x < tiles ? (tiles - 1 - (int)blockIdx.x) / G + 1 : 0);
-    }
-    const int items = whole_items + parts;
+    const int G = gridDim.x, tiles = p.tiles_m * p.tiles_n;
+    const int items = __builtin_amdgcn_readfirstlane((int)blockIdx.x < tiles ? (tiles - 1 - (int)blockIdx.x) / G + 1 : 0);
 
-    // ---- staging: where the next step's operands come from.  A is staged in two halves, the rows that are the first 64 of a wave's 128
-    // (half 0) and the others, because the two are read at different times.  A piece is one instruction of one wave, 1 KB of LDS.
-    // K-contiguous: image [256][64]; a piece is 8 rows, LDS position lane % 8 receives chunk (lane % 8) ^ (row & 7)
-    // A, K-strided: image [2 halves][64][128]; a piece is 4 rows, position lane % 16 receives chunk (lane % 16) ^ lx_swz(row)
-    // B, K-strided: image [64][256]; a piece is 2 rows, position lane % 32 receives chunk (lane % 32) ^ lx_swz(row)
-    int sv = 0, sk = 0, sk_end = 0;
+    // ---- staging: where the next step's operands come from.  A piece is one instruction of one wave, 1 KB of LDS: 8 rows, LDS position lane % 8
+    // receives chunk (lane % 8) ^ (row & 7).  A is staged in two halves, the rows that are the first 64 of a wave's 128 and the others.
+    int sv = 0, sk = 0;
     const bf16_t* sA = p.A;
     const bf16_t* sB = p.B;
     unsigned voA[4], voB[4];
-    // item v: where its tile is, its steps k0 .. k1 - 1, and which part it is (-1: a whole tile)
-    auto locate = [&](int v, int& m0, int& n0, int& k0, int& k1, int& part) {
-        k0 = 0;
-        k1 = p.steps;
-        part = -1;
-        int tm, tn;
-        if constexpr (EPI == LX_OUT) {
-            int row = v * p.teams + team;
-            if (v >= whole_items) {
-                part = v - whole_items;
-                row = p.whole + rt + part;
-                if (part == 0) k0 = r0 - rt * p.steps;
-                const int left = r1 - (rt + part) * p.steps;
-                k1 = left < p.steps ? left : p.steps;
-            }
-            const int blk = row / p.tiles_m;
-            tm = row - blk * p.tiles_m;
-            tn = blk * p.width + member;
-        } else {
-            const int tile = xcd_remap(blockIdx.x + v * G, p.tiles_m * p.tiles_n);
-            const int full = p.tiles_m * 8;
-            const int blk = tile / full;
-            const int rem = tile - blk * full;
-            const int c0 = blk * 8;
-            const int width = p.tiles_n - c0 < 8 ? p.tiles_n - c0 : 8;
-            tm = rem / width;
-            tn = c0 + rem - tm * width;
-        }
+    auto locate = [&](int v, int& m0, int& n0) {
+        const int tile = xcd_remap(blockIdx.x + v * G, tiles);
+        const int full = p.tiles_m * 8;
+        const int blk = tile / full;
+        const int rem = tile - blk * full;
+        const int c0 = blk * 8;
+        const int width = p.tiles_n - c0 < 8 ? p.tiles_n - c0 : 8;
+        const int tm = rem / width;
         // the divisions run on the vector unit: say that their results are the same in every lane
         m0 = __builtin_amdgcn_readfirstlane(tm * LX_TILE);
-        n0 = __builtin_amdgcn_readfirstlane(tn * LX_TILE);
+        n0 = __builtin_amdgcn_readfirstlane((c0 + rem - tm * width) * LX_TILE);
     };
     auto aim = [&](int v) {
-        int m0, n0, part;
-        locate(v, m0, n0, sk, sk_end, part);
-        sA = p.A + (AT ? (size_t)m0 : (size_t)m0 * p.lda);
-        sB = p.B + (BT ? (size_t)n0 : (size_t)n0 * p.ldb);
-        // rows and columns behind the edge of the output read the last valid ones: their results are not stored
+        int m0, n0;
+        locate(v, m0, n0);
+        sk = 0;
+        sA = p.A + (size_t)m0 * p.lda;
+        sB = p.B + (size_t)n0 * p.ldb;
+        // rows behind the edge of the output read the last valid ones: their results are not stored
         const int ma = p.M - 1 - m0, mb = p.N - 1 - n0;
         // the lane number passes through an empty asm, so that what is derived from it here is not kept in registers over the main loop
         int ln = lane;
         asm volatile("" : "+v"(ln));
         const int srow = ln >> 3, sch = (ln & 7) ^ srow;
-        const int shalf = ln >> 5, spos = ln & 31;
-        const int arow = ln >> 4, apos = ln & 15;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (AT) {
-                const int r = (wave * 2 + (j & 1)) * 4 + arow;
-                const int c = apos ^ lx_swz(r);
-                voA[j] = (unsigned)((r * p.lda + (c >> 3) * 128 + (j >> 1) * 64 + (c & 7) * 8) * 2);      // A's rows are padded to a multiple of 256
-            } else {
-                const int b = wave * 2 + (j & 1);
-                const int r = (b >> 3) * 128 + (j >> 1) * 64 + (b & 7) * 8 + srow;
-                voA[j] = (unsigned)(((r < ma ? r : ma) * p.lda + sch * 8) * 2);
-            }
-            if (BT) {
-                const int r = (wave * 4 + j) * 2 + shalf;
-                const int c = (spos ^ lx_swz(r)) * 8;
-                voB[j] = (unsigned)((r * p.ldb + (n0 + c < p.N ? c : p.N - 8 - n0)) * 2);
-            } else {
-                const int r = (wave * 4 + j) * 8 + srow;
-                voB[j] = (unsigned)(((r < mb ? r : mb) * p.ldb + sch * 8) * 2);
-            }
+            const int b = wave * 2 + (j & 1);
+            const int ra = (b >> 3) * 128 + (j >> 1) * 64 + (b & 7) * 8 + srow, rb = (wave * 4 + j) * 8 + srow;
+            voA[j] = (unsigned)(((ra < ma ? ra : ma) * p.lda + sch * 8) * 2);
+            voB[j] = (unsigned)(((rb < mb ? rb : mb) * p.ldb + sch * 8) * 2);
         }
     };
     // what lies behind the contraction's end comes from the zero row (the lane number passes through an empty asm as in aim)
     auto stageA = [&](int par, int half) {
-        const bf16_t* src = sA + (AT ? (size_t)sk * LX_BK * p.lda : (size_t)sk * LX_BK);
-        const unsigned dst = lds_base + (unsigned)(par * 2 * LX_ELEMS * 2) +
-                             (AT ? half * 16384 + wave * 2048 : (wave >> 2) * 16384 + half * 8192 + (wave & 3) * 2048);
+        const bf16_t* src = sA + (size_t)sk * LX_BK;
+        const unsigned dst = lds_base + (unsigned)(par * 2 * LX_ELEMS * 2) + (wave >> 2) * 16384 + half * 8192 + (wave & 3) * 2048;
         if ((sk + 1) * LX_BK <= p.KA) {
             glds16(src, voA[2 * half], dst);
             glds16(src, voA[2 * half + 1], dst + 1024);
@@ -283,32 +233,28 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
             int ln = lane;
             asm volatile("" : "+v"(ln));
             const void* zrow = (const char*)lx_zero_row + (ln & 31) * 16;
+            const int k = sk * LX_BK + ((ln & 7) ^ (ln >> 3)) * 8;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int k = sk * LX_BK + (AT ? (wave * 2 + j) * 4 + (ln >> 4) : ((ln & 7) ^ (ln >> 3)) * 8);
-                glds16_v(k < p.KA ? (const void*)((const char*)src + voA[2 * half + j]) : zrow, dst + j * 1024);
-            }
+            for (int j = 0; j < 2; ++j) glds16_v(k < p.KA ? (const void*)((const char*)src + voA[2 * half + j]) : zrow, dst + j * 1024);
         }
     };
     auto stageB = [&](int par) {
-        const bf16_t* src = sB + (BT ? (size_t)sk * LX_BK * p.ldb : (size_t)sk * LX_BK);
+        const bf16_t* src = sB + (size_t)sk * LX_BK;
         const unsigned dst = lds_base + (unsigned)((par * 2 + 1) * LX_ELEMS * 2) + lds_stage;
-        if ((sk + 1) * LX_BK <= p.KB) {
+        if ((sk + 1) * LX_BK <= p.KA) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) glds16(src, voB[j], dst + j * 1024);
         } else {
             int ln = lane;
             asm volatile("" : "+v"(ln));
             const void* zrow = (const char*)lx_zero_row + (ln & 31) * 16;
+            const int k = sk * LX_BK + ((ln & 7) ^ (ln >> 3)) * 8;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int k = sk * LX_BK + (BT ? (wave * 4 + j) * 2 + (ln >> 5) : ((ln & 7) ^ (ln >> 3)) * 8);
-                glds16_v(k < p.KB ? (const void*)((const char*)src + voB[j]) : zrow, dst + j * 1024);
-            }
+            for (int j = 0; j < 4; ++j) glds16_v(k < p.KA ? (const void*)((const char*)src + voB[j]) : zrow, dst + j * 1024);
         }
     };
     auto advance = [&]() {
-        if (++sk == sk_end) {
+        if (++sk == p.steps) {
             ++sv;
             if (sv < items) aim(sv);
         }
@@ -316,42 +262,21 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
 
     // ---- fragments
     int offA[2], offB[2];
-    int preA = 0, preB = 0, rbase = 0;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
         const int x = ((ks * 4 + lg) ^ (lr & 7)) << 3;
         offA[ks] = (wm * 128 + lr) * LX_BK + x;
         offB[ks] = (wn * 64 + lr) * LX_BK + x;
     }
-    if (AT || BT) {
-        const int sw = lx_swz(8 * lg + lq);
-        preA = ((wm * 8) | (lp >> 1)) ^ sw;
-        preB = ((wn * 8) | (lp >> 1)) ^ sw;
-        rbase = 8 * lg + lq;
-    }
     f32x4 acc[8][4];
     bf16x8 faE[4], faO[4], fbE[4], fbO[4];
     auto ldA = [&](bf16x8 (&f)[4], const bf16_t* cA, int ks, int h) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if (AT) {
-                const bf16_t* q = cA + h * 8192 + (ks * 32 + rbase) * 128 + (lp & 1) * 4 + ((preA ^ (2 * t)) << 3);
-                f[t] = lx_tr(q, q + 4 * 128);
-            } else {
-                f[t] = *reinterpret_cast<const bf16x8*>(cA + offA[ks] + (4 * h + t) * 16 * LX_BK);
-            }
-        }
+        for (int t = 0; t < 4; ++t) f[t] = *reinterpret_cast<const bf16x8*>(cA + offA[ks] + (4 * h + t) * 16 * LX_BK);
     };
     auto ldB = [&](bf16x8 (&f)[4], const bf16_t* cB, int ks) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if (BT) {
-                const bf16_t* q = cB + (ks * 32 + rbase) * 256 + (lp & 1) * 4 + ((preB ^ (2 * t)) << 3);
-                f[t] = lx_tr(q, q + 4 * 256);
-            } else {
-                f[t] = *reinterpret_cast<const bf16x8*>(cB + offB[ks] + t * 16 * LX_BK);
-            }
-        }
+        for (int t = 0; t < 4; ++t) f[t] = *reinterpret_cast<const bf16x8*>(cB + offB[ks] + t * 16 * LX_BK);
     };
     auto mma = [&](const bf16x8 (&fa)[4], const bf16x8 (&fb)[4], int h) {
 #pragma unroll
@@ -361,37 +286,24 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
                 acc[4 * h + tm][tn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[tn], fa[tm], acc[4 * h + tm][tn], 0, 0, 0);
     };
     // interleave a phase's 16 matrix instructions with its LDS reads
-    constexpr int RA = AT ? 8 : 4, RAB = (AT ? 8 : 4) + (BT ? 8 : 4);
 #define LX_MIX(reads)                                                                 \
     _Pragma("unroll") for (int i = 0; i < (reads); ++i) {                             \
         __builtin_amdgcn_sched_group_barrier(0x008, 16 / (reads), 0);                 \
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                            \
     }                                                                                 \
     __builtin_amdgcn_sched_barrier(0)
-#define LX_WAIT(n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n) : "memory")
-#define LX_BARRIER()                       \
-    __builtin_amdgcn_s_barrier();          \
-    asm volatile("" ::: "memory")
 
-    // The steps of all items of a workgroup form one stream, requested two steps ahead into the buffer of the current one.  A step is four
-    // phases: (A half 0, k 0..31), (half 0, k 32..63), (half 1, k 0..31), (half 1, k 32..63), fragments read one phase ahead, so that B
-    // and half 0 of the buffer have been read after the first phase and half 1 after the third.  Two schedules:
-    //   DEEP (dz W): barriers X behind the first and Y behind the third phase.  Behind X the requests for B and half 0 of step s + 2 go
-    //     out, behind Y those for half 1.  Y publishes B and half 0 of step s + 1, X half 1 of step s: a request has 1.25 to 1.5 steps to
-    //     arrive.  vmcnt counts in issue order (4 for B, 2 for a half): at X what is younger than half 1 of s are the 8 requests of s + 1,
-    //     at Y half 1 of s + 1 and the 6 of s + 2.
-    //   else: one barrier, Y.  Behind it the requests for A of step s + 2 go out, a phase later those for B; they have 0.75 to 1 step.
-    // The second barrier costs a step 8 % where the operands come out of the caches (x W^T, dz^T x: 2625 -> 2840 us and 2610 -> 2830
-    // us at 8192 x 100003 x 2048); dz W streams dz from memory along its long contraction and gains 9 % (2755 -> 2500 us).
+    // The steps of all tiles of a workgroup form one stream, requested two steps ahead into the buffer of the current one.  A step is four
+    // phases: (A half 0, k 0..31), (half 1, k 0..31), (half 0, k 32..63), (half 1, k 32..63), fragments read one phase ahead; behind the
+    // third the whole buffer has been read and the barrier opens it: the requests for A of step s + 2 go out, a phase later those for B;
+    // they have 0.75 to 1 step to arrive.  (Requesting B and half of A after the first phase, with a second barrier, costs a step 8 %.)
     // The output stores of a full tile (16 of a wave at least) between two steps may stay in flight over the first step's waits.
-    constexpr bool DEEP = LAY == LX_NN;
-    if (EPI != LX_OUT && blockIdx.x == 0 && tid == 0) *p.ticket = 0u;
+    if (blockIdx.x == 0 && tid == 0) *p.ticket = 0u;
     if (items == 0) return;
     aim(0);
     stageB(0); stageA(0, 0); stageA(0, 1);
     advance();
-    bool n1 = sv < items;       // step s + 1 is on its way
-    if (n1) {
+    if (sv < items) {
         stageB(1); stageA(1, 0); stageA(1, 1);
         advance();
         LX_WAIT(8);
@@ -403,8 +315,281 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
     ldA(faE, lsm, 0, 0);
     int par = 0;
     bool loose = false;         // at least 16 output stores of this wave are younger than its requests
-    bool pend = false;          // not DEEP: A of a step is on its way into the other buffer, B is not yet requested
+    bool pend = false;          // A of a step is on its way into the other buffer, B is not yet requested
 
+    for (int v = 0; v < items; ++v) {
+        int m0, n0;
+        locate(v, m0, n0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int kt = 0; kt < p.steps; ++kt) {
+            const bf16_t* cA = lsm + par * 2 * LX_ELEMS;
+            const bf16_t* cB = cA + LX_ELEMS;
+            const bf16_t* nA = lsm + (par ^ 1) * 2 * LX_ELEMS;
+            const bf16_t* nB = nA + LX_ELEMS;
+            if (pend) { stageB(par ^ 1); advance(); pend = false; }
+            mma(faE, fbE, 0);
+            ldA(faO, cA, 0, 1);
+            LX_MIX(4);
+            mma(faO, fbE, 1);
+            ldB(fbO, cB, 1);
+            ldA(faE, cA, 1, 0);
+            LX_MIX(8);
+            mma(faE, fbO, 0);
+            ldA(faO, cA, 1, 1);
+            LX_MIX(4);
+            if (loose) LX_WAIT(16);
+            else LX_WAIT(0);
+            LX_BARRIER();
+            if (sv < items) { stageA(par, 0); stageA(par, 1); pend = true; }
+            mma(faO, fbO, 1);
+            ldB(fbE, nB, 0);
+            ldA(faE, nA, 0, 0);
+            LX_MIX(8);
+            loose = false;
+            par ^= 1;
+        }
+        if (pend) { stageB(par ^ 1); advance(); pend = false; }      // before the stores: vmcnt counts in issue order
+        lx_loss_epilogue<8, EPI == LX_XENT_BIAS>(p, acc, m0 + wm * 128, n0 + wn * 64, reinterpret_cast<bf16_t*>(lsm + 4 * LX_ELEMS) + wave * (16 * 64 * 2));
+        loose = m0 + LX_TILE <= p.M && p.P != nullptr;       // every row is stored: 16 stores at least
+    }
+}
+
+template <int I> struct lx_int { static constexpr int value = I; };
+template <int FROM, int TO, class F>
+static __device__ __forceinline__ void lx_static_for(F&& f) {
+    if constexpr (FROM < TO) {
+        f(lx_int<FROM>{});
+        lx_static_for<FROM + 1, TO>(f);
+    }
+}
+template <int OFF>
+static __device__ __forceinline__ void lx_dma(const bf16_t* base, unsigned voff, unsigned lds_byte) {
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds_byte), "n"(OFF) : "memory", "m0", "scc");
+}
+static __device__ __forceinline__ void lx_mfma(f32x4& c, const bf16x8& a, const bf16x8& b) {
+    asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+static __device__ __forceinline__ bf16x8 lx_lds_tr(unsigned at) {
+    typedef __attribute__((address_space(3))) bf16x4* lds4;
+    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(__UINTPTR_TYPE__)at);
+    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(__UINTPTR_TYPE__)(at + 4 * 512));
+    return (bf16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+static __device__ __forceinline__ bf16x8 lx_lds_row(unsigned at) {
+    return *(const __attribute__((address_space(3))) bf16x8*)(__UINTPTR_TYPE__)at;
+}
+// to the other buffer, 64 KB on (the operands begin at LDS address 0, which the launch has no static LDS to move)
+static __device__ __forceinline__ void lx_flip(unsigned& at) { asm volatile("v_xor_b32 %0, 0x10000, %0" : "+v"(at)); }
+#define LX_PIN() __builtin_amdgcn_sched_barrier(0)
+#define LX_LDS_DONE() __builtin_amdgcn_s_waitcnt(0xc07f)         // lgkmcnt(0) as the compiler knows it: it adds no waits of its own behind it
+
+// The gradients, dx = dz W (NN) and dW = dz^T x (TN): persistent 256 x 256 tiles as above, but four waves (2 x 2) of 128 x 128, one on a SIMD with the
+// whole register file: 256 accumulators, fragments of a k half in use and of the next one arriving.  What bounds the eight-wave form is LDS:
+// its waves read 192 KB a step and the DMA writes 64 KB, together as many cycles at 128 bytes each as the matrix instructions take; four waves
+// read 128 KB.  But one wave to a SIMD hides nothing: every other instruction has to be issued in the 12 cycles a matrix instruction leaves, so
+// the order is written out instruction by instruction (the matrix instructions are inline assembly on accumulators that never move; a
+// scheduling barrier stands behind each), with one LDS read or request at a time between them, requests 5 to 7 matrix instructions
+// apart because a request occupies the path to LDS for 16 cycles and a wave that runs into another's waits, and the step's own
+// bookkeeping - addresses, buffer change - in the same gaps.
+// Operands whose rows run along the output (x, W, and dz for dW) sit in LDS as [64][256] and are read with the transposing ds_read_b64_tr_b16:
+// no transposed copy is made; dz for dx as [256][64] with ds_read_b128.
+//   8192 x 100003 x 2048: dz W 2520 -> 2170 us, dz^T x 2500 -> 2400 us (matrix pipe 82 % and 75 % busy; a library product of the same sizes and
+//   the layout it likes best 2117 and 2299 us).  25088 x 8192 x 768: 320 -> 284 and 289 -> 275 us.
+// Tiles are dealt by number as LxDeal says.
+template <int LAY>
+__global__ __launch_bounds__(256, 1) void lx_grad_kernel(const LxGemmParams p) {
+    constexpr bool AT = LAY == LX_TN;               // A is stored with the contraction as its slow dimension (B always is)
+    extern __shared__ __attribute__((aligned(16))) bf16_t lsm[];   // [2 buffers][A tile | B tile], [4 waves][16][64] fp32
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    const int lr = lane & 15, lg = lane >> 4;
+    const int lq = lr >> 2, lp = lr & 3;
+    const unsigned lds_base = __builtin_amdgcn_readfirstlane(lds_addr(lsm));
+
+    const int G = gridDim.x;
+    const int id = xcd_remap(blockIdx.x, G);        // a team's workgroups are neighbours on one XCD
+    const int team = __builtin_amdgcn_readfirstlane(id / p.width);
+    const int member = __builtin_amdgcn_readfirstlane(id - team * p.width);
+    const int whole_items = __builtin_amdgcn_readfirstlane(team < p.whole ? (p.whole - 1 - team) / p.teams + 1 : 0);
+    int parts = 0, r0 = 0, r1 = 0, rt = 0;
+    if (team < p.ranges) {
+        lx_range(team, p.rest * p.steps, p.ranges, r0, r1);
+        r0 = __builtin_amdgcn_readfirstlane(r0);
+        r1 = __builtin_amdgcn_readfirstlane(r1);
+        rt = __builtin_amdgcn_readfirstlane(r0 / p.steps);        // row (of the rest) of the first part
+        parts = r1 > (rt + 1) * p.steps ? 2 : 1;
+    }
+    const int items = whole_items + parts;
+
+    int sv = 0, sk = 0, sk_end = 0;
+    const bf16_t* sA = p.A;
+    const bf16_t* sB = p.B;
+    unsigned voA[8], voB[8];
+    // item v: where its tile is, its steps k0 .. k1 - 1, and which part it is (-1: a whole tile)
+    auto locate = [&](int v, int& m0, int& n0, int& k0, int& k1, int& part) {
+        k0 = 0;
+        k1 = p.steps;
+        part = -1;
+        int row = v * p.teams + team;
+        if (v >= whole_items) {
+            part = v - whole_items;
+            row = p.whole + rt + part;
+            if (part == 0) k0 = r0 - rt * p.steps;
+            const int left = r1 - (rt + part) * p.steps;
+            k1 = left < p.steps ? left : p.steps;
+        }
+        const int blk = row / p.tiles_m;
+        const int tm = row - blk * p.tiles_m, tn = blk * p.width + member;
+        m0 = __builtin_amdgcn_readfirstlane(tm * LX_TILE);
+        n0 = __builtin_amdgcn_readfirstlane(tn * LX_TILE);
+    };
+    // ---- requests.  A step's operand is eight pieces of 1 KB per wave, each an instruction.  [256][64]: 8 rows each, LDS position lane % 8 receives
+    // chunk (lane % 8) ^ (row & 7).  [64][256]: two rows each, pieces 0..3 of the contraction's first 32, position lane % 32 receives chunk
+    // (lane % 32) ^ lx_swz(row).  What lies behind the contraction's end needs no zeros in B, because A has them: dz is zero from the vocabulary's end
+    // to its row stride and, for dW, from the last row to a multiple of 64.  There B repeats its last row.
+    auto aim_rows = [&](unsigned (&vo)[8], int ld, int most) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int srow = ln >> 3, sch = (ln & 7) ^ srow;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int r = (wave * 8 + j) * 8 + srow;
+            vo[j] = (unsigned)(((r < most ? r : most) * ld + sch * 8) * 2);
+        }
+    };
+    auto aim_cols = [&](unsigned (&vo)[8], int ld, int last, int most) {        // last: rows behind it re-read it; most: likewise columns
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int shalf = ln >> 5, spos = ln & 31;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int r = (j >> 2) * 32 + (wave * 4 + (j & 3)) * 2 + shalf;
+            const int c = (spos ^ lx_swz(r)) * 8;
+            vo[j] = (unsigned)(((r < last ? r : last) * ld + (c < most ? c : most)) * 2);
+        }
+    };
+    int sm0 = 0, sn0 = 0;
+    const long long dA = AT ? (long long)LX_BK * p.lda : LX_BK, dB = (long long)LX_BK * p.ldb;
+    auto aim = [&](bool next) {
+        if (next) {
+            int part;
+            locate(sv, sm0, sn0, sk, sk_end, part);
+        }
+        sA = p.A + (AT ? (size_t)sm0 : (size_t)sm0 * p.lda) + sk * dA;
+        sB = p.B + sn0 + sk * dB;
+        if (AT) aim_cols(voA, p.lda, LX_BK - 1, LX_TILE - 1);
+        else aim_rows(voA, p.lda, p.M - 1 - sm0);
+        aim_cols(voB, p.ldb, p.KB - 1 - sk * LX_BK, p.N - 8 - sn0);
+    };
+    const unsigned dmaA = lds_base + wave * (AT ? 4096u : 8192u), dmaB = lds_base + LX_ELEMS * 2 + wave * 4096u;
+    auto stageA = [&](unsigned at, auto jt) __attribute__((always_inline)) {
+        constexpr int j = decltype(jt)::value;
+        lx_dma<AT ? (j >> 2) * 16384 + (j & 3) * 1024 : j * 1024>(sA, voA[j], dmaA + at);
+    };
+    auto stageB = [&](unsigned at, auto jt) __attribute__((always_inline)) {
+        constexpr int j = decltype(jt)::value;
+        lx_dma<(j >> 2) * 16384 + (j & 3) * 1024>(sB, voB[j], dmaB + at);
+    };
+    // A step has two phases, k 0..31 and k 32..63, and the fragments of a phase are read in the one before.  So a buffer's first half of a [64][256]
+    // image is free from phase 0 of its step on, its second half and a [256][64] image from phase 1 on; there they are requested for the step after
+    // next, the latter before the former, and have a step or more to arrive.  vmcnt counts in issue order: at the barrier before phase 0,
+    // 16 requests are younger than the second halves it reads; before phase 1, WX are younger than what that one reads.
+    constexpr int Q0 = AT ? 8 : 4, Q1 = 16 - Q0, WX = AT ? 16 : 8;
+    auto request = [&](unsigned at, auto pt, auto qt) __attribute__((always_inline)) {
+        constexpr int ph = decltype(pt)::value, q = decltype(qt)::value;
+        if constexpr (ph == 0) {
+            if constexpr (AT && q < 4) stageA(at, lx_int<q>{});
+            else stageB(at, lx_int<AT ? q - 4 : q>{});
+        } else if constexpr (AT) {
+            if constexpr (q < 4) stageA(at, lx_int<q + 4>{});
+            else stageB(at, lx_int<q>{});
+        } else {
+            if constexpr (q < 8) stageA(at, lx_int<q>{});
+            else stageB(at, lx_int<q - 4>{});
+        }
+    };
+    // sA and sB have been moved on by a step.  The last step of an item is aimed at anew (it may be a short one), the first one of the next item
+    // too; behind the last step of all the requests repeat it.
+    auto advance = [&]() {
+        if (++sk + 1 < sk_end) return;
+        bool next = false;
+        if (sk == sk_end) {
+            next = sv + 1 < items;
+            sv += next ? 1 : 0;
+            --sk;
+        }
+        aim(next);
+    };
+
+    // (read here, because a load that is in flight when the main loop begins would have to be waited for there)
+    float sc = 1.f;
+    if (p.scale != nullptr) sc = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(p.scale[0])));
+
+    // ---- fragments: where they lie in the first buffer, in bytes; the second is 64 KB further
+    unsigned atA[AT ? 8 : 2], atB[8];
+    {
+        const int rb = 8 * lg + lq, sw = lx_swz(rb);
+#pragma unroll
+        for (int t = 0; t < (AT ? 8 : 2); ++t)
+            atA[t] = lds_base + (AT ? (unsigned)(rb * 512 + (lp & 1) * 8 + ((((wm * 16) | (lp >> 1)) ^ sw ^ (2 * t)) << 4))
+                                    : (unsigned)((wm * 128 + lr) * 128 + (((t * 4 + lg) ^ (lr & 7)) << 4)));
+#pragma unroll
+        for (int t = 0; t < 8; ++t) atB[t] = lds_base + LX_ELEMS * 2 + (unsigned)(rb * 512 + (lp & 1) * 8 + ((((wn * 16) | (lp >> 1)) ^ sw ^ (2 * t)) << 4));
+    }
+    f32x4 acc[8][8];
+    bf16x8 faE[8], fbE[8], faO[8], fbO[8];          // of the two k halves of a step
+    auto ldA = [&](bf16x8& f, auto kt, auto tt) __attribute__((always_inline)) {
+        constexpr int ks = decltype(kt)::value, t = decltype(tt)::value;
+        if constexpr (AT) f = lx_lds_tr(atA[t] + ks * 16384);
+        else f = lx_lds_row(atA[ks] + t * 2048);
+    };
+    auto ldB = [&](bf16x8& f, auto kt, auto tt) __attribute__((always_inline)) {
+        constexpr int ks = decltype(kt)::value, t = decltype(tt)::value;
+        f = lx_lds_tr(atB[t] + ks * 16384);
+    };
+    // A phase: the 64 matrix instructions of a k half, one by one in this order; between them, evenly, the reads of the next phase's fragments, the
+    // requests, and in phase 0 behind the reads the step to the other buffer.
+    auto phase = [&](const bf16x8 (&fa)[8], const bf16x8 (&fb)[8], bf16x8 (&ga)[8], bf16x8 (&gb)[8], unsigned at, auto pt) __attribute__((always_inline)) {
+        constexpr int ph = decltype(pt)::value, Q = ph == 0 ? Q0 : Q1, GAP = 60 / Q;
+        lx_static_for<0, 64>([&](auto gt) __attribute__((always_inline)) {
+            constexpr int g = decltype(gt)::value, tm = g >> 3, tn = g & 7;
+            lx_mfma(acc[tm][tn], fb[tn], fa[tm]);
+            LX_PIN();
+            if constexpr (g % GAP == 1 && g / GAP < Q) { request(at, pt, lx_int<g / GAP>{}); LX_PIN(); }
+            if constexpr (g % 3 == 0 && g / 3 < 16) {
+                constexpr int i = g / 3;
+                if constexpr (i < 8) ldB(gb[i], lx_int<1 - ph>{}, lx_int<i>{});
+                else ldA(ga[i - 8], lx_int<1 - ph>{}, lx_int<i - 8>{});
+                LX_PIN();
+            }
+            if constexpr (ph == 0 && g >= 48) {
+                if constexpr (g - 48 < (AT ? 8 : 2)) lx_flip(atA[g - 48]);
+                if constexpr (g >= 56) lx_flip(atB[g - 56]);
+                LX_PIN();
+            }
+            if constexpr (ph == 1 && g == 62) { sA += dA; sB += dB; LX_PIN(); }
+        });
+    };
+    if (items == 0) return;
+    aim(true);
+    lx_static_for<0, 2>([&](auto st) __attribute__((always_inline)) {
+        constexpr unsigned at = decltype(st)::value * LX_ELEMS * 4u;
+        lx_static_for<0, Q0>([&](auto q) __attribute__((always_inline)) { request(at, lx_int<0>{}, q); });
+        lx_static_for<0, Q1>([&](auto q) __attribute__((always_inline)) { request(at, lx_int<1>{}, q); });
+        sA += dA; sB += dB;
+        advance();
+    });
+    LX_WAIT(16);
+    LX_BARRIER();
+    lx_static_for<0, 8>([&](auto t) __attribute__((always_inline)) { ldB(fbE[decltype(t)::value], lx_int<0>{}, t); });
+    lx_static_for<0, 8>([&](auto t) __attribute__((always_inline)) { ldA(faE[decltype(t)::value], lx_int<0>{}, t); });
+    unsigned at = 0;            // the current step's buffer
+    bool loose = false;         // at least 32 output stores of this wave are younger than its requests
     for (int v = 0; v < items; ++v) {
         int m0, n0, k0, k1, part;
         locate(v, m0, n0, k0, k1, part);
@@ -412,110 +597,71 @@ __global__ __launch_bounds__(512) void lx_gemm_kernel(const LxGemmParams p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < 8; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
         for (int kt = 0; kt < nk; ++kt) {
-            const bf16_t* cA = lsm + par * 2 * LX_ELEMS;
-            const bf16_t* cB = cA + LX_ELEMS;
-            const bf16_t* nA = lsm + (par ^ 1) * 2 * LX_ELEMS;
-            const bf16_t* nB = nA + LX_ELEMS;
-            if constexpr (DEEP) {
-                const bool n2 = sv < items;
-                mma(faE, fbE, 0);
-                ldB(fbO, cB, 1);
-                ldA(faO, cA, 1, 0);
-                LX_MIX(RAB);
-                if (!n1) LX_WAIT(0);
-                else if (loose) LX_WAIT(24);
-                else LX_WAIT(8);
-                LX_BARRIER();
-                if (n2) stageB(par);
-                mma(faO, fbO, 0);
-                ldA(faE, cA, 0, 1);
-                LX_MIX(RA);
-                if (n2) stageA(par, 0);
-                mma(faE, fbE, 1);
-                ldA(faO, cA, 1, 1);
-                LX_MIX(RA);
-                if (!n2) LX_WAIT(0);
-                else if (loose) LX_WAIT(24);
-                else LX_WAIT(8);
-                LX_BARRIER();
-                if (n2) { stageA(par, 1); advance(); }
-                mma(faO, fbO, 1);
-                n1 = n2;
-            } else {
-                if (pend) { stageB(par ^ 1); advance(); pend = false; }
-                mma(faE, fbE, 0);
-                ldA(faO, cA, 0, 1);
-                LX_MIX(RA);
-                mma(faO, fbE, 1);
-                ldB(fbO, cB, 1);
-                ldA(faE, cA, 1, 0);
-                LX_MIX(RAB);
-                mma(faE, fbO, 0);
-                ldA(faO, cA, 1, 1);
-                LX_MIX(RA);
-                if (loose) LX_WAIT(16);
-                else LX_WAIT(0);
-                LX_BARRIER();
-                if (sv < items) { stageA(par, 0); stageA(par, 1); pend = true; }
-                mma(faO, fbO, 1);
-            }
-            ldB(fbE, nB, 0);
-            ldA(faE, nA, 0, 0);
-            LX_MIX(RAB);
+            if (loose) LX_WAIT(48);
+            else LX_WAIT(16);
+            LX_LDS_DONE();
+            LX_BARRIER();
+            LX_PIN();
+            phase(faE, fbE, faO, fbO, at, lx_int<0>{});
+            if (loose) LX_WAIT(WX + 32);
+            else LX_WAIT(WX);
+            LX_LDS_DONE();
+            LX_BARRIER();
+            LX_PIN();
+            phase(faO, fbO, faE, fbE, at, lx_int<1>{});
+            advance();
             loose = false;
-            par ^= 1;
+            at ^= LX_ELEMS * 4u;
         }
-        if (pend) { stageB(par ^ 1); advance(); pend = false; }      // before the stores: vmcnt counts in issue order
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");          // the last matrix instructions' results
+        LX_PIN();
 
         const int srow = lane >> 3;
-        if constexpr (EPI == LX_OUT) {
-            // accumulators -> rows of 64 columns through the wave's 4 KB of LDS, so that a store covers whole lines
-            float* stg = reinterpret_cast<float*>(lsm + 4 * LX_ELEMS) + wave * (16 * 64);
-            const int n = n0 + wn * 64 + (lane & 7) * 8;
-            const float sc = p.scale != nullptr ? p.scale[0] : 1.0f;
+        // accumulators -> rows of 64 columns through the wave's 4 KB of LDS, so that a store covers whole lines
+        float* stg = reinterpret_cast<float*>(lsm + 4 * LX_ELEMS) + wave * (16 * 64);
 #pragma unroll
-            for (int tm = 0; tm < 8; ++tm) {
+        for (int u = 0; u < 16; ++u) {
+            const int tm = u >> 1, h = u & 1;
+            const int n = n0 + wn * 128 + h * 64 + (lane & 7) * 8;
 #pragma unroll
-                for (int tn = 0; tn < 4; ++tn)
-                    *reinterpret_cast<f32x4*>(stg + lr * 64 + (((tn * 4 + lg) ^ (lr & 7)) << 2)) = acc[tm][tn];
+            for (int tn = 0; tn < 4; ++tn)
+                *reinterpret_cast<f32x4*>(stg + lr * 64 + (((tn * 4 + lg) ^ (lr & 7)) << 2)) = acc[tm][4 * h + tn];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int r = half * 8 + srow;
-                    f32x4 lo = *reinterpret_cast<const f32x4*>(stg + r * 64 + (((2 * (lane & 7)) ^ srow) << 2));
-                    f32x4 hi = *reinterpret_cast<const f32x4*>(stg + r * 64 + (((2 * (lane & 7) + 1) ^ srow) << 2));
-                    const int m = m0 + wm * 128 + tm * 16 + r;
-                    if (m < p.M && n < p.N) {
-                        if (part >= 0) {
-                            float* q = p.slab + (size_t)((2 * team + part) * p.width + member) * 65536 + (m - m0) * 256 + (n - n0);
-                            __builtin_nontemporal_store(lo, reinterpret_cast<f32x4*>(q));
-                            __builtin_nontemporal_store(hi, reinterpret_cast<f32x4*>(q + 4));
+            for (int half = 0; half < 2; ++half) {
+                const int r = half * 8 + srow;
+                f32x4 lo = *reinterpret_cast<const f32x4*>(stg + r * 64 + (((2 * (lane & 7)) ^ srow) << 2));
+                f32x4 hi = *reinterpret_cast<const f32x4*>(stg + r * 64 + (((2 * (lane & 7) + 1) ^ srow) << 2));
+                const int m = m0 + wm * 128 + tm * 16 + r;
+                if (m < p.M && n < p.N) {
+                    if (part >= 0) {
+                        float* q = p.slab + (size_t)((2 * team + part) * p.width + member) * 65536 + (m - m0) * 256 + (n - n0);
+                        __builtin_nontemporal_store(lo, reinterpret_cast<f32x4*>(q));
+                        __builtin_nontemporal_store(hi, reinterpret_cast<f32x4*>(q + 4));
+                    } else {
+                        lo *= sc;
+                        hi *= sc;
+                        if (p.add != nullptr) {
+                            const float* q = p.add + (size_t)m * p.N + n;
+                            lo += *reinterpret_cast<const f32x4*>(q);
+                            hi += *reinterpret_cast<const f32x4*>(q + 4);
+                        }
+                        if (p.out_f32) {
+                            float* q = reinterpret_cast<float*>(p.out) + (size_t)m * p.ldo + n;
+                            *reinterpret_cast<f32x4*>(q) = lo;
+                            *reinterpret_cast<f32x4*>(q + 4) = hi;
                         } else {
-                            lo *= sc;
-                            hi *= sc;
-                            if (p.add != nullptr) {
-                                const float* q = p.add + (size_t)m * p.N + n;
-                                lo += *reinterpret_cast<const f32x4*>(q);
-                                hi += *reinterpret_cast<const f32x4*>(q + 4);
-                            }
-                            if (p.out_f32) {
-                                float* q = reinterpret_cast<float*>(p.out) + (size_t)m * p.ldo + n;
-                                *reinterpret_cast<f32x4*>(q) = lo;
-                                *reinterpret_cast<f32x4*>(q + 4) = hi;
-                            } else {
-                                const u32x4 o = {pack2bf(lo[0], lo[1]), pack2bf(lo[2], lo[3]), pack2bf(hi[0], hi[1]), pack2bf(hi[2], hi[3])};
-                                __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(reinterpret_cast<bf16_t*>(p.out) + (size_t)m * p.ldo + n));
-                            }
+                            const u32x4 o = {pack2bf(lo[0], lo[1]), pack2bf(lo[2], lo[3]), pack2bf(hi[0], hi[1]), pack2bf(hi[2], hi[3])};
+                            __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(reinterpret_cast<bf16_t*>(p.out) + (size_t)m * p.ldo + n));
                         }
                     }
                 }
             }
-        } else {
-            lx_loss_epilogue<8, EPI == LX_XENT_BIAS>(p, acc, m0 + wm * 128, n0 + wn * 64, reinterpret_cast<bf16_t*>(lsm + 4 * LX_ELEMS) + wave * (16 * 64 * 2));
         }
-        loose = m0 + LX_TILE <= p.M && (EPI != LX_OUT ? p.P != nullptr : n0 + LX_TILE <= p.N);       // a full tile: 16 stores at least
+        loose = m0 + LX_TILE <= p.M && n0 + LX_TILE <= p.N;       // a full tile: 32 stores at least
     }
+    LX_WAIT(0);         // nothing may arrive in LDS after the workgroup has ended
 }
 
 // ---------------------------------------------------------------------------------------------------- rows
@@ -528,7 +674,7 @@ struct LxRowParams {
     unsigned* ticket; float* scale; float* loss; int mean;      // loss not null: the last row to finish adds the rows up (see lx_loss_kernel)
     bf16_t* P; long long ldp;          // fp16 on entry, bf16 dz on exit; null: loss alone
     float* rows;
-    int V, D, rows_n;
+    int V, D, rows_n, pad_rows;         // pad_rows rows of zeros behind the last (lx_grad_kernel reads steps of 64 of them)
     float smoothing;
 };
 
@@ -624,14 +770,15 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
     __shared__ float sh[WAVES];
     const int tid = WAVES == 1 ? (int)threadIdx.x & 63 : (int)threadIdx.x;
     const int row = WAVES == 1 ? (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6) : (int)blockIdx.x;
-    if (row >= p.rows_n) return;
-    const long long t64 = p.target[row];
+    if (row >= p.rows_n + p.pad_rows) return;
+    const bool pad = row >= p.rows_n;
+    const long long t64 = pad ? 0 : p.target[row];
     bf16_t* P = p.P != nullptr ? p.P + (size_t)row * p.ldp : nullptr;
     const int chunks = (int)(p.ldp / 8);
-    if (t64 == p.ignore_index) {
+    if (pad || t64 == p.ignore_index) {
         if (P != nullptr)
             for (int c = tid; c < chunks; c += NT) __builtin_nontemporal_store((u32x4){0u, 0u, 0u, 0u}, reinterpret_cast<u32x4*>(P) + c);
-        lx_row_done(p, row, tid, 0.f);
+        if (!pad) lx_row_done(p, row, tid, 0.f);
         return;
     }
     // a label outside [0, V) never becomes an address: the row's loss and gradient are NaN
@@ -1190,7 +1337,7 @@ static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw
     q.stats = take((size_t)rows * q.stat_cols * sizeof(float2));
     q.zsum = smoothing ? take((size_t)rows * q.stat_cols * sizeof(float)) : 0;
     if (grad) {
-        q.P = take((size_t)rows * q.ldp * 2);
+        q.P = take((size_t)((rows + LX_BK - 1) / LX_BK * LX_BK) * q.ldp * 2);
         if (q.blocks > 1 && !dw_f32) q.acc = take((size_t)V * D * sizeof(float));
         const int cus = lx_cus();
         size_t slab = 0;            // dx and dW use it one after the other
@@ -1234,12 +1381,16 @@ static int lx_launch(LxGemmParams& p, const LxDeal& d, hipStream_t s, const char
         return d.splits > 1 ? lx_reduce(p, s, what) : VITK_OK;
     }
     static VitkLdsOnce once = {};
-    if (int rc = vitk_lds_once(once, (const void*)lx_gemm_kernel<LAY, EPI>, LX_LDS, what)) return rc;
-    p.width = d.width; p.teams = d.teams; p.whole = d.whole; p.rest = d.rest; p.ranges = d.ranges;
-    const int grid = EPI == LX_OUT ? d.teams * d.width : d.teams;
-    lx_gemm_kernel<LAY, EPI><<<grid, 512, LX_LDS, s>>>(p);
-    if (int rc = vitk_check_launch(what)) return rc;
-    if (EPI == LX_OUT && p.rest > 0) lx_join_kernel<<<p.rest * p.width * 32, 256, 0, s>>>(p);
+    if constexpr (EPI == LX_OUT) {
+        if (int rc = vitk_lds_once(once, (const void*)lx_grad_kernel<LAY>, LX_GRAD_LDS, what)) return rc;
+        p.width = d.width; p.teams = d.teams; p.whole = d.whole; p.rest = d.rest; p.ranges = d.ranges;
+        lx_grad_kernel<LAY><<<d.teams * d.width, 256, LX_GRAD_LDS, s>>>(p);
+        if (int rc = vitk_check_launch(what)) return rc;
+        if (p.rest > 0) lx_join_kernel<<<p.rest * p.width * 32, 256, 0, s>>>(p);
+    } else {
+        if (int rc = vitk_lds_once(once, (const void*)lx_logits_kernel<EPI>, LX_LDS, what)) return rc;
+        lx_logits_kernel<EPI><<<d.teams, 512, LX_LDS, s>>>(p);
+    }
     return vitk_check_launch(what);
 }
 
@@ -1301,21 +1452,23 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         const bool fused = q.blocks == 1 && T <= LX_FUSED_ROWS && (!grad || (size_t)T * q.ldp * 2 <= LX_FUSED_BYTES);
         r.ticket = ticket; r.scale = scale; r.loss = fused ? loss : nullptr; r.mean = mean;
         r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.rows_n = n; r.smoothing = smoothing;
+        r.pad_rows = grad && q.dw[last].kind == LX_BIG ? (LX_BK - n % LX_BK) % LX_BK : 0;
+        const int row_wgs = n + r.pad_rows;
         // long rows get more waves.  By the vocabulary alone, so that a row's sums do not depend on how many rows there are or what is wanted.
         // STREAM: past the caches, where the block is larger than they are.
         const bool stream = grad && (size_t)n * q.ldp * 2 > LX_CACHED;
         if (q.ldp >= 65536) {
-            if (stream) lx_row_kernel<16, true><<<n, 1024, 0, s>>>(r);
-            else lx_row_kernel<16, false><<<n, 1024, 0, s>>>(r);
+            if (stream) lx_row_kernel<16, true><<<row_wgs, 1024, 0, s>>>(r);
+            else lx_row_kernel<16, false><<<row_wgs, 1024, 0, s>>>(r);
         } else if (q.ldp >= 16384) {
-            if (stream) lx_row_kernel<8, true><<<n, 512, 0, s>>>(r);
-            else lx_row_kernel<8, false><<<n, 512, 0, s>>>(r);
+            if (stream) lx_row_kernel<8, true><<<row_wgs, 512, 0, s>>>(r);
+            else lx_row_kernel<8, false><<<row_wgs, 512, 0, s>>>(r);
         } else if (q.ldp >= 4096) {
-            if (stream) lx_row_kernel<4, true><<<n, 256, 0, s>>>(r);
-            else lx_row_kernel<4, false><<<n, 256, 0, s>>>(r);
+            if (stream) lx_row_kernel<4, true><<<row_wgs, 256, 0, s>>>(r);
+            else lx_row_kernel<4, false><<<row_wgs, 256, 0, s>>>(r);
         } else {
-            if (stream) lx_row_kernel<1, true><<<(n + 3) / 4, 256, 0, s>>>(r);
-            else lx_row_kernel<1, false><<<(n + 3) / 4, 256, 0, s>>>(r);
+            if (stream) lx_row_kernel<1, true><<<(row_wgs + 3) / 4, 256, 0, s>>>(r);
+            else lx_row_kernel<1, false><<<(row_wgs + 3) / 4, 256, 0, s>>>(r);
         }
         if (int rc = vitk_check_launch("linear_xent_rows")) return rc;
         if (last && !fused) {
