@@ -372,12 +372,10 @@ static __device__ __forceinline__ void lx_dma(const bf16_t* base, unsigned voff,
 static __device__ __forceinline__ void lx_mfma(f32x4& c, const bf16x8& a, const bf16x8& b) {
     asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
-static __device__ __forceinline__ bf16x8 lx_lds_tr(unsigned at) {
-    typedef __attribute__((address_space(3))) bf16x4* lds4;
-    const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(__UINTPTR_TYPE__)at);
-    const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(__UINTPTR_TYPE__)(at + 4 * 512));
-    return (bf16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+static __device__ __forceinline__ bf16x4 lx_lds_tr(unsigned at) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)(__UINTPTR_TYPE__)at);
 }
+static __device__ __forceinline__ bf16x8 lx_join(const bf16x4 a, const bf16x4 b) { return (bf16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
 static __device__ __forceinline__ bf16x8 lx_lds_row(unsigned at) {
     return *(const __attribute__((address_space(3))) bf16x8*)(__UINTPTR_TYPE__)at;
 }
@@ -391,13 +389,14 @@ static __device__ __forceinline__ void lx_flip(unsigned& at) { asm volatile("v_x
 // its waves read 192 KB a step and the DMA writes 64 KB, together as many cycles at 128 bytes each as the matrix instructions take; four waves
 // read 128 KB.  But one wave to a SIMD hides nothing: every other instruction has to be issued in the 12 cycles a matrix instruction leaves, so
 // the order is written out instruction by instruction (the matrix instructions are inline assembly on accumulators that never move; a
-// scheduling barrier stands behind each), with one LDS read or request at a time between them, requests 5 to 7 matrix instructions
-// apart because a request occupies the path to LDS for 16 cycles and a wave that runs into another's waits, and the step's own
-// bookkeeping - addresses, buffer change - in the same gaps.
+// scheduling barrier stands behind each), with one LDS read or one request (three instructions) in a gap, requests 3 to 6 matrix
+// instructions apart because each keeps the path to LDS busy for 16 cycles and a wave that runs into another's waits (issued in a burst,
+// or at every third gap of half the step, they cost a step 1000 cycles of 2060), and the step's own bookkeeping - addresses, buffer
+// change - in the same gaps.
 // Operands whose rows run along the output (x, W, and dz for dW) sit in LDS as [64][256] and are read with the transposing ds_read_b64_tr_b16:
 // no transposed copy is made; dz for dx as [256][64] with ds_read_b128.
-//   8192 x 100003 x 2048: dz W 2520 -> 2170 us, dz^T x 2500 -> 2400 us (matrix pipe 82 % and 75 % busy; a library product of the same sizes and
-//   the layout it likes best 2117 and 2299 us).  25088 x 8192 x 768: 320 -> 284 and 289 -> 275 us.
+//   8192 x 100003 x 2048: dz W 2520 -> 2180 us, dz^T x 2500 -> 2330 us (matrix pipe 81 % and 79 % busy at 1.8 and 1.7 GHz; a library product of the same sizes and
+//   the layout it likes best 2117 and 2299 us).  25088 x 8192 x 768: 320 -> 284 and 289 -> 277 us.
 // Tiles are dealt by number as LxDeal says.
 template <int LAY>
 __global__ __launch_bounds__(256, 1) void lx_grad_kernel(const LxGemmParams p) {
@@ -545,27 +544,41 @@ __global__ __launch_bounds__(256, 1) void lx_grad_kernel(const LxGemmParams p) {
     bf16x8 faE[8], fbE[8], faO[8], fbO[8];          // of the two k halves of a step
     auto ldA = [&](bf16x8& f, auto kt, auto tt) __attribute__((always_inline)) {
         constexpr int ks = decltype(kt)::value, t = decltype(tt)::value;
-        if constexpr (AT) f = lx_lds_tr(atA[t] + ks * 16384);
+        if constexpr (AT) f = lx_join(lx_lds_tr(atA[t] + ks * 16384), lx_lds_tr(atA[t] + ks * 16384 + 2048));
         else f = lx_lds_row(atA[ks] + t * 2048);
     };
     auto ldB = [&](bf16x8& f, auto kt, auto tt) __attribute__((always_inline)) {
         constexpr int ks = decltype(kt)::value, t = decltype(tt)::value;
-        f = lx_lds_tr(atB[t] + ks * 16384);
+        f = lx_join(lx_lds_tr(atB[t] + ks * 16384), lx_lds_tr(atB[t] + ks * 16384 + 2048));
     };
-    // A phase: the 64 matrix instructions of a k half, one by one in this order; between them, evenly, the reads of the next phase's fragments, the
-    // requests, and in phase 0 behind the reads the step to the other buffer.
+    // A phase: the 64 matrix instructions of a k half, one by one in this order; between them the reads of the next phase's fragments (B's
+    // first, which its first eight instructions need), the requests, and in phase 0 behind the reads the step to the other buffer.
     auto phase = [&](const bf16x8 (&fa)[8], const bf16x8 (&fb)[8], bf16x8 (&ga)[8], bf16x8 (&gb)[8], unsigned at, auto pt) __attribute__((always_inline)) {
-        constexpr int ph = decltype(pt)::value, Q = ph == 0 ? Q0 : Q1, GAP = 60 / Q;
+        constexpr int ph = decltype(pt)::value, Q = ph == 0 ? Q0 : Q1;
+        bf16x4 lo;
         lx_static_for<0, 64>([&](auto gt) __attribute__((always_inline)) {
             constexpr int g = decltype(gt)::value, tm = g >> 3, tn = g & 7;
             lx_mfma(acc[tm][tn], fb[tn], fa[tm]);
             LX_PIN();
-            if constexpr (g % GAP == 1 && g / GAP < Q) { request(at, pt, lx_int<g / GAP>{}); LX_PIN(); }
-            if constexpr (g % 3 == 0 && g / 3 < 16) {
+            // three gaps: half a [64][256] fragment each in the first two, a request in the third
+            if constexpr (g % 3 < 2 && g < 48) {
                 constexpr int i = g / 3;
-                if constexpr (i < 8) ldB(gb[i], lx_int<1 - ph>{}, lx_int<i>{});
-                else ldA(ga[i - 8], lx_int<1 - ph>{}, lx_int<i - 8>{});
+                if constexpr (i < 8) {
+                    if constexpr (g % 3 == 0) lo = lx_lds_tr(atB[i] + (1 - ph) * 16384);
+                    else gb[i] = lx_join(lo, lx_lds_tr(atB[i] + (1 - ph) * 16384 + 2048));
+                } else if constexpr (AT) {
+                    if constexpr (g % 3 == 0) lo = lx_lds_tr(atA[i - 8] + (1 - ph) * 16384);
+                    else ga[i - 8] = lx_join(lo, lx_lds_tr(atA[i - 8] + (1 - ph) * 16384 + 2048));
+                } else if constexpr (g % 3 == 0) {
+                    ldA(ga[i - 8], lx_int<1 - ph>{}, lx_int<i - 8>{});
+                }
                 LX_PIN();
+            }
+            if constexpr (g % 3 == 2) {
+                // which of the phase's 4, 8 or 12 requests: in every fifth, every second or two of three of these gaps
+                constexpr int h = g / 3;
+                constexpr int q = Q == 4 ? (h % 5 == 0 && h < 20 ? h / 5 : -1) : Q == 8 ? (h % 2 == 0 && h < 16 ? h / 2 : -1) : (h % 3 < 2 && h < 18 ? h / 3 * 2 + h % 3 : -1);
+                if constexpr (q >= 0) { request(at, pt, lx_int<q>{}); LX_PIN(); }
             }
             if constexpr (ph == 0 && g >= 48) {
                 if constexpr (g - 48 < (AT ? 8 : 2)) lx_flip(atA[g - 48]);
