@@ -352,8 +352,8 @@ int vitk_clip_grads(const void* const* src, void* const* dst, const int64_t* num
  * forward: out[t] = scale * table[ids[t]]; the row of an id outside [0, V) is NaN. */
 int vitk_embedding_fwd(const void* ids, int ids_are_64, const void* table, int table_type, int64_t ldt, void* out, int out_type, int64_t ldo,
                        int64_t T, int64_t V, int D, float scale, void* stream);
-/* gradient: dtable[v] = scale * sum over the tokens t with ids[t] == v of dout[t], in fp32 and in the order of the tokens whatever the
- * schedule (the tokens are sorted by id), rounded once; zero for rows without a token.  accumulate: added to what dtable holds, rows
+/* gradient: dtable[v] = scale * sum over the tokens t with ids[t] == v of dout[t], summed in fp32 in an order that the ids alone decide
+ * (the tokens are sorted by id; long runs are summed in stretches), rounded once; zero for rows without a token.  accumulate: added to what dtable holds, rows
  * without a token stay untouched.  Tokens with id padding_idx (negative: none) or an id outside [0, V) add nothing.
  * T, V < 2^31, D <= 2^23.  workspace: vitk_embedding_bwd_workspace(T, V, D) bytes. */
 size_t vitk_embedding_bwd_workspace(int64_t T, int64_t V, int D);

@@ -1252,9 +1252,11 @@ struct LxPlan {
 };
 // The kernel and its cut that a model of the time finds fastest, in microseconds on 256 compute units, from 28 shapes between 1 x 1000 x 192 and
 // 512 x 100003 x 1024 measured with each of the three kernels (time of x W^T / dz W / dz^T x in us, large : 128 : 64):
-//   1 x 1000 x 192       10 24 8 : 7 8 7 : 4 7 4              512 x 8192 x 768     22 32 17 : 15 21 14 : 19 19 16
-//   1024 x 1024 x 1024   30 31 29 : 16 17 16 : 11 12 10       8192 x 8192 x 768    92 129 129 : 157 114 99 : 244 154 156
-//   512 x 21843 x 768    25 50 31 : 31 36 34 : 47 33 36       512 x 100003 x 1024  117 131 125 : 158 156 189 : 245 262 260
+//   1 x 1000 x 192       10 23 12 : 7 8 7 : 4 7 4             512 x 8192 x 768     22 33 22 : 15 21 14 : 19 19 16
+//   1024 x 1024 x 1024   30 31 33 : 16 17 16 : 11 12 10       8192 x 8192 x 768    89 119 120 : 157 114 99 : 244 154 156
+//   512 x 21843 x 768    25 43 37 : 31 36 34 : 47 33 36       512 x 100003 x 1024  117 118 142 : 158 156 189 : 245 262 260
+// It is off by up to 15 %; where that makes it take the slower one (512 x 100003 x 1024: 308 us for both gradients, the large kernel 260), another
+// term for the memory cost as much elsewhere (512 x 50000 x 2048: 247, 264).
 // Large: whole rows alone take ceil(rows / teams) rounds; cutting what does not fill a round into ranges fills it at the price of parts written
 // and read, 0.13 us for one of 256 x 256 (512 KB at 4 TB/s).
 #define LX_US_STEP 1.25

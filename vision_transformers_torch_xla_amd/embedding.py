@@ -27,7 +27,7 @@ class _Embedding(torch.autograd.Function):
 
 def embedding(ids, weight, scale: float = 1.0, padding_idx=None, out_dtype=torch.bfloat16):
     """scale * weight[ids] in out_dtype (bf16 or fp32), differentiable in weight (fp32 or bf16 [V, D], D a multiple of 8); the gradient is summed
-    in the order of the tokens, so a step gives the same bits on every run.  Tokens with id padding_idx (negative: counted from the
+    in an order that the ids alone decide, so a step gives the same bits on every run.  Tokens with id padding_idx (negative: counted from the
     end) get their row and give no gradient.  An id outside the table gives a row of NaN."""
     if padding_idx is not None:
         V = weight.shape[0]

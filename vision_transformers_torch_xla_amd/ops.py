@@ -546,8 +546,8 @@ def embedding_fwd(ids, table, scale=1.0, out_dtype=None):
 
 
 def embedding_bwd(dout, ids, num_rows, scale=1.0, padding_idx=None, out=None, accumulate=False, out_dtype=None):
-    """Gradient of embedding_fwd's table: [num_rows, D] with row v = scale * sum of dout over the tokens with id v (fp32 sums in the order of
-    the tokens, the same bits on every run), zero where there is none; dout fp32 / bf16 [..., D].  Tokens with id padding_idx or an id
+    """Gradient of embedding_fwd's table: [num_rows, D] with row v = scale * sum of dout over the tokens with id v (fp32 sums in an order
+    that the ids alone decide: the same bits on every run), zero where there is none; dout fp32 / bf16 [..., D].  Tokens with id padding_idx or an id
     outside [0, num_rows) add nothing.  out: where it goes (fp32 / bf16 [num_rows, D]); with accumulate it is added there, and only the
     rows that have tokens are touched.  Without out: a new tensor of out_dtype (default: dout's type)."""
     if padding_idx is not None and not 0 <= int(padding_idx) < int(num_rows):
