@@ -126,6 +126,22 @@ def test_clip_grads_in_a_graph_on_another_stream(device):
 
 
 @pytest.mark.gpu
+def test_clip_grads_offsets_past_32_bits(device):
+    ops = _ops()
+    n = (1 << 32) + 12345
+    big, small = torch.full((n,), 0.5, dtype=bf16, device=device), torch.randn(1000, device=device)
+    big[-5:] = 3.0
+    before = small.clone()
+    norm = ops.clip_grads([small, big], 100.0)
+    want = math.sqrt(0.25 * (n - 5) + 45.0 + float(before.double().square().sum()))
+    assert abs(norm.item() - want) <= 2 * U32 * want
+    c = 100.0 / want
+    assert torch.all((small.double() - before.double() * c).abs() <= 8 * U32 * before.double().abs() * c)
+    for part, v in ((big[:1000], 0.5), (big[-1005:-5], 0.5), (big[-5:], 3.0)):
+        assert torch.all((part.double() - v * c).abs() <= v * c * (half_ulp(bf16) + 8 * U32))
+
+
+@pytest.mark.gpu
 def test_clip_grads_refuses(device):
     ops, err = _ops(), _error()
     a = torch.randn(64, device=device)
@@ -314,6 +330,31 @@ def test_embedding_bwd_in_a_graph(device, T, V):
         want = ops.embedding_bwd(dout, ids, V)
         torch.cuda.synchronize()
         assert torch.equal(got, want) and torch.equal(out, ops.embedding_fwd(ids, want))
+
+
+@pytest.mark.gpu
+def test_embedding_offsets_past_32_bits(device):
+    ops = _ops()
+    V, D, T = 3000001, 768, 3000                                                         # 4.6 GB of table, of its gradient
+    table = torch.randn(V, D, device=device, dtype=bf16)
+    ids = torch.randint(0, V, (T,), device=device)
+    ids[:50] = V - 1
+    assert torch.equal(ops.embedding_fwd(ids, table), table[ids])
+    dout = torch.randn(T, D, device=device)
+    got = ops.embedding_bwd(dout, ids, V, out_dtype=bf16)
+    rows, where = torch.unique(ids, return_inverse=True)
+    check_embedding_grad(got[rows], dout.cpu(), where.cpu(), len(rows), 1.0, None)
+    assert torch.count_nonzero(got.abs().amax(1)) == len(rows)
+    del got, dout
+    dout = table                                                                         # as many tokens, into a small table
+    ids = torch.randint(0, 500, (V,), device=device)
+    got = ops.embedding_bwd(dout, ids, 500, out_dtype=f32)
+    want, mag = (torch.zeros(500, D, dtype=f64, device=device) for _ in range(2))
+    for i in range(0, V, 1 << 18):
+        want.index_add_(0, ids[i:i + (1 << 18)], dout[i:i + (1 << 18)].double())
+        mag.index_add_(0, ids[i:i + (1 << 18)], dout[i:i + (1 << 18)].double().abs())
+    count = torch.bincount(ids, minlength=500).double()[:, None]
+    assert torch.all((got.double() - want).abs() <= (count + 3) * U32 * mag)
 
 
 @pytest.mark.gpu
@@ -555,6 +596,82 @@ def test_linear_xent_gradient_against_differences(device):
         allow = ((tol[2 + k] + half_ulp(r[2 + k].dtype) * (got.abs() + tol[2 + k])) * u.abs()).sum()
         assert abs((got * u).sum() - slope) <= allow + 1e-8
         assert allow < 0.2 * (got * u).abs().sum()                                             # the bound says something
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D", [(3, 1 << 22, 8), (3000001, 2, 8), (1, 2, 2000), (4097, 1, 64)])
+def test_linear_xent_longest_sides(device, T, V, D):
+    ops = _ops()
+    g = torch.Generator().manual_seed(T + V)
+    x, w, target = (t.to(device) for t in xent_inputs(T, V, D, g))
+    check_linear_xent(ops.linear_xent(x, w, target), x, w, target)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D", [(33000, 70001, 256), (600, 2200001, 1024)])           # probabilities, then weights and their gradient past 4 GiB
+def test_linear_xent_offsets_past_32_bits(device, T, V, D):
+    ops = _ops()
+    x = torch.randn(T, D, device=device).to(bf16)
+    w = (torch.randn(V, D, device=device) / math.sqrt(D)).to(bf16)
+    target = torch.randint(0, V, (T,), device=device)
+    r = ops.linear_xent(x, w, target, reduction="sum", block_bytes=8 << 30)
+    k = 64
+    rows = torch.cat([torch.arange(k), torch.arange(T - k, T)]).to(device)                # first and last rows of x, of the weight
+    cols = torch.cat([torch.arange(k), torch.arange(V - k, V)]).to(device)
+    lse = torch.full((T,), -math.inf, dtype=f64, device=device)
+    dx = torch.zeros(2 * k, D, dtype=f64, device=device)
+    step = max(1, (1 << 27) // T)
+    for c in range(0, V, step):
+        lse = torch.logaddexp(lse, torch.logsumexp(x.double() @ w[c:c + step].double().t(), 1))
+    dxt = torch.zeros_like(dx)
+    perr = 2 * (D + 2) * U32 * (x.abs().float().sum(1).max() * w.abs().max()).double() + (V / 64 + 200) * U32 * (1 + lse.abs().max())
+    err = lambda p, dz: p * (2.0 ** -11 + perr) * 1.01 + 2.0 ** -24 + dz.abs() * 2.0 ** -8 * 1.01              # noqa: E731   (see plain_linear_xent)
+    for c in range(0, V, 1 << 16):
+        wd = w[c:c + (1 << 16)].double()
+        p = (x[rows].double() @ wd.t() - lse[rows, None]).exp()
+        dz = p - (target[rows, None] == torch.arange(c, c + len(wd), device=device)).double()
+        dx += dz @ wd
+        dxt += err(p, dz) @ wd.abs() + (V + 4) * U32 * (dz.abs() @ wd.abs())
+    p = (x.double() @ w[cols].double().t() - lse[:, None]).exp()
+    dz = p - (target[:, None] == cols).double()
+    dw, dwt = dz.t() @ x.double(), err(p, dz).t() @ x.double().abs() + (T + 4) * U32 * (dz.abs().t() @ x.double().abs())
+    nll = lse - (x.double() * w[target].double()).sum(1)
+    assert torch.all((r.rows.double() - nll).abs() <= perr)
+    for got, want, tol in ((r.dx[rows], dx, dxt), (r.dweight[cols], dw, dwt)):
+        assert torch.all((got.double() - want).abs() <= tol + 2.0 ** -8 * 1.01 * (want.abs() + tol) + 2.0 ** -133)
+
+
+@pytest.mark.gpu
+def test_linear_xent_large_in_a_graph_and_on_two_streams_at_once(device):
+    ops = _ops()
+    g = torch.Generator().manual_seed(12)
+    sets = [tuple(t.to(device) for t in xent_inputs(*shape, g)) for shape in ((2050, 12001, 520), (1100, 25000, 424))]
+    eager = [ops.linear_xent(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    both = [[], []]
+    for k in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                both[i].append(ops.linear_xent(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(u, v) for r in both[i] for u, v in zip(r, eager[i]) if u is not None)
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    got = []
+    for graph, s in zip(graphs, sets):
+        with torch.cuda.graph(graph):
+            got.append(ops.linear_xent(*s))
+    for k in range(3):
+        for s in sets:
+            s[0].copy_(torch.randn(s[0].shape, generator=g))
+        torch.cuda.synchronize()
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for r, s in zip(got, sets):
+            assert all(torch.equal(u, v) for u, v in zip(r, ops.linear_xent(*s)) if u is not None)
 
 
 @pytest.mark.gpu
