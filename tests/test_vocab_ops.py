@@ -490,6 +490,22 @@ def test_linear_xent_large(device, T, V, D, block_bytes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D", [(3909, 8328, 432), (2534, 14114, 568), (6893, 5240, 600), (5541, 9060, 216)])      # logits by two kernels: split by classes, by rows
+def test_linear_xent_logits_by_two_kernels(device, T, V, D):
+    ops = _ops()
+    g = torch.Generator().manual_seed(T + D)
+    x, w, target = (t.to(device) for t in xent_inputs(T, V, D, g))
+    check_linear_xent(ops.linear_xent(x, w, target), x, w, target)
+    bias = (torch.randn(V, generator=g) * 0.5).to(bf16).to(device)
+    r = ops.linear_xent(x, w, target, bias, smoothing=0.1)
+    check_linear_xent(r, x, w, target, bias, 0.1)
+    e = ops.linear_xent(x, w, target, bias, smoothing=0.1, want_grad=False)
+    assert torch.equal(e.rows, r.rows) and torch.equal(e.loss, r.loss)
+    few = ops.linear_xent(x[-100:], w, target[-100:], bias, smoothing=0.1, want_grad=False)       # the same rows by one kernel alone
+    assert torch.equal(few.rows, r.rows[-100:])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("wtype", [bf16, f32])
 def test_linear_xent_in_several_blocks_of_rows(device, wtype):
     ops = _ops()
