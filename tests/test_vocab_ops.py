@@ -247,7 +247,7 @@ def test_embedding_bwd(device, T, V, D, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,V,D", [(262144, 511, 8), (262145, 70000, 16), (1000003, 300001, 8)])       # on both sides of the sort's scan; one pass and more
+@pytest.mark.parametrize("T,V,D", [(28672, 700, 40), (28673, 700, 40), (262144, 511, 8), (262145, 70000, 16), (1000003, 300001, 8)])       # on both sides of the borders: one launch, sort, sort with a scan; one pass and more
 def test_embedding_bwd_of_very_many_tokens(device, T, V, D):
     ops = _ops()
     g = torch.Generator().manual_seed(T)

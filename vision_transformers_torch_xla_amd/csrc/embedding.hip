@@ -80,7 +80,9 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const EmbFwdParams p
 // of range); it sorts behind every row.
 #define SORT_BINS 512
 #define SORT_BITS 9
-#define SORT_ITEMS 8            // (16: the four launches take 39 us for 100352 tokens, 8: 29 us, 4: 30 us)
+#define SORT_THREADS 1024
+#define SORT_WAVES (SORT_THREADS / 64)
+#define SORT_ITEMS 2            // 2048 tokens a workgroup (100352 tokens: the four launches take 21 us; with 4096 25; 256 threads of 8 28, of 16 39)
 
 template <typename I>
 static __device__ __forceinline__ unsigned emb_key(const void* ids, long long t, long long V, long long padding) {
@@ -120,14 +122,15 @@ static __device__ __forceinline__ unsigned sort_rank(unsigned* hist_wave, unsign
     return base + before;
 }
 
-// Grouping in one launch, for up to 49152 tokens of a vocabulary up to 2^18.  Workgroup g of 256 owns the ids that are g modulo 256.  It
+// Grouping in one launch, for up to 28672 tokens of a vocabulary up to 2^18.  Workgroup g of 256 owns the ids that are g modulo 256.  It
 // reads ALL ids (out of the L2 cache), counts how many belong to the workgroups before it - which is where its part of the sorted list
 // begins, so the workgroups need nothing from each other - and keeps its own tokens in a list in LDS, one in 256 of a text's.  Wave w has
 // a contiguous stretch of the tokens, so its list is in their order; a token's place is the wave's first one for its id plus the number of
 // equal ids before it in the wave.  A wave with more own tokens than its list holds reads its stretch again instead.  Tokens without a
 // gradient come last.  The workgroups behind the 256 zero the gradient meanwhile.  16384 tokens and 77 MB of zeros take 19 us together
-// (a radix sort in one workgroup 46 us); 100352 tokens 48 us, where the four launches below take 29 us.
-#define GROUP_MAX 49152
+// (a radix sort in one workgroup 46 us).  A whole gradient with it and with the four launches below, 8192 x 768: 1024 tokens 18 and 26 us, 16384 29 and
+// 33, 32768 39 and 37, 49152 50 and 42.
+#define GROUP_MAX 28672
 #define GROUP_WG 256
 #define GROUP_WAVES 16
 #define GROUP_LIST 192          // list entries of a wave
@@ -240,7 +243,7 @@ __global__ __launch_bounds__(1024) void emb_group_kernel(const void* ids, int T,
 // Several workgroups: per pass a histogram launch (counts[block][bin]) and a launch that turns the counts into ranks and scatters.  For that a
 // workgroup adds up the counts of all others; from SORT_DIRECT workgroups on, a launch in between turns the counts of SORT_GROUP workgroups
 // into sums over those before and a total per group, so that only the totals are added up.
-#define SORT_BLOCK (256 * SORT_ITEMS)       // tokens per workgroup
+#define SORT_BLOCK (SORT_THREADS * SORT_ITEMS)       // tokens per workgroup
 #define SORT_DIRECT 128
 #define SORT_GROUP 32
 
@@ -252,28 +255,26 @@ static __device__ __forceinline__ uint2 sort_item(const void* ids, const uint2* 
 }
 
 template <typename I, bool FIRST>
-__global__ __launch_bounds__(256) void emb_hist_kernel(const void* ids, const uint2* in, long long T, long long V, long long padding, int shift,
+__global__ __launch_bounds__(SORT_THREADS) void emb_hist_kernel(const void* ids, const uint2* in, long long T, long long V, long long padding, int shift,
                                                        unsigned* counts, int blocks, uint4* zero, long long zero16) {
     __shared__ unsigned hist[SORT_BINS];
     if ((int)blockIdx.x >= blocks) {        // the blocks behind the sort's zero the gradient (first pass only)
         const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-        const long long step = (long long)(gridDim.x - blocks) * 256;
-        for (long long i = (long long)(blockIdx.x - blocks) * 256 + threadIdx.x; i < zero16; i += step) zero[i] = z;
+        const long long step = (long long)(gridDim.x - blocks) * SORT_THREADS;
+        for (long long i = (long long)(blockIdx.x - blocks) * SORT_THREADS + threadIdx.x; i < zero16; i += step) zero[i] = z;
         return;
     }
-    hist[threadIdx.x] = 0;
-    hist[threadIdx.x + 256] = 0;
+    if (threadIdx.x < SORT_BINS) hist[threadIdx.x] = 0;
     __syncthreads();
     const long long t0 = (long long)blockIdx.x * SORT_BLOCK;
 #pragma unroll
     for (int j = 0; j < SORT_ITEMS; ++j) {
-        const long long t = t0 + j * 256 + threadIdx.x;
+        const long long t = t0 + j * SORT_THREADS + threadIdx.x;
         const uint2 it = sort_item<I, FIRST>(ids, in, t, T, V, padding);
         if (t < T) atomicAdd(&hist[(it.x >> shift) & (SORT_BINS - 1)], 1u);
     }
     __syncthreads();
-    counts[(size_t)blockIdx.x * SORT_BINS + threadIdx.x] = hist[threadIdx.x];
-    counts[(size_t)blockIdx.x * SORT_BINS + threadIdx.x + 256] = hist[threadIdx.x + 256];
+    if (threadIdx.x < SORT_BINS) counts[(size_t)blockIdx.x * SORT_BINS + threadIdx.x] = hist[threadIdx.x];
 }
 
 __global__ __launch_bounds__(SORT_BINS) void emb_scan_kernel(unsigned* counts, int blocks, unsigned* totals) {
@@ -292,13 +293,14 @@ __global__ __launch_bounds__(SORT_BINS) void emb_scan_kernel(unsigned* counts, i
 
 // totals: the counts themselves and entries = blocks, or the groups' totals
 template <typename I, bool FIRST>
-__global__ __launch_bounds__(256) void emb_scatter_kernel(const void* ids, const uint2* in, long long T, long long V, long long padding, int shift,
+__global__ __launch_bounds__(SORT_THREADS) void emb_scatter_kernel(const void* ids, const uint2* in, long long T, long long V, long long padding, int shift,
                                                           const unsigned* __restrict__ counts, const unsigned* __restrict__ totals, int entries, uint2* out) {
-    __shared__ unsigned hist[4 * SORT_BINS];
-    __shared__ unsigned sums[4];
+    __shared__ unsigned hist[SORT_WAVES * SORT_BINS];
+    __shared__ unsigned sums[SORT_WAVES];
+    __shared__ unsigned odd[2][SORT_BINS];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     unsigned* mine = hist + wave * SORT_BINS;
-    for (int i = threadIdx.x; i < 4 * SORT_BINS; i += 256) hist[i] = 0;
+    for (int i = threadIdx.x; i < SORT_WAVES * SORT_BINS; i += SORT_THREADS) hist[i] = 0;
     __syncthreads();
     uint2 item[SORT_ITEMS];
     const long long t0 = (long long)blockIdx.x * SORT_BLOCK + wave * (64 * SORT_ITEMS);
@@ -308,31 +310,35 @@ __global__ __launch_bounds__(256) void emb_scatter_kernel(const void* ids, const
         item[j] = sort_item<I, FIRST>(ids, in, t, T, V, padding);
         if (t < T) atomicAdd(&mine[(item[j].x >> shift) & (SORT_BINS - 1)], 1u);
     }
-    // thread i owns bins 2i and 2i + 1: their totals and the share of the blocks before this one
-    const int b0 = 2 * threadIdx.x;
+    // threads i and 512 + i add up the even and the odd entries of bin i: its total and the share of the blocks before this one
+    const int bin = (int)threadIdx.x & (SORT_BINS - 1);
     const int own = totals == counts ? (int)blockIdx.x : (int)blockIdx.x / SORT_GROUP;
-    unsigned tot0 = 0, tot1 = 0, pre0 = 0, pre1 = 0;
-    if (totals != counts) {
-        const uint2 c = *reinterpret_cast<const uint2*>(counts + (size_t)blockIdx.x * SORT_BINS + b0);
-        pre0 = c.x; pre1 = c.y;
-    }
+    unsigned tot = 0, pre = 0;
 #pragma unroll 8
-    for (int b = 0; b < entries; ++b) {
-        const uint2 c = *reinterpret_cast<const uint2*>(totals + (size_t)b * SORT_BINS + b0);
-        const bool before = b < own;
-        pre0 += before ? c.x : 0u; pre1 += before ? c.y : 0u;
-        tot0 += c.x; tot1 += c.y;
+    for (int b = threadIdx.x / SORT_BINS; b < entries; b += SORT_THREADS / SORT_BINS) {
+        const unsigned c = totals[(size_t)b * SORT_BINS + bin];
+        pre += b < own ? c : 0u;
+        tot += c;
     }
-    const unsigned incl = wave_scan(tot0 + tot1);
-    if (lane == 63) sums[wave] = incl;
+    if (threadIdx.x >= SORT_BINS) { odd[0][bin] = tot; odd[1][bin] = pre; }
     __syncthreads();
-    unsigned base = incl - tot0 - tot1;
-    for (int w = 0; w < wave; ++w) base += sums[w];
-    unsigned r0 = base + pre0, r1 = base + tot0 + pre1;
-    for (int w = 0; w < 4; ++w) {
-        const unsigned c0 = hist[w * SORT_BINS + b0], c1 = hist[w * SORT_BINS + b0 + 1];
-        hist[w * SORT_BINS + b0] = r0; hist[w * SORT_BINS + b0 + 1] = r1;
-        r0 += c0; r1 += c1;
+    unsigned incl = 0;
+    if (threadIdx.x < SORT_BINS) {
+        tot += odd[0][bin];
+        pre += odd[1][bin] + (totals != counts ? counts[(size_t)blockIdx.x * SORT_BINS + bin] : 0u);
+        incl = wave_scan(tot);
+        if (lane == 63) sums[wave] = incl;
+    }
+    __syncthreads();
+    if (threadIdx.x < SORT_BINS) {
+        unsigned r = incl - tot + pre;
+        for (int w = 0; w < wave; ++w) r += sums[w];
+#pragma unroll
+        for (int w = 0; w < SORT_WAVES; ++w) {
+            const unsigned c = hist[w * SORT_BINS + bin];
+            hist[w * SORT_BINS + bin] = r;
+            r += c;
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -698,9 +704,9 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
         for (int pass = 0; pass < passes; ++pass) {
             const int shift = pass * SORT_BITS, extra = pass == 0 ? zero_blocks : 0;
 #define EMB_PASS(I, F)                                                                                                                       \
-    emb_hist_kernel<I, F><<<blocks + extra, 256, 0, s>>>(ids, from, T, V, padding_idx, shift, counts, blocks, (uint4*)dtable, zero16);      \
+    emb_hist_kernel<I, F><<<blocks + extra, SORT_THREADS, 0, s>>>(ids, from, T, V, padding_idx, shift, counts, blocks, (uint4*)dtable, zero16);      \
     if (groups > 0) emb_scan_kernel<<<groups, SORT_BINS, 0, s>>>(counts, blocks, totals);                                                    \
-    emb_scatter_kernel<I, F><<<blocks, 256, 0, s>>>(ids, from, T, V, padding_idx, shift, counts, totals, entries, to)
+    emb_scatter_kernel<I, F><<<blocks, SORT_THREADS, 0, s>>>(ids, from, T, V, padding_idx, shift, counts, totals, entries, to)
             if (pass > 0) { EMB_PASS(int64_t, false); }
             else if (ids_are_64) { EMB_PASS(int64_t, true); }
             else { EMB_PASS(int32_t, true); }
