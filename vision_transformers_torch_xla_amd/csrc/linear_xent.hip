@@ -855,8 +855,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
 }
 
 // Count of the counted rows, the scale of the gradients (1 / count, or 1 for a sum; 0 without a counted row) and the loss.  Workgroup b sums
-// a stretch of the rows into part[b]; the last one to finish adds the parts in order (the kernel that made the logits has zeroed the ticket).
-#define LX_LOSS_WGS 64
+// a stretch of the rows into part[b]; the last one to finish adds the parts up, one to a lane (the kernel that made the logits has zeroed the ticket).
+#define LX_LOSS_WGS 64          // at most a wave's lanes
 struct LxLossPart { double sum; long long count; };
 __global__ __launch_bounds__(256) void lx_loss_kernel(const long long* __restrict__ target, long long ignore_index, const float* __restrict__ rows, int T, int per,
                                                       int mean, LxLossPart* part, unsigned* ticket, float* __restrict__ scale, float* __restrict__ loss) {
@@ -885,21 +885,25 @@ __global__ __launch_bounds__(256) void lx_loss_kernel(const long long* __restric
     for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); n += __shfl_xor(n, o, 64); }
     if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = s; shc[threadIdx.x >> 6] = n; }
     __syncthreads();
-    if (threadIdx.x != 0) return;
+    if (threadIdx.x >= 64) return;
     s = (sh[0] + sh[1]) + (sh[2] + sh[3]);
     long long count = (long long)shc[0] + shc[1] + shc[2] + shc[3];
     if (gridDim.x > 1) {
-        __hip_atomic_store(&part[blockIdx.x].sum, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(&part[blockIdx.x].count, count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (__hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) != gridDim.x - 1) return;
-        s = 0.0;
-        count = 0;
-        for (unsigned b = 0; b < gridDim.x; ++b) {
-            s += __hip_atomic_load(&part[b].sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            count += __hip_atomic_load(&part[b].count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        unsigned nth = 0;
+        if (threadIdx.x == 0) {
+            __hip_atomic_store(&part[blockIdx.x].sum, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(&part[blockIdx.x].count, count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            nth = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
         }
+        if (__builtin_amdgcn_readfirstlane(nth) != gridDim.x - 1) return;
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        const bool mine = threadIdx.x < gridDim.x;
+        s = mine ? __hip_atomic_load(&part[threadIdx.x].sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+        count = mine ? __hip_atomic_load(&part[threadIdx.x].count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); count += __shfl_xor(count, o, 64); }
     }
-    lx_finish(s, count, mean, scale, loss);
+    if (threadIdx.x == 0) lx_finish(s, count, mean, scale, loss);
 }
 
 // The same products for outputs too small to fill the chip with 256 x 256 tiles, which also cost a call 8 to 10 us of pipeline fill and epilogue
