@@ -1082,12 +1082,43 @@ __global__ __launch_bounds__(256) void lx_small_kernel(const LxGemmParams p) {
     if (EPI != LX_OUT && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0u;
     lx_small_body<LAY, EPI, FM, WM, WN>(p, sm, blockIdx.x, gridDim.x);
 }
-// dx and dW in one launch: both need dz alone.  The first `blocks` workgroups are those of dx.
+// db of up to 1024 rows: a workgroup sums 128 columns, 16 rows at a time
+struct LxColsum { const bf16_t* dz; long long ldp; int T, V; const float* scale; void* db; int db_f32; };
+static __device__ __forceinline__ void lx_colsum_few(const LxColsum& c, float (*sh)[128], int block) {
+    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
+    const long long col = (long long)block * 128 + lane * 8;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int r = group; r < c.T; r += 16) {
+        float v[8];
+        load8(c.dz + (size_t)r * c.ldp + col, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += v[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sh[group][lane * 8 + k] = acc[k];
+    __syncthreads();
+    const int n = block * 128 + (int)threadIdx.x;
+    if (threadIdx.x >= 128 || n >= c.V) return;
+    float s = 0.f;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) s += sh[g][threadIdx.x];
+    s *= c.scale[0];
+    if (c.db_f32) reinterpret_cast<float*>(c.db)[n] = s;
+    else reinterpret_cast<bf16_t*>(c.db)[n] = f2bf(s);
+}
+__global__ __launch_bounds__(256) void lx_colsum_few_kernel(const LxColsum c) {
+    __shared__ float sh[16][128];
+    lx_colsum_few(c, sh, blockIdx.x);
+}
+// dx, dW and db of few rows in one launch: they need dz alone.  The first bx workgroups are those of dx, the next bw those of dW.
 template <int FM, int WM, int WN>
-__global__ __launch_bounds__(256) void lx_small_grads_kernel(const LxGemmParams dx, const LxGemmParams dw, int blocks) {
+__global__ __launch_bounds__(256) void lx_small_grads_kernel(const LxGemmParams dx, const LxGemmParams dw, const LxColsum db, int bx, int bw) {
     __shared__ __attribute__((aligned(1024))) bf16_t sm[LxSmall<FM, WM, WN>::lds];
-    if ((int)blockIdx.x < blocks) lx_small_body<LX_NN, LX_OUT, FM, WM, WN>(dx, sm, blockIdx.x, blocks);
-    else lx_small_body<LX_TN, LX_OUT, FM, WM, WN>(dw, sm, blockIdx.x - blocks, gridDim.x - blocks);
+    const int block = blockIdx.x;
+    if (block < bx) lx_small_body<LX_NN, LX_OUT, FM, WM, WN>(dx, sm, block, bx);
+    else if (block < bx + bw) lx_small_body<LX_TN, LX_OUT, FM, WM, WN>(dw, sm, block - bx, bw);
+    else lx_colsum_few(db, reinterpret_cast<float (*)[128]>(sm), block - bx - bw);
 }
 
 // out = scale * sum over the splits of slab[s] (+ add), fixed order; N % 4 == 0
@@ -1188,32 +1219,6 @@ __global__ __launch_bounds__(256) void lx_colsum_final_kernel(const float* __res
     float s = first ? 0.f : sum[n];
     for (int r = 0; r < ranges; ++r) s += partial[(size_t)r * ldp + n];
     if (db == nullptr) { sum[n] = s; return; }
-    s *= scale[0];
-    if (db_f32) reinterpret_cast<float*>(db)[n] = s;
-    else reinterpret_cast<bf16_t*>(db)[n] = f2bf(s);
-}
-
-// the same for up to 1024 rows in one launch: a workgroup sums 128 columns, 16 rows at a time
-__global__ __launch_bounds__(256) void lx_colsum_few_kernel(const bf16_t* __restrict__ dz, long long ldp, int T, int V, const float* __restrict__ scale, void* __restrict__ db, int db_f32) {
-    __shared__ float sh[16][128];
-    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
-    const long long col = (long long)blockIdx.x * 128 + lane * 8;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int r = group; r < T; r += 16) {
-        float v[8];
-        load8(dz + (size_t)r * ldp + col, v);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] += v[k];
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) sh[group][lane * 8 + k] = acc[k];
-    __syncthreads();
-    const int n = blockIdx.x * 128 + (int)threadIdx.x;
-    if (threadIdx.x >= 128 || n >= V) return;
-    float s = 0.f;
-#pragma unroll
-    for (int g = 0; g < 16; ++g) s += sh[g][threadIdx.x];
     s *= scale[0];
     if (db_f32) reinterpret_cast<float*>(db)[n] = s;
     else reinterpret_cast<bf16_t*>(db)[n] = f2bf(s);
@@ -1547,6 +1552,8 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         e.add = b > 0 ? acc : nullptr;
         if (last) { e.out = dw; e.ldo = lddw; e.out_f32 = dw_f32; }
         else { e.out = acc; e.ldo = D; e.out_f32 = 1; }
+        const LxColsum c = {dz, q.ldp, n, V, scale, db, db_f32};
+        const bool few = db != nullptr && q.blocks == 1 && n <= 1024;
         const LxDeal& dd = q.dx[last];
         const LxDeal& de = q.dw[last];
         if (lx_one_launch(dd, de)) {
@@ -1554,8 +1561,9 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
             lx_tiles(e, de);
             e.slab = d.slab + dd.slab;
             const int bx = d.tiles_m * d.tiles_n * dd.splits, bw = e.tiles_m * e.tiles_n * de.splits;
-            if (dd.kind == LX_SMALL64) lx_small_grads_kernel<1, 4, 1><<<bx + bw, 256, 0, s>>>(d, e, bx);
-            else lx_small_grads_kernel<4, 2, 2><<<bx + bw, 256, 0, s>>>(d, e, bx);
+            const int bc = few ? (int)(q.ldp / 128) : 0;
+            if (dd.kind == LX_SMALL64) lx_small_grads_kernel<1, 4, 1><<<bx + bw + bc, 256, 0, s>>>(d, e, c, bx, bw);
+            else lx_small_grads_kernel<4, 2, 2><<<bx + bw + bc, 256, 0, s>>>(d, e, c, bx, bw);
             if (int rc = vitk_check_launch("linear_xent_grads")) return rc;
             if (dd.splits > 1)
                 if (int rc = lx_reduce(d, s, "linear_xent_dx_sum")) return rc;
@@ -1565,8 +1573,8 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
             if (int rc = lx_launch<LX_NN, LX_OUT>(d, dd, s, "linear_xent_dx")) return rc;
             if (int rc = lx_launch<LX_TN, LX_OUT>(e, de, s, "linear_xent_dw")) return rc;
         }
-        if (db != nullptr && q.blocks == 1 && n <= 1024) {
-            lx_colsum_few_kernel<<<(unsigned)(q.ldp / 128), 256, 0, s>>>(dz, q.ldp, n, V, scale, db, db_f32);
+        if (few) {
+            if (!lx_one_launch(dd, de)) lx_colsum_few_kernel<<<(unsigned)(q.ldp / 128), 256, 0, s>>>(c);
             if (int rc = vitk_check_launch("linear_xent_db")) return rc;
         } else if (db != nullptr) {
             float* part = (float*)(ws + q.colpart);
