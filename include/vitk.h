@@ -307,12 +307,12 @@ int vitk_kd_kl_fwd_bwd(const float* student, int lds_, const float* teacher, int
  * loss[0] = sum of rows / number of counted rows (mean != 0) or their sum; 0 without a counted row.  A target outside [0, V) that is not
  * ignore_index makes its row, the loss and the gradients it reaches NaN.
  * x bf16 [T, D], w bf16 [V, D] (row strides ldx, ldw), bias [V] (0 fp32, 1 bf16) or NULL, target int64 [T].  D and the strides are
- * multiples of 8, rows 16-byte aligned; T <= 2^30, V <= 2^22.  With dx and dw (both or neither): dx bf16 [T, D], dw [V, D] (bf16, or fp32 with dw_f32) and, with
- * db, db [V] (bf16, or fp32 with db_f32) receive the gradients of loss[0].  Products are of bf16 factors with fp32 sums; the factor dloss/dz
+ * multiples of 8, rows 16-byte aligned; T <= 2^30, V <= 2^22.  dx bf16 [T, D], dw [V, D] (bf16, or fp32 with dw_f32) and db [V] (bf16, or fp32 with
+ * db_f32) receive the gradients of loss[0]; each may be NULL, and what only it needs is not computed.  Products are of bf16 factors with fp32 sums; the factor dloss/dz
  * is rounded to bf16 once, without the 1 / count, which multiplies the sums.
  * Rows are worked through in blocks whose probabilities (2 bytes each) and statistics take about block_bytes at most (at least 256
  * rows); dw is summed over the blocks in fp32 (an fp32 dw in place: its rows must then be contiguous).  An ignored row adds 0 * x to dw: its x
- * has to be finite there, as with separate products.  workspace: vitk_linear_xent_workspace(...) bytes for the same arguments, 256-byte aligned. */
+ * has to be finite there, as with separate products.  want_grad: whether any gradient is asked for.  workspace: vitk_linear_xent_workspace(...) bytes for the same arguments, 256-byte aligned. */
 size_t vitk_linear_xent_workspace(int64_t T, int V, int D, int want_grad, int smoothing, int dw_f32, int bias, size_t block_bytes);
 int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_type, const int64_t* target, int64_t T, int V, int D,
                      float smoothing, int64_t ignore_index, int mean, float* loss, float* rows, void* dx, int64_t lddx, void* dw, int64_t lddw, int dw_f32,

@@ -718,6 +718,30 @@ def test_linear_xent_in_a_graph_on_another_stream(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D,block_bytes", [(40, 500, 64, 1 << 30), (700, 3000, 192, 1 << 30), (2050, 12001, 520, 1 << 30), (1500, 2000, 72, 1 << 20)])
+def test_linear_xent_some_of_the_gradients(device, T, V, D, block_bytes):
+    ops = _ops()
+    g = torch.Generator().manual_seed(T + V)
+    x, w, target = (t.to(device) for t in xent_inputs(T, V, D, g))
+    bias = torch.randn(V, generator=g).to(device)
+    args = dict(smoothing=0.1, block_bytes=block_bytes)
+    full = ops.linear_xent(x, w, target, bias, **args)
+    check_linear_xent(full, x, w, target, bias, 0.1)
+    for grads in ((), ("x",), ("weight",), ("bias",), ("x", "bias"), ("weight", "bias"), ["x", "weight"]):
+        r = ops.linear_xent(x, w, target, bias, grads=grads, **args)
+        assert torch.equal(r.loss, full.loss) and torch.equal(r.rows, full.rows)
+        for name, got, want in (("x", r.dx, full.dx), ("weight", r.dweight, full.dweight), ("bias", r.dbias, full.dbias)):
+            assert torch.equal(got, want) if name in grads else got is None
+    head = w.float().requires_grad_(True)                               # frozen features, then a frozen head
+    from vision_transformers_torch_xla_amd import losses
+    losses.linear_cross_entropy(x, head, target, bias, smoothing=0.1).backward()
+    assert close(head.grad, full.dweight.cpu(), 0.005)
+    feats = x.clone().requires_grad_(True)
+    losses.linear_cross_entropy(feats, w, target, bias, smoothing=0.1).backward()
+    assert close(feats.grad, full.dx.cpu(), 0.005)
+
+
+@pytest.mark.gpu
 def test_linear_xent_refuses(device):
     ops, err = _ops(), _error()
     x, w, t = torch.randn(6, 16, device=device).to(bf16), torch.randn(9, 16, device=device).to(bf16), torch.zeros(6, dtype=torch.int64, device=device)
@@ -728,6 +752,7 @@ def test_linear_xent_refuses(device):
                  lambda: ops.linear_xent(x, w, t, smoothing=1.5), lambda: ops.linear_xent(x, w, t, smoothing=math.nan),
                  lambda: ops.linear_xent(x, w, t, reduction="none"), lambda: ops.linear_xent(x, w, t, dweight_dtype=f16),
                  lambda: ops.linear_xent(x[:, ::2], w[:, ::2], t), lambda: ops.linear_xent(x[:, 1:9], w[:, 1:9], t), lambda: ops.linear_xent(x, w[:0], t),
+                 lambda: ops.linear_xent(x, w, t, grads="x"), lambda: ops.linear_xent(x, w, t, grads=("x", "w")),
                  lambda: ops.linear_xent(x, w, t, block_bytes=0), lambda: ops.linear_xent(x[:1].expand(6, 16), w, t)):
         with pytest.raises(err):
             call()
@@ -1024,7 +1049,7 @@ def test_entry_points_check_before_they_launch():
         return lib.vitk_linear_xent(x, ldx, w, 16, None, 0, p, T, V, D, eps, -100, 1, p, p, dx, ld, dw, ld, 0, db, 0, p, nbytes, 1 << 20, None)
     assert need > 0 and lib.vitk_linear_xent_workspace(0, 4, 16, 1, 0, 0, 0, 1 << 20) == 0
     assert xent(nbytes=need - 1) == -28
-    for kw in ({"x": None}, {"ldx": 12}, {"D": 12}, {"V": 0}, {"V": 1 << 23}, {"eps": -0.1}, {"eps": 1.1}, {"dx": None}, {"db": p}, {"x": p + 8}, {"T": 0}, {"ld": 8}):
+    for kw in ({"x": None}, {"ldx": 12}, {"D": 12}, {"V": 0}, {"V": 1 << 23}, {"eps": -0.1}, {"eps": 1.1}, {"dx": None, "dw": None, "db": p}, {"db": p}, {"dx": p + 8}, {"dw": p + 8}, {"x": p + 8}, {"T": 0}, {"ld": 8}):
         assert xent(**kw) == -22, kw
 
 

@@ -1457,13 +1457,12 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
     VITK_REQUIRE(vitk_aligned(x, 16) && vitk_aligned(w, 16) && vitk_aligned(workspace, 256) && vitk_aligned(target, 8), "linear_xent: rows must be 16-byte aligned");
     VITK_REQUIRE(smoothing >= 0.f && smoothing <= 1.f, "linear_xent: smoothing %g outside [0, 1]", (double)smoothing);
     VITK_REQUIRE(!bias || bias_type == 0 || bias_type == 1, "linear_xent: bias types are 0 (fp32) and 1 (bf16)");
-    VITK_REQUIRE((dx != nullptr) == (dw != nullptr), "linear_xent: dx and dw go together");
-    const bool grad = dx != nullptr;
-    VITK_REQUIRE(!grad || (lddx % 8 == 0 && lddx >= D && lddw % 8 == 0 && lddw >= D && vitk_aligned(dx, 16) && vitk_aligned(dw, 16)),
+    const bool grad = dx || dw || db;
+    VITK_REQUIRE((!dx || (lddx % 8 == 0 && lddx >= D && vitk_aligned(dx, 16))) && (!dw || (lddw % 8 == 0 && lddw >= D && vitk_aligned(dw, 16))),
                  "linear_xent: gradient rows must be 16-byte aligned with strides that are multiples of 8 (lddx=%lld lddw=%lld)", (long long)lddx, (long long)lddw);
-    VITK_REQUIRE(!db || (grad && bias), "linear_xent: db needs a bias and the other gradients");
+    VITK_REQUIRE(!db || bias, "linear_xent: db needs a bias");
     const LxPlan q = lx_plan(T, V, D, grad, smoothing > 0.f, dw_f32, db != nullptr, block_bytes);
-    VITK_REQUIRE(!grad || !dw_f32 || q.blocks == 1 || lddw == D, "linear_xent: an fp32 dw over several blocks of rows must be contiguous");
+    VITK_REQUIRE(!dw || !dw_f32 || q.blocks == 1 || lddw == D, "linear_xent: an fp32 dw over several blocks of rows must be contiguous");
     if (workspace_bytes < q.total) {
         vitk_set_error("linear_xent: workspace %zu < %zu", workspace_bytes, q.total);
         return VITK_ENOSPC;
@@ -1512,7 +1511,7 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         const bool fused = q.blocks == 1 && T <= LX_FUSED_ROWS && (!grad || (size_t)T * q.ldp * 2 <= LX_FUSED_BYTES);
         r.ticket = ticket; r.scale = scale; r.loss = fused ? loss : nullptr; r.mean = mean;
         r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.rows_n = n; r.smoothing = smoothing;
-        r.pad_rows = grad && q.dw[last].kind == LX_BIG ? (LX_BK - n % LX_BK) % LX_BK : 0;
+        r.pad_rows = dw && q.dw[last].kind == LX_BIG ? (LX_BK - n % LX_BK) % LX_BK : 0;
         const int row_wgs = n + r.pad_rows;
         // long rows get more waves.  By the vocabulary alone, so that a row's sums do not depend on how many rows there are or what is wanted.
         // STREAM: past the caches, where the block is larger than they are.
@@ -1556,7 +1555,8 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         const bool few = db != nullptr && q.blocks == 1 && n <= 1024;
         const LxDeal& dd = q.dx[last];
         const LxDeal& de = q.dw[last];
-        if (lx_one_launch(dd, de)) {
+        const bool together = dx && dw && lx_one_launch(dd, de);
+        if (together) {
             lx_tiles(d, dd);
             lx_tiles(e, de);
             e.slab = d.slab + dd.slab;
@@ -1570,11 +1570,13 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
             if (de.splits > 1)
                 if (int rc = lx_reduce(e, s, "linear_xent_dw_sum")) return rc;
         } else {
-            if (int rc = lx_launch<LX_NN, LX_OUT>(d, dd, s, "linear_xent_dx")) return rc;
-            if (int rc = lx_launch<LX_TN, LX_OUT>(e, de, s, "linear_xent_dw")) return rc;
+            if (dx)
+                if (int rc = lx_launch<LX_NN, LX_OUT>(d, dd, s, "linear_xent_dx")) return rc;
+            if (dw)
+                if (int rc = lx_launch<LX_TN, LX_OUT>(e, de, s, "linear_xent_dw")) return rc;
         }
         if (few) {
-            if (!lx_one_launch(dd, de)) lx_colsum_few_kernel<<<(unsigned)(q.ldp / 128), 256, 0, s>>>(c);
+            if (!together) lx_colsum_few_kernel<<<(unsigned)(q.ldp / 128), 256, 0, s>>>(c);
             if (int rc = vitk_check_launch("linear_xent_db")) return rc;
         } else if (db != nullptr) {
             float* part = (float*)(ws + q.colpart);

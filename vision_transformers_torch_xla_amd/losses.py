@@ -108,8 +108,9 @@ class _LinearXent(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, smoothing, ignore_index, reduction, want):
         wtype = weight.dtype
+        grads = [n for n, need in zip(("x", "weight", "bias"), ctx.needs_input_grad) if need]
         r = ops.linear_xent(_bf16_rows(x), _bf16_rows(weight), target, None if bias is None else bias.detach(), smoothing=smoothing,
-                            ignore_index=ignore_index, reduction=reduction, want_grad=want, dweight_dtype=wtype if wtype in (bf16, f32) else None)
+                            ignore_index=ignore_index, reduction=reduction, want_grad=want, dweight_dtype=wtype if wtype in (bf16, f32) else None, grads=grads)
         ctx.grads = (r.dx, r.dweight, r.dbias) if want else None
         ctx.xtype = x.dtype
         return r.loss
@@ -120,9 +121,8 @@ class _LinearXent(torch.autograd.Function):
         if ctx.grads is None:
             raise VitkError("linear_cross_entropy: backward was called a second time (the gradients are handed over, not kept)")
         (dx, dw, db), ctx.grads = ctx.grads, None
-        need = ctx.needs_input_grad
-        dx = _times(dx, go).to(ctx.xtype) if need[0] else None
-        return dx, _times(dw, go) if need[1] else None, _times(db, go) if need[2] else None, None, None, None, None, None
+        dx = _times(dx, go)
+        return None if dx is None else dx.to(ctx.xtype), _times(dw, go), _times(db, go), None, None, None, None, None
 
 
 def linear_cross_entropy(x, weight, target, bias=None, smoothing: float = 0.0, ignore_index: int = -100, reduction: str = "mean"):

@@ -590,7 +590,7 @@ LINEAR_XENT_BLOCK = 2 << 30          # bytes of probabilities that linear_xent h
 
 
 def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, reduction="mean", want_grad=True, dweight_dtype=None,
-                block_bytes=LINEAR_XENT_BLOCK):
+                block_bytes=LINEAR_XENT_BLOCK, grads=("x", "weight", "bias")):
     """Cross entropy of the logits x @ weight.T + bias against int64 targets, with the gradients of the reduced loss, without the logits in
     memory: x bf16 [T, D], weight bf16 [V, D] (rows may have a stride), bias fp32 / bf16 [V], target [T].  D % 8 == 0, V <= 2^22.
 
@@ -598,6 +598,7 @@ def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, 
     rows, or their sum (reduction 'sum'); 0 with zero gradients where no row counts.  Any other target outside [0, V) gives NaN.
     An ignored row of x must still be finite where dweight is wanted (0 times the row is added, as with separate products).
     want_grad: dx bf16 [T, D], dweight [V, D] in dweight_dtype (bf16, the default, or float32), dbias in the bias's type.
+    grads: which of them; a frozen head or frozen features cost one product less.
     block_bytes: the rows are worked through in blocks that hold about this many bytes of probabilities (at least 256 rows); more than
     one block costs an fp32 copy of a bf16 dweight."""
     for t, n in ((x, "x"), (weight, "weight")):
@@ -613,6 +614,8 @@ def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, 
         raise _lib.VitkError(f"linear_xent: target must be int64 [{T}], got {target.dtype} {tuple(target.shape)}")
     if int(block_bytes) <= 0:
         raise _lib.VitkError(f"linear_xent: block_bytes must be positive, got {block_bytes}")
+    if isinstance(grads, str) or not set(grads) <= {"x", "weight", "bias"}:
+        raise _lib.VitkError(f"linear_xent: grads must be some of ('x', 'weight', 'bias'), got {grads!r}")
     if reduction not in ("mean", "sum"):
         raise _lib.VitkError(f"linear_xent: reduction must be 'mean' or 'sum' (rows are returned beside either), got {reduction!r}")
     btype = 0
@@ -631,9 +634,12 @@ def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, 
     loss = torch.empty((), dtype=f32, device=dev)
     dx = dw = db = None
     if want_grad:
-        dx = torch.empty((T, D), dtype=bf16, device=dev)
-        dw = torch.empty((V, D), dtype=wtype, device=dev)
-        db = torch.empty(V, dtype=bias.dtype, device=dev) if bias is not None else None
+        if "x" in grads:
+            dx = torch.empty((T, D), dtype=bf16, device=dev)
+        if "weight" in grads:
+            dw = torch.empty((V, D), dtype=wtype, device=dev)
+        if "bias" in grads and bias is not None:
+            db = torch.empty(V, dtype=bias.dtype, device=dev)
     if T == 0 and V > 0:
         for t in (loss, dw, db):
             if t is not None:
@@ -641,7 +647,7 @@ def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, 
         return LinearXent(loss, rows, dx, dw, db)
     lib = _lib.load()
     wf32, smooth = int(wtype == f32), float(smoothing)
-    need = lib.vitk_linear_xent_workspace(T, V, D, int(want_grad), int(smooth > 0), wf32, int(db is not None), int(block_bytes))
+    need = lib.vitk_linear_xent_workspace(T, V, D, int(any(t is not None for t in (dx, dw, db))), int(smooth > 0), wf32, int(db is not None), int(block_bytes))
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
     check(lib.vitk_linear_xent(_ptr(x), x.stride(0) if T > 1 else max(D, 1), _ptr(weight), weight.stride(0) if V > 1 else max(D, 1), _ptr(bias), btype, _ptr(target),
                                T, V, D, smooth, int(ignore_index), int(reduction == "mean"), _ptr(loss), _ptr(rows), _ptr(dx), D, _ptr(dw), D, wf32,
