@@ -355,7 +355,7 @@ int vitk_embedding_fwd(const void* ids, int ids_are_64, const void* table, int t
 /* gradient: dtable[v] = scale * sum over the tokens t with ids[t] == v of dout[t], summed in fp32 in an order that the ids alone decide
  * (the tokens are sorted by id; long runs are summed in stretches), rounded once; zero for rows without a token.  accumulate: added to what dtable holds, rows
  * without a token stay untouched.  Tokens with id padding_idx (negative: none) or an id outside [0, V) add nothing.
- * T, V < 2^31, D <= 2^23.  workspace: vitk_embedding_bwd_workspace(T, V, D) bytes. */
+ * T, V < 2^31, D <= 2^23.  workspace: vitk_embedding_bwd_workspace(T, V, D) bytes, 16-byte aligned; NULL where that is 0 (few tokens). */
 size_t vitk_embedding_bwd_workspace(int64_t T, int64_t V, int D);
 int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void* ids, int ids_are_64, void* dtable, int dtable_type, int64_t ldo,
                        int64_t T, int64_t V, int D, float scale, int64_t padding_idx, int accumulate, void* workspace, size_t workspace_bytes,

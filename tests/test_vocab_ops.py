@@ -374,6 +374,7 @@ def test_embedding_refuses(device):
                  lambda: ops.embedding_bwd(dout, ids, 10, out=torch.empty(9, 16, device=device)),
                  lambda: ops.embedding_bwd(dout, ids, 10, out=torch.empty(10, 32, device=device)[:, :16]),    # a stride without accumulate
                  lambda: ops.embedding_bwd(dout, ids, 10, out=torch.empty(10, 16, device=device), out_dtype=bf16),
+                 lambda: ops.embedding_bwd(dout, ids, 10, out_dtype=f16),
                  lambda: ops.embedding_bwd(dout[:, :12], ids, 10),
                  lambda: ops.embedding_bwd(dout.half(), ids, 10),
                  lambda: ops.embedding_bwd(dout, ids, 10, padding_idx=-1),
@@ -1038,8 +1039,9 @@ def test_entry_points_check_before_they_launch():
     assert lib.vitk_embedding_fwd(p, 1, p, 2, 16, p, 0, 16, 4, 4, 16, 1.0, None) == -22
     assert lib.vitk_embedding_fwd(p, 1, p + 4, 0, 16, p, 0, 16, 4, 4, 16, 1.0, None) == -22
     assert lib.vitk_embedding_fwd(None, 1, None, 0, 16, None, 0, 16, 0, 4, 16, 1.0, None) == 0          # nothing to do
-    need = lib.vitk_embedding_bwd_workspace(4, 4, 16)
-    assert lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 16, 4, 4, 16, 1.0, -1, 0, p, need - 1, None) == -28
+    need = lib.vitk_embedding_bwd_workspace(1000, 4, 16)
+    assert need > 0 and lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 16, 1000, 4, 16, 1.0, -1, 0, p, need - 1, None) == -28
+    assert lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 16, 1000, 4, 16, 1.0, -1, 0, None, need, None) == -22
     assert lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 24, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22
     assert lib.vitk_embedding_bwd(p, 0, 8, p, 1, p, 0, 16, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22
     assert lib.vitk_embedding_bwd(None, 0, 16, p, 1, p, 0, 16, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22

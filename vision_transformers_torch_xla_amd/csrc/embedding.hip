@@ -626,7 +626,7 @@ int vitk_embedding_fwd(const void* ids, int ids_are_64, const void* table, int t
 }
 
 size_t vitk_embedding_bwd_workspace(int64_t T, int64_t V, int D) {
-    if (T <= FEW_MAX || V <= 0 || D <= 0) return 16;
+    if (T <= FEW_MAX || V <= 0 || D <= 0) return 0;
     const long long pieces = (T + emb_piece(T, D) - 1) / emb_piece(T, D);
     size_t n = emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)pieces * 2 * D * sizeof(float));
     if (!emb_one(T, V)) n += emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)(emb_sort_blocks(T) + emb_sort_groups(T)) * SORT_BINS * sizeof(unsigned));
@@ -639,7 +639,7 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
     VITK_REQUIRE(T >= 0 && V > 0 && D > 0, "embedding_bwd: bad shape T=%lld V=%lld D=%d", (long long)T, (long long)V, D);
     VITK_REQUIRE((dout_type == 0 || dout_type == 1) && (dtable_type == 0 || dtable_type == 1), "embedding_bwd: types are 0 (fp32) and 1 (bf16)");
     VITK_REQUIRE(T < 0x7fffffffll && V < 0x7fffffffll && D <= (1 << 23), "embedding_bwd: T and V must be below 2^31, D at most 2^23");
-    VITK_REQUIRE(dtable && workspace && (T == 0 || (dout && ids)), "embedding_bwd: null pointer");
+    VITK_REQUIRE(dtable && (workspace || T <= FEW_MAX) && (T == 0 || (dout && ids)), "embedding_bwd: null pointer");
     VITK_REQUIRE(D % 8 == 0 && ldd % 8 == 0 && ldo % 8 == 0 && ldd >= D && ldo >= D, "embedding_bwd: D and the row strides must be multiples of 8, strides >= D (D=%d ldd=%lld ldo=%lld)",
                  D, (long long)ldd, (long long)ldo);
     VITK_REQUIRE(vitk_aligned(dtable, 16) && vitk_aligned(workspace, 16) && (T == 0 || (vitk_aligned(dout, 16) && vitk_aligned(ids, ids_are_64 ? 8 : 4))),

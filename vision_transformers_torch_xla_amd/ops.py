@@ -552,28 +552,33 @@ def embedding_bwd(dout, ids, num_rows, scale=1.0, padding_idx=None, out=None, ac
     rows that have tokens are touched.  Without out: a new tensor of out_dtype (default: dout's type)."""
     if padding_idx is not None and not 0 <= int(padding_idx) < int(num_rows):
         raise _lib.VitkError(f"embedding_bwd: padding_idx {padding_idx} outside the table of {num_rows} rows")
-    if dout.dim() < 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
+    if dout.dim() < 1 or dout.shape[:-1] != ids.shape:
         raise _lib.VitkError(f"embedding_bwd: dout must be {tuple(ids.shape)} + (D,), got {tuple(dout.shape)}")
-    D = dout.shape[-1]
+    D, num_rows = dout.shape[-1], int(num_rows)
     flat = _ids1d(ids)
-    rows = dout.reshape(flat.numel(), D)
+    T = flat.numel()
+    rows = dout if dout.dim() == 2 else dout.reshape(T, D)
     if D > 1 and rows.stride(1) != 1:
         rows = rows.contiguous()
     dcode, ldd = _rows2d(rows, "dout")
     if out is None:
         if accumulate:
             raise _lib.VitkError("embedding_bwd: accumulate needs out")
-        out = torch.empty((int(num_rows), D), dtype=dout.dtype if out_dtype is None else out_dtype, device=dout.device)
+        ocode, ldo = _ROW_TYPES.get(dout.dtype if out_dtype is None else out_dtype), D
+        if ocode is None:
+            raise _lib.VitkError(f"embedding_bwd: out_dtype must be float32 or bfloat16, got {out_dtype}")
+        out = torch.empty((num_rows, D), dtype=bf16 if ocode else f32, device=dout.device)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise _lib.VitkError(f"embedding_bwd: out is {out.dtype}, out_dtype says {out_dtype}")
-    if tuple(out.shape) != (int(num_rows), D):
+    elif out.shape != (num_rows, D):
         raise _lib.VitkError(f"embedding_bwd: out must be [{num_rows}, {D}], got {tuple(out.shape)}")
-    ocode, ldo = _rows2d(out, "out")
+    else:
+        ocode, ldo = _rows2d(out, "out")
     lib = _lib.load()
-    ws = torch.empty(lib.vitk_embedding_bwd_workspace(flat.numel(), int(num_rows), D), dtype=torch.uint8, device=out.device)
-    check(lib.vitk_embedding_bwd(_ptr(rows), dcode, ldd, _ptr(flat), int(flat.dtype == torch.int64), _ptr(out), ocode, ldo, flat.numel(), int(num_rows),
-                                 D, float(scale), -1 if padding_idx is None else int(padding_idx), int(bool(accumulate)), _ptr(ws), ws.numel(),
-                                 _stream()), "embedding_bwd")
+    need = lib.vitk_embedding_bwd_workspace(T, num_rows, D)
+    ws = torch.empty(need, dtype=torch.uint8, device=out.device) if need else None
+    check(lib.vitk_embedding_bwd(rows.data_ptr(), dcode, ldd, flat.data_ptr(), int(flat.dtype == torch.int64), out.data_ptr(), ocode, ldo, T, num_rows, D,
+                                 float(scale), -1 if padding_idx is None else int(padding_idx), int(bool(accumulate)), _ptr(ws), need, _stream()), "embedding_bwd")
     return out
 
 
