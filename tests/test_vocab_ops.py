@@ -257,8 +257,8 @@ def test_embedding_bwd_of_very_many_tokens(device, T, V, D):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T", [1, 9, 256, 257, 511, 512, 513])                   # on both sides of the form for few tokens
-@pytest.mark.parametrize("V,D", [(3, 8), (4099, 24), (40, 256), (700, 264), (100, 1032), (1, 16384), (300001, 8)])
+@pytest.mark.parametrize("T", [1, 9, 256, 257, 511, 512, 513, 682, 683, 1024, 1025])       # on both sides of the form for few tokens
+@pytest.mark.parametrize("V,D", [(3, 8), (4099, 24), (40, 256), (700, 264), (90, 768), (100, 1032), (1, 16384), (300001, 8)])
 def test_embedding_bwd_of_few_tokens(device, T, V, D):
     ops = _ops()
     g = torch.Generator().manual_seed(T * V)
@@ -1039,9 +1039,9 @@ def test_entry_points_check_before_they_launch():
     assert lib.vitk_embedding_fwd(p, 1, p, 2, 16, p, 0, 16, 4, 4, 16, 1.0, None) == -22
     assert lib.vitk_embedding_fwd(p, 1, p + 4, 0, 16, p, 0, 16, 4, 4, 16, 1.0, None) == -22
     assert lib.vitk_embedding_fwd(None, 1, None, 0, 16, None, 0, 16, 0, 4, 16, 1.0, None) == 0          # nothing to do
-    need = lib.vitk_embedding_bwd_workspace(1000, 4, 16)
-    assert need > 0 and lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 16, 1000, 4, 16, 1.0, -1, 0, p, need - 1, None) == -28
-    assert lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 16, 1000, 4, 16, 1.0, -1, 0, None, need, None) == -22
+    need = lib.vitk_embedding_bwd_workspace(2000, 4, 16)
+    assert need > 0 and lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 16, 2000, 4, 16, 1.0, -1, 0, p, need - 1, None) == -28
+    assert lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 16, 2000, 4, 16, 1.0, -1, 0, None, need, None) == -22
     assert lib.vitk_embedding_bwd(p, 0, 16, p, 1, p, 0, 24, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22
     assert lib.vitk_embedding_bwd(p, 0, 8, p, 1, p, 0, 16, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22
     assert lib.vitk_embedding_bwd(None, 0, 16, p, 1, p, 0, 16, 4, 4, 16, 1.0, -1, 0, p, need, None) == -22

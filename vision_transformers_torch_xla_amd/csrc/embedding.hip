@@ -479,9 +479,10 @@ __global__ __launch_bounds__(1024) void embedding_join_kernel(const EmbBwdParams
 // Few tokens: everything in one launch, without a list.  The last workgroups zero the rows that no token has; each of the others is one token
 // and a slice of the columns, and if its token is the first with its id it collects the tokens that have the same one, in order, and
 // adds them up: up to eight by one group of threads, more by 256 / lanes groups, a stretch each, whose sums are joined in order.
-// A call takes 13 us instead of 19 (512 tokens, 1000 x 768), with 50021 x 768 to zero 16 instead of 21; the worst mix, one id alone before so
-// large a table, 28 instead of 22.
-#define FEW_MAX 512
+// A call takes 9 us instead of 16 (512 tokens, 1000 x 768), with 50021 x 768 to zero 16 instead of 21; the worst mix, one id alone before so large a
+// table, 28 instead of 22.  Most workgroups end at once, but 4096 of them take as long to start as the other form needs.
+#define FEW_MAX 1024
+#define FEW_WGS 2048            // tokens times slices
 #define FEW_AHEAD 16
 #define FEW_ROWS 2048           // rows of the gradient a workgroup zeroes at a time, at most
 template <typename I, typename TI, typename TO>
@@ -588,6 +589,9 @@ static int emb_passes(long long V) {
     return (bits + SORT_BITS - 1) / SORT_BITS;
 }
 static bool emb_one(long long T, long long V) { return T <= GROUP_MAX && V <= (1 << 18); }
+static int emb_few_lanes(int D) { return D > 256 ? 32 : emb_lanes(D); }
+static int emb_few_slices(int D) { return (D / 8 + emb_few_lanes(D) - 1) / emb_few_lanes(D); }
+static bool emb_few(long long T, int D) { return T <= FEW_MAX && T * emb_few_slices(D) <= FEW_WGS; }
 static long long emb_sort_blocks(long long T) { return (T + SORT_BLOCK - 1) / SORT_BLOCK; }
 static long long emb_sort_groups(long long T) { return emb_sort_blocks(T) > SORT_DIRECT ? (emb_sort_blocks(T) + SORT_GROUP - 1) / SORT_GROUP : 0; }
 static size_t emb_up(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -626,7 +630,7 @@ int vitk_embedding_fwd(const void* ids, int ids_are_64, const void* table, int t
 }
 
 size_t vitk_embedding_bwd_workspace(int64_t T, int64_t V, int D) {
-    if (T <= FEW_MAX || V <= 0 || D <= 0) return 0;
+    if (T <= 0 || V <= 0 || D <= 0 || emb_few(T, D)) return 0;
     const long long pieces = (T + emb_piece(T, D) - 1) / emb_piece(T, D);
     size_t n = emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)pieces * 2 * D * sizeof(float));
     if (!emb_one(T, V)) n += emb_up((size_t)T * sizeof(uint2)) + emb_up((size_t)(emb_sort_blocks(T) + emb_sort_groups(T)) * SORT_BINS * sizeof(unsigned));
@@ -639,7 +643,7 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
     VITK_REQUIRE(T >= 0 && V > 0 && D > 0, "embedding_bwd: bad shape T=%lld V=%lld D=%d", (long long)T, (long long)V, D);
     VITK_REQUIRE((dout_type == 0 || dout_type == 1) && (dtable_type == 0 || dtable_type == 1), "embedding_bwd: types are 0 (fp32) and 1 (bf16)");
     VITK_REQUIRE(T < 0x7fffffffll && V < 0x7fffffffll && D <= (1 << 23), "embedding_bwd: T and V must be below 2^31, D at most 2^23");
-    VITK_REQUIRE(dtable && (workspace || T <= FEW_MAX) && (T == 0 || (dout && ids)), "embedding_bwd: null pointer");
+    VITK_REQUIRE(dtable && (workspace || emb_few(T, D)) && (T == 0 || (dout && ids)), "embedding_bwd: null pointer");
     VITK_REQUIRE(D % 8 == 0 && ldd % 8 == 0 && ldo % 8 == 0 && ldd >= D && ldo >= D, "embedding_bwd: D and the row strides must be multiples of 8, strides >= D (D=%d ldd=%lld ldo=%lld)",
                  D, (long long)ldd, (long long)ldo);
     VITK_REQUIRE(vitk_aligned(dtable, 16) && vitk_aligned(workspace, 16) && (T == 0 || (vitk_aligned(dout, 16) && vitk_aligned(ids, ids_are_64 ? 8 : 4))),
@@ -654,8 +658,8 @@ int vitk_embedding_bwd(const void* dout, int dout_type, int64_t ldd, const void*
     EmbBwdParams p = {};
     p.dout = dout; p.out = dtable; p.T = T; p.V = V; p.ldd = ldd; p.ldo = ldo; p.D = D; p.accumulate = accumulate; p.scale = scale;
     const int types = (dout_type << 1) | dtable_type;
-    if (T <= FEW_MAX) {
-        const int lanes = D > 256 ? 32 : emb_lanes(D), few_slices = (D / 8 + lanes - 1) / lanes;
+    if (emb_few(T, D)) {
+        const int lanes = emb_few_lanes(D), few_slices = emb_few_slices(D);
         const long long bytes = (long long)D * (dtable_type == 0 ? 4 : 2);
         const int zero_rows = (int)(bytes >= 65536 ? 1 : 65536 / bytes < FEW_ROWS ? 65536 / bytes : FEW_ROWS);
         const int zero_wgs = accumulate ? 0 : (int)((V + zero_rows - 1) / zero_rows < 1024 ? (V + zero_rows - 1) / zero_rows : 1024);
