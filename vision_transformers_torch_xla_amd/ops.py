@@ -515,12 +515,12 @@ _ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1}
 def _rows2d(t, name):
     """an fp32 / bf16 matrix with contiguous rows -> (type code, row stride)"""
     _here(t, name)
-    code = _ROW_TYPES.get(t.dtype)
+    code, shape, stride = _ROW_TYPES.get(t.dtype), t.shape, t.stride()
     if code is None:
         raise _lib.VitkError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise _lib.VitkError(f"{name}: expected a matrix with contiguous rows, got shape {tuple(t.shape)} with strides {t.stride()}")
-    return code, t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
+        raise _lib.VitkError(f"{name}: expected a matrix with contiguous rows, got shape {tuple(shape)} with strides {stride}")
+    return code, stride[0] if shape[0] > 1 else max(shape[1], 1)
 
 
 def _ids1d(ids):
@@ -536,11 +536,13 @@ def embedding_fwd(ids, table, scale=1.0, out_dtype=None):
     code, ldt = _rows2d(table, "table")
     V, D = table.shape
     flat = _ids1d(ids)
-    out_dtype = table.dtype if out_dtype is None else out_dtype
-    if out_dtype not in _ROW_TYPES:
+    if out_dtype is None or out_dtype == table.dtype:
+        ocode, out = code, table.new_empty((*ids.shape, D))
+    elif out_dtype in _ROW_TYPES:
+        ocode, out = _ROW_TYPES[out_dtype], table.new_empty((*ids.shape, D), dtype=out_dtype)
+    else:
         raise _lib.VitkError(f"embedding_fwd: out_dtype must be float32 or bfloat16, got {out_dtype}")
-    out = torch.empty((*ids.shape, D), dtype=out_dtype, device=table.device)
-    check(_lib.load().vitk_embedding_fwd(_ptr(flat), int(flat.dtype == torch.int64), _ptr(table), code, ldt, _ptr(out), _ROW_TYPES[out_dtype], D,
+    check(_lib.load().vitk_embedding_fwd(flat.data_ptr(), flat.dtype == torch.int64, table.data_ptr(), code, ldt, out.data_ptr(), ocode, D,
                                          flat.numel(), V, D, float(scale), _stream()), "embedding_fwd")
     return out
 
@@ -607,15 +609,14 @@ def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, 
     block_bytes: the rows are worked through in blocks that hold about this many bytes of probabilities (at least 256 rows); more than
     one block costs an fp32 copy of a bf16 dweight."""
     for t, n in ((x, "x"), (weight, "weight")):
-        _here(t, n)
-        if t.dtype != bf16 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-            raise _lib.VitkError(f"linear_xent: {n} must be a bf16 matrix with contiguous rows, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
-    T, D = x.shape
-    V = weight.shape[0]
-    if weight.shape[1] != D:
-        raise _lib.VitkError(f"linear_xent: x has {D} columns, weight {weight.shape[1]}")
+        if t.dtype != bf16 or t.dim() != 2:
+            raise _lib.VitkError(f"linear_xent: {n} must be a bf16 matrix, got {t.dtype} {tuple(t.shape)}")
+    ldx, ldw = _rows2d(x, "linear_xent: x")[1], _rows2d(weight, "linear_xent: weight")[1]
+    (T, D), (V, width) = x.shape, weight.shape
+    if width != D:
+        raise _lib.VitkError(f"linear_xent: x has {D} columns, weight {width}")
     _here(target, "target")
-    if target.dtype != torch.int64 or tuple(target.shape) != (T,):
+    if target.dtype != torch.int64 or target.shape != (T,):
         raise _lib.VitkError(f"linear_xent: target must be int64 [{T}], got {target.dtype} {tuple(target.shape)}")
     if int(block_bytes) <= 0:
         raise _lib.VitkError(f"linear_xent: block_bytes must be positive, got {block_bytes}")
@@ -626,7 +627,7 @@ def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, 
     btype = 0
     if bias is not None:
         _here(bias, "bias")
-        if bias.dtype not in _ROW_TYPES or tuple(bias.shape) != (V,):
+        if bias.dtype not in _ROW_TYPES or bias.shape != (V,):
             raise _lib.VitkError(f"linear_xent: bias must be float32 or bfloat16 [{V}], got {bias.dtype} {tuple(bias.shape)}")
         bias = bias.contiguous()
         btype = _ROW_TYPES[bias.dtype]
@@ -654,7 +655,7 @@ def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, 
     wf32, smooth = int(wtype == f32), float(smoothing)
     need = lib.vitk_linear_xent_workspace(T, V, D, int(any(t is not None for t in (dx, dw, db))), int(smooth > 0), wf32, int(db is not None), int(block_bytes))
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-    check(lib.vitk_linear_xent(_ptr(x), x.stride(0) if T > 1 else max(D, 1), _ptr(weight), weight.stride(0) if V > 1 else max(D, 1), _ptr(bias), btype, _ptr(target),
+    check(lib.vitk_linear_xent(x.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(bias), btype, _ptr(target),
                                T, V, D, smooth, int(ignore_index), int(reduction == "mean"), _ptr(loss), _ptr(rows), _ptr(dx), D, _ptr(dw), D, wf32,
                                _ptr(db), int(db is not None and db.dtype == f32), _ptr(ws), ws.numel(), int(block_bytes), _stream()), "linear_xent")
     return LinearXent(loss, rows, dx, dw, db)
