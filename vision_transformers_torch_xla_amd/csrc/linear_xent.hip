@@ -393,6 +393,8 @@ static __device__ __forceinline__ void lx_flip(unsigned& at) { asm volatile("v_x
 // instructions apart because each keeps the path to LDS busy for 16 cycles and a wave that runs into another's waits (issued in a burst,
 // or at every third gap of half the step, they cost a step 1000 cycles of 2060), and the step's own bookkeeping - addresses, buffer
 // change - in the same gaps.
+// Power is the limit behind that: 32 x 32 x 16 instructions take the same cycles at a 10 % lower clock (2260 -> 2480 us), and every second row of the
+// 8 x 8 runs backwards, so that an operand stays from row to row (0.4 %).
 // Operands whose rows run along the output (x, W, and dz for dW) sit in LDS as [64][256] and are read with the transposing ds_read_b64_tr_b16:
 // no transposed copy is made; dz for dx as [256][64] with ds_read_b128.
 //   8192 x 100003 x 2048: dz W 2520 -> 2180 us, dz^T x 2500 -> 2330 us (matrix pipe 81 % and 79 % busy at 1.8 and 1.7 GHz; a library product of the same sizes and
@@ -551,13 +553,13 @@ __global__ __launch_bounds__(256, 1) void lx_grad_kernel(const LxGemmParams p) {
         constexpr int ks = decltype(kt)::value, t = decltype(tt)::value;
         f = lx_join(lx_lds_tr(atB[t] + ks * 16384), lx_lds_tr(atB[t] + ks * 16384 + 2048));
     };
-    // A phase: the 64 matrix instructions of a k half, one by one in this order; between them the reads of the next phase's fragments (B's
+    // A phase: the 64 matrix instructions of a k half, one by one; between them the reads of the next phase's fragments (B's
     // first, which its first eight instructions need), the requests, and in phase 0 behind the reads the step to the other buffer.
     auto phase = [&](const bf16x8 (&fa)[8], const bf16x8 (&fb)[8], bf16x8 (&ga)[8], bf16x8 (&gb)[8], unsigned at, auto pt) __attribute__((always_inline)) {
         constexpr int ph = decltype(pt)::value, Q = ph == 0 ? Q0 : Q1;
         bf16x4 lo;
         lx_static_for<0, 64>([&](auto gt) __attribute__((always_inline)) {
-            constexpr int g = decltype(gt)::value, tm = g >> 3, tn = g & 7;
+            constexpr int g = decltype(gt)::value, tm = g >> 3, tn = (tm & 1) ? 7 - (g & 7) : g & 7;
             lx_mfma(acc[tm][tn], fb[tn], fa[tm]);
             LX_PIN();
             // three gaps: half a [64][256] fragment each in the first two, a request in the third
