@@ -66,14 +66,98 @@ static __device__ __forceinline__ unsigned lx_pack_h(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector(v, f16x2));
 }
 
+// v combined over the four lanes that share a row (lane ^ 16, lane ^ 32), by the lane swaps of the vector unit: no trip through LDS
+template <class F>
+static __device__ __forceinline__ float lx_over_row(float v, F&& f) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // The loss's epilogue of a wave that holds FM * 16 rows (from m0) by 64 columns (from n0) of logits: lane (lr, lg) has columns 16 tn + 4 lg + j
 // of row 16 tm + lr.  stg: 2 KB of LDS of the wave's own, through which P leaves in rows of 64 columns so that a store covers whole lines.
-// EXTRA: with a bias or the sums of the logits.
+// EXTRA: with a bias or the sums of the logits.  WANT_P, FULL (every row is one of the matrix): so that the code of the rows has no branch and the
+// rows' chains of maximum, exponentials and sum overlap (with a branch per row and the sums through LDS: 2804 instead of 2750 us at 8192 x 100003 x
+// 2048, 174 instead of 167 at 2047 x 50021 x 1024).
+template <int FM, bool EXTRA, bool WANT_P, bool FULL>
+static __device__ __forceinline__ void lx_loss_rows(const LxGemmParams& p, f32x4 (&acc)[FM][4], int m0, int n0, bf16_t* stg) {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));          // what is derived from it is not to be kept in registers over the main loop
+    const int lr = lane & 15, lg = lane >> 4, srow = lane >> 3;
+    const int room = p.N - n0 - 4 * lg;              // the lane's columns with 16 tn + j < room are columns of the vocabulary
+    float mxs[FM], sums[FM], zsums[FM];
+#pragma unroll
+    for (int tm = 0; tm < FM; ++tm) {
+        float z[4][4], mx = acc[tm][0][0];
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mx = fmaxf(mx, acc[tm][tn][j]);
+        if constexpr (EXTRA) {
+            float q[4];
+#pragma unroll
+            for (int tn = 0; tn < 4; ++tn) {
+                float v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = tn * 16 + j < room ? acc[tm][tn][j] : 0.f;
+                q[tn] = (v[0] + v[1]) + (v[2] + v[3]);
+            }
+            zsums[tm] = lx_over_row((q[0] + q[1]) + (q[2] + q[3]), [](float a, float b) { return a + b; });
+        }
+        mx = lx_over_row(mx, [](float a, float b) { return fmaxf(a, b); });
+        // From here on in powers of two, relative to m = max * log2(e) as rounded: z * log2(e) - m is one fma, exact up to its own rounding
+        mx *= 1.44269504088896340736f;
+        const float ref = mx == -INFINITY ? 0.f : mx;        // a row of -inf only: 2^(-inf - 0) = 0
+        float q[4];
+#pragma unroll
+        for (int tn = 0; tn < 4; ++tn) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[tn][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][j], 1.44269504088896340736f, -ref));
+            q[tn] = (z[tn][0] + z[tn][1]) + (z[tn][2] + z[tn][3]);
+        }
+        mxs[tm] = mx;
+        sums[tm] = lx_over_row((q[0] + q[1]) + (q[2] + q[3]), [](float a, float b) { return a + b; });
+        if constexpr (WANT_P) {
+#pragma unroll
+            for (int tn = 0; tn < 4; ++tn) {
+                uint2 w;
+                w.x = lx_pack_h(z[tn][0], z[tn][1]);
+                w.y = lx_pack_h(z[tn][2], z[tn][3]);
+                *reinterpret_cast<uint2*>(stg + lr * 64 + (((tn * 2 + (lg >> 1)) ^ (lr & 7)) << 3) + (lg & 1) * 4) = w;
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = half * 8 + srow;
+                const u32x4 o = *reinterpret_cast<const u32x4*>(stg + r * 64 + (((lane & 7) ^ srow) << 3));
+                const int mr = m0 + tm * 16 + r;
+                if (FULL || mr < p.M) __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(p.P + (size_t)mr * p.ldp + n0 + (lane & 7) * 8));
+            }
+        }
+    }
+    // lane group lg stores the statistics of the rows of tm = lg, lg + 4
+#pragma unroll
+    for (int h = 0; h < (FM + 3) / 4; ++h) {
+        float mx = mxs[4 * h], sum = sums[4 * h], zsum = EXTRA ? zsums[4 * h] : 0.f;
+#pragma unroll
+        for (int k = 1; k < 4 && 4 * h + k < FM; ++k) {
+            mx = lg == k ? mxs[4 * h + k] : mx;
+            sum = lg == k ? sums[4 * h + k] : sum;
+            if constexpr (EXTRA) zsum = lg == k ? zsums[4 * h + k] : zsum;
+        }
+        const int m = m0 + (4 * h + lg) * 16 + lr;
+        if (4 * h + lg < FM && (FULL || m < p.M)) {
+            const size_t at = (size_t)m * p.stat_cols + (n0 >> 6);
+            p.stats[at] = make_float2(mx, sum);
+            if (EXTRA && p.zsum != nullptr) p.zsum[at] = zsum;
+        }
+    }
+}
 template <int FM, bool EXTRA>
 static __device__ __forceinline__ void lx_loss_epilogue(const LxGemmParams& p, f32x4 (&acc)[FM][4], int m0, int n0, bf16_t* stg) {
-    const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4, srow = lane >> 3;
-    const int first = n0 + 4 * lg;                   // the lane's columns are first + 16 tn + j
-    const int room = p.N - first;                    // those with 16 tn + j < room are columns of the vocabulary
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int first = n0 + 4 * (lane >> 4), room = p.N - first;
     if constexpr (EXTRA) {
         if (p.bias != nullptr) {
 #pragma unroll
@@ -96,56 +180,13 @@ static __device__ __forceinline__ void lx_loss_epilogue(const LxGemmParams& p, f
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[tm][tn][j] = tn * 16 + j < room ? acc[tm][tn][j] : -INFINITY;
     }
-    const int sc = n0 >> 6;
-#pragma unroll
-    for (int tm = 0; tm < FM; ++tm) {
-        const int m = m0 + tm * 16 + lr;
-        float z[4][4], mx = -INFINITY, zs = 0.f;
-#pragma unroll
-        for (int tn = 0; tn < 4; ++tn)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                z[tn][j] = acc[tm][tn][j];
-                mx = fmaxf(mx, z[tn][j]);
-                if constexpr (EXTRA) zs += tn * 16 + j < room ? z[tn][j] : 0.f;
-            }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        // From here on in powers of two, relative to m = max * log2(e) as rounded: z * log2(e) - m is one fma, exact up to its own rounding
-        mx *= 1.44269504088896340736f;
-        const float ref = mx == -INFINITY ? 0.f : mx;        // a row of -inf only: 2^(-inf - 0) = 0
-        float s = 0.f;
-#pragma unroll
-        for (int tn = 0; tn < 4; ++tn)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                z[tn][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[tn][j], 1.44269504088896340736f, -ref));
-                s += z[tn][j];
-            }
-        s += __shfl_xor(s, 16, 64);
-        s += __shfl_xor(s, 32, 64);
-        if (lg == 0 && m < p.M) p.stats[(size_t)m * p.stat_cols + sc] = make_float2(mx, s);
-        if (EXTRA && p.zsum != nullptr) {
-            zs += __shfl_xor(zs, 16, 64);
-            zs += __shfl_xor(zs, 32, 64);
-            if (lg == 0 && m < p.M) p.zsum[(size_t)m * p.stat_cols + sc] = zs;
-        }
-        if (p.P != nullptr) {
-#pragma unroll
-            for (int tn = 0; tn < 4; ++tn) {
-                uint2 w;
-                w.x = lx_pack_h(z[tn][0], z[tn][1]);
-                w.y = lx_pack_h(z[tn][2], z[tn][3]);
-                *reinterpret_cast<uint2*>(stg + lr * 64 + (((tn * 2 + (lg >> 1)) ^ (lr & 7)) << 3) + (lg & 1) * 4) = w;
-            }
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int r = half * 8 + srow;
-                const u32x4 o = *reinterpret_cast<const u32x4*>(stg + r * 64 + (((lane & 7) ^ srow) << 3));
-                const int mr = m0 + tm * 16 + r;
-                if (mr < p.M) __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(p.P + (size_t)mr * p.ldp + n0 + (lane & 7) * 8));
-            }
-        }
+    const bool full = m0 + FM * 16 <= p.M;
+    if (p.P != nullptr) {
+        if (full) lx_loss_rows<FM, EXTRA, true, true>(p, acc, m0, n0, stg);
+        else lx_loss_rows<FM, EXTRA, true, false>(p, acc, m0, n0, stg);
+    } else {
+        if (full) lx_loss_rows<FM, EXTRA, false, true>(p, acc, m0, n0, stg);
+        else lx_loss_rows<FM, EXTRA, false, false>(p, acc, m0, n0, stg);
     }
 }
 
