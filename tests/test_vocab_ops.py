@@ -743,6 +743,30 @@ def test_linear_xent_some_of_the_gradients(device, T, V, D, block_bytes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [300, 1024, 1025, 5000])
+@pytest.mark.parametrize("V", [40, 1000, 3001])
+def test_linear_xent_bias_gradient_keeps_the_hits(device, T, V):
+    """1 - smoothing is no bf16 number: a hit must not be off by its rounding in the same direction every time"""
+    ops = _ops()
+    g = torch.Generator().manual_seed(T + V)
+    x, w = (torch.randn(T, 64, generator=g) * 0.05).to(bf16), (torch.randn(V, 64, generator=g) * 0.05).to(bf16)
+    target = torch.randint(0, 8, (T,), generator=g) * (V // 8)
+    target[::7] = -100
+    bias = torch.zeros(V)
+    for reduction in ("sum", "mean"):
+        r = ops.linear_xent(x.to(device), w.to(device), target.to(device), bias.to(device), smoothing=0.1, reduction=reduction, grads=("bias",))
+        (_, _, _, _, db), _ = plain_linear_xent(x, w, target, bias, 0.1, -100, reduction == "mean")
+        counted = target != -100
+        p = torch.softmax(x[counted].double() @ w.double().t(), 1)
+        n = int(counted.sum())
+        # fp16 and bf16 roundings of what is not a hit, of the size of p; the sums
+        tol = 1.01 * (2.0 ** -9 + 2.0 ** -8) * (p + 0.1 / V).sum(0) + n * 2.0 ** -24 + (n + 4) * U32 * (p.sum(0) + torch.bincount(target[counted], minlength=V))
+        assert torch.all((r.dbias.cpu().double() - db).abs() <= tol * (1.0 / n if reduction == "mean" else 1.0))
+        hit = db[target[counted][0]].abs()
+        assert (tol * (1.0 / n if reduction == "mean" else 1.0)).min() < 0.0017 * hit or V == 40        # it would see 0.9 rounded to bf16
+
+
+@pytest.mark.gpu
 def test_linear_xent_refuses(device):
     ops, err = _ops(), _error()
     x, w, t = torch.randn(6, 16, device=device).to(bf16), torch.randn(9, 16, device=device).to(bf16), torch.zeros(6, dtype=torch.int64, device=device)

@@ -11,7 +11,7 @@
 //   2. one workgroup per row (lx_row_kernel): lse from the table, the target's logit as a dot product of its own, the row's loss, and
 //      P -> dz in place, now bf16: the one rounding of the gradient's factor.  g is not in it: a constant such as 1 / count would be
 //      rounded 1 part in 256 in the same direction everywhere; it multiplies the fp32 sums of the next step.
-//   3. dx = dz W and dW = dz^T x (lx_grad_kernel), and the column sums for db.
+//   3. dx = dz W and dW = dz^T x (lx_grad_kernel), and the column sums for db, to which each target's dz adds what its rounding took.
 // 6 T V D floating-point operations: nothing is computed twice.  Keeping one 16-bit factor per logit of a block costs 4 bytes of
 // traffic per logit for step 2, where computing the logits again for the gradients would cost 2 D operations.
 #include "common.h"
@@ -730,6 +730,7 @@ struct LxRowParams {
     unsigned* ticket; float* scale; float* loss; int mean;      // loss not null: the last row to finish adds the rows up (see lx_loss_kernel)
     bf16_t* P; long long ldp;          // fp16 on entry, bf16 dz on exit; null: loss alone
     float* rows;
+    float* delta;                      // what the target's dz lost to bf16, per row (0 where it is ignored); null: no db
     int V, D, rows_n, pad_rows;         // pad_rows rows of zeros behind the last (lx_grad_kernel reads steps of 64 of them)
     float smoothing;
 };
@@ -834,7 +835,10 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
     if (pad || t64 == p.ignore_index) {
         if (P != nullptr)
             for (int c = tid; c < chunks; c += NT) __builtin_nontemporal_store((u32x4){0u, 0u, 0u, 0u}, reinterpret_cast<u32x4*>(P) + c);
-        if (!pad) lx_row_done(p, row, tid, 0.f);
+        if (!pad) {
+            if (p.delta != nullptr && tid == 0) p.delta[row] = 0.f;
+            lx_row_done(p, row, tid, 0.f);
+        }
         return;
     }
     // a label outside [0, V) never becomes an address: the row's loss and gradient are NaN
@@ -889,7 +893,17 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
         for (int j = 0; j < LX_AHEAD; ++j) {
             const int c = c0 + j * NT;
             if (c < chunks) {
-                const u32x4 o = lx_dz8(r[j], __builtin_amdgcn_exp2f(m[j] - lse2), u, hit, c * 8, t, p.V, valid);
+                const float f = __builtin_amdgcn_exp2f(m[j] - lse2);
+                const u32x4 o = lx_dz8(r[j], f, u, hit, c * 8, t, p.V, valid);
+                if (p.delta != nullptr && c == (t >> 3)) {
+                    const int shift = (t & 1) * 16;
+                    unsigned in = 0, out = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (k == ((t & 7) >> 1)) { in = r[j][k]; out = o[k]; }
+                    const float v = __builtin_fmaf((float)__builtin_bit_cast(_Float16, (unsigned short)(in >> shift)), f, -u) - hit;
+                    p.delta[row] = valid ? v - bf2f((unsigned short)(out >> shift)) : 0.f;
+                }
                 if (STREAM) __builtin_nontemporal_store(o, q + c);
                 else q[c] = o;
             }
@@ -1125,19 +1139,43 @@ __global__ __launch_bounds__(256) void lx_small_kernel(const LxGemmParams p) {
     if (EPI != LX_OUT && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0u;
     lx_small_body<LAY, EPI, FM, WM, WN>(p, sm, blockIdx.x, gridDim.x);
 }
+// Rows first, first + STEP, ... < end of dz, 8 columns, for db, with what the targets' dz lost to bf16: without that every hit of 1 - smoothing is off in
+// the same direction (0.9 by 0.17 %).  Eight rows are in flight; the targets, which are rare, are looked at behind them.
+template <int STEP>
+static __device__ __forceinline__ void lx_colsum_rows(float (&acc)[8], const bf16_t* dz, long long ldp, long long col, const long long* target, const float* delta,
+                                                      int first, int end) {
+    for (int r0 = first; r0 < end; r0 += 8 * STEP) {
+        float v[8][8], d[8];
+        int t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int r = r0 + j * STEP < end ? r0 + j * STEP : r0;
+            load8(dz + (size_t)r * ldp + col, v[j]);
+            const long long c = target[r] - col;
+            t[j] = c >= 0 && c < 8 && r0 + j * STEP < end ? (int)c : 8;
+            d[j] = delta[r];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool in = r0 + j * STEP < end;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] += in ? v[j][k] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (t[j] < 8) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) acc[k] += t[j] == k ? d[j] : 0.f;
+            }
+    }
+}
 // db of up to 1024 rows: a workgroup sums 128 columns, 16 rows at a time
-struct LxColsum { const bf16_t* dz; long long ldp; int T, V; const float* scale; void* db; int db_f32; };
+struct LxColsum { const bf16_t* dz; long long ldp; int T, V; const float* scale; void* db; int db_f32; const long long* target; const float* delta; };
 static __device__ __forceinline__ void lx_colsum_few(const LxColsum& c, float (*sh)[128], int block) {
     const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
     const long long col = (long long)block * 128 + lane * 8;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int r = group; r < c.T; r += 16) {
-        float v[8];
-        load8(c.dz + (size_t)r * c.ldp + col, v);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] += v[k];
-    }
+    lx_colsum_rows<16>(acc, c.dz, c.ldp, col, c.target, c.delta, group, c.T);
 #pragma unroll
     for (int k = 0; k < 8; ++k) sh[group][lane * 8 + k] = acc[k];
     __syncthreads();
@@ -1232,21 +1270,14 @@ __global__ __launch_bounds__(256) void lx_join_kernel(const LxGemmParams p) {
 }
 
 // db: column sums of dz.  A block sums 512 columns over a range of rows into partial[range][ldp]; the second kernel adds the ranges in order.
-__global__ __launch_bounds__(256) void lx_colsum_kernel(const bf16_t* __restrict__ dz, long long ldp, int T, int rows_per_range, float* __restrict__ partial) {
+__global__ __launch_bounds__(256) void lx_colsum_kernel(const bf16_t* __restrict__ dz, long long ldp, int T, int rows_per_range, float* __restrict__ partial,
+                                                        const long long* __restrict__ target, const float* __restrict__ delta) {
     __shared__ float sh[4][512];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long col = (long long)blockIdx.x * 512 + lane * 8;
     const int r0 = blockIdx.y * rows_per_range, r1 = r0 + rows_per_range < T ? r0 + rows_per_range : T;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (col < ldp) {
-#pragma unroll 4
-        for (int r = r0 + wave; r < r1; r += 4) {
-            float v[8];
-            load8(dz + (size_t)r * ldp + col, v);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) acc[k] += v[k];
-        }
-    }
+    if (col < ldp) lx_colsum_rows<4>(acc, dz, ldp, col, target, delta, r0 + wave, r1);
 #pragma unroll
     for (int k = 0; k < 8; ++k) sh[wave][lane * 8 + k] = acc[k];
     __syncthreads();
@@ -1260,6 +1291,7 @@ __global__ __launch_bounds__(256) void lx_colsum_final_kernel(const float* __res
     const int n = blockIdx.x * 256 + threadIdx.x;
     if (n >= V) return;
     float s = first ? 0.f : sum[n];
+#pragma unroll 16
     for (int r = 0; r < ranges; ++r) s += partial[(size_t)r * ldp + n];
     if (db == nullptr) { sum[n] = s; return; }
     s *= scale[0];
@@ -1268,7 +1300,6 @@ __global__ __launch_bounds__(256) void lx_colsum_final_kernel(const float* __res
 }
 
 // ---------------------------------------------------------------------------------------------------- host
-#define LX_RANGES 64
 // the rows' kernel adds the losses up itself for up to 512 rows, unless it rewrites more than 1 MB of P (each row's ticket waits for the
 // stores before it to reach memory)
 #define LX_FUSED_ROWS 512
@@ -1286,6 +1317,8 @@ static int lx_cus() {
     }
     return cache[dev];
 }
+// ranges of rows that the column sums are cut into: more where there are few columns (25088 x 1000: 64 of them 23 + 4 us, 128 15 + 5)
+static int lx_ranges(long long ldp) { return ldp <= 2048 ? 128 : 64; }
 static size_t lx_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // How the tiles of dx and dW are dealt.  `width` column tiles side by side form a row, worked on by a team of as many workgroups in step, so
@@ -1300,7 +1333,7 @@ struct LxPlan {
     long long ldp, stat_cols;
     int block, blocks;              // rows per block, blocks
     LxDeal dx[2], dw[2];            // of a block, of the last one
-    size_t scale, stats, zsum, P, acc, slab, colpart, colsum, total;
+    size_t scale, stats, zsum, P, acc, slab, colpart, colsum, delta, total;
 };
 // The kernel and its cut that a model of the time finds fastest, in microseconds on 256 compute units, from 28 shapes between 1 x 1000 x 192 and
 // 512 x 100003 x 1024 measured with each of the three kernels (time of x W^T / dz W / dz^T x in us, large : 128 : 64):
@@ -1439,8 +1472,9 @@ static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw
         }
         if (slab > 0) q.slab = take(slab * sizeof(float));
         if (bias) {
-            q.colpart = take((size_t)LX_RANGES * q.ldp * sizeof(float));
+            q.colpart = take((size_t)lx_ranges(q.ldp) * q.ldp * sizeof(float));
             q.colsum = take((size_t)V * sizeof(float));
+            q.delta = take((size_t)rows * sizeof(float));
         }
     }
     q.total = at;
@@ -1555,6 +1589,7 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         r.ticket = ticket; r.scale = scale; r.loss = fused ? loss : nullptr; r.mean = mean;
         r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.rows_n = n; r.smoothing = smoothing;
         r.pad_rows = dw && q.dw[last].kind == LX_BIG ? (LX_BK - n % LX_BK) % LX_BK : 0;
+        r.delta = db ? (float*)(ws + q.delta) : nullptr;
         const int row_wgs = n + r.pad_rows;
         // long rows get more waves.  By the vocabulary alone, so that a row's sums do not depend on how many rows there are or what is wanted.
         // STREAM: past the caches, where the block is larger than they are.
@@ -1594,7 +1629,7 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         e.add = b > 0 ? acc : nullptr;
         if (last) { e.out = dw; e.ldo = lddw; e.out_f32 = dw_f32; }
         else { e.out = acc; e.ldo = D; e.out_f32 = 1; }
-        const LxColsum c = {dz, q.ldp, n, V, scale, db, db_f32};
+        const LxColsum c = {dz, q.ldp, n, V, scale, db, db_f32, r.target, r.delta};
         const bool few = db != nullptr && q.blocks == 1 && n <= 1024;
         const LxDeal& dd = q.dx[last];
         const LxDeal& de = q.dw[last];
@@ -1623,10 +1658,10 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
             if (int rc = vitk_check_launch("linear_xent_db")) return rc;
         } else if (db != nullptr) {
             float* part = (float*)(ws + q.colpart);
-            int per = (n + LX_RANGES - 1) / LX_RANGES;
+            int per = (n + lx_ranges(q.ldp) - 1) / lx_ranges(q.ldp);
             if (per < 32) per = 32;
             const int ranges = (n + per - 1) / per;
-            lx_colsum_kernel<<<dim3((unsigned)((q.ldp + 511) / 512), ranges), 256, 0, s>>>(dz, q.ldp, n, per, part);
+            lx_colsum_kernel<<<dim3((unsigned)((q.ldp + 511) / 512), ranges), 256, 0, s>>>(dz, q.ldp, n, per, part, r.target, r.delta);
             lx_colsum_final_kernel<<<(V + 255) / 256, 256, 0, s>>>(part, q.ldp, ranges, V, scale, (float*)(ws + q.colsum), b == 0, last ? db : nullptr, db_f32);
             if (int rc = vitk_check_launch("linear_xent_db")) return rc;
         }
