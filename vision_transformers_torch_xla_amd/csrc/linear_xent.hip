@@ -34,7 +34,7 @@ struct LxGemmParams {
     const bf16_t* A; const bf16_t* B;       // NT: A [M][KA], B [N][KB];  NN: B [KB][N];  TN: A [KA][M], B [KB][N]
     int lda, ldb;
     int M, N;
-    int KA, KB;             // valid extent of the contraction in each operand; behind it zeros are read
+    int KA, KB;             // valid extent of the contraction in each operand; behind it zeros are read (lx_grad_kernel: A holds them)
     int steps;              // 64-deep steps over the whole contraction
     int tiles_m, tiles_n;
     // work, LX_XENT*: workgroup g of G takes the tiles g, g + G, ... (in bands of 8 column tiles)
