@@ -593,6 +593,53 @@ def test_linear_xent_extreme_logits(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D", [(300, 200, 64), (1680, 21915, 72)])                   # logits by the small and by the large kernel
+def test_linear_xent_gradient_of_classes_far_below_a_neighbour(device, T, V, D):
+    """every class has a row of dweight and an entry of dbias of its own, in which no larger class stands beside it: a probability is held to so many
+    bits of ITSELF, 40 powers of e below the largest of its neighbours too"""
+    ops = _ops()
+    g = torch.Generator().manual_seed(T)
+    x, w = (torch.randn(T, D, generator=g) * 0.3).to(bf16).to(device), (torch.randn(V, D, generator=g) * 0.3).to(bf16).to(device)
+    target = (torch.randint(64, V, (T,), generator=g)).to(device)                        # never one of the first 64 classes
+    bias = torch.randn(V, generator=g)
+    bias[0], bias[1:64] = 8.0, 8.0 - torch.linspace(2.0, 40.0, 63)
+    bias = bias.to(device)
+    r = ops.linear_xent(x, w, target, bias, reduction="sum", dweight_dtype=f32)
+    z = x.double() @ w.double().t() + bias.double()
+    lse = torch.logsumexp(z, 1)
+    p = (z[:, :64] - lse[:, None]).exp()
+    # as in plain_linear_xent, without anything that does not shrink with p
+    zerr = ((D + 2) * U32 * (x.double().abs() @ w.double().abs().t() + bias.double().abs())).max()
+    perr = 2 * zerr + (V / 64 + 200) * U32 * (1 + lse.abs().max())
+    E = p * (2.0 ** -11 + 2.0 ** -8 + perr + (T + 4) * U32) * 1.01
+    assert torch.all((r.dweight[:64].double() - p.t() @ x.double()).abs() <= E.t() @ x.double().abs())
+    assert torch.all((r.dbias[:64].double() - p.sum(0)).abs() <= E.sum(0))
+    assert float(p.sum(0)[63] / p.sum(0)[0]) < 1e-16 and torch.all(r.dbias[:64] > 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [2.0 ** 9, 2.0 ** 12, 2.0 ** 15])
+def test_linear_xent_of_logits_of_millions(device, scale):
+    """one class has everything, however large the logits: whole numbers here, so that fp32 holds them exactly"""
+    ops = _ops()
+    g = torch.Generator().manual_seed(3)
+    x, w = torch.randint(-8, 9, (90, 64), generator=g).to(bf16), torch.randint(-8, 9, (300, 64), generator=g).to(bf16)
+    x, w = (x * scale).to(device), (w * scale).to(device)                                # logits in units of scale^2 = 2^18 .. 2^30
+    z = x.double() @ w.double().t()
+    first, second = z.topk(2, 1).values.unbind(1)
+    x, z = x[first > second], z[first > second]                                          # without ties
+    assert len(x) > 60 and z.abs().max() < 2.0 ** 24 * scale ** 2
+    target = z.argmax(1)
+    target[::2] = 7
+    r = ops.linear_xent(x, w, target, dweight_dtype=f32, reduction="sum")
+    want = z.max(1).values - z.gather(1, target[:, None])[:, 0]
+    assert torch.all((r.rows.double() - want).abs() <= 8 * U32 * z.abs().max())
+    dz = torch.nn.functional.one_hot(z.argmax(1), 300).double() - torch.nn.functional.one_hot(target, 300).double()
+    assert torch.equal(r.dweight.double(), dz.t() @ x.double())
+    assert torch.equal(r.dx.double(), (dz @ w.double()).to(bf16).double())
+
+
+@pytest.mark.gpu
 def test_linear_xent_gradient_against_differences(device):
     ops = _ops()
     g = torch.Generator().manual_seed(9)

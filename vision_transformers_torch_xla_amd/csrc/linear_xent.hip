@@ -5,9 +5,10 @@
 //
 // x bf16 [T, D], W bf16 [V, D].  The rows are worked through in blocks whose size the workspace bounds; per block
 //   1. x W^T tile by tile (lx_logits_kernel).  The epilogue takes a tile's logits in fp32 from the accumulators: per row and 64
-//      columns their maximum m and s = sum exp(z - m) go to a small table (in powers of two); exp(z - m) itself, in [0, 1], goes to the block's
-//      matrix P in fp16 (11 bits; bf16 would round it 8 times as far; what falls below fp16's 6e-8 of its maximum is below what the
-//      later bf16 rounding of its larger neighbours leaves).  Loss alone: only the table is written.
+//      columns their maximum m and s = sum exp(z - m) go to a small table; exp(z - m) itself, in [0, 1], goes to the block's
+//      matrix P in 16 bits of its own: no sign, 6 bits of exponent, 10 of fraction, from 1 down to 2^-62 (lx_pack_p).  fp16 has the same 11 bits
+//      but ends at 6e-8 of the piece's maximum, and a class that stays 18 powers of e below a neighbour would lose its row of dW and its
+//      db, which have no larger neighbour in their sums; bf16 would round 8 times as far.  Loss alone: only the table is written.
 //   2. one workgroup per row (lx_row_kernel): lse from the table, the target's logit as a dot product of its own, the row's loss, and
 //      P -> dz in place, now bf16: the one rounding of the gradient's factor.  g is not in it: a constant such as 1 / count would be
 //      rounded 1 part in 256 in the same direction everywhere; it multiplies the fp32 sums of the next step.
@@ -48,9 +49,9 @@ struct LxGemmParams {
     float* slab;
     // LX_XENT
     const void* bias; int bias_type;        // 0 fp32, 1 bf16, null: none
-    float2* stats; int stat_cols;           // [M][stat_cols]: (m log2 e, s) of 64 columns
+    float2* stats; int stat_cols;           // [M][stat_cols]: (m, s) of 64 columns
     float* zsum;                            // [M][stat_cols] sums of the logits, null: not wanted (no smoothing)
-    _Float16* P; long long ldp;             // null: loss alone
+    unsigned short* P; long long ldp;       // (lx_pack_p) null: loss alone
     unsigned* ticket;                       // zeroed here for the kernels that follow
 };
 
@@ -60,11 +61,15 @@ static __device__ __forceinline__ bf16x8 lx_tr(const bf16_t* lo, const bf16_t* h
     const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)hi);
     return (bf16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
-typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
-static __device__ __forceinline__ unsigned lx_pack_h(float a, float b) {
-    const f32x2_t v = {a, b};
-    return __builtin_bit_cast(unsigned, __builtin_convertvector(v, f16x2));
+// P's numbers.  The epilogue forms 2^(z - m - 64), whose fp32 exponent field ends at 63 (6 bits); 10 bits of the fraction are kept, to nearest.  Read
+// back, the 16 bits in place are that number again (its subnormals too: exponent field 0), and 2^64 goes into the factor it is multiplied with.
+// Two of them to a word take three instructions, as fp16's conversion does.
+#define LX_P_SCALE 64
+static __device__ __forceinline__ unsigned lx_pack_p(float a, float b) {
+    const unsigned x = (__float_as_uint(a) + 0x1000u) << 3, y = (__float_as_uint(b) + 0x1000u) << 3;
+    return __builtin_amdgcn_perm(y, x, 0x07060302u);        // the upper halves of both
 }
+static __device__ __forceinline__ float lx_unpack_p(unsigned v) { return __uint_as_float(v << 13); }
 
 // v combined over the four lanes that share a row (lane ^ 16, lane ^ 32), by the lane swaps of the vector unit: no trip through LDS
 template <class F>
@@ -106,24 +111,24 @@ static __device__ __forceinline__ void lx_loss_rows(const LxGemmParams& p, f32x4
             zsums[tm] = lx_over_row((q[0] + q[1]) + (q[2] + q[3]), [](float a, float b) { return a + b; });
         }
         mx = lx_over_row(mx, [](float a, float b) { return fmaxf(a, b); });
-        // From here on in powers of two, relative to m = max * log2(e) as rounded: z * log2(e) - m is one fma, exact up to its own rounding
-        mx *= 1.44269504088896340736f;
-        const float ref = mx == -INFINITY ? 0.f : mx;        // a row of -inf only: 2^(-inf - 0) = 0
+        // The maximum is taken off before the product with log2(e), so that the largest gives 1 exactly however large the logits are.  (With
+        // z * log2(e) - fl(m * log2(e)) as one fma a logit saves an instruction, but from logits of 10^7 on the product's rounding is whole powers of two.)
+        const float off = mx == -INFINITY ? 0.f : mx;         // a row of -inf only: 2^(-inf) = 0
         float q[4];
 #pragma unroll
         for (int tn = 0; tn < 4; ++tn) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) z[tn][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][j], 1.44269504088896340736f, -ref));
+            for (int j = 0; j < 4; ++j) z[tn][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][j] - off, 1.44269504088896340736f, -(float)LX_P_SCALE));
             q[tn] = (z[tn][0] + z[tn][1]) + (z[tn][2] + z[tn][3]);
         }
         mxs[tm] = mx;
-        sums[tm] = lx_over_row((q[0] + q[1]) + (q[2] + q[3]), [](float a, float b) { return a + b; });
+        sums[tm] = lx_over_row((q[0] + q[1]) + (q[2] + q[3]), [](float a, float b) { return a + b; }) * 0x1p+64f;
         if constexpr (WANT_P) {
 #pragma unroll
             for (int tn = 0; tn < 4; ++tn) {
                 uint2 w;
-                w.x = lx_pack_h(z[tn][0], z[tn][1]);
-                w.y = lx_pack_h(z[tn][2], z[tn][3]);
+                w.x = lx_pack_p(z[tn][0], z[tn][1]);
+                w.y = lx_pack_p(z[tn][2], z[tn][3]);
                 *reinterpret_cast<uint2*>(stg + lr * 64 + (((tn * 2 + (lg >> 1)) ^ (lr & 7)) << 3) + (lg & 1) * 4) = w;
             }
 #pragma unroll
@@ -728,7 +733,7 @@ struct LxRowParams {
     const long long* target; long long ignore_index;
     const float2* stats; const float* zsum; int stat_cols;
     unsigned* ticket; float* scale; float* loss; int mean;      // loss not null: the last row to finish adds the rows up (see lx_loss_kernel)
-    bf16_t* P; long long ldp;          // fp16 on entry, bf16 dz on exit; null: loss alone
+    bf16_t* P; long long ldp;          // P on entry (lx_pack_p), bf16 dz on exit; null: loss alone
     float* rows;
     float* delta;                      // what the target's dz lost to bf16, per row (0 where it is ignored); null: no db
     int V, D, rows_n, pad_rows;         // pad_rows rows of zeros behind the last (lx_grad_kernel reads steps of 64 of them)
@@ -760,15 +765,17 @@ static __device__ __forceinline__ float lx_block_sum(float v, float* sh) {
     return v;
 }
 
-// 8 columns of P -> dz
+// exp(m - mx) * 2^-s2 for a piece's maximum m <= the row's mx; infinite ones, and the lowest logits of a type, are equal to themselves
+static __device__ __forceinline__ float lx_below(float m, float mx, float s2 = 0.f) {
+    return __builtin_amdgcn_exp2f((m == mx ? 0.f : (m - mx) * 1.44269504088896340736f) - s2);
+}
+// 8 columns of P -> dz; f holds the 2^64 of lx_unpack_p
 static __device__ __forceinline__ u32x4 lx_dz8(const u32x4 r, float f, float u, float hit, int n, int t, int V, bool valid) {
     float v[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const unsigned word = r[k];         // (a bit cast of the vector's element itself reads element 0)
-        const f16x2 h = __builtin_bit_cast(f16x2, word);
-        v[2 * k] = __builtin_fmaf((float)h[0], f, -u);
-        v[2 * k + 1] = __builtin_fmaf((float)h[1], f, -u);
+        v[2 * k] = __builtin_fmaf(lx_unpack_p(r[k] & 0xffffu), f, -u);
+        v[2 * k + 1] = __builtin_fmaf(lx_unpack_p(r[k] >> 16), f, -u);
     }
     if ((t & ~7) == n) {
 #pragma unroll
@@ -861,19 +868,18 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
 #pragma unroll 4
     for (int c = tid; c < entries; c += NT) mx = fmaxf(mx, st[c].x);
     mx = lx_block_max<WAVES>(mx, sh);
-    const float ref = mx == -INFINITY ? 0.f : mx;
     float s = 0.f, zs = 0.f;
 #pragma unroll 4
     for (int c = tid; c < entries; c += NT) {
         const float2 v = st[c];
-        s += v.y * (v.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(v.x - ref));         // an all -inf entry has s = 0, or NaN where a logit was NaN
+        s += v.y * lx_below(v.x, mx);           // an all -inf entry has s = 0, or NaN where a logit was NaN
         if (p.smoothing > 0.f) zs += p.zsum[(size_t)row * p.stat_cols + c];
     }
     s = lx_block_sum<WAVES>(s, sh);
     dot = lx_block_sum<WAVES>(dot, sh);
     if (p.smoothing > 0.f) zs = lx_block_sum<WAVES>(zs, sh);
     if (p.bias != nullptr) dot += p.bias_type == 1 ? bf2f(reinterpret_cast<const bf16_t*>(p.bias)[t]) : reinterpret_cast<const float*>(p.bias)[t];
-    const float lse2 = ref + log2f(s), lse = lse2 * 0.69314718055994530942f;
+    const float s2 = log2f(s), lse = mx + s2 * 0.69314718055994530942f;
     float l = lse - dot;
     if (p.smoothing > 0.f) l = (1.f - p.smoothing) * l + p.smoothing * (lse - zs / (float)p.V);
     lx_row_done(p, row, tid, valid ? l : __builtin_nanf(""));
@@ -893,7 +899,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
         for (int j = 0; j < LX_AHEAD; ++j) {
             const int c = c0 + j * NT;
             if (c < chunks) {
-                const float f = __builtin_amdgcn_exp2f(m[j] - lse2);
+                const float f = lx_below(m[j], mx, s2) * 0x1p+64f;
                 const u32x4 o = lx_dz8(r[j], f, u, hit, c * 8, t, p.V, valid);
                 if (p.delta != nullptr && c == (t >> 3)) {
                     const int shift = (t & 1) * 16;
@@ -901,7 +907,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         if (k == ((t & 7) >> 1)) { in = r[j][k]; out = o[k]; }
-                    const float v = __builtin_fmaf((float)__builtin_bit_cast(_Float16, (unsigned short)(in >> shift)), f, -u) - hit;
+                    const float v = __builtin_fmaf(lx_unpack_p((in >> shift) & 0xffffu), f, -u) - hit;
                     p.delta[row] = valid ? v - bf2f((unsigned short)(out >> shift)) : 0.f;
                 }
                 if (STREAM) __builtin_nontemporal_store(o, q + c);
@@ -1563,7 +1569,7 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         g.M = n; g.N = V; g.KA = g.KB = D; g.steps = (D + LX_BK - 1) / LX_BK;
         g.bias = bias; g.bias_type = bias_type;
         g.stats = (float2*)(ws + q.stats); g.stat_cols = (int)q.stat_cols; g.zsum = smoothing > 0.f ? (float*)(ws + q.zsum) : nullptr;
-        g.P = grad ? (_Float16*)(ws + q.P) : nullptr; g.ldp = q.ldp; g.ticket = ticket;
+        g.P = grad ? (unsigned short*)(ws + q.P) : nullptr; g.ldp = q.ldp; g.ticket = ticket;
         const LxLogits deal = lx_deal_logits(n, V, g.steps, cus);
         auto logits = [&](LxGemmParams q, const LxDeal& how) {
             return q.bias || q.zsum ? lx_launch<LX_NT, LX_XENT_BIAS>(q, how, s, "linear_xent_logits") : lx_launch<LX_NT, LX_XENT>(q, how, s, "linear_xent_logits");
