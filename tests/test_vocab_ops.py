@@ -640,6 +640,51 @@ def test_linear_xent_of_logits_of_millions(device, scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("top", [65, 1000, 10000])
+def test_linear_xent_loss_of_certain_rows(device, top):
+    """the loss of a row does not know how large its logits are: log(1 + k e^-gap) to fp32's rounding of numbers near 1"""
+    ops = _ops()
+    V, D = 700, 64
+    x, w = torch.zeros(40, D), torch.zeros(V, D)
+    w[:, 0], w[:, 1] = 1.0, 0.0
+    w[torch.arange(0, V, 5), 1] = 1.0                                                    # every fifth class is `gap` above the others
+    gap = torch.arange(40) % 20
+    x[:, 0], x[:, 1] = (top // 8) * 8 if top > 256 else top, gap
+    w[333, 2], x[:, 2] = 1.0, 2.0 * gap                                                  # the target: as much again above those
+    x, w = x.to(bf16).to(device), w.to(bf16).to(device)
+    z = x.double() @ w.double().t()
+    assert torch.equal(z, (x.float() @ w.float().t()).double())                          # whole numbers: nothing is rounded on the way
+    target = torch.full((40,), 333, device=device)
+    want = torch.log1p(((z - z[:, 333:334]).exp().sum(1) - 1.0))
+    for smoothing in (0.0, 0.1):
+        r = ops.linear_xent(x, w, target, smoothing=smoothing, want_grad=False)
+        exact = (1 - smoothing) * want + smoothing * (want + z[:, 333] - z.mean(1))
+        # the sum s: an exponential and its argument, V / 64 sums; its logarithm; with smoothing the mean, of the logits' size
+        tol = (V / 64 + 16) * U32 * (1 + want) + smoothing * 16 * U32 * z.abs().max()
+        assert torch.all((r.rows.double() - exact).abs() <= tol)
+    # whatever the logits, no loss is negative
+    g = torch.Generator().manual_seed(top)
+    x, w = torch.randn(500, 64, generator=g).to(bf16).to(device), torch.randn(90, 64, generator=g).to(bf16).to(device)
+    x = x * (top / 65.0)
+    rows = ops.linear_xent(x, w, (x @ w.t()).argmax(1), want_grad=False).rows
+    assert torch.all(rows >= 0) and (rows < 1e-3).any()
+
+
+@pytest.mark.gpu
+def test_linear_xent_row_whose_mask_leaves_nothing(device):
+    """every class masked out with the type's lowest value: equal logits, as a softmax has it; with -inf: NaN, as a softmax has it"""
+    ops = _ops()
+    g = torch.Generator().manual_seed(4)
+    x, w, target = (t.to(device) for t in xent_inputs(50, 300, 64, g, ignored=0.0))
+    r = ops.linear_xent(x, w, target, torch.full((300,), torch.finfo(f32).min, device=device))
+    assert torch.all((r.rows - math.log(300)).abs() <= 8 * U32 * math.log(300))
+    p = torch.full((50, 300), 1 / 300, dtype=f64, device=device) - torch.nn.functional.one_hot(target, 300).double()
+    assert torch.all((r.dx.double() - p @ w.double() / 50).abs() <= (2.0 ** -11 + 2.0 ** -7) * 1.01 * (p.abs() @ w.double().abs() / 50))
+    r = ops.linear_xent(x, w, target, torch.full((300,), -math.inf, device=device))
+    assert torch.isnan(r.rows).all() and torch.isnan(r.dx).all()
+
+
+@pytest.mark.gpu
 def test_linear_xent_gradient_against_differences(device):
     ops = _ops()
     g = torch.Generator().manual_seed(9)

@@ -879,9 +879,12 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
     dot = lx_block_sum<WAVES>(dot, sh);
     if (p.smoothing > 0.f) zs = lx_block_sum<WAVES>(zs, sh);
     if (p.bias != nullptr) dot += p.bias_type == 1 ? bf2f(reinterpret_cast<const bf16_t*>(p.bias)[t]) : reinterpret_cast<const float*>(p.bias)[t];
-    const float s2 = log2f(s), lse = mx + s2 * 0.69314718055994530942f;
-    float l = lse - dot;
-    if (p.smoothing > 0.f) l = (1.f - p.smoothing) * l + p.smoothing * (lse - zs / (float)p.V);
+    // lse - z as (max - z) + log s: lse as one number would be rounded to its own size, which is 30 times the loss of a certain row.  Neither loss
+    // is negative; the target's logit, a sum of its own, may be an ulp above the maximum.
+    const float s2 = log2f(s);
+    auto above = [&](float z) { const float l = __builtin_fmaf(s2, 0.69314718055994530942f, mx - z); return l < 0.f ? 0.f : l; };
+    float l = above(dot);
+    if (p.smoothing > 0.f) l = (1.f - p.smoothing) * l + p.smoothing * above(zs / (float)p.V);
     lx_row_done(p, row, tid, valid ? l : __builtin_nanf(""));
     if (P == nullptr) return;
     const float u = p.smoothing / (float)p.V, hit = 1.f - p.smoothing;
