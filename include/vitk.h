@@ -309,7 +309,7 @@ int vitk_kd_kl_fwd_bwd(const float* student, int lds_, const float* teacher, int
  * x bf16 [T, D], w bf16 [V, D] (row strides ldx, ldw), bias [V] (0 fp32, 1 bf16) or NULL, target int64 [T].  D and the strides are
  * multiples of 8, rows 16-byte aligned; T <= 2^30, V <= 2^22.  dx bf16 [T, D], dw [V, D] (bf16, or fp32 with dw_f32) and db [V] (bf16, or fp32 with
  * db_f32) receive the gradients of loss[0]; each may be NULL, and what only it needs is not computed.  Products are of bf16 factors with fp32 sums; the factor dloss/dz
- * is rounded to bf16 once, without the 1 / count, which multiplies the sums.
+ * is rounded to bf16 once, without the 1 / count and a part of 1 - smoothing, which multiply the sums.
  * Rows are worked through in blocks whose probabilities (2 bytes each) and statistics take about block_bytes at most (at least 256
  * rows); dw is summed over the blocks in fp32 (an fp32 dw in place: its rows must then be contiguous).  An ignored row adds 0 * x to dw: its x
  * has to be finite there, as with separate products.  want_grad: whether any gradient is asked for.  workspace: vitk_linear_xent_workspace(...) bytes for the same arguments, 256-byte aligned. */

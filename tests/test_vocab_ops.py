@@ -859,6 +859,55 @@ def test_linear_xent_bias_gradient_keeps_the_hits(device, T, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,V", [(2000, 3001), (900, 21843), (700, 100003)])
+def test_linear_xent_smoothing_is_not_rounded_the_same_way_in_every_row(device, T, V):
+    """1 - smoothing at the targets and smoothing / V at all other classes are no bf16 numbers (0.9 is off by 0.17 %, 0.1 / 21843 by 0.25 %): sums over many rows must
+    not be off by the rounding of a constant"""
+    ops = _ops()
+    g = torch.Generator().manual_seed(V)
+    D = 64
+    x = (1.0 + 0.3 * torch.randn(T, D, generator=g)).to(bf16).to(device)                 # all of one sign: nothing averages out in dweight
+    w = (torch.randn(V, D, generator=g) * 0.02).to(bf16).to(device)
+    target = (torch.randint(0, 8, (T,), generator=g) * (V // 8)).to(device)
+    bias = torch.zeros(V)
+    never = torch.arange(1, V // 8)                                                      # classes of a probability of nothing: smoothing / V is all they get
+    bias[never] = -60.0
+    never, bias = never.to(device), bias.to(device)
+    r = ops.linear_xent(x, w, target, bias, smoothing=0.1, reduction="sum", dweight_dtype=f32)
+    X, W, u = x.double(), w.double(), 0.1 / V
+    p = torch.softmax(X @ W.t() + bias.double(), 1)
+    hits = torch.nn.functional.one_hot(target, V).double()
+    dz = p - u - 0.9 * hits
+    # as in plain_linear_xent, but at a target what is rounded is no constant: at most what stands there beside 0.9, p + u, is lost; and
+    # what a class of no probability gets, u, is held to 2e-4 (of these three V: lx_factor, 8e-6, 1.1e-4 and 8e-7)
+    E = (p * 2.0 ** -11 + (p - u).abs() * 2.0 ** -8) * 1.01 * (1 - hits) + (p + u) * hits + (T + 300) * U32 * dz.abs() + 2.0 ** -30 * p
+    E[:, never] = 2e-4 * u
+    for got, want, tol in ((r.dweight, dz.t() @ X, E.t() @ X.abs()), (r.dbias, dz.sum(0), E.sum(0))):
+        assert torch.all((got.double() - want).abs() <= tol)
+        hit = target.unique()
+        assert (tol[hit] / want[hit].abs()).max() < 1.2e-3                               # it would see 0.9 rounded to bf16
+    # dx: its own rounding to bf16 is as far and has either sign; over all T * D elements it leaves 2^-8 / sqrt(3 T D) < 1.1e-5 of their size (six times
+    # that is allowed), a constant's rounding all of itself.  At the target p - u beside 0.9 is lost here too: of a want that is 0.9 of W's row, up to
+    # the other classes' share, that is (p + u) / 0.9
+    want = dz @ W
+    lost = float((hits * (p + u)).sum(1).max()) / 0.9
+    assert lost < 1.2e-3 and abs(float((r.dx.double() * want).sum() / (want * want).sum()) - 1) <= 6.6e-5 + 1.02 * lost
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("smoothing", [1e-6, 0.5, 0.97, 1.0])
+def test_linear_xent_any_smoothing(device, smoothing):
+    ops = _ops()
+    g = torch.Generator().manual_seed(2)
+    x, w, target = xent_inputs(130, 333, 64, g)
+    bias = torch.randn(333, generator=g)
+    dev = [t.to(device) for t in (x, w, target, bias)]
+    for reduction in ("mean", "sum"):
+        r = ops.linear_xent(*dev, smoothing=smoothing, reduction=reduction, dweight_dtype=f32)
+        check_linear_xent(r, x, w, target, bias, smoothing, mean=reduction == "mean")
+
+
+@pytest.mark.gpu
 def test_linear_xent_refuses(device):
     ops, err = _ops(), _error()
     x, w, t = torch.randn(6, 16, device=device).to(bf16), torch.randn(9, 16, device=device).to(bf16), torch.zeros(6, dtype=torch.int64, device=device)

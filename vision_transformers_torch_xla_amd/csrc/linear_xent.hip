@@ -10,9 +10,11 @@
 //      but ends at 6e-8 of the piece's maximum, and a class that stays 18 powers of e below a neighbour would lose its row of dW and its
 //      db, which have no larger neighbour in their sums; bf16 would round 8 times as far.  Loss alone: only the table is written.
 //   2. one workgroup per row (lx_row_kernel): lse from the table, the target's logit as a dot product of its own, the row's loss, and
-//      P -> dz in place, now bf16: the one rounding of the gradient's factor.  g is not in it: a constant such as 1 / count would be
-//      rounded 1 part in 256 in the same direction everywhere; it multiplies the fp32 sums of the next step.
-//   3. dx = dz W and dW = dz^T x (lx_grad_kernel), and the column sums for db, to which each target's dz adds what its rounding took.
+//      P -> dz in place, now bf16: the one rounding of the gradient's factor.  Constants are kept out of it, because each would be rounded
+//      by up to 1 part in 256 in the same direction everywhere: dz is divided by g and by a number that makes 1 - e a bf16 number and
+//      e/V nearly one (lx_factor); both multiply the fp32 sums of the next step.
+//   3. dx = dz W and dW = dz^T x (lx_grad_kernel), and the column sums for db, to which each target's dz adds what its rounding took (near
+//      -(1 - e) a probability of less than 2^-9 vanishes).
 // 6 T V D floating-point operations: nothing is computed twice.  Keeping one 16-bit factor per logit of a block costs 4 bytes of
 // traffic per logit for step 2, where computing the logits again for the gradients would cost 2 D operations.
 #include "common.h"
@@ -738,6 +740,8 @@ struct LxRowParams {
     float* delta;                      // what the target's dz lost to bf16, per row (0 where it is ignored); null: no db
     int V, D, rows_n, pad_rows;         // pad_rows rows of zeros behind the last (lx_grad_kernel reads steps of 64 of them)
     float smoothing;
+    float a, u, hit;                   // dz = a p - u - hit [the target], see lx_factor
+    double unit;                       // what dz is multiplied by
 };
 
 template <int WAVES>
@@ -795,8 +799,8 @@ static __device__ __forceinline__ u32x4 lx_dz8(const u32x4 r, float f, float u, 
 }
 
 // scale of the gradients and loss from the sum of the rows' losses and the count of the counted rows
-static __device__ __forceinline__ void lx_finish(double s, long long count, int mean, float* scale, float* loss) {
-    if (scale != nullptr) *scale = count == 0 ? 0.f : mean ? (float)(1.0 / (double)count) : 1.f;
+static __device__ __forceinline__ void lx_finish(double s, long long count, int mean, double unit, float* scale, float* loss) {
+    if (scale != nullptr) *scale = (float)(count == 0 ? 0.0 : mean ? unit / (double)count : unit);
     if (loss != nullptr) *loss = (float)(count == 0 ? 0.0 : mean ? s / (double)count : s);
 }
 // A row's loss is known: it is stored, and where p.loss is set the wave that is the last of all rows' first waves adds them up, lane by lane, then
@@ -822,7 +826,7 @@ static __device__ __forceinline__ void lx_row_done(const LxRowParams& p, int row
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); count += __shfl_xor(count, o, 64); }
-    if (tid == 0) lx_finish(s, count, p.mean, p.scale, p.loss);
+    if (tid == 0) lx_finish(s, count, p.mean, p.unit, p.scale, p.loss);
 }
 
 // WAVES waves per row: one workgroup, or for short rows one wave of a workgroup of four.  Bound by memory: 4 bytes per logit where the gradient
@@ -887,7 +891,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
     if (p.smoothing > 0.f) l = (1.f - p.smoothing) * l + p.smoothing * above(zs / (float)p.V);
     lx_row_done(p, row, tid, valid ? l : __builtin_nanf(""));
     if (P == nullptr) return;
-    const float u = p.smoothing / (float)p.V, hit = 1.f - p.smoothing;
+    const float u = p.u, hit = p.hit, a = p.a * 0x1p+64f;
     u32x4* q = reinterpret_cast<u32x4*>(P);
     for (int c0 = tid; c0 < chunks; c0 += LX_AHEAD * NT) {
         u32x4 r[LX_AHEAD];
@@ -902,7 +906,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
         for (int j = 0; j < LX_AHEAD; ++j) {
             const int c = c0 + j * NT;
             if (c < chunks) {
-                const float f = lx_below(m[j], mx, s2) * 0x1p+64f;
+                const float f = lx_below(m[j], mx, s2) * a;
                 const u32x4 o = lx_dz8(r[j], f, u, hit, c * 8, t, p.V, valid);
                 if (p.delta != nullptr && c == (t >> 3)) {
                     const int shift = (t & 1) * 16;
@@ -920,12 +924,12 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
     }
 }
 
-// Count of the counted rows, the scale of the gradients (1 / count, or 1 for a sum; 0 without a counted row) and the loss.  Workgroup b sums
+// Count of the counted rows, the scale of the gradients (unit / count, or unit for a sum; 0 without a counted row) and the loss.  Workgroup b sums
 // a stretch of the rows into part[b]; the last one to finish adds the parts up, one to a lane (the kernel that made the logits has zeroed the ticket).
 #define LX_LOSS_WGS 64          // at most a wave's lanes
 struct LxLossPart { double sum; long long count; };
 __global__ __launch_bounds__(256) void lx_loss_kernel(const long long* __restrict__ target, long long ignore_index, const float* __restrict__ rows, int T, int per,
-                                                      int mean, LxLossPart* part, unsigned* ticket, float* __restrict__ scale, float* __restrict__ loss) {
+                                                      int mean, double unit, LxLossPart* part, unsigned* ticket, float* __restrict__ scale, float* __restrict__ loss) {
     __shared__ double sh[4];
     __shared__ int shc[4];
     const int i1 = (int)((blockIdx.x + 1ll) * per < T ? (blockIdx.x + 1ll) * per : T);
@@ -969,7 +973,7 @@ __global__ __launch_bounds__(256) void lx_loss_kernel(const long long* __restric
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); count += __shfl_xor(count, o, 64); }
     }
-    if (threadIdx.x == 0) lx_finish(s, count, mean, scale, loss);
+    if (threadIdx.x == 0) lx_finish(s, count, mean, unit, scale, loss);
 }
 
 // The same products for outputs too small to fill the chip with 256 x 256 tiles, which also cost a call 8 to 10 us of pipeline fill and epilogue
@@ -1148,8 +1152,8 @@ __global__ __launch_bounds__(256) void lx_small_kernel(const LxGemmParams p) {
     if (EPI != LX_OUT && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0u;
     lx_small_body<LAY, EPI, FM, WM, WN>(p, sm, blockIdx.x, gridDim.x);
 }
-// Rows first, first + STEP, ... < end of dz, 8 columns, for db, with what the targets' dz lost to bf16: without that every hit of 1 - smoothing is off in
-// the same direction (0.9 by 0.17 %).  Eight rows are in flight; the targets, which are rare, are looked at behind them.
+// Rows first, first + STEP, ... < end of dz, 8 columns, for db, with what the targets' dz lost to bf16: without that the target's own probability
+// would be missing from every hit while it is small.  Eight rows are in flight; the targets, which are rare, are looked at behind them.
 template <int STEP>
 static __device__ __forceinline__ void lx_colsum_rows(float (&acc)[8], const bf16_t* dz, long long ldp, long long col, const long long* target, const float* delta,
                                                       int first, int end) {
@@ -1328,6 +1332,26 @@ static int lx_cus() {
 }
 // ranges of rows that the column sums are cut into: more where there are few columns (25088 x 1000: 64 of them 23 + 4 us, 128 15 + 5)
 static int lx_ranges(long long ldp) { return ldp <= 2048 ? 128 : 64; }
+// dz / unit = a p - u - hit [the target].  Of the 128 bf16 numbers from 1 up, hit is the one for which u = hit e / (V (1 - e)) is nearest to a bf16 number
+// too: half of all V within 1.4e-5, nine in ten within 5e-5 (1 - e and e/V themselves are off by up to 2^-8; 0.9 by 0.17 %, 0.1 / 21843 by 0.25 %).
+// u stays inside the rounded factor: taken off the sums instead (as e/V times the sums of x and of W's rows), the factor would be rounded to
+// 2^-8 of p also where p - e/V nearly cancels.
+struct LxFactor { float a, u, hit; double unit; };
+static LxFactor lx_factor(float smoothing, int V) {
+    const double e = smoothing;
+    if (e <= 0.0) return {1.f, 0.f, 1.f, 1.0};
+    if (e >= 1.0) return {(float)V, 1.f, 0.f, 1.0 / V};
+    const double r = e / (V * (1.0 - e));
+    int exponent, best = 128;
+    const double f = frexp(r, &exponent);
+    double least = 1.0;
+    for (int m = 128; m < 256; ++m) {
+        const double t = f * m < 128.0 ? 2.0 * f * m : f * m, off = fabs(rint(t) - t) / t;
+        if (off < least) { least = off; best = m; }
+    }
+    const double hit = best / 128.0, unit = (1.0 - e) / hit;
+    return {(float)(1.0 / unit), (float)(r * hit), (float)hit, unit};
+}
 static size_t lx_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // How the tiles of dx and dW are dealt.  `width` column tiles side by side form a row, worked on by a team of as many workgroups in step, so
@@ -1555,12 +1579,13 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
     }
     hipStream_t s = (hipStream_t)stream;
     const int cus = lx_cus();
+    const LxFactor factor = grad ? lx_factor(smoothing, V) : LxFactor{};
     char* ws = (char*)workspace;
     float* scale = (float*)(ws + q.scale);
     unsigned* ticket = (unsigned*)(ws + q.scale + 8);
     const long long* tg = (const long long*)target;
     if (q.blocks > 1 && grad) {
-        lx_loss_kernel<<<1, 256, 0, s>>>(tg, ignore_index, nullptr, (int)T, (int)T, mean, nullptr, nullptr, scale, nullptr);
+        lx_loss_kernel<<<1, 256, 0, s>>>(tg, ignore_index, nullptr, (int)T, (int)T, mean, factor.unit, nullptr, nullptr, scale, nullptr);
         if (int rc = vitk_check_launch("linear_xent_count")) return rc;
     }
     for (int b = 0; b < q.blocks; ++b) {
@@ -1597,6 +1622,7 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         const bool fused = q.blocks == 1 && T <= LX_FUSED_ROWS && (!grad || (size_t)T * q.ldp * 2 <= LX_FUSED_BYTES);
         r.ticket = ticket; r.scale = scale; r.loss = fused ? loss : nullptr; r.mean = mean;
         r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.rows_n = n; r.smoothing = smoothing;
+        r.a = factor.a; r.u = factor.u; r.hit = factor.hit; r.unit = factor.unit;
         r.pad_rows = dw && q.dw[last].kind == LX_BIG ? (LX_BK - n % LX_BK) % LX_BK : 0;
         r.delta = db ? (float*)(ws + q.delta) : nullptr;
         const int row_wgs = n + r.pad_rows;
@@ -1620,7 +1646,7 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         if (last && !fused) {
             int per = (int)((T + LX_LOSS_WGS - 1) / LX_LOSS_WGS);
             if (per < 1024) per = 1024;
-            lx_loss_kernel<<<(int)((T + per - 1) / per), 256, 0, s>>>(tg, ignore_index, rows, (int)T, per, mean, (LxLossPart*)(ws + q.scale + 16), ticket,
+            lx_loss_kernel<<<(int)((T + per - 1) / per), 256, 0, s>>>(tg, ignore_index, rows, (int)T, per, mean, factor.unit, (LxLossPart*)(ws + q.scale + 16), ticket,
                                                                       q.blocks > 1 ? nullptr : scale, loss);
             if (int rc = vitk_check_launch("linear_xent_loss")) return rc;
         }
