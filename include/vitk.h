@@ -311,8 +311,8 @@ int vitk_kd_kl_fwd_bwd(const float* student, int lds_, const float* teacher, int
  * db_f32) receive the gradients of loss[0]; each may be NULL, and what only it needs is not computed.  Products are of bf16 factors with fp32 sums; the factor dloss/dz
  * is rounded to bf16 once, without the 1 / count and a part of 1 - smoothing, which multiply the sums.
  * Rows are worked through in blocks whose probabilities (2 bytes each) and statistics take about block_bytes at most (at least 256
- * rows); dw is summed over the blocks in fp32 (an fp32 dw in place: its rows must then be contiguous).  An ignored row adds 0 * x to dw: its x
- * has to be finite there, as with separate products.  want_grad: whether any gradient is asked for.  workspace: vitk_linear_xent_workspace(...) bytes for the same arguments, 256-byte aligned. */
+ * rows), with a copy of their x beside them; dw is summed over the blocks in fp32 (an fp32 dw in place: its rows must then be contiguous).  A row of x
+ * whose target is ignored adds nothing, whatever it holds.  want_grad: whether any gradient is asked for.  workspace: vitk_linear_xent_workspace(...) bytes for the same arguments, 256-byte aligned. */
 size_t vitk_linear_xent_workspace(int64_t T, int V, int D, int want_grad, int smoothing, int dw_f32, int bias, size_t block_bytes);
 int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_type, const int64_t* target, int64_t T, int V, int D,
                      float smoothing, int64_t ignore_index, int mean, float* loss, float* rows, void* dx, int64_t lddx, void* dw, int64_t lddw, int dw_f32,

@@ -685,6 +685,26 @@ def test_linear_xent_row_whose_mask_leaves_nothing(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D,block_bytes", [(1, 1000, 192, 1 << 30), (70, 500, 64, 1 << 30), (700, 3000, 192, 1 << 30), (2050, 12001, 520, 1 << 30), (1500, 2000, 72, 1 << 20)])
+def test_linear_xent_ignored_rows_may_hold_anything(device, T, V, D, block_bytes):
+    ops = _ops()
+    g = torch.Generator().manual_seed(T + V)
+    x, w, target = (t.to(device) for t in xent_inputs(T, V, D, g, ignored=0.4))
+    target[-1] = -100                                                                     # the last row of x too: short blocks repeat it
+    bias = torch.randn(V, generator=g).to(device)
+    dirty, clean = x.clone(), x.clone()
+    ignored = target == -100
+    dirty[ignored] = torch.tensor([math.nan, math.inf, -math.inf, 3e38], device=device).to(bf16).repeat(int(ignored.sum()), D // 4)
+    clean[ignored] = 0.0
+    for smoothing in (0.0, 0.1):
+        got = ops.linear_xent(dirty, w, target, bias, smoothing=smoothing, dweight_dtype=f32, block_bytes=block_bytes)
+        want = ops.linear_xent(clean, w, target, bias, smoothing=smoothing, dweight_dtype=f32, block_bytes=block_bytes)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.isfinite(t).all() for t in got) and torch.all(got.dx[ignored] == 0)
+        check_linear_xent(want, clean, w, target, bias, smoothing)
+
+
+@pytest.mark.gpu
 def test_linear_xent_gradient_against_differences(device):
     ops = _ops()
     g = torch.Generator().manual_seed(9)

@@ -13,6 +13,8 @@
 //      P -> dz in place, now bf16: the one rounding of the gradient's factor.  Constants are kept out of it, because each would be rounded
 //      by up to 1 part in 256 in the same direction everywhere: dz is divided by g and by a number that makes 1 - e a bf16 number and
 //      e/V nearly one (lx_factor); both multiply the fp32 sums of the next step.
+//      Where dW is wanted it also copies x, with zeros for the rows that are not counted: their dz is zero, but zero times what such a row may
+//      hold (infinities, NaN) would not be.  2 T D bytes written beside the 4 T V of P: under 1 % of a call.
 //   3. dx = dz W and dW = dz^T x (lx_grad_kernel), and the column sums for db, to which each target's dz adds what its rounding took (near
 //      -(1 - e) a probability of less than 2^-9 vanishes).
 // 6 T V D floating-point operations: nothing is computed twice.  Keeping one 16-bit factor per logit of a block costs 4 bytes of
@@ -737,6 +739,7 @@ struct LxRowParams {
     unsigned* ticket; float* scale; float* loss; int mean;      // loss not null: the last row to finish adds the rows up (see lx_loss_kernel)
     bf16_t* P; long long ldp;          // P on entry (lx_pack_p), bf16 dz on exit; null: loss alone
     float* rows;
+    bf16_t* xs;                        // [rows_n][D]: x, zero where a row is not counted; null: no dW
     float* delta;                      // what the target's dz lost to bf16, per row (0 where it is ignored); null: no db
     int V, D, rows_n, pad_rows;         // pad_rows rows of zeros behind the last (lx_grad_kernel reads steps of 64 of them)
     float smoothing;
@@ -847,6 +850,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
         if (P != nullptr)
             for (int c = tid; c < chunks; c += NT) __builtin_nontemporal_store((u32x4){0u, 0u, 0u, 0u}, reinterpret_cast<u32x4*>(P) + c);
         if (!pad) {
+            if (p.xs != nullptr)
+                for (int c = tid; c < p.D / 8; c += NT) reinterpret_cast<u32x4*>(p.xs + (size_t)row * p.D)[c] = (u32x4){0u, 0u, 0u, 0u};
             if (p.delta != nullptr && tid == 0) p.delta[row] = 0.f;
             lx_row_done(p, row, tid, 0.f);
         }
@@ -865,6 +870,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void lx_row_kernel(c
         float a[8], b[8];
         load8(xr + c * 8, a);
         load8(wr + c * 8, b);
+        if (p.xs != nullptr) reinterpret_cast<u32x4*>(p.xs + (size_t)row * p.D)[c] = reinterpret_cast<const u32x4*>(xr)[c];
 #pragma unroll
         for (int k = 0; k < 8; ++k) dot = __builtin_fmaf(a[k], b[k], dot);
     }
@@ -1366,7 +1372,7 @@ struct LxPlan {
     long long ldp, stat_cols;
     int block, blocks;              // rows per block, blocks
     LxDeal dx[2], dw[2];            // of a block, of the last one
-    size_t scale, stats, zsum, P, acc, slab, colpart, colsum, delta, total;
+    size_t scale, stats, zsum, P, xs, acc, slab, colpart, colsum, delta, total;
 };
 // The kernel and its cut that a model of the time finds fastest, in microseconds on 256 compute units, from 28 shapes between 1 x 1000 x 192 and
 // 512 x 100003 x 1024 measured with each of the three kernels (time of x W^T / dz W / dz^T x in us, large : 128 : 64):
@@ -1493,6 +1499,7 @@ static LxPlan lx_plan(long long T, int V, int D, int grad, int smoothing, int dw
     q.zsum = smoothing ? take((size_t)rows * q.stat_cols * sizeof(float)) : 0;
     if (grad) {
         q.P = take((size_t)((rows + LX_BK - 1) / LX_BK * LX_BK) * q.ldp * 2);
+        q.xs = take((size_t)rows * D * 2);
         if (q.blocks > 1 && !dw_f32) q.acc = take((size_t)V * D * sizeof(float));
         const int cus = lx_cus();
         size_t slab = 0;            // dx and dW use it one after the other
@@ -1624,6 +1631,7 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         r.P = (bf16_t*)g.P; r.ldp = q.ldp; r.rows = rows + r0; r.V = V; r.D = D; r.rows_n = n; r.smoothing = smoothing;
         r.a = factor.a; r.u = factor.u; r.hit = factor.hit; r.unit = factor.unit;
         r.pad_rows = dw && q.dw[last].kind == LX_BIG ? (LX_BK - n % LX_BK) % LX_BK : 0;
+        r.xs = dw ? (bf16_t*)(ws + q.xs) : nullptr;
         r.delta = db ? (float*)(ws + q.delta) : nullptr;
         const int row_wgs = n + r.pad_rows;
         // long rows get more waves.  By the vocabulary alone, so that a row's sums do not depend on how many rows there are or what is wanted.
@@ -1658,7 +1666,7 @@ int vitk_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, con
         d.scale = scale; d.out = (bf16_t*)dx + r0 * lddx; d.ldo = lddx; d.slab = (float*)(ws + q.slab);
         // dW = dz^T x, summed over the blocks in fp32
         LxGemmParams e = {};
-        e.A = dz; e.lda = (int)q.ldp; e.B = g.A; e.ldb = (int)ldx; e.M = V; e.N = D; e.KA = e.KB = n; e.steps = (n + LX_BK - 1) / LX_BK;
+        e.A = dz; e.lda = (int)q.ldp; e.B = r.xs; e.ldb = D; e.M = V; e.N = D; e.KA = e.KB = n; e.steps = (n + LX_BK - 1) / LX_BK;
         e.scale = scale; e.slab = d.slab;
         float* acc = dw_f32 ? (float*)dw : (float*)(ws + q.acc);
         e.add = b > 0 ? acc : nullptr;

@@ -603,7 +603,7 @@ def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, 
 
     rows[i] = (1 - smoothing) * nll + smoothing * mean_j(-logp_ij), 0 where target == ignore_index; loss = their mean over the counted
     rows, or their sum (reduction 'sum'); 0 with zero gradients where no row counts.  Any other target outside [0, V) gives NaN.
-    An ignored row of x must still be finite where dweight is wanted (0 times the row is added, as with separate products).
+    What an ignored row of x holds (infinities, NaN) goes nowhere; its row of dx is zero.
     want_grad: dx bf16 [T, D], dweight [V, D] in dweight_dtype (bf16, the default, or float32), dbias in the bias's type.
     grads: which of them; a frozen head or frozen features cost one product less.
     block_bytes: the rows are worked through in blocks that hold about this many bytes of probabilities (at least 256 rows); more than
