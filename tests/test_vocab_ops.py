@@ -142,6 +142,30 @@ def test_clip_grads_offsets_past_32_bits(device):
 
 
 @pytest.mark.gpu
+def test_clip_grads_of_lazy_clones(device):
+    """a lazy clone that is written gets memory of its own: the original keeps its values"""
+    ops = _ops()
+    a, b = torch.randn(300, device=device), torch.randn(70, device=device)
+    keep = [a.clone(), b.clone()]
+    lazy = [torch._lazy_clone(a), torch._lazy_clone(b)]
+    _, want = plain_clip([t.cpu() for t in keep], 1.0)
+    ops.clip_grads(lazy, 1.0)                                                        # in place
+    assert torch.equal(a, keep[0]) and torch.equal(b, keep[1])
+    check_clipped(lazy, want)
+    out = [torch._lazy_clone(a), torch._lazy_clone(b)]                               # outputs that share the gradients' own memory so far
+    ops.clip_grads([a, b], 1.0, out=out)
+    assert torch.equal(a, keep[0]) and torch.equal(b, keep[1])
+    check_clipped(out, want)
+    half = torch._lazy_clone(a)
+    ops.clip_grads([half, b], 1.0, out=[half, out[1]])
+    assert torch.equal(a, keep[0])
+    check_clipped([half, out[1]], want)
+    with pytest.raises(_error()):
+        ops.clip_grads([a, a.view(300)], 1.0)
+    assert torch.equal(a, keep[0])
+
+
+@pytest.mark.gpu
 def test_clip_grads_refuses(device):
     ops, err = _ops(), _error()
     a = torch.randn(64, device=device)

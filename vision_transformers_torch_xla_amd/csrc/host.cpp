@@ -54,14 +54,11 @@ static PyObject* clip_table(PyObject*, PyObject* args) {
         for (Py_ssize_t i = 0; i < n; ++i) {
             const at::Tensor& t = tensor_at(list, i, "tensors");
             check_one(t, i, "tensors", device);
-            src[i] = (int64_t)t.const_data_ptr();
             numel[i] = t.numel();
             types[i] = type_code(t);
         }
         if (out != Py_None) {
             if (PyList_GET_SIZE(out) != n) throw std::to_string(n) + " tensors, " + std::to_string(PyList_GET_SIZE(out)) + " outputs";
-            std::vector<std::pair<int64_t, int64_t>> ranges;       // written memory, and read memory that is not written in place
-            ranges.reserve(2 * n);
             for (Py_ssize_t i = 0; i < n; ++i) {
                 const at::Tensor& t = tensor_at(list, i, "tensors");
                 const at::Tensor& o = tensor_at(out, i, "out");
@@ -70,8 +67,16 @@ static PyObject* clip_table(PyObject*, PyObject* args) {
                     if (o.scalar_type() != t.scalar_type() || o.sizes() != t.sizes() || o.strides() != t.strides())
                         throw "out[" + std::to_string(i) + "] must have the shape, strides and type of tensors[" + std::to_string(i) + "]";
                 }
-                dst[i] = (int64_t)o.const_data_ptr();
-                const int64_t bytes = numel[i] * (int64_t)t.element_size();
+            }
+            // what is written gets memory of its own first where it is a lazy clone that still shares its original's; that may move what is read
+            for (Py_ssize_t i = 0; i < n; ++i) dst[i] = (int64_t)tensor_at(out, i, "out").mutable_data_ptr();
+        }
+        for (Py_ssize_t i = 0; i < n; ++i) src[i] = (int64_t)tensor_at(list, i, "tensors").const_data_ptr();
+        if (out != Py_None) {
+            std::vector<std::pair<int64_t, int64_t>> ranges;       // written memory, and read memory that is not written in place
+            ranges.reserve(2 * n);
+            for (Py_ssize_t i = 0; i < n; ++i) {
+                const int64_t bytes = numel[i] * (types[i] == 0 ? 4 : 2);
                 if (bytes == 0) continue;
                 ranges.emplace_back(dst[i], bytes);
                 if (dst[i] != src[i]) ranges.emplace_back(src[i], -bytes);
