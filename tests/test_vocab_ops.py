@@ -1007,6 +1007,30 @@ def test_linear_cross_entropy_module(device, wtype, reduction):
 
 
 @pytest.mark.gpu
+def test_upstream_scalar_is_not_rounded_to_the_gradients_type(device):
+    from vision_transformers_torch_xla_amd import losses
+    g = torch.Generator().manual_seed(13)
+    x, w, t = (v.to(device) for v in xent_inputs(90, 50, 32, g))
+    bias = torch.randn(50, generator=g).to(device, bf16)
+    up = 1.0 + 2.0 ** -8 + 2.0 ** -9                                 # bf16 has 1 + 2^-7 for it
+    want = _ops().linear_xent(x, w, t, bias)
+    leaves = [v.clone().requires_grad_(True) for v in (x, w, bias)]
+    (up * losses.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])).backward()
+    for leaf, v in zip(leaves, want[2:]):
+        assert torch.equal(leaf.grad, (v.float() * up).to(bf16))
+
+
+def test_upstream_scalar_is_multiplied_in_place():
+    """a gradient of the weight's size is not held twice"""
+    from vision_transformers_torch_xla_amd.losses import _times
+    for g, go in ((torch.randn(8, 16), torch.tensor(0.7)), (torch.randn(40), torch.tensor(0.7, dtype=f64)), (torch.randn(40).to(bf16), torch.tensor(0.7))):
+        want = (g.float() * go.float()).to(g.dtype)
+        got = _times(g, go)
+        assert got is g and torch.equal(g, want)
+    assert _times(None, torch.tensor(2.0)) is None
+
+
+@pytest.mark.gpu
 def test_linear_cross_entropy_inputs_of_every_layout(device, monkeypatch):
     from vision_transformers_torch_xla_amd import losses
     g = torch.Generator().manual_seed(8)

@@ -99,7 +99,9 @@ def _times(g, go):
         return g
     if g.dtype == bf16 and g.dim() == 2:
         return ops.rowscale(g, go.reshape(1).float(), g.shape[0], out=g)
-    return (g * go.float()).to(g.dtype)
+    if g.dtype == f32:
+        return g.mul_(go.float())
+    return g.copy_(g.float() * go.float())          # bf16 times a scalar on the GPU would round the scalar first
 
 
 class _LinearXent(torch.autograd.Function):
