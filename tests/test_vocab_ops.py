@@ -1126,6 +1126,37 @@ def test_token_embedding_module(device):
     check_embedding_grad(m.weight.grad, torch.ones(7, 30, 16), ids.cpu(), 50, 4.0, 49)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [bf16, f32])
+def test_token_embedding_backward_of_every_layout(device, out_dtype):
+    """what autograd hands to the lookup's backward where the vectors are summed, averaged or joined with others"""
+    from vision_transformers_torch_xla_amd.embedding import TokenEmbedding
+    torch.manual_seed(7)
+    m = TokenEmbedding(50, 16, scale=2.0, out_dtype=out_dtype).to(device)
+    ids = torch.randint(0, 50, (30,), device=device)
+    other = torch.ones(30, 3, device=device, dtype=out_dtype)
+    up = torch.randn(30, 40, device=device).to(out_dtype)
+    row = torch.randn(16, device=device).to(out_dtype)
+    cases = {
+        "summed over the tokens": (ids, lambda e: (e.sum(0), row), row.expand(30, 16)),
+        "one sequence, summed": (ids[None], lambda e: (e.sum(1)[0], row), row.expand(30, 16)),
+        "one sequence of several, summed": (ids.view(5, 6), lambda e: (e.sum(1), up[:5, :16]), up[:5, None, :16].expand(5, 6, 16)),
+        "before others": (ids, lambda e: (torch.cat([e, other], 1), up[:, :19]), up[:, :16]),
+        "behind others": (ids, lambda e: (torch.cat([other, e], 1), up[:, :19]), up[:, 3:19]),
+        "one token, behind others": (ids[:1], lambda e: (torch.cat([other[:1], e], 1), up[:1, :19]), up[:1, 3:19]),
+        "columns first": (ids, lambda e: (e.t(), up[:16, :30]), up[:16, :30].t()),
+        "no token": (ids[:0], lambda e: (e.sum(0), row), row.expand(0, 16)),
+    }
+    for name, (i, use, dout) in cases.items():
+        m.weight.grad = None
+        out, v = use(m(i))
+        out.backward(v)
+        if i.numel() == 0:
+            assert torch.all(m.weight.grad == 0)
+        else:
+            check_embedding_grad(m.weight.grad, dout.cpu(), i.cpu(), 50, 2.0, None)
+
+
 def test_module_arguments_are_checked():
     from vision_transformers_torch_xla_amd.embedding import TokenEmbedding, embedding
     from vision_transformers_torch_xla_amd.losses import LinearCrossEntropy, linear_cross_entropy

@@ -549,7 +549,8 @@ def embedding_fwd(ids, table, scale=1.0, out_dtype=None):
 
 def embedding_bwd(dout, ids, num_rows, scale=1.0, padding_idx=None, out=None, accumulate=False, out_dtype=None):
     """Gradient of embedding_fwd's table: [num_rows, D] with row v = scale * sum of dout over the tokens with id v (fp32 sums in an order
-    that the ids alone decide: the same bits on every run), zero where there is none; dout fp32 / bf16 [..., D].  Tokens with id padding_idx or an id
+    that the ids alone decide: the same bits on every run), zero where there is none; dout fp32 / bf16 [..., D] of any layout (copied where its
+    rows are not contiguous, a multiple of 8 values apart and 16-byte aligned).  Tokens with id padding_idx or an id
     outside [0, num_rows) add nothing.  out: where it goes (fp32 / bf16 [num_rows, D]); with accumulate it is added there, and only the
     rows that have tokens are touched.  Without out: a new tensor of out_dtype (default: dout's type)."""
     if padding_idx is not None and not 0 <= int(padding_idx) < int(num_rows):
@@ -560,8 +561,12 @@ def embedding_bwd(dout, ids, num_rows, scale=1.0, padding_idx=None, out=None, ac
     flat = _ids1d(ids)
     T = flat.numel()
     rows = dout if dout.dim() == 2 else dout.reshape(T, D)
-    if D > 1 and rows.stride(1) != 1:
+    # autograd hands over whatever the operation behind the lookup leaves: one row for all tokens (a sum over them), a part of wider rows (a concatenation)
+    s0, s1 = rows.stride()
+    if (s1 != 1 and D > 1) or (T > 1 and (s0 < D or s0 % 8)):
         rows = rows.contiguous()
+    if rows.data_ptr() % 16:
+        rows = rows.clone()
     dcode, ldd = _rows2d(rows, "dout")
     if out is None:
         if accumulate:
