@@ -31,6 +31,13 @@ def _core_model(model):
     return m.student if hasattr(m, "student") else m
 
 
+def _head_parameters(criterion):
+    """the trainable parameters of a criterion that holds the model's head (LinearCrossEntropy, also inside a wrapper with .module); a criterion
+    that merely has parameters is its owner's affair"""
+    core = getattr(criterion, "module", criterion)
+    return [p for p in core.parameters() if p.requires_grad] if getattr(core, "takes_features", False) else []
+
+
 def _grad_tensors(source):
     """the gradient tensors behind a module, a tensor or a nested iterable of them; a flat-buffer model counts as its one buffer"""
     if isinstance(source, torch.Tensor):
@@ -168,6 +175,7 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
     metric_logger = utils.MetricLogger(delimiter="  ")      # device scalars stay on the GPU until the meters are read
     header = f"Epoch: [{epoch}]"
     reducer = getattr(model, "reducer", None)
+    head = _head_parameters(criterion)
     optimizer.zero_grad()
     graphed = None
     if GraphedStep.wanted(model, update_freq):      # VITK_GRAPH_STEP=1: the captured step is kept on the model from epoch to epoch
@@ -212,15 +220,14 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
                 if reducer is not None:
                     reducer.wait()
                 if max_norm is not None and max_norm > 0:
-                    own = isinstance(criterion, torch.nn.Module) and any(p.grad is not None for p in criterion.parameters())
-                    clip_grad_norm_([model, criterion] if own else model, max_norm)      # a criterion may hold a head (LinearCrossEntropy)
+                    clip_grad_norm_([model, head] if any(p.grad is not None for p in head) else model, max_norm)
                 optimizer.step()
                 optimizer.zero_grad()
                 if model_ema is not None:
                     model_ema.update(model)
 
             class_acc = None
-            if mixup_fn is None and not getattr(criterion, "takes_features", False):
+            if mixup_fn is None and not getattr(getattr(criterion, "module", criterion), "takes_features", False):
                 out0 = output[0] if isinstance(output, tuple) else output
                 class_acc = (ops.argmax_rows(out0.detach().float()) == targets).float().mean()
 
