@@ -93,3 +93,65 @@ def test_only_a_head_is_clipped_with_the_model(monkeypatch):
     clipped.clear()
     engine.train_one_epoch(model, criterion, batches(1), torch.optim.SGD(model.parameters(), lr=0.1), torch.device("cpu"), 0, max_norm=0.5, mixup_fn=same)
     assert clipped == [model]
+
+
+# ------------------------------------------------------------------------------------------- several ranks (gloo)
+def _train(model, criterion, data, max_norm, update_freq=1):
+    from vision_transformers_torch_xla_amd import engine
+    engine.ops.clip_grads = torch_clip                                   # (a process of its own)
+    opt = torch.optim.SGD([*model.parameters(), *criterion.parameters()], lr=0.5)
+    engine.train_one_epoch(model, criterion, data, opt, torch.device("cpu"), 0, max_norm=max_norm, update_freq=update_freq)
+    return torch.cat([p.detach().reshape(-1) for p in (*model.parameters(), *criterion.parameters())])
+
+
+def _worker(rank, world, port, tmp):
+    sys.path.insert(0, str(ROOT))
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank))
+    torch.set_num_threads(1)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        for case, (max_norm, update_freq) in enumerate(((0.3, 1), (0.0, 1), (0.3, 2))):
+            torch.manual_seed(5)
+            model, criterion = Features(reducer=True), Head()
+            torch.manual_seed(50 + rank)                                 # a head of its own on every rank: rank 0's is the one that counts
+            with torch.no_grad():
+                criterion.weight.add_(torch.randn(criterion.weight.shape) * (rank + 0.5))
+                start = [p.detach().clone() for p in criterion.parameters()]
+            data = batches(6)
+            mine = [(x[4 * rank:4 * rank + 4], t[4 * rank:4 * rank + 4]) for x, t in data]
+            got = _train(model, criterion, mine, max_norm, update_freq)
+            other = got.clone()
+            dist.broadcast(other, src=0)
+            assert torch.equal(got, other), f"case {case}: the ranks differ by {float((got - other).abs().max())}"
+            if rank == 0:
+                torch.save((start, got), Path(tmp) / f"case{case}.pt")
+    finally:
+        dist.destroy_process_group()
+
+
+def _alone(tmp):
+    """one process, the whole batches, from rank 0's head"""
+    sys.path.insert(0, str(ROOT))
+    torch.set_num_threads(1)
+    for case, (max_norm, update_freq) in enumerate(((0.3, 1), (0.0, 1), (0.3, 2))):
+        start, got = torch.load(Path(tmp) / f"case{case}.pt", weights_only=True)
+        torch.manual_seed(5)
+        model, criterion = Features(), Head()
+        with torch.no_grad():
+            for p, v in zip(criterion.parameters(), start):
+                p.copy_(v)
+        want = _train(model, criterion, batches(6), max_norm, update_freq)
+        # the same sums of fp32 numbers in another order: 6 steps of a few dozen terms
+        assert torch.all((got - want).abs() <= 6 * 64 * 2.0 ** -24 * (1 + want.abs())), float((got - want).abs().max())
+
+
+def test_a_head_in_the_criterion_trains_alike_on_two_ranks(tmp_path):
+    s = socket.socket()
+    s.bind(("127.0.0.1", 0))
+    port = s.getsockname()[1]
+    s.close()
+    mp.spawn(_worker, args=(2, port, str(tmp_path)), nprocs=2, join=True)
+    p = mp.get_context("spawn").Process(target=_alone, args=(str(tmp_path),))
+    p.start()
+    p.join()
+    assert p.exitcode == 0

@@ -145,6 +145,38 @@ class GradReducer:
             self._timed = []
         return total, n, elems
 
+    @torch.no_grad()
+    def average(self, params):
+        """Averages the gradients of parameters outside the flat buffer (a criterion's head) over the ranks, in place, one collective each on the
+        current stream.  Call it on every rank with the same parameters, after backward; a parameter without a gradient on this rank
+        contributes zeros and receives the average, as in torch's DistributedDataParallel."""
+        if self._skip:
+            return
+        for p in params:
+            if p.grad is None:
+                p.grad = torch.zeros_like(p)
+            g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
+            if dist.get_backend(self.pg) == "nccl":
+                dist.all_reduce(g, op=dist.ReduceOp.AVG, group=self.pg)
+            else:                                    # gloo has no AVG and is given host memory only (see _launch)
+                host = g.to("cpu", torch.float32).mul_(1.0 / self.world)
+                dist.all_reduce(host, op=dist.ReduceOp.SUM, group=self.pg)
+                g.copy_(host)
+            if g is not p.grad:
+                p.grad.copy_(g)
+
+    @torch.no_grad()
+    def share(self, params):
+        """Rank 0's values of these parameters on every rank."""
+        if self._skip:
+            return
+        direct = dist.get_backend(self.pg) == "nccl"
+        for p in params:
+            # gloo is given host memory only (see _launch)
+            t = p.detach().contiguous() if direct else p.detach().to("cpu", torch.float32).contiguous()
+            dist.broadcast(t, src=0, group=self.pg)
+            p.copy_(t)
+
     def wait(self):
         """Make the current stream (or the host, for CPU tensors) wait for every outstanding bucket.  Backward already does
         this when it reports its last gradients, so after a complete backward this is a no-op kept for callers that reduce

@@ -176,6 +176,8 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
     header = f"Epoch: [{epoch}]"
     reducer = getattr(model, "reducer", None)
     head = _head_parameters(criterion)
+    if reducer is not None:
+        reducer.share(head)                         # the model's own parameters were shared when it was wrapped
     optimizer.zero_grad()
     graphed = None
     if GraphedStep.wanted(model, update_freq):      # VITK_GRAPH_STEP=1: the captured step is kept on the model from epoch to epoch
@@ -219,6 +221,7 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
             if last_micro:
                 if reducer is not None:
                     reducer.wait()
+                    reducer.average(head)             # before the norm: every rank clips by the same one
                 if max_norm is not None and max_norm > 0:
                     clip_grad_norm_([model, head] if any(p.grad is not None for p in head) else model, max_norm)
                 optimizer.step()
