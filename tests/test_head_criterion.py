@@ -155,3 +155,120 @@ def test_a_head_in_the_criterion_trains_alike_on_two_ranks(tmp_path):
     p.start()
     p.join()
     assert p.exitcode == 0
+
+
+# --------------------------------------------------------------------------------------------- the captured step
+def test_a_step_with_parameters_in_the_criterion_is_not_captured(monkeypatch):
+    from vision_transformers_torch_xla_amd import engine
+    monkeypatch.setenv("VITK_GRAPH_STEP", "1")
+    model = Features()
+    model.begin_static_droppath = lambda *a: None
+    head = Head()
+    wanted = lambda c: engine.GraphedStep.wanted(model, 1, c)          # noqa: E731
+    assert engine.GraphedStep.wanted(model, 1) and wanted(torch.nn.CrossEntropyLoss()) and wanted(torch.nn.functional.cross_entropy)
+    assert not wanted(head) and not wanted(WithTemperature())
+    for p in head.parameters():
+        p.requires_grad_(False)
+    assert wanted(head)
+
+
+@pytest.mark.gpu
+def test_vit_and_head_train_alike_with_and_without_the_graph_switch(device, monkeypatch):
+    """a ViT whose outputs are the features, LinearCrossEntropy on them, clipping by the common norm, one fused AdamW over both: the same weights
+    with VITK_GRAPH_STEP=1, after five steps; the head learns in every one of them"""
+    from vision_transformers_torch_xla_amd import engine, optim_factory
+    from vision_transformers_torch_xla_amd.losses import LinearCrossEntropy
+    from vision_transformers_torch_xla_amd.vit import create_model
+    monkeypatch.setenv("VITK_DROPPATH_COMPACT", "0")
+    g = torch.Generator().manual_seed(2)
+    data = [(torch.randn(8, 3, 224, 224, generator=g), torch.randint(0, 300, (8,), generator=g)) for _ in range(5)]
+
+    class Args:
+        opt, lr, weight_decay, opt_eps, opt_betas = "adamw", 1e-3, 0.05, 1e-8, None
+
+    def run(flag):
+        monkeypatch.setenv("VITK_GRAPH_STEP", flag)
+        torch.manual_seed(5)
+        model = create_model("vit_tiny_patch16_224", num_classes=64, global_pool="avg", drop_path_rate=0.1, depth=2).to(device)
+        criterion = LinearCrossEntropy(64, 300, smoothing=0.1).to(device)
+        opt = optim_factory.create_optimizer(Args, model)
+        opt.add_param_group({"params": list(criterion.parameters()), "weight_decay": 0.0})
+        seen, norms = [], []
+        step, clip = opt.step, engine.clip_grad_norm_
+        monkeypatch.setattr(opt, "step", lambda: (step(), seen.append(criterion.weight.detach().clone())))
+        with monkeypatch.context() as m:
+            m.setattr(engine, "clip_grad_norm_", lambda what, max_norm: norms.append(clip(what, max_norm)))
+            engine.train_one_epoch(model, criterion, data, opt, device, 0, max_norm=0.05, update_freq=1, log_freq=1)
+        torch.cuda.synchronize()
+        return model._flat["p"].detach().clone(), seen, torch.stack(norms)
+
+    before = engine.GraphedStep.total_replays
+    with_flag, without = run("1"), run("0")
+    assert engine.GraphedStep.total_replays == before
+    assert torch.equal(with_flag[0], without[0]) and torch.equal(with_flag[2], without[2])
+    assert all(torch.equal(a, b) for a, b in zip(with_flag[1], without[1]))
+    assert len(without[1]) == 5 and all(not torch.equal(a, b) for a, b in zip(without[1], without[1][1:]))
+
+
+@pytest.mark.gpu
+def test_vit_features_and_head_gradients(device):
+    """the gradients that the joined pair computes, against the formula on the features that the model gave"""
+    from tests.test_vocab_ops import half_ulp, plain_linear_xent
+    from vision_transformers_torch_xla_amd.losses import LinearCrossEntropy
+    from vision_transformers_torch_xla_amd.vit import create_model
+    torch.manual_seed(6)
+    model = create_model("vit_tiny_patch16_224", num_classes=64, global_pool="avg", drop_path_rate=0.0, depth=2).to(device)
+    criterion = LinearCrossEntropy(64, 211).to(device)
+    with torch.no_grad():
+        criterion.weight.mul_(20)
+    x, t = torch.randn(8, 3, 224, 224, device=device), torch.randint(0, 211, (8,), device=device)
+    t[2] = -100
+    out = model(x)
+    out.retain_grad()
+    loss = criterion(out, t)
+    loss.backward()
+    (want, _, dx, dw, db), (lt, _, dxt, dwt, dbt) = plain_linear_xent(out.detach().to(torch.bfloat16), criterion.weight.detach().to(torch.bfloat16), t,
+                                                                      criterion.bias.detach(), 0.0, -100, True)
+    assert abs(loss.item() - want.item()) <= lt + 2.0 ** -24 * abs(want)
+    for got, v, tol in ((out.grad, dx, dxt), (criterion.weight.grad, dw, dwt), (criterion.bias.grad, db, dbt)):
+        # dx is rounded to bf16 on the way (the features are products' factors), whatever the features' type
+        assert torch.all((got.double() - v).abs() <= tol + 1.01 * half_ulp(torch.bfloat16) * (v.abs() + tol) + 2.0 ** -133)
+    flat = model._flat["g"].detach().clone()
+    again = model(x)                                                     # the same gradient by hand through the model alone
+    model.zero_grad()
+    again.backward(out.grad)
+    assert torch.equal(model._flat["g"], flat) and flat.abs().max() > 0
+
+
+def _rccl_worker(rank, port, tmp):
+    sys.path.insert(0, str(ROOT))
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK="0", WORLD_SIZE="1", LOCAL_RANK="0")
+    torch.cuda.set_device(0)
+    dev = torch.device("cuda", 0)
+    from vision_transformers_torch_xla_amd.dp import GradReducer
+    dist.init_process_group("nccl", rank=0, world_size=1, device_id=dev)
+    try:
+        red = GradReducer(lambda: None, single_rank_collectives=True)
+        params = [torch.nn.Parameter(torch.randn(300, 64, device=dev)), torch.nn.Parameter(torch.randn(33, device=dev, dtype=torch.bfloat16)),
+                  torch.nn.Parameter(torch.randn(5, device=dev))]
+        for p in params[:2]:
+            p.grad = torch.randn_like(p)
+        keep = [(p.detach().clone(), None if p.grad is None else p.grad.clone()) for p in params]
+        red.share(params)
+        red.average(params)
+        torch.cuda.synchronize()
+        for p, (v, g) in zip(params, keep):                              # one rank: the average is the identity
+            assert torch.equal(p, v) and (torch.equal(p.grad, g) if g is not None else torch.all(p.grad == 0))
+        (Path(tmp) / "ok").write_text("ok")
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.gpu
+def test_head_collectives_over_rccl(device, tmp_path):
+    s = socket.socket()
+    s.bind(("127.0.0.1", 0))
+    port = s.getsockname()[1]
+    s.close()
+    mp.spawn(_rccl_worker, args=(port, str(tmp_path)), nprocs=1, join=True)
+    assert (tmp_path / "ok").exists()

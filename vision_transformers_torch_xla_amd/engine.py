@@ -82,7 +82,9 @@ class GraphedStep:
     and scaled, as timm does, instead of the compact kept-samples batches whose shapes change per step); the optimizer step, EMA,
     clipping and metrics stay outside the graph (learning rate and weight decay change per step and are kernel arguments).
     Results are those of the eager step with VITK_DROPPATH_COMPACT=0, bit for bit.  Not used with a gradient reducer (collectives
-    are not captured) or with gradient accumulation."""
+    are not captured), with gradient accumulation, or with a criterion that has trainable parameters: the gradients of those are made by
+    autograd's accumulation, whose captured memory no .grad would refer to after the next zero_grad, and which must not be captured while
+    an eager step's graph of the same parameters lives."""
 
     WARMUP = 2          # eager steps before the capture (allocator, lazy attributes, weight copies)
     total_replays = 0   # replays made by all instances (diagnostics, tests)
@@ -95,7 +97,9 @@ class GraphedStep:
         self.x = self.y = self.output = self.loss = None
 
     @staticmethod
-    def wanted(model, update_freq):
+    def wanted(model, update_freq, criterion=None):
+        if isinstance(criterion, torch.nn.Module) and any(p.requires_grad for p in criterion.parameters()):
+            return False
         return (os.environ.get("VITK_GRAPH_STEP") == "1" and update_freq == 1 and getattr(model, "reducer", None) is None
                 and hasattr(_core_model(model), "begin_static_droppath"))
 
@@ -180,7 +184,7 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
         reducer.share(head)                         # the model's own parameters were shared when it was wrapped
     optimizer.zero_grad()
     graphed = None
-    if GraphedStep.wanted(model, update_freq):      # VITK_GRAPH_STEP=1: the captured step is kept on the model from epoch to epoch
+    if GraphedStep.wanted(model, update_freq, criterion):      # VITK_GRAPH_STEP=1: the captured step is kept on the model from epoch to epoch
         holder = _core_model(model)                 # (its deep copies - an EMA model - are rebuilt from scratch and do not inherit it)
         graphed = getattr(holder, "_vitk_graphed_step", None)
         if graphed is None or graphed.criterion is not criterion or graphed.model is not model:
