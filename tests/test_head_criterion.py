@@ -272,3 +272,45 @@ def test_head_collectives_over_rccl(device, tmp_path):
     s.close()
     mp.spawn(_rccl_worker, args=(port, str(tmp_path)), nprocs=1, join=True)
     assert (tmp_path / "ok").exists()
+
+
+# -------------------------------------------------------------------------------------------- evaluation, checkpoints
+@pytest.mark.gpu
+@pytest.mark.parametrize("classes", [211, 300])
+def test_evaluate_with_the_head_of_the_criterion(device, classes, monkeypatch):
+    from vision_transformers_torch_xla_amd import engine
+    from vision_transformers_torch_xla_amd.losses import LinearCrossEntropy
+    from vision_transformers_torch_xla_amd.vit import create_model
+    torch.manual_seed(7)
+    model = create_model("vit_tiny_patch16_224", num_classes=64, global_pool="avg", drop_path_rate=0.0, depth=1).to(device).eval()
+    head = LinearCrossEntropy(64, classes, smoothing=0.1).to(device)
+    with torch.no_grad():
+        head.weight.mul_(30), head.bias.normal_()
+    data = [(torch.randn(n, 3, 224, 224), torch.randint(0, classes, (n,))) for n in (7, 8, 3)]
+    data[1][1][2:5] = -100
+    data[2][1][:] = -100                                                  # nothing counts in the last batch
+    loss, top1, top5, n = 0.0, 0, 0, 0
+    for x, t in data:
+        with torch.no_grad():
+            f = model(x.to(device)).to(torch.bfloat16).double()
+        z = f @ head.weight.detach().to(torch.bfloat16).double().t() + head.bias.detach().double()
+        keep = t != -100
+        z, t = z.cpu()[keep], t[keep]
+        if len(t):
+            # fp32 sums of 64 products and the bias
+            assert torch.all((head.logits(f.float()).cpu().double()[keep] - z).abs() <= 66 * 2.0 ** -24 * 64 * float(z.abs().max()))
+            order = z.topk(5, 1).indices == t[:, None]
+            loss += float(torch.nn.functional.cross_entropy(z, t, reduction="sum"))
+            top1, top5, n = top1 + int(order[:, 0].sum()), top5 + int(order.sum()), n + len(t)
+    for most in (1 << 28, 2 * classes):                                   # whole batches, two rows at a time
+        with monkeypatch.context() as m:
+            m.setattr(engine._by_head, "__defaults__", (most,))
+            got = engine.evaluate(data, model, device, criterion=head)
+        assert abs(got["loss"] - loss / n) <= 1e-4 * loss / n
+        assert abs(got["acc1"] - 100.0 * top1 / n) < 1e-3 and abs(got["acc5"] - 100.0 * top5 / n) < 1e-3
+    assert head.logits(torch.zeros(0, 64, device=device)).shape == (0, classes)
+    from vision_transformers_torch_xla_amd._lib import VitkError
+    with pytest.raises(VitkError, match="no target counts"):
+        engine.evaluate(data[2:], model, device, criterion=head)
+    with pytest.raises(VitkError):
+        head.logits(torch.zeros(4, 32, device=device))

@@ -23,6 +23,7 @@ from typing import Iterable, Optional
 import torch
 
 from . import ops, utils
+from ._lib import VitkError
 from .losses import CrossEntropyLoss
 
 
@@ -268,8 +269,26 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
     return {k: meter.global_avg for k, meter in metric_logger.meters.items()}
 
 
+def _by_head(head, features, target, loss_of, most=1 << 28):
+    """(loss, acc1, acc5, rows) of features through a criterion's head: over the targets that count, in pieces of at most `most` logits"""
+    features, target = features.reshape(-1, features.shape[-1]), target.reshape(-1)
+    counted = target != head.ignore_index
+    features, target = features[counted], target[counted]
+    rows, sums = target.shape[0], None
+    per = max(1, most // head.weight.shape[0])
+    for i in range(0, rows, per):
+        z, t = head.logits(features[i:i + per]), target[i:i + per]
+        part = torch.stack([loss_of(z, t), *utils.accuracy(z, t, topk=(1, 5))]) * t.shape[0]
+        sums = part if sums is None else sums + part
+    return (*(sums / rows), rows) if rows else (0.0, 0.0, 0.0, 0)         # (the meters exist on every rank all the same)
+
+
 @torch.no_grad()
-def evaluate(data_loader, model, device, use_amp=False, tpu: bool = False):
+def evaluate(data_loader, model, device, use_amp=False, tpu: bool = False, criterion=None):
+    """criterion: the training criterion where it holds the model's head (LinearCrossEntropy); the model's outputs are then features [..., D],
+    every target that counts is a row, and the loss is weighted by rows.  Any other criterion is not looked at (the loss is the cross entropy)."""
+    head = getattr(criterion, "module", criterion)
+    head = head if getattr(head, "takes_features", False) else None
     criterion = CrossEntropyLoss()
     metric_logger = utils.MetricLogger(delimiter="  ")
     model.eval()
@@ -278,14 +297,20 @@ def evaluate(data_loader, model, device, use_amp=False, tpu: bool = False):
         images = images.to(device, non_blocking=True)
         target = target.to(device, non_blocking=True)
         output = model(images)
-        loss = criterion(output, target)
-        acc1, acc5 = utils.accuracy(output, target, topk=(1, 5))
-        bs = target.shape[0]
-        metric_logger.update(loss=loss)
+        if head is not None:
+            loss, acc1, acc5, bs = _by_head(head, output, target, criterion)
+            metric_logger.meters["loss"].update(loss, n=bs)
+        else:
+            loss = criterion(output, target)
+            acc1, acc5 = utils.accuracy(output, target, topk=(1, 5))
+            bs = target.shape[0]
+            metric_logger.update(loss=loss)
         metric_logger.meters["acc1"].update(acc1, n=bs)
         metric_logger.meters["acc5"].update(acc5, n=bs)
     metric_logger.flush()
     metric_logger.synchronize_between_processes()
+    if head is not None and "loss" in metric_logger.meters and metric_logger.meters["loss"].count == 0:
+        raise VitkError("evaluate: no target counts (every one is the head's ignore_index)")
     if utils.is_main_process() and metric_logger.meters:
         print("* Acc@1 {top1.global_avg:.3f} Acc@5 {top5.global_avg:.3f} loss {losses.global_avg:.3f}".format(
             top1=metric_logger.meters["acc1"], top5=metric_logger.meters["acc5"], losses=metric_logger.meters["loss"]))

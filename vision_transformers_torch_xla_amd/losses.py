@@ -15,7 +15,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
-from ._lib import VitkError
+from ._lib import EPI_BIAS_F32, VitkError
 
 bf16, f32 = torch.bfloat16, torch.float32
 
@@ -162,6 +162,23 @@ class LinearCrossEntropy(nn.Module):
 
     def forward(self, x, target):
         return linear_cross_entropy(x, self.weight, target, self.bias, self.smoothing, self.ignore_index, self.reduction)
+
+    @torch.no_grad()
+    def logits(self, x):
+        """fp32 logits [rows, num_classes] of features [rows, in_features], for evaluation and prediction: no gradient, and as large as they are"""
+        V, D = self.weight.shape
+        if x.dim() != 2 or x.shape[1] != D:
+            raise VitkError(f"LinearCrossEntropy.logits: expected features [rows, {D}], got {tuple(x.shape)}")
+        ops._here(x, "LinearCrossEntropy.logits: features")
+        if x.shape[0] == 0:
+            return x.new_empty((0, V), dtype=f32)
+        w, b, room = self.weight.detach(), self.bias, (V + 3) // 4 * 4           # the product wants a multiple of 4 classes
+        if room != V:
+            w = torch.nn.functional.pad(w, (0, 0, 0, room - V))
+        bias = torch.zeros(room, dtype=f32, device=x.device)
+        if b is not None:
+            bias[:V] = b.detach()
+        return ops.gemm_nt(_bf16_rows(x), _bf16_rows(w), epilogue=EPI_BIAS_F32, bias=bias)[:, :V].contiguous()
 
 
 class DistillationLoss(nn.Module):
