@@ -314,3 +314,39 @@ def test_evaluate_with_the_head_of_the_criterion(device, classes, monkeypatch):
         engine.evaluate(data[2:], model, device, criterion=head)
     with pytest.raises(VitkError):
         head.logits(torch.zeros(4, 32, device=device))
+
+
+def test_the_head_of_the_criterion_is_saved_and_restored(tmp_path):
+    import argparse
+
+    from vision_transformers_torch_xla_amd import utils
+    from vision_transformers_torch_xla_amd._lib import VitkError
+    from vision_transformers_torch_xla_amd.losses import CrossEntropyLoss, LinearCrossEntropy
+    args = lambda: argparse.Namespace(output_dir=str(tmp_path), auto_resume=True, resume="", start_epoch=0)          # noqa: E731
+
+    def fresh(seed):
+        torch.manual_seed(seed)
+        model, head = torch.nn.Linear(8, 8), LinearCrossEntropy(8, 33)
+        opt = torch.optim.AdamW([*model.parameters(), *head.parameters()], lr=0.1)
+        for p in (*model.parameters(), *head.parameters()):
+            p.grad = torch.randn_like(p)
+        opt.step()
+        return model, head, opt
+    model, head, opt = fresh(0)
+    utils.save_model(args(), 4, model, model, opt, None, criterion=head)
+    assert set(torch.load(tmp_path / "checkpoint-4.pth", weights_only=True)["criterion"]) == {"weight", "bias"}
+    model2, head2, opt2 = fresh(1)
+    a = args()
+    utils.auto_load_model(a, model2, model2, opt2, None, criterion=head2)
+    assert a.start_epoch == 5 and torch.equal(head.weight, head2.weight) and torch.equal(head.bias, head2.bias) and torch.equal(model.weight, model2.weight)
+    assert torch.equal(opt.state[head.weight]["exp_avg"], opt2.state[head2.weight]["exp_avg"])
+    # a criterion without parameters: as before; a file without the head is refused before anything is changed
+    utils.save_model(args(), 5, model, model, opt, None, criterion=CrossEntropyLoss())
+    assert "criterion" not in torch.load(tmp_path / "checkpoint-5.pth", weights_only=True)
+    model3, head3, opt3 = fresh(2)
+    keep = model3.weight.detach().clone()
+    with pytest.raises(VitkError, match="criterion"):
+        utils.auto_load_model(args(), model3, model3, opt3, None, criterion=head3)
+    assert torch.equal(model3.weight, keep)
+    utils.auto_load_model(args(), model3, model3, opt3, None)
+    assert torch.equal(model3.weight, model.weight)

@@ -325,10 +325,17 @@ def _plain_args(args):
             for k, v in src.items()}
 
 
-def save_model(args, epoch, model, model_without_ddp, optimizer, loss_scaler, model_ema=None):
+def _criterion_module(criterion):
+    """the criterion behind a wrapper, where it has something of its own to keep (a head); else None"""
+    core = getattr(criterion, "module", criterion)
+    return core if isinstance(core, torch.nn.Module) and len(core.state_dict()) > 0 else None
+
+
+def save_model(args, epoch, model, model_without_ddp, optimizer, loss_scaler, model_ema=None, criterion=None):
     """checkpoint-{epoch}.pth under args.output_dir, written by rank 0: {'model', 'optimizer', 'epoch', 'scaler', 'args'
     [, 'model_ema']} with timm parameter names, then the checkpoint save_ckpt_num * save_ckpt_freq epochs back is removed
-    (utils/__init__.py:686-732).  'args' is stored as a dict of plain values."""
+    (utils/__init__.py:686-732).  'args' is stored as a dict of plain values.  criterion: a criterion with parameters (a head,
+    losses.LinearCrossEntropy) is stored beside the model as 'criterion'; its optimizer state is the optimizer's."""
     from pathlib import Path
     output_dir = Path(args.output_dir)
     output_dir.mkdir(parents=True, exist_ok=True)
@@ -343,6 +350,8 @@ def save_model(args, epoch, model, model_without_ddp, optimizer, loss_scaler, mo
     if model_ema is not None:
         ema = model_ema.ema if hasattr(model_ema, "ema") else model_ema
         to_save["model_ema"] = {k: v.detach().cpu() for k, v in ema.state_dict().items()}
+    if _criterion_module(criterion) is not None:
+        to_save["criterion"] = {k: v.detach().cpu() for k, v in _criterion_module(criterion).state_dict().items()}
     save_on_master(to_save, checkpoint_path)
     if is_main_process() and isinstance(epoch, int):
         to_del = epoch - getattr(args, "save_ckpt_num", 3) * getattr(args, "save_ckpt_freq", 1)
@@ -399,10 +408,11 @@ def save_safetensors(model, path):
     safetensors.torch.save_file({k: v.detach().cpu().contiguous() for k, v in model.state_dict().items()}, str(path))
 
 
-def auto_load_model(args, model, model_without_ddp, optimizer, loss_scaler, model_ema=None):
+def auto_load_model(args, model, model_without_ddp, optimizer, loss_scaler, model_ema=None, criterion=None):
     """Resume from args.resume, or with args.auto_resume from the highest-numbered checkpoint-*.pth in args.output_dir:
     restores the model, and when the file holds them the optimizer state, args.start_epoch = epoch + 1, the EMA weights
-    and the scaler (utils/__init__.py:735-770)."""
+    and the scaler (utils/__init__.py:735-770).  criterion: a criterion with parameters gets those that save_model stored for it; a
+    file without them is refused (the model would go on with another head)."""
     import glob
     from pathlib import Path
     output_dir = Path(args.output_dir)
@@ -417,7 +427,13 @@ def auto_load_model(args, model, model_without_ddp, optimizer, loss_scaler, mode
         print("Auto resume checkpoint: %s" % getattr(args, "resume", ""))
     if getattr(args, "resume", ""):
         checkpoint = _load_checkpoint_file(args.resume)
+        holder = _criterion_module(criterion)
+        if holder is not None and "criterion" not in checkpoint:
+            from ._lib import VitkError
+            raise VitkError(f"{args.resume} holds no parameters for the criterion (save_model(criterion=...) stores them)")
         model_without_ddp.load_state_dict(checkpoint["model"])
+        if holder is not None:
+            holder.load_state_dict(checkpoint["criterion"])
         print("Resume checkpoint %s" % args.resume)
         if "optimizer" in checkpoint and "epoch" in checkpoint:
             optimizer.load_state_dict(checkpoint["optimizer"])
