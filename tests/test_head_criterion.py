@@ -350,3 +350,34 @@ def test_the_head_of_the_criterion_is_saved_and_restored(tmp_path):
     assert torch.equal(model3.weight, keep)
     utils.auto_load_model(args(), model3, model3, opt3, None)
     assert torch.equal(model3.weight, model.weight)
+
+
+@pytest.mark.gpu
+def test_a_model_without_a_gradient_stays_out_of_the_common_norm(device):
+    """zero_grad only marks the flat buffer; where the next step trains the head alone, the values of the step before are no part of its norm"""
+    from vision_transformers_torch_xla_amd import engine
+    from vision_transformers_torch_xla_amd.losses import LinearCrossEntropy
+    from vision_transformers_torch_xla_amd.vit import create_model
+    torch.manual_seed(8)
+    model = create_model("vit_tiny_patch16_224", num_classes=64, global_pool="avg", drop_path_rate=0.0, depth=1).to(device)
+    head = LinearCrossEntropy(64, 50).to(device)
+    x, t = torch.randn(4, 3, 224, 224, device=device), torch.randint(0, 50, (4,), device=device)
+    of = lambda *ts: float(torch.sqrt(sum(v.double().square().sum() for v in ts)))          # noqa: E731
+    for set_to_none in (True, False):
+        head.zero_grad()
+        head(model(x), t).backward()
+        flat = model._flat["g"].clone()
+        own = [p.grad.clone() for p in head.parameters()]
+        assert abs(engine.clip_grad_norm_([model, head], 1e9).item() / of(flat, *own) - 1) < 1e-6
+        model.zero_grad(set_to_none)
+        head.zero_grad()
+        with torch.no_grad():
+            f = model(x)
+        head(f, t).backward()                                            # linear probing
+        own = [p.grad.clone() for p in head.parameters()]
+        norm = engine.clip_grad_norm_([model, head], 0.5 * of(*own))
+        assert abs(norm.item() / of(*own) - 1) < 1e-6 and abs(of(*(p.grad for p in head.parameters())) / (0.5 * of(*own)) - 1) < 1e-5
+        assert torch.equal(model._flat["g"], flat)
+    for p in model.parameters():                                         # a foreign optimizer's zero_grad
+        p.grad = None
+    assert abs(engine.clip_grad_norm_([model, head], 1e9).item() / of(*(p.grad for p in head.parameters())) - 1) < 1e-6

@@ -46,6 +46,9 @@ def _grad_tensors(source):
     if isinstance(source, torch.nn.Module):
         core = _core_model(source)
         if hasattr(core, "_ensure_grad_buffer"):
+            # zero_grad leaves the buffer's values where they are: without a backward pass since, they are nobody's gradient
+            if core._grad_touched and not (core._grad_valid and any(p.grad is not None for p in core._plist)):
+                return []
             return [core._ensure_grad_buffer()]
         return [p.grad.detach() for p in source.parameters() if p.grad is not None]
     return [g for item in source for g in _grad_tensors(item)]

@@ -446,6 +446,8 @@ class VisionTransformer(nn.Module):
         o = self._offs["pos_embed"]
         self._gpos2d = flat_g[o:o + self.num_tokens * D].view(self.num_tokens, D)
 
+    _grad_touched = False           # whether a backward pass has written the gradient buffer since the model was made
+
     def _ensure_grad_buffer(self):
         """the flat fp32 gradient buffer of a model built with a lazy one (deep copies: an EMA copy never trains)"""
         if self._flat["g"] is None:
@@ -974,7 +976,7 @@ class VisionTransformer(nn.Module):
         for n, p in zip(self._pnames, self._plist):
             if p.grad is None or p.grad.data_ptr() != self._gview[n].data_ptr():
                 p.grad = self._gview[n]
-        self._grad_valid = True
+        self._grad_valid = self._grad_touched = True
         if pending_ln:
             ev = torch.cuda.Event()
             ev.record()
