@@ -695,6 +695,24 @@ def test_linear_xent_loss_of_certain_rows(device, top):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [2, 3, 6, 13])
+@pytest.mark.parametrize("grad", [False, True])
+def test_linear_xent_loss_of_few_classes(device, V, grad):
+    """few terms to a sum: nothing averages a rounding out"""
+    ops = _ops()
+    g = torch.Generator().manual_seed(V)
+    x, w = torch.zeros(400, 8), torch.zeros(V, 8)
+    x[:, :3], w[:, :3] = torch.randint(-2, 3, (400, 3), generator=g).float(), torch.randint(-1, 2, (V, 3), generator=g).float()
+    x, w = x.to(bf16).to(device), w.to(bf16).to(device)
+    target = torch.randint(0, V, (400,), generator=g).to(device)
+    r = ops.linear_xent(x, w, target, want_grad=grad)
+    z = x.double() @ w.double().t()                                                      # whole numbers up to 6
+    want = torch.logsumexp(z, 1) - z.gather(1, target[:, None])[:, 0]
+    # exp(-d): the argument's rounding, d e^-d < 0.4, and the exponential's own ulp; the sum, its logarithm, ln 2, the result
+    assert torch.all((r.rows.double() - want).abs() <= 8 * U32 * (1 + want))
+
+
+@pytest.mark.gpu
 def test_linear_xent_row_whose_mask_leaves_nothing(device):
     """every class masked out with the type's lowest value: equal logits, as a softmax has it; with -inf: NaN, as a softmax has it"""
     ops = _ops()

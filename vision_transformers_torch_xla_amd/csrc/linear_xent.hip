@@ -1,4 +1,5 @@
-// Softmax cross entropy of a linear layer over a large vocabulary, with its gradients, without the logits in memory.
+// Softmax cross entropy of a linear layer over a large vocabulary, with its gradients.  The logits stay in registers; what the gradients need of
+// them is kept in 2 bytes each, for a block of rows at a time.
 //
 //   z = x W^T + b      lse_i = log sum_j exp z_ij      loss_i = lse_i - (1 - e) z_i,t(i) - e/V sum_j z_ij
 //   dz_ij = p_ij - (1 - e) [j = t(i)] - e/V            dx = g dz W      dW = g dz^T x      db = g sum_i dz_i
@@ -14,7 +15,7 @@
 //      by up to 1 part in 256 in the same direction everywhere: dz is divided by g and by a number that makes 1 - e a bf16 number and
 //      e/V nearly one (lx_factor); both multiply the fp32 sums of the next step.
 //      Where dW is wanted it also copies x, with zeros for the rows that are not counted: their dz is zero, but zero times what such a row may
-//      hold (infinities, NaN) would not be.  2 T D bytes written beside the 4 T V of P: under 1 % of a call.
+//      hold (infinities, NaN) would not be.  2 T D bytes written beside the 4 T V of P: 0.3 to 1.4 % of a call.
 //   3. dx = dz W and dW = dz^T x (lx_grad_kernel), and the column sums for db, to which each target's dz adds what its rounding took (near
 //      -(1 - e) a probability of less than 2^-9 vanishes).
 // 6 T V D floating-point operations: nothing is computed twice.  Keeping one 16-bit factor per logit of a block costs 4 bytes of
@@ -65,12 +66,11 @@ static __device__ __forceinline__ bf16x8 lx_tr(const bf16_t* lo, const bf16_t* h
     const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)hi);
     return (bf16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
-// P's numbers.  The epilogue forms 2^(z - m - 64), whose fp32 exponent field ends at 63 (6 bits); 10 bits of the fraction are kept, to nearest.  Read
-// back, the 16 bits in place are that number again (its subnormals too: exponent field 0), and 2^64 goes into the factor it is multiplied with.
-// Two of them to a word take three instructions, as fp16's conversion does.
-#define LX_P_SCALE 64
+// P's numbers, at most 1.  Times 2^-64 their fp32 exponent field ends at 63 (6 bits); 10 bits of the fraction are kept, to nearest.  Read back, the 16
+// bits in place are that number again (its subnormals too: exponent field 0), and 2^64 goes into the factor it is multiplied with.  (2^-64 within
+// the exponential's argument saves the product, but rounds the argument to 4e-6 there: the row sums of few classes were twice as far off.)
 static __device__ __forceinline__ unsigned lx_pack_p(float a, float b) {
-    const unsigned x = (__float_as_uint(a) + 0x1000u) << 3, y = (__float_as_uint(b) + 0x1000u) << 3;
+    const unsigned x = (__float_as_uint(a * 0x1p-64f) + 0x1000u) << 3, y = (__float_as_uint(b * 0x1p-64f) + 0x1000u) << 3;
     return __builtin_amdgcn_perm(y, x, 0x07060302u);        // the upper halves of both
 }
 static __device__ __forceinline__ float lx_unpack_p(unsigned v) { return __uint_as_float(v << 13); }
@@ -87,8 +87,8 @@ static __device__ __forceinline__ float lx_over_row(float v, F&& f) {
 // The loss's epilogue of a wave that holds FM * 16 rows (from m0) by 64 columns (from n0) of logits: lane (lr, lg) has columns 16 tn + 4 lg + j
 // of row 16 tm + lr.  stg: 2 KB of LDS of the wave's own, through which P leaves in rows of 64 columns so that a store covers whole lines.
 // EXTRA: with a bias or the sums of the logits.  WANT_P, FULL (every row is one of the matrix): so that the code of the rows has no branch and the
-// rows' chains of maximum, exponentials and sum overlap (with a branch per row and the sums through LDS: 2804 instead of 2750 us at 8192 x 100003 x
-// 2048, 174 instead of 167 at 2047 x 50021 x 1024).
+// rows' chains of maximum, exponentials and sum overlap (a branch per row and the sums through LDS cost 2 % of the logits at 8192 x 100003 x
+// 2048, 4 % at 2047 x 50021 x 1024).
 template <int FM, bool EXTRA, bool WANT_P, bool FULL>
 static __device__ __forceinline__ void lx_loss_rows(const LxGemmParams& p, f32x4 (&acc)[FM][4], int m0, int n0, bf16_t* stg) {
     int lane = threadIdx.x & 63;
@@ -116,17 +116,18 @@ static __device__ __forceinline__ void lx_loss_rows(const LxGemmParams& p, f32x4
         }
         mx = lx_over_row(mx, [](float a, float b) { return fmaxf(a, b); });
         // The maximum is taken off before the product with log2(e), so that the largest gives 1 exactly however large the logits are.  (With
-        // z * log2(e) - fl(m * log2(e)) as one fma a logit saves an instruction, but from logits of 10^7 on the product's rounding is whole powers of two.)
+        // z * log2(e) - fl(m * log2(e)) as one fma a logit saves an instruction, 0.5 to 1.2 % of a call, but from logits of 10^7 on the product's
+        // rounding is whole powers of two; a second form for those, behind a branch, spills the accumulators.)
         const float off = mx == -INFINITY ? 0.f : mx;         // a row of -inf only: 2^(-inf) = 0
         float q[4];
 #pragma unroll
         for (int tn = 0; tn < 4; ++tn) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) z[tn][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[tm][tn][j] - off, 1.44269504088896340736f, -(float)LX_P_SCALE));
+            for (int j = 0; j < 4; ++j) z[tn][j] = __builtin_amdgcn_exp2f((acc[tm][tn][j] - off) * 1.44269504088896340736f);
             q[tn] = (z[tn][0] + z[tn][1]) + (z[tn][2] + z[tn][3]);
         }
         mxs[tm] = mx;
-        sums[tm] = lx_over_row((q[0] + q[1]) + (q[2] + q[3]), [](float a, float b) { return a + b; }) * 0x1p+64f;
+        sums[tm] = lx_over_row((q[0] + q[1]) + (q[2] + q[3]), [](float a, float b) { return a + b; });
         if constexpr (WANT_P) {
 #pragma unroll
             for (int tn = 0; tn < 4; ++tn) {
@@ -1379,7 +1380,7 @@ struct LxPlan {
 //   1 x 1000 x 192       10 23 12 : 7 8 7 : 4 7 4             512 x 8192 x 768     22 33 22 : 15 21 14 : 19 19 16
 //   1024 x 1024 x 1024   30 31 33 : 16 17 16 : 11 12 10       8192 x 8192 x 768    89 119 120 : 157 114 99 : 244 154 156
 //   512 x 21843 x 768    25 43 37 : 31 36 34 : 47 33 36       512 x 100003 x 1024  117 118 142 : 158 156 189 : 245 262 260
-// It is off by up to 15 %; where that makes it take the slower one (512 x 100003 x 1024: 308 us for both gradients, the large kernel 260), another
+// It is off by up to 18 %; where that makes it take the slower one (512 x 100003 x 1024: 308 us for both gradients, the large kernel 260), another
 // term for the memory cost as much elsewhere (512 x 50000 x 2048: 247, 264).
 // Large: whole rows alone take ceil(rows / teams) rounds; cutting what does not fill a round into ranges fills it at the price of parts written
 // and read, 0.13 us for one of 256 x 256 (512 KB at 4 TB/s).
