@@ -301,7 +301,7 @@ int vitk_xent_soft_fwd_bwd(const float* logits, int ld, const float* target, int
  * main.py:939-970 / test_kd.py:43-88 */
 int vitk_kd_kl_fwd_bwd(const float* student, int lds_, const float* teacher, int ldt, float temperature,
                        float* loss_rows, float* dstudent, int ldd, float grad_scale, int B, int C, void* stream);
-/* ---- cross entropy of a linear layer over a large vocabulary, with its gradients, without the logits in memory (the head's
+/* ---- cross entropy of a linear layer over a large vocabulary, with its gradients; no logits are stored, 2 bytes of each at most (the head's
  * nn.Linear followed by the criterion, main.py:926-935, in one call):  z = x w^T + bias;
  * rows[i] = (1-smoothing) * (lse_i - z_i,target) + smoothing * (lse_i - mean_j z_ij), 0 where target == ignore_index;
  * loss[0] = sum of rows / number of counted rows (mean != 0) or their sum; 0 without a counted row.  A target outside [0, V) that is not

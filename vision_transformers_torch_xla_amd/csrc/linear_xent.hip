@@ -116,7 +116,7 @@ static __device__ __forceinline__ void lx_loss_rows(const LxGemmParams& p, f32x4
         }
         mx = lx_over_row(mx, [](float a, float b) { return fmaxf(a, b); });
         // The maximum is taken off before the product with log2(e), so that the largest gives 1 exactly however large the logits are.  (With
-        // z * log2(e) - fl(m * log2(e)) as one fma a logit saves an instruction, 0.5 to 1.2 % of a call, but from logits of 10^7 on the product's
+        // z * log2(e) - fl(m * log2(e)) as one fma a logit saves an instruction, 0.5 to 1 % of a call, but from logits of 10^7 on the product's
         // rounding is whole powers of two; a second form for those, behind a branch, spills the accumulators.)
         const float off = mx == -INFINITY ? 0.f : mx;         // a row of -inf only: 2^(-inf) = 0
         float q[4];

@@ -1,6 +1,6 @@
 """Criteria of the reference's training loop, computed by fused HIP kernels (log-softmax, loss and gradient in
 one pass over fp32 logits; linear_cross_entropy / LinearCrossEntropy take the features and the head's weight instead, for label sets
-whose logits are too large to hold).
+whose fp32 logits and their gradient are too large to hold).
 
 Mirrors main.py:926-935 (criterion choice: timm SoftTargetCrossEntropy when mixup is on, timm
 LabelSmoothingCrossEntropy(smoothing) when smoothing > 0, else nn.CrossEntropyLoss) and the inline knowledge
@@ -128,7 +128,7 @@ class _LinearXent(torch.autograd.Function):
 
 
 def linear_cross_entropy(x, weight, target, bias=None, smoothing: float = 0.0, ignore_index: int = -100, reduction: str = "mean"):
-    """cross entropy of the logits x @ weight.T + bias without the logits in memory (ops.linear_xent): x [..., D], weight [V, D] (bf16, or fp32
+    """cross entropy of the logits x @ weight.T + bias, of which 2 bytes each are held for a block of rows at a time (ops.linear_xent): x [..., D], weight [V, D] (bf16, or fp32
     masters, which are rounded to bf16 for the products as every linear of this package does), bias [V], target [...] int64.
     Differentiable in x, weight and bias, once.  reduction 'mean' (over the targets that are not ignore_index) or 'sum'."""
     if x.dim() < 1 or tuple(x.shape[:-1]) != tuple(target.shape):
@@ -145,7 +145,9 @@ class LinearCrossEntropy(nn.Module):
     """A classification head and its criterion in one: owns weight [num_classes, in_features] and bias (fp32 masters, timm's head
     initialisation), takes the features instead of the logits.  For label sets so large that the logits and their gradient are what fills
     the memory: 21 843 classes, or the vocabulary of a token-prediction objective over every position.  As a criterion of train_one_epoch it is
-    clipped together with the model; its parameters belong into the optimizer beside the model's."""
+    clipped together with the model and averaged over its ranks; its parameters belong into the optimizer beside the model's
+    (optimizer.add_param_group), itself into evaluate, save_model and auto_load_model (criterion=...).  A weight average (utils.ModelEma)
+    does not cover it."""
 
     takes_features = True           # train_one_epoch: the model's output is not a matrix of logits
 

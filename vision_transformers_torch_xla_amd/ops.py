@@ -603,16 +603,17 @@ LINEAR_XENT_BLOCK = 2 << 30          # bytes of probabilities that linear_xent h
 
 def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, reduction="mean", want_grad=True, dweight_dtype=None,
                 block_bytes=LINEAR_XENT_BLOCK, grads=("x", "weight", "bias")):
-    """Cross entropy of the logits x @ weight.T + bias against int64 targets, with the gradients of the reduced loss, without the logits in
-    memory: x bf16 [T, D], weight bf16 [V, D] (rows may have a stride), bias fp32 / bf16 [V], target [T].  D % 8 == 0, V <= 2^22.
+    """Cross entropy of the logits x @ weight.T + bias against int64 targets, with the gradients of the reduced loss; of the logits 2 bytes each
+    are held, for a block of rows at a time: x bf16 [T, D], weight bf16 [V, D] (rows may have a stride), bias fp32 / bf16 [V], target [T].
+    D % 8 == 0, V <= 2^22.
 
     rows[i] = (1 - smoothing) * nll + smoothing * mean_j(-logp_ij), 0 where target == ignore_index; loss = their mean over the counted
     rows, or their sum (reduction 'sum'); 0 with zero gradients where no row counts.  Any other target outside [0, V) gives NaN.
     What an ignored row of x holds (infinities, NaN) goes nowhere; its row of dx is zero.
     want_grad: dx bf16 [T, D], dweight [V, D] in dweight_dtype (bf16, the default, or float32), dbias in the bias's type.
     grads: which of them; a frozen head or frozen features cost one product less.
-    block_bytes: the rows are worked through in blocks that hold about this many bytes of probabilities (at least 256 rows); more than
-    one block costs an fp32 copy of a bf16 dweight."""
+    block_bytes: the rows are worked through in blocks that hold about this many bytes of probabilities (at least 256 rows), and a copy of
+    their x; more than one block costs an fp32 copy of a bf16 dweight."""
     for t, n in ((x, "x"), (weight, "weight")):
         if t.dtype != bf16 or t.dim() != 2:
             raise _lib.VitkError(f"linear_xent: {n} must be a bf16 matrix, got {t.dtype} {tuple(t.shape)}")
