@@ -104,15 +104,19 @@ def _train(model, criterion, data, max_norm, update_freq=1):
     return torch.cat([p.detach().reshape(-1) for p in (*model.parameters(), *criterion.parameters())])
 
 
+CASES = ((0.3, 1, False), (0.0, 1, False), (0.3, 2, False), (0.3, 1, True))          # max_norm, micro-steps to a step, a frozen weight
+
+
 def _worker(rank, world, port, tmp):
     sys.path.insert(0, str(ROOT))
     os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank))
     torch.set_num_threads(1)
     dist.init_process_group("gloo", rank=rank, world_size=world)
     try:
-        for case, (max_norm, update_freq) in enumerate(((0.3, 1), (0.0, 1), (0.3, 2))):
+        for case, (max_norm, update_freq, frozen) in enumerate(CASES):
             torch.manual_seed(5)
             model, criterion = Features(reducer=True), Head()
+            criterion.weight.requires_grad_(not frozen)
             torch.manual_seed(50 + rank)                                 # a head of its own on every rank: rank 0's is the one that counts
             with torch.no_grad():
                 criterion.weight.add_(torch.randn(criterion.weight.shape) * (rank + 0.5))
@@ -133,10 +137,11 @@ def _alone(tmp):
     """one process, the whole batches, from rank 0's head"""
     sys.path.insert(0, str(ROOT))
     torch.set_num_threads(1)
-    for case, (max_norm, update_freq) in enumerate(((0.3, 1), (0.0, 1), (0.3, 2))):
+    for case, (max_norm, update_freq, frozen) in enumerate(CASES):
         start, got = torch.load(Path(tmp) / f"case{case}.pt", weights_only=True)
         torch.manual_seed(5)
         model, criterion = Features(), Head()
+        criterion.weight.requires_grad_(not frozen)
         with torch.no_grad():
             for p, v in zip(criterion.parameters(), start):
                 p.copy_(v)

@@ -33,10 +33,10 @@ def _core_model(model):
 
 
 def _head_parameters(criterion):
-    """the trainable parameters of a criterion that holds the model's head (LinearCrossEntropy, also inside a wrapper with .module); a criterion
-    that merely has parameters is its owner's affair"""
+    """the parameters of a criterion that holds the model's head (LinearCrossEntropy, also inside a wrapper with .module); a criterion that merely
+    has parameters is its owner's affair"""
     core = getattr(criterion, "module", criterion)
-    return [p for p in core.parameters() if p.requires_grad] if getattr(core, "takes_features", False) else []
+    return list(core.parameters()) if getattr(core, "takes_features", False) else []
 
 
 def _grad_tensors(source):
@@ -185,7 +185,8 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
     reducer = getattr(model, "reducer", None)
     head = _head_parameters(criterion)
     if reducer is not None:
-        reducer.share(head)                         # the model's own parameters were shared when it was wrapped
+        reducer.share(head)                         # frozen ones too; the model's own parameters were shared when it was wrapped
+    head = [p for p in head if p.requires_grad]
     optimizer.zero_grad()
     graphed = None
     if GraphedStep.wanted(model, update_freq, criterion):      # VITK_GRAPH_STEP=1: the captured step is kept on the model from epoch to epoch
