@@ -986,6 +986,16 @@ def test_linear_xent_refuses(device):
             call()
 
 
+@pytest.mark.gpu
+def test_linear_xent_without_rows_checks_its_arguments(device):
+    ops, err = _ops(), _error()
+    x, w, t = torch.empty(0, 16, device=device, dtype=bf16), torch.zeros(9, 16, device=device, dtype=bf16), torch.empty(0, dtype=torch.int64, device=device)
+    assert ops.linear_xent(x, w, t, smoothing=0.1).loss.item() == 0.0
+    for kw in ({"smoothing": 1.5}, {"smoothing": math.nan}, {"smoothing": -0.1}, {"reduction": "none"}, {"block_bytes": 0}):
+        with pytest.raises(err):
+            ops.linear_xent(x, w, t, **kw)
+
+
 # --------------------------------------------------------------------------------------- modules and the path
 def close(got, want, rel):
     got, want = got.detach().double().cpu(), want.double()

@@ -628,6 +628,9 @@ def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, 
         raise _lib.VitkError(f"linear_xent: block_bytes must be positive, got {block_bytes}")
     if isinstance(grads, str) or not set(grads) <= {"x", "weight", "bias"}:
         raise _lib.VitkError(f"linear_xent: grads must be some of ('x', 'weight', 'bias'), got {grads!r}")
+    smooth = float(smoothing)
+    if not 0.0 <= smooth <= 1.0:
+        raise _lib.VitkError(f"linear_xent: smoothing {smoothing} outside [0, 1]")
     if reduction not in ("mean", "sum"):
         raise _lib.VitkError(f"linear_xent: reduction must be 'mean' or 'sum' (rows are returned beside either), got {reduction!r}")
     btype = 0
@@ -658,7 +661,7 @@ def linear_xent(x, weight, target, bias=None, smoothing=0.0, ignore_index=-100, 
                 t.zero_()
         return LinearXent(loss, rows, dx, dw, db)
     lib = _lib.load()
-    wf32, smooth = int(wtype == f32), float(smoothing)
+    wf32 = int(wtype == f32)
     need = lib.vitk_linear_xent_workspace(T, V, D, int(any(t is not None for t in (dx, dw, db))), int(smooth > 0), wf32, int(db is not None), int(block_bytes))
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
     check(lib.vitk_linear_xent(x.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(bias), btype, _ptr(target),
